@@ -1,0 +1,96 @@
+/*
+ * C-ABI of the dense operators around deformable attention in an encoder or
+ * decoder layer: the linear layer with its epilogue and gradients, its 8-bit
+ * input checkpoint, and layer norm with its gradients. Part of
+ * `libmuspace_msda.so`, MI355X (gfx950).
+ *
+ * Tensors are device pointers, dense, row-major, all of one type: float32 (0),
+ * float16 (1) or bfloat16 (2), unless noted. Products and statistics are summed
+ * in float32, in a fixed order; every result is rounded once, to its type. Any
+ * sizes and any alignment of the type are allowed; rows of whole 16-byte pieces
+ * on 16-byte boundaries are the fast case.
+ *
+ * linear        z = x weight^T + bias;  output = act(z) + residual
+ *               x [rows, in], weight [out, in], bias [out] or NULL,
+ *               residual [rows, out] or NULL, output [rows, out]
+ * activation    0 none, 1 relu, 2 gelu (z * Phi(z), by the error function)
+ * relu_mask     [rows, ceil(out / 8)] bytes: bit i of byte j is set where the
+ *               derivative of relu at z[8 j + i] is one (z > 0, or NaN)
+ * pre_activation [rows, out] z in the tensors' type, kept for gelu's derivative
+ * codes, scales an 8-bit checkpoint of x: [rows, pad32(in)] int8 and
+ *               [rows, pad32(in) / 32] bytes. 32 values share 2^e, the smallest
+ *               power of two with 127 * 2^e at or over their largest magnitude;
+ *               the byte is e + 127, or 255 where one of them is an infinity or
+ *               NaN: such a block reads back as NaN. code * 2^e is a number of
+ *               the tensors' type, so products read back exactly what is kept.
+ *
+ * Conventions: launches are ordered on `stream`, on the current device; nothing
+ * synchronises or allocates. Return 0 or a MUSPACE_E* code with
+ * muspace_last_error() set (muspace_msda.h). rows may be 0 (gradients of weight
+ * and bias are then zero). in, out at most 2^20; rows below 2^31 - 256.
+ */
+#ifndef MUSPACE_LAYER_H_
+#define MUSPACE_LAYER_H_
+
+#include <stddef.h>
+#include <stdint.h>
+
+#include "muspace_msda.h"
+
+#ifdef __cplusplus
+extern "C" {
+#endif
+
+/* relu_mask and pre_activation may be NULL (no gradient wanted); relu_mask is
+ * written for activation 1 only, pre_activation for activation 2 only. */
+MUSPACE_API int linear_forward(const void *x, int dtype, const void *weight, const void *bias,
+                               const void *residual, void *output, uint8_t *relu_mask,
+                               void *pre_activation, int64_t rows, int64_t in_features,
+                               int64_t out_features, int activation, void *stream);
+
+MUSPACE_API int linear_checkpoint(const void *x, int dtype, int8_t *codes, uint8_t *scales,
+                                  int64_t rows, int64_t in_features, void *stream);
+
+/* Bytes of workspace of linear_backward (256-byte aligned; 0: none needed). */
+MUSPACE_API size_t linear_backward_workspace_size(int dtype, int64_t rows, int64_t in_features,
+                                                  int64_t out_features, int activation);
+
+/* dz = grad_output * act'(z); grad_input = dz weight; grad_weight = dz^T x;
+ * grad_bias = sum of dz over rows. A NULL gradient is not computed. x is needed
+ * for grad_weight unless codes and scales are given in its place; weight for
+ * grad_input; relu_mask for activation 1; pre_activation for activation 2.
+ * The gradient of the residual is grad_output itself. Outputs are overwritten. */
+MUSPACE_API int linear_backward(const void *grad_output, int dtype, const void *x,
+                                const int8_t *codes, const uint8_t *scales, const void *weight,
+                                const uint8_t *relu_mask, const void *pre_activation,
+                                void *grad_input, void *grad_weight, void *grad_bias,
+                                int64_t rows, int64_t in_features, int64_t out_features,
+                                int activation, void *workspace, size_t workspace_bytes,
+                                void *stream);
+
+/* layer norm over the last dimension:
+ *   c = x - mean(x);  s = 1 / sqrt(mean(c^2) + eps);  output = c s weight + bias
+ * x, output [rows, cols]; weight, bias [cols] of weight_dtype (dtype or float32),
+ * each may be NULL (ones, zeros). statistics [rows, 2] float32 or NULL: the mean
+ * as an offset from the row's first value, and s; the backward reads them. */
+MUSPACE_API int layer_norm_forward(const void *x, int dtype, const void *weight, const void *bias,
+                                   int weight_dtype, void *output, float *statistics, int64_t rows,
+                                   int64_t cols, float eps, void *stream);
+
+MUSPACE_API size_t layer_norm_backward_workspace_size(int dtype, int64_t rows, int64_t cols);
+
+/* With h = c s and w = grad_output weight:
+ *   grad_input = s (w - mean(w) - h mean(w h));  grad_weight = sum of grad_output h over rows;
+ *   grad_bias = sum of grad_output over rows (both of weight_dtype).
+ * A NULL gradient is not computed; the workspace is needed for the last two. */
+MUSPACE_API int layer_norm_backward(const void *grad_output, int dtype, const void *x,
+                                    const void *weight, int weight_dtype, const float *statistics,
+                                    void *grad_input, void *grad_weight, void *grad_bias,
+                                    int64_t rows, int64_t cols, void *workspace,
+                                    size_t workspace_bytes, void *stream);
+
+#ifdef __cplusplus
+}
+#endif
+
+#endif /* MUSPACE_LAYER_H_ */

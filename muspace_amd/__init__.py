@@ -7,7 +7,11 @@ as mu_space`` gives code written against the reference the same names.
 """
 
 from .ops import (
+    checkpoint_int8,
+    checkpoint_restore,
     explain_dispatch,
+    layer_norm,
+    linear,
     multi_scale_deformable_attn,
     multi_scale_deformable_attn_pytorch,
     multi_scale_deformable_attn_pytorch_compat,
@@ -28,10 +32,14 @@ __all__ = [
     "DispatchDecision",
     "DispatchReport",
     "__version__",
+    "checkpoint_int8",
+    "checkpoint_restore",
     "clear_dispatch_report",
     "explain_dispatch",
     "get_dispatch_reports",
     "get_last_dispatch_report",
+    "layer_norm",
+    "linear",
     "multi_scale_deformable_attn",
     "multi_scale_deformable_attn_pytorch",
     "multi_scale_deformable_attn_pytorch_compat",

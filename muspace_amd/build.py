@@ -17,7 +17,12 @@ from pathlib import Path
 
 PACKAGE_DIR = Path(__file__).resolve().parent
 REPO_DIR = PACKAGE_DIR.parent
-SOURCES = (PACKAGE_DIR / "csrc" / "msda_capi.hip", PACKAGE_DIR / "csrc" / "dfa_capi.hip")
+SOURCES = (
+    PACKAGE_DIR / "csrc" / "msda_capi.hip",
+    PACKAGE_DIR / "csrc" / "dfa_capi.hip",
+    PACKAGE_DIR / "csrc" / "linear_capi.hip",
+    PACKAGE_DIR / "csrc" / "layer_norm_capi.hip",
+)
 DEPENDS = (
     PACKAGE_DIR / "csrc" / "capi_errors.hpp",
     PACKAGE_DIR / "csrc" / "msda_device.hpp",
@@ -26,8 +31,12 @@ DEPENDS = (
     PACKAGE_DIR / "csrc" / "msda_forward_bin.hpp",
     PACKAGE_DIR / "csrc" / "msda_forward_slab.hpp",
     PACKAGE_DIR / "csrc" / "dfa_kernels.hpp",
+    PACKAGE_DIR / "csrc" / "linear_device.hpp",
+    PACKAGE_DIR / "csrc" / "linear_kernels.hpp",
+    PACKAGE_DIR / "csrc" / "layer_norm_kernels.hpp",
     REPO_DIR / "include" / "muspace_msda.h",
     REPO_DIR / "include" / "muspace_dfa.h",
+    REPO_DIR / "include" / "muspace_layer.h",
 )
 LIBRARY = PACKAGE_DIR / "native" / "libmuspace_msda.so"
 # memory-system probes for bench.py (--gather-probe, --atomic-probe); not

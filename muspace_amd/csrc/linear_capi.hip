@@ -1,0 +1,353 @@
+// C-ABI entry points of the linear layer (declared in include/muspace_layer.h).
+// Plans (tile sizes, parts of k) are functions of sizes, type and alignment only.
+#include <hip/hip_runtime.h>
+
+#include <climits>
+#include <cstdint>
+
+#include "../../include/muspace_layer.h"
+#include "capi_errors.hpp"
+#include "linear_kernels.hpp"
+
+namespace {
+
+using capi::check_launch;
+using capi::fail;
+using capi::ok;
+using dense::Job;
+using dense::Product;
+
+constexpr int64_t kMaxRows = INT_MAX - 256;
+constexpr int64_t kMaxFeatures = 1 << 20;
+constexpr int kCus = 256;
+
+int validate(const char *fn, int dtype, int64_t rows, int64_t in, int64_t out, int act) {
+  if (dtype < 0 || dtype > 2) {
+    return fail(MUSPACE_EINVAL, "%s: tensors must be float32, float16 or bfloat16", fn);
+  }
+  if (rows < 0 || in < 0 || out < 0) {
+    return fail(MUSPACE_EINVAL, "%s: invalid dims rows=%lld in_features=%lld out_features=%lld",
+                fn, (long long)rows, (long long)in, (long long)out);
+  }
+  if (act < dense::kNone || act > dense::kGelu) {
+    return fail(MUSPACE_EINVAL, "%s: activation must be 0 (none), 1 (relu) or 2 (gelu), got %d",
+                fn, act);
+  }
+  // the tiles of the smallest size, over any two of the three dimensions
+  const int64_t r = rows / 32 + 1, i = in / 32 + 1, o = out / 32 + 1;
+  if (rows > kMaxRows || in > kMaxFeatures || out > kMaxFeatures || r * i > INT_MAX ||
+      r * o > INT_MAX) {
+    return fail(MUSPACE_ERANGE, "%s: dims exceed the kernels' 32-bit indexing", fn);
+  }
+  return ok();
+}
+
+int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+bool aligned16(const void *p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
+int value_bytes(int dtype) { return dtype == 0 ? 4 : 2; }
+int chunk_values(int dtype) { return 16 / value_bytes(dtype); }
+int step_values(int dtype) { return dense::kRowBytes / value_bytes(dtype); }
+size_t pad256(size_t n) { return (n + 255) & ~static_cast<size_t>(255); }
+
+// Tiles of 128 x 128 where they give every CU one, else 64 x 64.
+bool large_tiles(int64_t m, int64_t n) {
+  return ceil_div(m, 128) * ceil_div(n, 128) >= kCus;
+}
+
+struct WeightPlan {
+  bool large;
+  int splits, k_split;  // parts of the rows, rows in each
+};
+
+// dz^T x has few tiles and a long sum: the sum is cut into parts until there are
+// about two workgroups a CU, each of at least four steps.
+WeightPlan plan_weight(int dtype, int64_t rows, int64_t in, int64_t out) {
+  WeightPlan p;
+  p.large = in > 64 && out > 64;
+  const int b = p.large ? 128 : 64;
+  const int64_t tiles = ceil_div(out, b) * (in > 0 ? ceil_div(in, b) : 1);
+  const int64_t steps = ceil_div(rows, step_values(dtype));
+  int64_t splits = tiles > 0 ? 2 * kCus / tiles : 1;
+  if (splits > steps / 4) splits = steps / 4;
+  if (splits < 1) splits = 1;
+  const int64_t per = ceil_div(steps, splits);
+  p.k_split = static_cast<int>((per > 0 ? per : 1) * step_values(dtype));
+  p.splits = static_cast<int>(rows > 0 ? ceil_div(rows, p.k_split) : 1);
+  return p;
+}
+
+size_t partial_bytes(const WeightPlan &p, int64_t in, int64_t out) {
+  if (p.splits == 1) return 0;
+  const size_t ld = static_cast<size_t>((in + 7) & ~int64_t{7});
+  return pad256(static_cast<size_t>(p.splits) * out * ld * 4) +
+         pad256(static_cast<size_t>(p.splits) * out * 4);
+}
+
+template <typename T, Job kJob, int B, bool kMask, bool kCodes>
+void launch_tight(const Product &a, int blocks, bool tight, hipStream_t st) {
+  if (tight) {
+    dense::linear_product<T, kJob, B, B, true, kMask, kCodes>
+        <<<blocks, dense::kThreads, 0, st>>>(a);
+  } else {
+    dense::linear_product<T, kJob, B, B, false, kMask, kCodes>
+        <<<blocks, dense::kThreads, 0, st>>>(a);
+  }
+}
+
+template <typename T, Job kJob, bool kMask, bool kCodes>
+void launch_product(Product a, bool large, bool tight, hipStream_t st) {
+  const int b = large ? 128 : 64;
+  a.tiles_n = static_cast<int>(ceil_div(a.n > 0 ? a.n : 1, b));
+  a.tiles = static_cast<int>(ceil_div(a.m, b)) * a.tiles_n;
+  const int blocks = a.tiles * a.splits;
+  if (blocks == 0) return;
+  if (large) {
+    launch_tight<T, kJob, 128, kMask, kCodes>(a, blocks, tight, st);
+  } else {
+    launch_tight<T, kJob, 64, kMask, kCodes>(a, blocks, tight, st);
+  }
+}
+
+template <typename T, int kWaves>
+void launch_few(const Product &a, bool tight, hipStream_t st) {
+  if (tight) {
+    dense::linear_forward_few<T, kWaves, true><<<a.tiles, kWaves * 64, 0, st>>>(a);
+  } else {
+    dense::linear_forward_few<T, kWaves, false><<<a.tiles, kWaves * 64, 0, st>>>(a);
+  }
+}
+
+template <typename T>
+void run_forward(Product a, bool tight, hipStream_t st) {
+  if (ceil_div(a.m, 64) * ceil_div(a.n, 64) < kCus) {
+    a.tiles_n = static_cast<int>(ceil_div(a.n, 32));
+    a.tiles = static_cast<int>(ceil_div(a.m, 32)) * a.tiles_n;
+    launch_few<T, 4>(a, tight, st);
+    return;
+  }
+  launch_product<T, Job::kForward, false, false>(a, large_tiles(a.m, a.n), tight, st);
+}
+
+template <typename T>
+void run_weight(const Product &a, const WeightPlan &plan, bool tight, bool codes, void *dw, void *db,
+                hipStream_t st) {
+  if (a.mask != nullptr) {
+    if (codes) {
+      launch_product<T, Job::kWeight, true, true>(a, plan.large, tight, st);
+    } else {
+      launch_product<T, Job::kWeight, true, false>(a, plan.large, tight, st);
+    }
+  } else if (codes) {
+    launch_product<T, Job::kWeight, false, true>(a, plan.large, tight, st);
+  } else {
+    launch_product<T, Job::kWeight, false, false>(a, plan.large, tight, st);
+  }
+  if (plan.splits > 1) {
+    const int64_t work = static_cast<int64_t>(a.m) * ((a.n + 7) / 8 * 2) + a.m;
+    dense::linear_weight_sum<T>
+        <<<static_cast<unsigned>(ceil_div(work, dense::kThreads)), dense::kThreads, 0, st>>>(
+            a.partial, a.bias_partial, static_cast<T *>(dw), static_cast<T *>(db), a.m, a.n,
+            plan.splits);
+  }
+}
+
+template <typename T>
+void run_input(const Product &a, bool tight, hipStream_t st) {
+  const bool large = large_tiles(a.m, a.n);
+  if (a.mask != nullptr) {
+    launch_product<T, Job::kInput, true, false>(a, large, tight, st);
+  } else {
+    launch_product<T, Job::kInput, false, false>(a, large, tight, st);
+  }
+}
+
+int grid_for(int64_t work) {
+  const int64_t b = ceil_div(work, dense::kThreads);
+  return static_cast<int>(b > 65536 ? 65536 : (b < 1 ? 1 : b));
+}
+
+template <typename F>
+void by_type(int dtype, F &&f) {
+  if (dtype == 0) {
+    f(float{});
+  } else if (dtype == 1) {
+    f(__half{});
+  } else {
+    f(dense::bf16_t{});
+  }
+}
+
+}  // namespace
+
+extern "C" {
+
+int linear_forward(const void *x, int dtype, const void *weight, const void *bias,
+                   const void *residual, void *output, uint8_t *relu_mask, void *pre_activation,
+                   int64_t rows, int64_t in_features, int64_t out_features, int activation,
+                   void *stream) {
+  int rc = validate("linear_forward", dtype, rows, in_features, out_features, activation);
+  if (rc != MUSPACE_OK) return rc;
+  if (rows == 0 || out_features == 0) return ok();
+  if (output == nullptr || (in_features > 0 && (x == nullptr || weight == nullptr))) {
+    return fail(MUSPACE_EINVAL, "linear_forward: null tensor pointer");
+  }
+  Product a = {};
+  a.p = x;
+  a.q = weight;
+  a.ldp = a.ldq = in_features;
+  a.m = static_cast<int>(rows);
+  a.n = static_cast<int>(out_features);
+  a.k = static_cast<int>(in_features);
+  a.splits = 1;
+  a.bias = bias;
+  a.residual = residual;
+  a.out = output;
+  a.z_out = activation == dense::kGelu ? pre_activation : nullptr;
+  a.mask_out = activation == dense::kRelu ? relu_mask : nullptr;
+  a.mask_ld = ceil_div(out_features, 8);
+  a.act = activation;
+  const bool tight =
+      in_features % chunk_values(dtype) == 0 && aligned16(x) && aligned16(weight);
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  by_type(dtype, [&](auto t) { run_forward<decltype(t)>(a, tight, st); });
+  return check_launch("linear_forward");
+}
+
+int linear_checkpoint(const void *x, int dtype, int8_t *codes, uint8_t *scales, int64_t rows,
+                      int64_t in_features, void *stream) {
+  int rc = validate("linear_checkpoint", dtype, rows, in_features, 0, 0);
+  if (rc != MUSPACE_OK) return rc;
+  if (rows == 0 || in_features == 0) return ok();
+  if (x == nullptr || codes == nullptr || scales == nullptr) {
+    return fail(MUSPACE_EINVAL, "linear_checkpoint: null tensor pointer");
+  }
+  const int64_t work = rows * (((in_features + 31) & ~int64_t{31}) / chunk_values(dtype));
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  by_type(dtype, [&](auto t) {
+    using T = decltype(t);
+    dense::linear_checkpoint<T><<<grid_for(work), dense::kThreads, 0, st>>>(
+        static_cast<const T *>(x), reinterpret_cast<uint8_t *>(codes), scales, rows,
+        static_cast<int>(in_features));
+  });
+  return check_launch("linear_checkpoint");
+}
+
+size_t linear_backward_workspace_size(int dtype, int64_t rows, int64_t in_features,
+                                      int64_t out_features, int activation) {
+  if (validate("linear_backward_workspace_size", dtype, rows, in_features, out_features,
+               activation) != MUSPACE_OK) {
+    return 0;
+  }
+  const WeightPlan plan = plan_weight(dtype, rows, in_features, out_features);
+  size_t bytes = partial_bytes(plan, in_features, out_features);
+  if (activation == dense::kGelu) {
+    bytes += pad256(static_cast<size_t>(rows) * out_features * value_bytes(dtype));
+  }
+  return bytes;
+}
+
+int linear_backward(const void *grad_output, int dtype, const void *x, const int8_t *codes,
+                    const uint8_t *scales, const void *weight, const uint8_t *relu_mask,
+                    const void *pre_activation, void *grad_input, void *grad_weight,
+                    void *grad_bias, int64_t rows, int64_t in_features, int64_t out_features,
+                    int activation, void *workspace, size_t workspace_bytes, void *stream) {
+  const char *fn = "linear_backward";
+  int rc = validate(fn, dtype, rows, in_features, out_features, activation);
+  if (rc != MUSPACE_OK) return rc;
+  const bool want_input = grad_input != nullptr && rows > 0 && in_features > 0;
+  const bool want_weight = grad_weight != nullptr && in_features > 0 && out_features > 0;
+  const bool want_bias = grad_bias != nullptr && out_features > 0;
+  if (!want_input && !want_weight && !want_bias) return ok();
+  const bool summed = rows > 0 && out_features > 0;  // dz has values
+  if ((codes == nullptr) != (scales == nullptr)) {
+    return fail(MUSPACE_EINVAL, "%s: codes and scales come together", fn);
+  }
+  if (summed &&
+      (grad_output == nullptr || (want_input && weight == nullptr) ||
+       (want_weight && x == nullptr && codes == nullptr) ||
+       (activation == dense::kRelu && relu_mask == nullptr) ||
+       (activation == dense::kGelu && pre_activation == nullptr))) {
+    return fail(MUSPACE_EINVAL, "%s: null tensor pointer", fn);
+  }
+  const size_t need =
+      linear_backward_workspace_size(dtype, rows, in_features, out_features, activation);
+  if (need > 0 && (workspace == nullptr || workspace_bytes < need ||
+                   reinterpret_cast<uintptr_t>(workspace) % 256 != 0)) {
+    return fail(MUSPACE_EINVAL, "%s: needs a 256-byte aligned workspace of %zu bytes, got %zu", fn,
+                need, workspace == nullptr ? size_t{0} : workspace_bytes);
+  }
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  char *ws = static_cast<char *>(workspace);
+  const void *dz = grad_output;
+  if (activation == dense::kGelu && summed) {
+    const int64_t count = rows * out_features;
+    by_type(dtype, [&](auto t) {
+      using T = decltype(t);
+      dense::linear_gelu_grad<T>
+          <<<grid_for(ceil_div(count, chunk_values(dtype))), dense::kThreads, 0, st>>>(
+              static_cast<const T *>(grad_output), static_cast<const T *>(pre_activation),
+              reinterpret_cast<T *>(ws), count);
+    });
+    dz = ws;
+    ws += pad256(static_cast<size_t>(count) * value_bytes(dtype));
+  }
+  const int v = chunk_values(dtype);
+  const bool whole_out = out_features % v == 0 && aligned16(dz);
+  const uint8_t *mask = activation == dense::kRelu && summed ? relu_mask : nullptr;
+
+  if (want_input) {
+    Product a = {};
+    a.p = dz;
+    a.q = weight;
+    a.ldp = out_features;
+    a.ldq = in_features;
+    a.m = static_cast<int>(rows);
+    a.n = static_cast<int>(in_features);
+    a.k = static_cast<int>(out_features);
+    a.mask = mask;
+    a.mask_ld = ceil_div(out_features, 8);
+    a.splits = 1;
+    a.out = grad_input;
+    const bool tight = whole_out && in_features % v == 0 && aligned16(weight);
+    by_type(dtype, [&](auto t) { run_input<decltype(t)>(a, tight, st); });
+  }
+  if (want_weight || want_bias) {
+    const WeightPlan plan = plan_weight(dtype, rows, in_features, out_features);
+    Product a = {};
+    a.p = dz;
+    a.ldp = out_features;
+    a.m = static_cast<int>(out_features);
+    // without a weight gradient: no columns, the first column of tiles sums dz
+    a.n = want_weight ? static_cast<int>(in_features) : 0;
+    a.k = static_cast<int>(rows);
+    const bool coded = want_weight && codes != nullptr;
+    a.q = coded ? static_cast<const void *>(codes) : x;
+    a.ldq = coded ? (in_features + 31) & ~int64_t{31} : in_features;
+    a.scales = coded ? scales : nullptr;
+    a.scale_ld = a.ldq / 32;
+    a.mask = mask;
+    a.mask_ld = ceil_div(out_features, 8);
+    a.splits = plan.splits;
+    a.k_split = plan.k_split;
+    a.out = grad_weight;
+    if (plan.splits > 1) {
+      a.partial = reinterpret_cast<float *>(ws);
+      if (want_bias) {
+        const size_t ld = static_cast<size_t>((in_features + 7) & ~int64_t{7});
+        a.bias_partial = reinterpret_cast<float *>(
+            ws + pad256(static_cast<size_t>(plan.splits) * out_features * ld * 4));
+      }
+    } else if (want_bias) {
+      a.bias_out = grad_bias;
+    }
+    const bool tight =
+        whole_out && (!want_weight || coded || (in_features % v == 0 && aligned16(x)));
+    by_type(dtype, [&](auto t) {
+      run_weight<decltype(t)>(a, plan, tight, coded, grad_weight, want_bias ? grad_bias : nullptr,
+                              st);
+    });
+  }
+  return check_launch(fn);
+}
+
+}  // extern "C"

@@ -1,0 +1,349 @@
+// Building blocks of the dense-layer kernels (linear_kernels.hpp): 16-byte
+// pieces of a row ("chunks"), their layouts in LDS and the matrix instructions.
+//
+// A chunk is 16 bytes of a row: 8 values of a 16-bit type or 4 float32 values.
+// A tile of an operand is staged in LDS in one of two layouts, by how the
+// operand lies in memory against the product's summed index k:
+//
+//   along    k is the contiguous index (x and W of x W^T). LDS holds a row of
+//            128 bytes (kStep values of k) per tile row. Chunk c of row r sits in
+//            slot c ^ (r & 7), so that the 8 lanes which an LDS access serves at
+//            a time, 8 rows of one chunk column, touch all banks once.
+//   across   k is the row index (both operands of dz^T x, W of dz W). LDS holds a
+//            row per k. 16-bit operands are read with the transposing LDS read
+//            (four rows of 16 values per 16 lanes): 32-byte pieces are rotated by
+//            XOR with k, so that the four rows lie in different banks. float32
+//            operands are read a dword a lane, 32 consecutive ones a row.
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include <type_traits>
+
+#include "msda_device.hpp"
+
+namespace dense {
+
+using msda::bf16_t;
+using msda::from_float;
+using msda::to_float;
+
+constexpr int kWave = 64;
+constexpr int kThreads = 256;
+constexpr int kRowBytes = 128;  // of k per tile row and step
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef short i16x4 __attribute__((ext_vector_type(4)));
+typedef short i16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
+typedef unsigned int u32x2 __attribute__((ext_vector_type(2)));
+
+// values per chunk, and k per step
+template <typename T>
+struct Piece {
+  static constexpr int kValues = 16 / static_cast<int>(sizeof(T));
+  static constexpr int kStep = kRowBytes / static_cast<int>(sizeof(T));
+};
+
+// A chunk at any alignment of its type: global_load_dwordx4 takes byte
+// addresses, the packed type tells the compiler so.
+struct __attribute__((packed, aligned(2))) Loose16 {
+  u32x4 v;
+};
+struct __attribute__((packed, aligned(2))) Loose8 {
+  u32x2 v;
+};
+
+template <typename T>
+__device__ __forceinline__ void unpack(const u32x4 &v, float (&o)[Piece<T>::kValues]);
+template <>
+__device__ __forceinline__ void unpack<float>(const u32x4 &v, float (&o)[4]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) o[i] = __uint_as_float(v[i]);
+}
+template <>
+__device__ __forceinline__ void unpack<bf16_t>(const u32x4 &v, float (&o)[8]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    o[2 * i] = __uint_as_float(v[i] << 16);
+    o[2 * i + 1] = __uint_as_float(v[i] & 0xffff0000u);
+  }
+}
+template <>
+__device__ __forceinline__ void unpack<__half>(const u32x4 &v, float (&o)[8]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    o[2 * i] = __half2float(__ushort_as_half(static_cast<unsigned short>(v[i] & 0xffffu)));
+    o[2 * i + 1] = __half2float(__ushort_as_half(static_cast<unsigned short>(v[i] >> 16)));
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ uint32_t bits_of(T v);
+template <>
+__device__ __forceinline__ uint32_t bits_of<float>(float v) {
+  return __float_as_uint(v);
+}
+template <>
+__device__ __forceinline__ uint32_t bits_of<bf16_t>(bf16_t v) {
+  return v.bits;
+}
+template <>
+__device__ __forceinline__ uint32_t bits_of<__half>(__half v) {
+  return __half_as_ushort(v);
+}
+
+// round to nearest even, once: the results' only rounding below 32 bits
+template <typename T>
+__device__ __forceinline__ u32x4 pack(const float (&v)[Piece<T>::kValues]);
+template <>
+__device__ __forceinline__ u32x4 pack<float>(const float (&v)[4]) {
+  return u32x4{__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]),
+               __float_as_uint(v[3])};
+}
+template <>
+__device__ __forceinline__ u32x4 pack<__half>(const float (&v)[8]) {
+  u32x4 o;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    o[i] = bits_of(from_float<__half>(v[2 * i])) | bits_of(from_float<__half>(v[2 * i + 1])) << 16;
+  }
+  return o;
+}
+template <>
+__device__ __forceinline__ u32x4 pack<bf16_t>(const float (&v)[8]) {
+  // the conversion instruction of gfx950 rounds to nearest even and keeps NaN
+  u32x4 o;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const __bf16 a = static_cast<__bf16>(v[2 * i]);
+    const __bf16 b = static_cast<__bf16>(v[2 * i + 1]);
+    o[i] = static_cast<uint32_t>(__builtin_bit_cast(unsigned short, a)) |
+           static_cast<uint32_t>(__builtin_bit_cast(unsigned short, b)) << 16;
+  }
+  return o;
+}
+
+// ------------------------------------------------------------ row loads ---
+
+// Loads of one operand's chunks. kTight: every chunk starts on a 16-byte
+// boundary and a row's length is a whole number of chunks; the loads are then
+// unconditional buffer loads, whose range check returns zeros past the operand.
+// Otherwise rows start anywhere: a chunk inside its row is one load at its own
+// alignment, the last one of a row value by value.
+struct Source {
+  const char *base;   // first byte of the step's window (uniform)
+  uint32_t bytes;     // of the window: what lies beyond reads as zero
+};
+
+__device__ __forceinline__ u32x4 tight_load(const Source &s, uint32_t offset) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  const __amdgpu_buffer_rsrc_t r =
+      __builtin_amdgcn_make_buffer_rsrc(const_cast<char *>(s.base), 0, s.bytes, 0x00020000);
+  return __builtin_amdgcn_raw_buffer_load_b128(r, offset, 0, 0);
+#else
+  return u32x4{};
+#endif
+}
+
+__device__ __forceinline__ uint32_t tight_load_byte(const Source &s, uint32_t offset) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  const __amdgpu_buffer_rsrc_t r =
+      __builtin_amdgcn_make_buffer_rsrc(const_cast<char *>(s.base), 0, s.bytes, 0x00020000);
+  return __builtin_amdgcn_raw_buffer_load_b8(r, offset, 0, 0);
+#else
+  return 0;
+#endif
+}
+
+__device__ __forceinline__ u32x2 tight_load8(const Source &s, uint32_t offset) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  const __amdgpu_buffer_rsrc_t r =
+      __builtin_amdgcn_make_buffer_rsrc(const_cast<char *>(s.base), 0, s.bytes, 0x00020000);
+  return __builtin_amdgcn_raw_buffer_load_b64(r, offset, 0, 0);
+#else
+  return u32x2{};
+#endif
+}
+
+__device__ __forceinline__ uint32_t tight_load4(const Source &s, uint32_t offset) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  const __amdgpu_buffer_rsrc_t r =
+      __builtin_amdgcn_make_buffer_rsrc(const_cast<char *>(s.base), 0, s.bytes, 0x00020000);
+  return __builtin_amdgcn_raw_buffer_load_b32(r, offset, 0, 0);
+#else
+  return 0;
+#endif
+}
+
+constexpr uint32_t kPast = 0x80000000u;  // an offset past every window
+
+// `left` values of a row from `p` on (at most a chunk of them; none when <= 0)
+template <typename T>
+__device__ __forceinline__ u32x4 loose_load(const T *p, int left) {
+  if (left >= Piece<T>::kValues) return reinterpret_cast<const Loose16 *>(p)->v;
+  u32x4 o = {0, 0, 0, 0};
+  if (left > 0) {
+#pragma unroll
+    for (int i = 0; i < Piece<T>::kValues; ++i) {
+      if (i < left) {
+        const uint32_t b = bits_of(p[i]);
+        if constexpr (sizeof(T) == 4) {
+          o[i] = b;
+        } else {
+          o[i / 2] |= b << (16 * (i & 1));
+        }
+      }
+    }
+  }
+  return o;
+}
+
+template <typename T>
+__device__ __forceinline__ void loose_store(T *p, const u32x4 &v, int left) {
+  if (left >= Piece<T>::kValues) {
+    reinterpret_cast<Loose16 *>(p)->v = v;
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < Piece<T>::kValues; ++i) {
+    if (i < left) {
+      if constexpr (sizeof(T) == 4) {
+        reinterpret_cast<uint32_t *>(p)[i] = v[i];
+      } else {
+        reinterpret_cast<uint16_t *>(p)[i] = static_cast<uint16_t>(v[i / 2] >> (16 * (i & 1)));
+      }
+    }
+  }
+}
+
+// ------------------------------------------------- masks and 8-bit codes ---
+
+// Keep the values whose bit is set (the others become zero, whatever they are).
+template <typename T>
+__device__ __forceinline__ u32x4 keep_bits(u32x4 v, uint32_t bits) {
+  u32x4 o;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (sizeof(T) == 4) {
+      o[i] = v[i] & static_cast<uint32_t>(-static_cast<int>((bits >> i) & 1u));
+    } else {
+      const uint32_t lo = static_cast<uint32_t>(-static_cast<int>((bits >> (2 * i)) & 1u));
+      const uint32_t hi = static_cast<uint32_t>(-static_cast<int>((bits >> (2 * i + 1)) & 1u));
+      o[i] = v[i] & ((lo & 0xffffu) | (hi & 0xffff0000u));
+    }
+  }
+  return o;
+}
+
+// The value of a scale byte: 2^(s - 127); 255 stands for a block that held an
+// infinity or NaN and reads back as NaN.
+__device__ __forceinline__ float scale_value(uint32_t s) {
+  // s is at least 1 by construction (the writer clamps), so 2^(s - 127) is normal
+  return __uint_as_float(s == 255u ? 0x7fc00000u : s << 23);
+}
+
+// Values of a chunk from its codes. code * 2^e needs 7 bits and is exact in every
+// type (the writer keeps e within the type's range).
+template <typename T>
+__device__ __forceinline__ u32x4 decode(const uint32_t (&w)[Piece<T>::kValues / 4], float scale) {
+  float v[Piece<T>::kValues];
+#pragma unroll
+  for (int i = 0; i < Piece<T>::kValues; ++i) {
+    const int code = static_cast<int>(w[i / 4] << (24 - 8 * (i & 3))) >> 24;
+    v[i] = static_cast<float>(code) * scale;
+  }
+  return pack<T>(v);
+}
+
+// ------------------------------------------------------------ LDS layouts ---
+
+__device__ __forceinline__ uint32_t along_offset(int row, int chunk) {
+  return row * kRowBytes + ((chunk ^ (row & 7)) << 4);
+}
+
+// chunk `c` of row `k` of an across tile of R values a row
+template <typename T, int R>
+__device__ __forceinline__ uint32_t across_offset(int k, int c) {
+  if constexpr (sizeof(T) == 4) {
+    return (k * R + c * 4) * 4;
+  } else {
+    constexpr int kPairs = R / 16;  // 32-byte pieces of a row
+    constexpr int kMask = (kPairs < 8 ? kPairs : 8) - 1;
+    return k * (R * 2) + ((((c >> 1) ^ (k & kMask)) << 1 | (c & 1)) << 4);
+  }
+}
+
+// A lane's part of 32 rows by 8 (float32) or 16 (16-bit) of k: lane l holds row
+// l % 32 and, with h = l / 32, the chunk 2 s + h of a step's 8.
+template <typename T, bool kAlong, int R>
+__device__ __forceinline__ u32x4 read_fragment(const char *tile, int row0, int s, int lane) {
+  if constexpr (kAlong) {
+    const int row = row0 + (lane & 31);
+    return *reinterpret_cast<const u32x4 *>(tile + along_offset(row, 2 * s + (lane >> 5)));
+  } else if constexpr (sizeof(T) == 4) {
+    u32x4 o;
+    const int k = (2 * s + (lane >> 5)) * 4;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      o[i] = *reinterpret_cast<const uint32_t *>(tile + ((k + i) * R + row0 + (lane & 31)) * 4);
+    }
+    return o;
+  } else {
+    // a group of 16 lanes hands in four k rows of 16 values (lane i: row i / 4,
+    // values 4 (i % 4) on) and gets back, lane i, the four k of value i
+#if defined(__HIP_DEVICE_COMPILE__)
+    const int group = lane >> 4, i = lane & 15;
+    const int k = (2 * s + (group >> 1)) * 8 + (i >> 2);
+    const int c = (row0 + (group & 1) * 16) / 8 + ((i & 3) >> 1);
+    typedef __attribute__((address_space(3))) i16x4 *lds_ptr;
+    const uint32_t o0 = across_offset<T, R>(k, c) + (i & 1) * 8;
+    const uint32_t o1 = across_offset<T, R>(k + 4, c) + (i & 1) * 8;
+    const i16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+        (lds_ptr)const_cast<char *>(tile + o0));
+    const i16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+        (lds_ptr)const_cast<char *>(tile + o1));
+    const i16x8 v = __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+    return __builtin_bit_cast(u32x4, v);
+#else
+    return u32x4{};
+#endif
+  }
+}
+
+// acc[i][j] += sum over the fragments' k of a[i] b[j], i and j in 0..31. Lane l
+// holds column j = l % 32 of acc, register r row 8 (r / 4) + 4 (l / 32) + r % 4.
+template <typename T>
+__device__ __forceinline__ f32x16 multiply(const u32x4 &a, const u32x4 &b, f32x16 acc) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      acc = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(a[i]), __uint_as_float(b[i]),
+                                                 acc, 0, 0, 0);
+    }
+    return acc;
+  } else if constexpr (std::is_same_v<T, bf16_t>) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a),
+                                                   __builtin_bit_cast(bf16x8, b), acc, 0, 0, 0);
+  } else {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a),
+                                                  __builtin_bit_cast(f16x8, b), acc, 0, 0, 0);
+  }
+#else
+  return acc;
+#endif
+}
+
+// LDS that only one wavefront touches: its accesses run in order, the compiler
+// must not reorder them.
+__device__ __forceinline__ void wave_lds_sync() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+}
+
+}  // namespace dense

@@ -1,0 +1,635 @@
+// Kernels of the dense layer (include/muspace_layer.h):
+//
+//   y  = act(x W^T + b) + r          linear_product<Job::kForward> / linear_forward_few
+//   dz = g * act'(x W^T + b)         on the fly from a bit mask (relu), or
+//                                    linear_gelu_grad (gelu, from the kept x W^T + b)
+//   dx = dz W                        linear_product<Job::kInput>
+//   dW = dz^T x, db = sum of dz      linear_product<Job::kWeight> + linear_weight_sum
+//   x in 8 bits                      linear_checkpoint; read back by kWeight's loader
+//
+// linear_product: a workgroup of four wavefronts makes a BM x BN tile of the
+// result, each wavefront a quarter. Both operands go through LDS in steps of 128
+// bytes of k, two buffers: the chunks of step i + 1 are in registers on their way
+// while step i is multiplied. Products run on the matrix cores with float32 sums:
+// 32x32x16 for 16-bit types, 32x32x2 for float32. The wavefront multiplies with
+// the result's columns as the matrix instruction's rows, so that a lane holds
+// runs of four columns of a row and the tile goes through LDS in 16-byte pieces
+// into whole 128-byte row segments, where bias, activation, residual and mask
+// are applied once per value.
+//
+// All sums are in float32 and in a fixed order: results do not change from run to
+// run. Results are rounded once, to the tensors' type.
+#pragma once
+
+#include <type_traits>
+
+#include "linear_device.hpp"
+
+namespace dense {
+
+enum class Job { kForward, kInput, kWeight };
+enum Activation : int { kNone = 0, kRelu = 1, kGelu = 2 };
+
+struct Product {
+  const void *p;         // rows of the result: x, dz or dz^T
+  const void *q;         // columns: W, W^T or x
+  int64_t ldp, ldq;      // values per row in memory
+  int m, n, k;           // result rows, columns; summed index
+  const uint8_t *mask;   // relu's bits for p (0: none), one byte per 8 columns
+  int64_t mask_ld;
+  const uint8_t *scales;  // kWeight with codes: q are codes, a scale byte per 32
+  int64_t scale_ld;
+  int tiles_n, tiles;    // tiles along n; all tiles of the result
+  int splits, k_split;   // kWeight: parts of k, steps' values in each
+  // forward
+  const void *bias, *residual;
+  void *out, *z_out;     // z_out: kept x W^T + b (gelu under training)
+  uint8_t *mask_out;     // kept sign bits (relu under training)
+  int act;
+  // kWeight
+  float *partial, *bias_partial;  // [splits][m][pad8(n)], [splits][m]
+  void *bias_out;                 // splits == 1: db (0: none)
+};
+
+// Workgroups go to the eight XCDs in turn. Give each XCD a contiguous run of the
+// tile order, so that the tiles of one row strip (or one part of k) share an L2.
+__device__ __forceinline__ int xcd_order(int id, int count) {
+  const int xcd = id & 7, per = count >> 3, rest = count & 7;
+  return xcd * per + (xcd < rest ? xcd : rest) + (id >> 3);
+}
+
+// --------------------------------------------------------- operand loader ---
+
+// One operand's R rows (of the result) by a step of k: kCount chunks per thread,
+// fetched into registers, then put into LDS.
+template <typename T, bool kAlong, int R, bool kTight, bool kMask, bool kCodes>
+struct Loader {
+  static constexpr int kV = Piece<T>::kValues;
+  static constexpr int kStep = Piece<T>::kStep;
+  static constexpr int kCount = R / 32;
+  static constexpr int kAcross = R / kV;              // chunks per k row (across)
+  static constexpr int kStride = kThreads / kAcross;  // k rows between a thread's chunks
+
+  const T *ptr;
+  const uint8_t *bytes;   // mask or scales
+  int64_t ld, bytes_ld;
+  int row0, rows, k_end;  // first result row, their number in all, end of k
+  int r, c;               // thread's first row (along) or k row (across); its chunk
+  u32x4 v[kCount];
+  uint32_t side[kCount];  // mask byte or scale byte
+
+  __device__ __forceinline__ void init(const void *src, int64_t ld_, const uint8_t *b,
+                                       int64_t b_ld, int row0_, int rows_, int k_end_) {
+    ptr = static_cast<const T *>(src);
+    bytes = b;
+    ld = ld_;
+    bytes_ld = b_ld;
+    row0 = row0_;
+    rows = rows_;
+    k_end = k_end_;
+    const int t = threadIdx.x;
+    if constexpr (kAlong) {
+      r = t >> 3;
+      c = t & 7;
+    } else {
+      r = t / kAcross;
+      c = t % kAcross;
+    }
+  }
+
+  static __device__ __forceinline__ uint32_t window(int64_t bytes_left) {
+    return bytes_left > 0x7fffffff ? 0x7fffffffu
+                                   : (bytes_left < 0 ? 0u : static_cast<uint32_t>(bytes_left));
+  }
+
+  // memory rows from `first` on, columns from `col` on, of `count` rows in all
+  template <typename U>
+  static __device__ __forceinline__ Source view(const U *p, int64_t ld_, int64_t first, int col,
+                                                int64_t count) {
+    Source s;
+    s.base = reinterpret_cast<const char *>(p + first * ld_ + col);
+    s.bytes = window(((count - first) * ld_ - col) * static_cast<int64_t>(sizeof(U)));
+    return s;
+  }
+
+  __device__ __forceinline__ void fetch(int k0) {
+    if constexpr (kAlong) {
+      const bool inside = k0 + c * kV < k_end;
+      if constexpr (kTight) {
+        const Source s = view(ptr, ld, row0, k0, rows);
+#pragma unroll
+        for (int i = 0; i < kCount; ++i) {
+          const uint32_t off = static_cast<uint32_t>((r + 32 * i) * ld + c * kV) *
+                               static_cast<uint32_t>(sizeof(T));
+          v[i] = tight_load(s, inside ? off : kPast);
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < kCount; ++i) {
+          const int row = row0 + r + 32 * i;
+          v[i] = loose_load<T>(ptr + row * ld + k0 + c * kV,
+                               row < rows ? k_end - (k0 + c * kV) : 0);
+        }
+      }
+      if constexpr (kMask) {
+        const Source s = view(bytes, bytes_ld, row0, k0 / 8, rows);
+#pragma unroll
+        for (int i = 0; i < kCount; ++i) {
+          side[i] = tight_load_byte(
+              s, static_cast<uint32_t>((r + 32 * i) * bytes_ld) + (c * kV) / 8);
+        }
+      }
+    } else {
+      const bool inside = row0 + c * kV < rows;
+      if constexpr (kCodes) {
+        const uint8_t *codes = reinterpret_cast<const uint8_t *>(ptr);
+        const Source s = view(codes, ld, k0, row0, k_end);
+        const Source f = view(bytes, bytes_ld, k0, row0 / 32, k_end);
+#pragma unroll
+        for (int i = 0; i < kCount; ++i) {
+          const uint32_t kr = r + i * kStride;
+          const uint32_t off = kr * static_cast<uint32_t>(ld) + c * kV;
+          if constexpr (kV == 8) {
+            const u32x2 w = tight_load8(s, inside ? off : kPast);
+            v[i][0] = w[0];
+            v[i][1] = w[1];
+          } else {
+            v[i][0] = tight_load4(s, inside ? off : kPast);
+          }
+          side[i] = tight_load_byte(
+              f, inside ? kr * static_cast<uint32_t>(bytes_ld) + (c * kV) / 32 : kPast);
+        }
+      } else if constexpr (kTight) {
+        const Source s = view(ptr, ld, k0, row0, k_end);
+#pragma unroll
+        for (int i = 0; i < kCount; ++i) {
+          const uint32_t off = static_cast<uint32_t>((r + i * kStride) * ld + c * kV) *
+                               static_cast<uint32_t>(sizeof(T));
+          v[i] = tight_load(s, inside ? off : kPast);
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < kCount; ++i) {
+          const int64_t kr = k0 + r + i * kStride;
+          v[i] = loose_load<T>(ptr + kr * ld + row0 + c * kV,
+                               kr < k_end ? rows - (row0 + c * kV) : 0);
+        }
+      }
+      if constexpr (kMask) {
+        const Source s = view(bytes, bytes_ld, k0, row0 / 8, k_end);
+#pragma unroll
+        for (int i = 0; i < kCount; ++i) {
+          side[i] = tight_load_byte(
+              s, static_cast<uint32_t>((r + i * kStride) * bytes_ld) + (c * kV) / 8);
+        }
+      }
+    }
+  }
+
+  // the fetched chunk as the product reads it
+  __device__ __forceinline__ u32x4 chunk(int i) const {
+    if constexpr (kCodes) {
+      uint32_t w[kV / 4];
+      w[0] = v[i][0];
+      if constexpr (kV == 8) w[1] = v[i][1];
+      return decode<T>(w, scale_value(side[i]));
+    } else if constexpr (kMask) {
+      return keep_bits<T>(v[i], side[i] >> ((c * kV) & 7));
+    } else {
+      return v[i];
+    }
+  }
+
+  __device__ __forceinline__ void put(char *tile, int i, const u32x4 &value) const {
+    const uint32_t at = kAlong ? along_offset(r + 32 * i, c)
+                               : across_offset<T, R>(r + i * kStride, c);
+    *reinterpret_cast<u32x4 *>(tile + at) = value;
+  }
+};
+
+// ---------------------------------------------------------------- epilogue ---
+
+__device__ __forceinline__ float gelu(float z) {
+  return 0.5f * z * (1.0f + erff(z * 0.70710678118654752f));
+}
+
+__device__ __forceinline__ float gelu_slope(float z) {
+  const float cdf = 0.5f * (1.0f + erff(z * 0.70710678118654752f));
+  return cdf + z * (0.39894228040143268f * expf(-0.5f * z * z));
+}
+
+// `left` values of bias from `p` on
+template <typename T>
+__device__ __forceinline__ void load_bias(const T *p, int left, float (&b)[Piece<T>::kValues]) {
+  const u32x4 v = loose_load<T>(p, left);
+  unpack<T>(v, b);
+}
+
+// A chunk of the forward's result: z holds x W^T + b. `half`: the lane holds the
+// upper four columns of a mask byte (float32).
+template <typename T>
+__device__ __forceinline__ void finish_forward(const Product &a, int64_t row, int col, int left,
+                                               float (&z)[Piece<T>::kValues]) {
+  constexpr int kV = Piece<T>::kValues;
+  const int64_t at = row * a.n + col;
+  if (a.act == kRelu) {
+    uint32_t bits = 0;
+#pragma unroll
+    for (int i = 0; i < kV; ++i) {
+      const bool keep = !(z[i] <= 0.0f);  // NaN stays NaN
+      bits |= (keep && i < left ? 1u : 0u) << i;
+      z[i] = keep ? z[i] : 0.0f;
+    }
+    if (a.mask_out != nullptr) {
+      if constexpr (kV == 4) {
+        // lanes l and l ^ 1 hold the two halves of a byte
+        const uint32_t other = __shfl_xor(bits, 1);
+        if ((col & 4) == 0 && left > 0) {
+          a.mask_out[row * a.mask_ld + col / 8] = static_cast<uint8_t>(bits | other << 4);
+        }
+      } else if (left > 0) {
+        a.mask_out[row * a.mask_ld + col / 8] = static_cast<uint8_t>(bits);
+      }
+    }
+  } else if (a.act == kGelu) {
+    if (a.z_out != nullptr && left > 0) {
+      loose_store(static_cast<T *>(a.z_out) + at, pack<T>(z), left);
+    }
+#pragma unroll
+    for (int i = 0; i < kV; ++i) z[i] = gelu(z[i]);
+  }
+  if (left <= 0) return;
+  if (a.residual != nullptr) {
+    float r[kV];
+    unpack<T>(loose_load<T>(static_cast<const T *>(a.residual) + at, left), r);
+#pragma unroll
+    for (int i = 0; i < kV; ++i) z[i] += r[i];
+  }
+  loose_store(static_cast<T *>(a.out) + at, pack<T>(z), left);
+}
+
+// ------------------------------------------------------------- tile kernel ---
+
+template <typename T, Job kJob, int BM, int BN, bool kTight, bool kMask, bool kCodes>
+__global__ __launch_bounds__(kThreads) void linear_product(const Product a) {
+  constexpr int kV = Piece<T>::kValues;
+  constexpr int kStep = Piece<T>::kStep;
+  constexpr bool kPAlong = kJob != Job::kWeight;
+  constexpr bool kQAlong = kJob == Job::kForward;
+  constexpr int WM = BM / 2, WN = BN / 2;  // a wavefront's quarter
+  constexpr int kI = WM / 32, kJ = WN / 32;
+  constexpr int kTileP = BM * kRowBytes, kTileQ = BN * kRowBytes;
+  constexpr int kBuffer = kTileP + kTileQ;
+  constexpr int kStageLd = WN + 4;  // floats; the pad spreads rows over the banks
+  static_assert(4 * 32 * kStageLd * 4 <= 2 * kBuffer, "result stage exceeds the tiles' LDS");
+  __shared__ __attribute__((aligned(16))) char lds[2 * kBuffer];
+
+  int tile = xcd_order(blockIdx.x, gridDim.x);
+  int split = 0;
+  if constexpr (kJob == Job::kWeight) {
+    split = tile / a.tiles;
+    tile -= split * a.tiles;
+  }
+  const int row0 = tile / a.tiles_n * BM, col0 = tile % a.tiles_n * BN;
+  const int k_begin = split * a.k_split;
+  const int k_end = kJob == Job::kWeight ? min(a.k, k_begin + a.k_split) : a.k;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int wr = (wave >> 1) * WM, wc = (wave & 1) * WN;
+
+  Loader<T, kPAlong, BM, kTight, kMask, false> p;
+  Loader<T, kQAlong, BN, kTight, false, kCodes> q;
+  p.init(a.p, a.ldp, a.mask, a.mask_ld, row0, a.m, k_end);
+  q.init(a.q, a.ldq, a.scales, a.scale_ld, col0, a.n, k_end);
+
+  f32x16 acc[kI][kJ];
+#pragma unroll
+  for (int i = 0; i < kI; ++i) {
+#pragma unroll
+    for (int j = 0; j < kJ; ++j) acc[i][j] = f32x16{};
+  }
+  // kWeight's first tile column also sums dz over its rows: a thread's chunks all
+  // lie in one column of chunks
+  float sums[kV] = {};
+  const bool sum_p = kJob == Job::kWeight && col0 == 0;
+
+  auto put = [&](char *buffer) {
+#pragma unroll
+    for (int i = 0; i < p.kCount; ++i) {
+      const u32x4 v = p.chunk(i);
+      if constexpr (kJob == Job::kWeight) {
+        if (sum_p) {
+          float f[kV];
+          unpack<T>(v, f);
+#pragma unroll
+          for (int e = 0; e < kV; ++e) sums[e] += f[e];
+        }
+      }
+      p.put(buffer, i, v);
+    }
+#pragma unroll
+    for (int i = 0; i < q.kCount; ++i) q.put(buffer + kTileP, i, q.chunk(i));
+  };
+
+  if (k_begin < k_end) {
+    p.fetch(k_begin);
+    q.fetch(k_begin);
+    put(lds);
+  }
+  __syncthreads();
+  int at = 0;
+  for (int k0 = k_begin; k0 < k_end; k0 += kStep) {
+    const bool more = k0 + kStep < k_end;
+    if (more) {
+      p.fetch(k0 + kStep);
+      q.fetch(k0 + kStep);
+    }
+    const char *tile_p = lds + at, *tile_q = lds + at + kTileP;
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {
+      u32x4 fp[kI], fq[kJ];
+#pragma unroll
+      for (int i = 0; i < kI; ++i) fp[i] = read_fragment<T, kPAlong, BM>(tile_p, wr + 32 * i, s, lane);
+#pragma unroll
+      for (int j = 0; j < kJ; ++j) fq[j] = read_fragment<T, kQAlong, BN>(tile_q, wc + 32 * j, s, lane);
+#pragma unroll
+      for (int i = 0; i < kI; ++i) {
+#pragma unroll
+        for (int j = 0; j < kJ; ++j) acc[i][j] = multiply<T>(fq[j], fp[i], acc[i][j]);
+      }
+    }
+    at ^= kBuffer;
+    if (more) put(lds + at);
+    __syncthreads();
+  }
+
+  // the bias gradient: threads of one chunk column add their sums, in thread order
+  if constexpr (kJob == Job::kWeight) {
+    if (sum_p && (a.bias_partial != nullptr || a.bias_out != nullptr)) {
+      constexpr int kGroups = kThreads / (BM / kV);
+      float *s = reinterpret_cast<float *>(lds);
+      const int c = threadIdx.x % (BM / kV), g = threadIdx.x / (BM / kV);
+#pragma unroll
+      for (int e = 0; e < kV; ++e) s[g * BM + c * kV + e] = sums[e];
+      __syncthreads();
+      const int row = row0 + threadIdx.x;
+      if (threadIdx.x < BM && row < a.m) {
+        float total = 0.0f;
+#pragma unroll
+        for (int i = 0; i < kGroups; ++i) total += s[i * BM + threadIdx.x];
+        if (a.bias_partial != nullptr) {
+          a.bias_partial[static_cast<int64_t>(split) * a.m + row] = total;
+        } else {
+          static_cast<T *>(a.bias_out)[row] = from_float<T>(total);
+        }
+      }
+      __syncthreads();
+    }
+  }
+
+  // the tile, 32 rows of a wavefront at a time, through the wavefront's own LDS
+  float *stage = reinterpret_cast<float *>(lds) + wave * 32 * kStageLd;
+  constexpr int kLanes = WN / kV;         // lanes per row
+  constexpr int kRows = kWave / kLanes;   // rows at a time
+  const int chunk = lane % kLanes;
+  const int col = col0 + wc + chunk * kV, left = a.n - col;
+  float bias[kV] = {};
+  if constexpr (kJob == Job::kForward) {
+    if (a.bias != nullptr) load_bias<T>(static_cast<const T *>(a.bias) + col, left, bias);
+  }
+#pragma unroll
+  for (int i = 0; i < kI; ++i) {
+#pragma unroll
+    for (int j = 0; j < kJ; ++j) {
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        f32x4 v;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = acc[i][j][4 * g + e];
+        *reinterpret_cast<f32x4 *>(stage + (lane & 31) * kStageLd + 32 * j + 8 * g +
+                                   4 * (lane >> 5)) = v;
+      }
+    }
+    wave_lds_sync();
+#pragma unroll
+    for (int r0 = 0; r0 < 32; r0 += kRows) {
+      const int r = r0 + lane / kLanes;
+      const int64_t row = row0 + wr + 32 * i + r;
+      const float *src = stage + r * kStageLd + chunk * kV;
+      float z[kV];
+#pragma unroll
+      for (int e = 0; e < kV; e += 4) {
+        const f32x4 v = *reinterpret_cast<const f32x4 *>(src + e);
+#pragma unroll
+        for (int x = 0; x < 4; ++x) z[e + x] = v[x];
+      }
+      const int here = row < a.m ? left : 0;
+      if constexpr (kJob == Job::kForward) {
+#pragma unroll
+        for (int e = 0; e < kV; ++e) z[e] += bias[e];
+        finish_forward<T>(a, row, col, here, z);
+      } else {
+        if (here > 0) {
+          if (kJob == Job::kWeight && a.partial != nullptr) {
+            const int64_t ld = (a.n + 7) & ~7;
+            float *to = a.partial + (static_cast<int64_t>(split) * a.m + row) * ld + col;
+#pragma unroll
+            for (int e = 0; e < kV; e += 4) {
+              f32x4 v = {z[e], z[e + 1], z[e + 2], z[e + 3]};
+              *reinterpret_cast<f32x4 *>(to + e) = v;
+            }
+          } else {
+            loose_store(static_cast<T *>(a.out) + row * a.n + col, pack<T>(z), here);
+          }
+        }
+      }
+    }
+    wave_lds_sync();
+  }
+}
+
+// ---------------------------------------------------- forward, few results ---
+
+// A workgroup makes 32 x 32 results with kWaves wavefronts that share k, chunks
+// straight from memory into the matrix instruction: nothing waits for another
+// wavefront until the sums are joined in LDS, in wavefront order.
+template <typename T, int kWaves, bool kTight>
+__global__ __launch_bounds__(kWaves * kWave) void linear_forward_few(const Product a) {
+  constexpr int kV = Piece<T>::kValues;
+  constexpr int kStep = Piece<T>::kStep;
+  constexpr int kLd = 36;
+  __shared__ __attribute__((aligned(16))) float lds[kWaves][32 * kLd];
+  const int tile = xcd_order(blockIdx.x, gridDim.x);
+  const int row0 = tile / a.tiles_n * 32, col0 = tile % a.tiles_n * 32;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const T *x = static_cast<const T *>(a.p) + static_cast<int64_t>(row0) * a.ldp;
+  const T *w = static_cast<const T *>(a.q) + static_cast<int64_t>(col0) * a.ldq;
+  const int r = lane & 31, h = lane >> 5;
+  const bool row_in = row0 + r < a.m, col_in = col0 + r < a.n;
+  f32x16 acc = {};
+  for (int k0 = wave * kStep; k0 < a.k; k0 += kWaves * kStep) {
+    u32x4 fp[4], fq[4];
+    if constexpr (kTight) {
+      using L = Loader<T, true, 32, true, false, false>;
+      const Source sp = L::view(x, a.ldp, 0, k0, a.m - row0);
+      const Source sq = L::view(w, a.ldq, 0, k0, a.n - col0);
+#pragma unroll
+      for (int s = 0; s < 4; ++s) {
+        const int k = (2 * s + h) * kV;
+        const bool inside = k0 + k < a.k;
+        fp[s] = tight_load(sp, inside ? static_cast<uint32_t>((r * a.ldp + k) * sizeof(T)) : kPast);
+        fq[s] = tight_load(sq, inside ? static_cast<uint32_t>((r * a.ldq + k) * sizeof(T)) : kPast);
+      }
+    } else {
+#pragma unroll
+      for (int s = 0; s < 4; ++s) {
+        const int k = k0 + (2 * s + h) * kV;
+        fp[s] = loose_load<T>(x + r * a.ldp + k, row_in ? a.k - k : 0);
+        fq[s] = loose_load<T>(w + r * a.ldq + k, col_in ? a.k - k : 0);
+      }
+    }
+#pragma unroll
+    for (int s = 0; s < 4; ++s) acc = multiply<T>(fq[s], fp[s], acc);
+  }
+#pragma unroll
+  for (int g = 0; g < 4; ++g) {
+    const f32x4 v = {acc[4 * g], acc[4 * g + 1], acc[4 * g + 2], acc[4 * g + 3]};
+    *reinterpret_cast<f32x4 *>(&lds[wave][r * kLd + 8 * g + 4 * h]) = v;
+  }
+  __syncthreads();
+  constexpr int kLanes = 32 / kV;
+  // whole wavefronts take part (the mask's halves are exchanged between lanes)
+  for (int i = threadIdx.x; i < 32 * kLanes; i += kWaves * kWave) {
+    const int chunk = i % kLanes, rr = i / kLanes;
+    const int col = col0 + chunk * kV;
+    const int64_t row = row0 + rr;
+    const int left = row < a.m ? a.n - col : 0;
+    float z[kV], b[kV] = {};
+    if (a.bias != nullptr) load_bias<T>(static_cast<const T *>(a.bias) + col, a.n - col, b);
+#pragma unroll
+    for (int e = 0; e < kV; ++e) z[e] = 0.0f;
+#pragma unroll
+    for (int u = 0; u < kWaves; ++u) {
+#pragma unroll
+      for (int e = 0; e < kV; ++e) z[e] += lds[u][rr * kLd + chunk * kV + e];
+    }
+#pragma unroll
+    for (int e = 0; e < kV; ++e) z[e] += b[e];
+    finish_forward<T>(a, row, col, left, z);
+  }
+}
+
+// ----------------------------------------------------- gradient's last step ---
+
+// dW and db from the parts of k, summed in their order.
+template <typename T>
+__global__ __launch_bounds__(kThreads) void linear_weight_sum(const float *partial,
+                                                              const float *bias_partial, T *dw,
+                                                              T *db, int m, int n, int splits) {
+  const int ld = (n + 7) & ~7, per_row = ld / 4;
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
+  const int64_t count = static_cast<int64_t>(m) * per_row;
+  if (i < count) {
+    const int64_t row = i / per_row;
+    const int col = static_cast<int>(i - row * per_row) * 4;
+    const float *src = partial + row * ld + col;
+    const int64_t stride = static_cast<int64_t>(m) * ld;
+    f32x4 s = {0.0f, 0.0f, 0.0f, 0.0f};
+    int u = 0;
+    for (; u + 8 <= splits; u += 8) {
+      f32x4 v[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = *reinterpret_cast<const f32x4 *>(src + (u + e) * stride);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) s += v[e];
+    }
+    for (; u < splits; ++u) s += *reinterpret_cast<const f32x4 *>(src + u * stride);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      if (col + e < n) dw[row * n + col + e] = from_float<T>(s[e]);
+    }
+    return;
+  }
+  const int64_t row = i - count;
+  if (db != nullptr && row < m) {
+    float s = 0.0f;
+    for (int u = 0; u < splits; ++u) s += bias_partial[static_cast<int64_t>(u) * m + row];
+    db[row] = from_float<T>(s);
+  }
+}
+
+// ------------------------------------------------------------- elementwise ---
+
+// dz = g * gelu'(z), z the kept pre-activation. dz is rounded to the tensors'
+// type: it is an operand of two matrix products.
+template <typename T>
+__global__ __launch_bounds__(kThreads) void linear_gelu_grad(const T *g, const T *z, T *dz,
+                                                             int64_t count) {
+  constexpr int kV = Piece<T>::kValues;
+  const int64_t chunks = (count + kV - 1) / kV;
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x; i < chunks;
+       i += static_cast<int64_t>(gridDim.x) * kThreads) {
+    const int64_t at = i * kV;
+    const int left = count - at < kV ? static_cast<int>(count - at) : kV;
+    float a[kV], b[kV];
+    unpack<T>(loose_load<T>(g + at, left), a);
+    unpack<T>(loose_load<T>(z + at, left), b);
+#pragma unroll
+    for (int e = 0; e < kV; ++e) a[e] *= gelu_slope(b[e]);
+    loose_store(dz + at, pack<T>(a), left);
+  }
+}
+
+// x in 8 bits. A block of 32 values of a row shares 2^e, the smallest power of two
+// with 127 * 2^e >= its largest magnitude; a code is the nearest integer to
+// x / 2^e (ties to even). codes [rows][pad32(cols)], zero past cols; scales
+// [rows][pad32(cols) / 32] hold e + 127, or 255 for a block with an infinity or
+// NaN. e stays where 2^e is a normal number (and, for float16, a float16 number),
+// and codes end at 63 where 64 * 2^e is past the type's range, so that every
+// code * 2^e is a number of the type.
+template <typename T>
+__global__ __launch_bounds__(kThreads) void linear_checkpoint(const T *x, uint8_t *codes,
+                                                              uint8_t *scales, int64_t rows,
+                                                              int cols) {
+  constexpr int kV = Piece<T>::kValues;
+  constexpr int kGroup = 32 / kV;  // lanes per block of 32
+  constexpr bool kHalf = std::is_same_v<T, __half>;
+  constexpr uint32_t kLow = kHalf ? 127 - 24 : 1, kHigh = kHalf ? 127 + 10 : 127 + 122;
+  const int padded = (cols + 31) & ~31, per_row = padded / kV;
+  const int64_t chunks = rows * per_row;
+  // per_row and the launch's stride are multiples of kGroup: a block's lanes stay together
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x; i < chunks;
+       i += static_cast<int64_t>(gridDim.x) * kThreads) {
+    const int64_t row = i / per_row;
+    const int col = static_cast<int>(i - row * per_row) * kV;
+    float v[kV];
+    unpack<T>(loose_load<T>(x + row * cols + col, cols - col), v);
+    uint32_t top = 0;
+#pragma unroll
+    for (int e = 0; e < kV; ++e) top = max(top, __float_as_uint(v[e]) & 0x7fffffffu);
+#pragma unroll
+    for (int d = 1; d < kGroup; d <<= 1) top = max(top, static_cast<uint32_t>(__shfl_xor(top, d)));
+    const bool finite = top < 0x7f800000u;
+    const int s0 = static_cast<int>(top >> 23) - 6 + ((top & 0x7fffffu) > 0x7e0000u ? 1 : 0);
+    const uint32_t s = s0 < static_cast<int>(kLow) ? kLow : static_cast<uint32_t>(s0);
+    const float inverse = __uint_as_float((254u - s) << 23);
+    const float limit = s >= kHigh ? 63.0f : 127.0f;
+    uint32_t w[kV / 4] = {};
+#pragma unroll
+    for (int e = 0; e < kV; ++e) {
+      float q = rintf(v[e] * inverse);
+      q = finite ? fminf(fmaxf(q, -limit), limit) : 1.0f;  // 1 * NaN reads back as NaN
+      w[e / 4] |= (static_cast<uint32_t>(static_cast<int>(q)) & 0xffu) << (8 * (e & 3));
+    }
+    uint8_t *to = codes + row * padded + col;
+    if constexpr (kV == 8) {
+      *reinterpret_cast<u32x2 *>(to) = u32x2{w[0], w[1]};
+    } else {
+      *reinterpret_cast<uint32_t *>(to) = w[0];
+    }
+    if (col % 32 == 0) {
+      scales[row * (padded / 32) + col / 32] = static_cast<uint8_t>(finite ? s : 255u);
+    }
+  }
+}
+
+}  // namespace dense

@@ -15,15 +15,23 @@ from .deformable_aggregation import (
     deformable_aggregation_reference,
     feature_maps_format,
 )
+from .layer_norm import layer_norm, layer_norm_pytorch
+from .linear import checkpoint_int8, checkpoint_restore, linear, linear_pytorch
 
 __all__ = [
     "attention_softmax",
+    "checkpoint_int8",
+    "checkpoint_restore",
     "deformable_aggregation",
     "deformable_aggregation_function",
     "deformable_aggregation_reference",
     "feature_maps_format",
     "explain_dispatch",
+    "layer_norm",
+    "layer_norm_pytorch",
     "level_start_index_from_shapes",
+    "linear",
+    "linear_pytorch",
     "multi_scale_deformable_attn",
     "multi_scale_deformable_attn_pytorch",
     "multi_scale_deformable_attn_pytorch_compat",

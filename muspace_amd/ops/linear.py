@@ -1,0 +1,286 @@
+"""The linear layer of an encoder or decoder block, with its epilogue fused.
+
+Deformable-attention layers surround the attention with dense products: value,
+offset, weight and output projections and a feed-forward block, each followed by
+a bias, sometimes an activation, often the layer's input:
+
+    out = activation(input @ weight.T + bias) + residual
+
+``linear`` computes this in one kernel, on the matrix cores with float32 sums,
+rounded once. Its backward recomputes nothing and keeps little: relu keeps one
+bit per value (not the output), gelu the pre-activation, and the input either
+as it is or, with ``checkpoint="int8"``, in 8 bits: blocks of 32 values share a
+power of two, and the weight's gradient is the product with exactly the values
+that were kept (``checkpoint_int8``, ``checkpoint_restore``). Such a call keeps
+1.03 bytes of input per value instead of 2 or 4; every other result is the
+same as without. The input's gradient needs no input at all.
+
+No reference counterpart: the reference leaves these products to torch
+(/root/reference/mu_space/ops/multi_scale_deformable_attn.py:215-338 starts at the projected value).
+"""
+
+from __future__ import annotations
+
+import math
+
+import torch
+import torch.nn.functional as F
+from torch.autograd.function import once_differentiable
+
+from ..runtime.kernel_dispatch import (
+    NATIVE_BACKEND,
+    DispatchReport,
+    explain_dispatch as _explain_dispatch,
+    is_rocm_tensor,
+    record_dispatch_report,
+)
+from ..runtime.native import native_error
+from .multi_scale_deformable_attn import _native_extension
+
+OPERATOR_NAME = "linear"
+BLOCK = 32  # values of a row that share a scale in an 8-bit checkpoint
+ACTIVATIONS = {None: 0, "relu": 1, "gelu": 2}
+
+_DTYPES = (torch.float32, torch.float16, torch.bfloat16)
+# by type: the smallest scale exponent, and the one whose codes end at 63 since
+# 64 * 2^e is past the type's largest number
+_SCALE_RANGE = {torch.float16: (-24, 10), torch.bfloat16: (-126, 122), torch.float32: (-126, 122)}
+
+
+# ------------------------------------------------------------- checkpoints ---
+
+
+def checkpoint_int8(input: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """``input`` [..., cols] in 8 bits: ``(codes int8 [rows, padded], scales
+    uint8 [rows, padded / 32])``, cols padded to a multiple of 32.
+
+    A block of 32 values of a row shares 2^e, the smallest power of two with
+    127 * 2^e at or over the block's largest magnitude; a code is x / 2^e
+    rounded to the nearest integer, ties to even; a scale byte is e + 127, or 255
+    where the block holds an infinity or NaN: it reads back as NaN.
+    """
+    if input.dtype not in _DTYPES:
+        raise TypeError("input must be float16, bfloat16 or float32")
+    if input.dim() == 0:
+        raise ValueError("input must have at least one dimension")
+    cols = input.shape[-1]
+    rows = math.prod(input.shape[:-1])
+    padded = (cols + BLOCK - 1) // BLOCK * BLOCK
+    if is_rocm_tensor(input):
+        ext = _native_extension()
+        if ext is None:
+            raise RuntimeError(f"muSPACE HIP native library is unavailable: {native_error()}")
+        codes = torch.empty((rows, padded), dtype=torch.int8, device=input.device)
+        scales = torch.empty((rows, padded // BLOCK), dtype=torch.uint8, device=input.device)
+        ext.linear_checkpoint(input.contiguous().view(rows, cols), codes, scales)
+        return codes, scales
+    low, high = _SCALE_RANGE[input.dtype]
+    x = F.pad(input.reshape(rows, cols).float(), (0, padded - cols)).view(rows, -1, BLOCK)
+    finite = torch.isfinite(x).all(-1, keepdim=True)
+    mantissa, exponent = torch.frexp(torch.where(finite, x, 0.0).abs().amax(-1, keepdim=True))
+    exponent = (exponent - 7 + (mantissa > 127.0 / 128.0).int()).clamp_min(low)
+    exponent = torch.where(mantissa == 0, low, exponent)  # a block of zeros
+    limit = torch.where(exponent >= high, 63.0, 127.0)
+    # two factors: 2^-e alone leaves float32's range of normal numbers
+    half = exponent // 2
+    codes = torch.ldexp(torch.ldexp(x, -half), half - exponent).round()
+    codes = torch.where(finite, torch.minimum(torch.maximum(codes, -limit), limit), 1.0)
+    scales = torch.where(finite, exponent + 127, 255)
+    return codes.view(rows, padded).to(torch.int8), scales.view(rows, -1).to(torch.uint8)
+
+
+def checkpoint_restore(codes: torch.Tensor, scales: torch.Tensor, cols: int,
+                       dtype: torch.dtype) -> torch.Tensor:
+    """The values an 8-bit checkpoint stands for, ``[rows, cols]`` in ``dtype``
+    (exact: a code times its power of two is a number of the type)."""
+    rows = codes.shape[0]
+    exponent = scales.to(torch.int32) - 127
+    # 2^e straight from its bits: e is in [-126, 122]
+    factor = ((exponent + 127).clamp(1, 254) << 23).view(torch.float32)
+    factor = torch.where(scales == 255, math.nan, factor)
+    values = codes.view(rows, -1, BLOCK).float() * factor.unsqueeze(-1)
+    return values.view(rows, -1)[:, :cols].to(dtype)
+
+
+# ---------------------------------------------------------- PyTorch path ---
+
+
+def _activate(z: torch.Tensor, activation: str | None) -> torch.Tensor:
+    if activation == "relu":
+        return F.relu(z)
+    if activation == "gelu":
+        return F.gelu(z)
+    return z
+
+
+class _CheckpointedInput(torch.autograd.Function):
+    """``F.linear`` whose backward reads the input from its 8-bit checkpoint."""
+
+    @staticmethod
+    def forward(ctx, input, weight):
+        ctx.shape, ctx.dtype = input.shape, input.dtype
+        ctx.save_for_backward(weight, *checkpoint_int8(input))
+        return F.linear(input, weight)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad):
+        weight, codes, scales = ctx.saved_tensors
+        kept = checkpoint_restore(codes, scales, ctx.shape[-1], ctx.dtype)
+        flat = grad.reshape(-1, grad.shape[-1])
+        return grad @ weight, flat.t() @ kept
+
+
+def linear_pytorch(input, weight, bias=None, *, activation=None, residual=None, checkpoint=None):
+    """``linear`` in PyTorch operations, on any device."""
+    if checkpoint is None:
+        z = F.linear(input, weight, bias)
+    else:
+        z = _CheckpointedInput.apply(input, weight)
+        if bias is not None:
+            z = z + bias
+    out = _activate(z, activation)
+    return out if residual is None else out + residual
+
+
+# ------------------------------------------------------------ native path ---
+
+
+def _forward(ext, input, weight, bias, residual, activation, keep):
+    """The output, and what the gradient of the activation needs (``keep``)."""
+    rows = math.prod(input.shape[:-1])
+    features = weight.shape[0]
+    output = input.new_empty((*input.shape[:-1], features))
+    kept = None
+    if keep and activation == 1:
+        kept = torch.empty((rows, (features + 7) // 8), dtype=torch.uint8, device=input.device)
+    elif keep and activation == 2:
+        kept = input.new_empty((rows, features))
+    ext.linear_forward(input, weight, bias, residual, output, kept, activation)
+    return output, kept
+
+
+class _NativeLinearFunction(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, input, weight, bias, residual, activation, checkpoint):
+        ext = _native_extension()
+        if ext is None:
+            raise RuntimeError("muSPACE HIP native library is unavailable")
+        need_input, need_weight, need_bias = ctx.needs_input_grad[:3]
+        keep = need_input or need_weight or need_bias
+        output, kept = _forward(ext, input, weight, bias, residual, activation, keep)
+        codes = scales = None
+        if need_weight and checkpoint:
+            codes, scales = checkpoint_int8(input)
+        ctx.activation = activation
+        ctx.input_shape = input.shape
+        ctx.weight_shape = weight.shape
+        ctx.save_for_backward(input if need_weight and not checkpoint else None, codes, scales,
+                              weight if need_input else None, kept)
+        return output
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad_output):
+        need_input, need_weight, need_bias, need_residual = ctx.needs_input_grad[:4]
+        grad_residual = grad_output if need_residual else None
+        if not (need_input or need_weight or need_bias):
+            return None, None, None, grad_residual, None, None
+        ext = _native_extension()
+        if ext is None:
+            raise RuntimeError("muSPACE HIP native library is unavailable")
+        input, codes, scales, weight, kept = ctx.saved_tensors
+        grad = grad_output.contiguous()
+        new = grad.new_empty
+        grad_input = new(ctx.input_shape) if need_input else None
+        grad_weight = new(ctx.weight_shape) if need_weight else None
+        grad_bias = new(ctx.weight_shape[0]) if need_bias else None
+        ext.linear_backward(grad, input, codes, scales, weight, kept, grad_input, grad_weight,
+                            grad_bias, ctx.weight_shape, ctx.activation)
+        return grad_input, grad_weight, grad_bias, grad_residual, None, None
+
+
+def _report(backend, selected, decision, native_available):
+    record_dispatch_report(
+        DispatchReport(
+            operator=OPERATOR_NAME,
+            requested_backend=backend,
+            selected_backend=selected,
+            device=decision.device,
+            reason=decision.reason,
+            native_available=native_available,
+        )
+    )
+
+
+def _validate(input, weight, bias, activation, residual, checkpoint) -> None:
+    if input.dtype not in _DTYPES:
+        raise TypeError("input must be float16, bfloat16 or float32")
+    if activation not in ACTIVATIONS:
+        raise ValueError(f"activation must be None, 'relu' or 'gelu', got {activation!r}")
+    if checkpoint is not None and checkpoint != "int8":
+        raise ValueError(f"checkpoint must be None or 'int8', got {checkpoint!r}")
+    if input.dim() == 0:
+        raise ValueError("input must have at least one dimension")
+    if weight.dim() != 2 or weight.shape[1] != input.shape[-1]:
+        raise ValueError(f"weight must be [out_features, {input.shape[-1]}], "
+                         f"got {list(weight.shape)}")
+    if bias is not None and bias.shape != weight.shape[:1]:
+        raise ValueError(f"bias must be [{weight.shape[0]}], got {list(bias.shape)}")
+    if residual is not None and residual.shape != (*input.shape[:-1], weight.shape[0]):
+        raise ValueError(f"residual must have the output's shape "
+                         f"{[*input.shape[:-1], weight.shape[0]]}, got {list(residual.shape)}")
+    for name, tensor in (("weight", weight), ("bias", bias), ("residual", residual)):
+        if tensor is not None and tensor.dtype != input.dtype:
+            raise TypeError(f"{name} must be {input.dtype} like the input, got {tensor.dtype}")
+
+
+def linear(
+    input: torch.Tensor,
+    weight: torch.Tensor,
+    bias: torch.Tensor | None = None,
+    *,
+    activation: str | None = None,
+    residual: torch.Tensor | None = None,
+    checkpoint: str | None = None,
+    backend: str = "auto",
+) -> torch.Tensor:
+    """``activation(input @ weight.T + bias) + residual``, in ``input.dtype``.
+
+    ``input`` [..., in_features], ``weight`` [out_features, in_features], ``bias``
+    [out_features], ``residual`` of the output's shape [..., out_features]; all of
+    one type, float32, float16 or bfloat16, any strides. ``activation``: None,
+    ``"relu"`` or ``"gelu"`` (by the error function). ``checkpoint="int8"`` keeps the
+    input for the weight's gradient in 8 bits (see the module's text).
+
+    ``backend``: ``"auto"`` (HIP kernels on ROCm tensors, the PyTorch path
+    elsewhere), ``"hip"`` (native kernels or an error) or ``"reference"``. A native
+    failure is raised, not hidden behind the PyTorch path. Gradients can be taken
+    once (no gradients of gradients) on the HIP path.
+    """
+    _validate(input, weight, bias, activation, residual, checkpoint)
+    ext = _native_extension()
+    decision = _explain_dispatch(input, backend=backend, native_available=ext is not None)
+    if decision.backend == "error":
+        _report(backend, "error", decision, ext is not None)
+        detail = native_error() if ext is None and is_rocm_tensor(input) else None
+        raise RuntimeError(f"{decision.reason}: {detail}" if detail else decision.reason)
+    if decision.backend == "reference":
+        _report(backend, "reference", decision, ext is not None)
+        return linear_pytorch(input, weight, bias, activation=activation, residual=residual,
+                              checkpoint=checkpoint)
+    input, weight = input.contiguous(), weight.contiguous()
+    bias = None if bias is None else bias.contiguous()
+    residual = None if residual is None else residual.contiguous()
+    code = ACTIVATIONS[activation]
+    if torch.is_grad_enabled() and any(
+            t is not None and t.requires_grad for t in (input, weight, bias, residual)):
+        output = _NativeLinearFunction.apply(input, weight, bias, residual, code,
+                                             checkpoint is not None)
+    else:
+        output, _ = _forward(ext, input, weight, bias, residual, code, False)
+    _report(backend, NATIVE_BACKEND, decision, True)
+    return output
+
+
+__all__ = ["checkpoint_int8", "checkpoint_restore", "linear", "linear_pytorch"]

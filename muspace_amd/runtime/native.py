@@ -19,6 +19,7 @@ carrying the library's message.
 from __future__ import annotations
 
 import ctypes
+import math
 from functools import lru_cache
 from importlib.resources import files
 from pathlib import Path
@@ -145,6 +146,30 @@ _EXPORTS: dict[str, tuple[Any, list[Any]]] = {
     "deformable_aggregation_backward_ws": (
         _c_int, [_c_ptr] * 9 + [_c_int64] * 8 + [_c_ptr, ctypes.c_size_t, _c_ptr]
     ),
+    # include/muspace_layer.h
+    "linear_forward": (
+        _c_int, [_c_ptr, _c_int] + [_c_ptr] * 6 + [_c_int64] * 3 + [_c_int, _c_ptr]
+    ),
+    "linear_checkpoint": (
+        _c_int, [_c_ptr, _c_int, _c_ptr, _c_ptr, _c_int64, _c_int64, _c_ptr]
+    ),
+    "linear_backward_workspace_size": (ctypes.c_size_t, [_c_int] + [_c_int64] * 3 + [_c_int]),
+    "linear_backward": (
+        _c_int,
+        [_c_ptr, _c_int] + [_c_ptr] * 9 + [_c_int64] * 3
+        + [_c_int, _c_ptr, ctypes.c_size_t, _c_ptr],
+    ),
+    "layer_norm_forward": (
+        _c_int,
+        [_c_ptr, _c_int, _c_ptr, _c_ptr, _c_int, _c_ptr, _c_ptr, _c_int64, _c_int64,
+         ctypes.c_float, _c_ptr],
+    ),
+    "layer_norm_backward_workspace_size": (ctypes.c_size_t, [_c_int, _c_int64, _c_int64]),
+    "layer_norm_backward": (
+        _c_int,
+        [_c_ptr, _c_int, _c_ptr, _c_ptr, _c_int] + [_c_ptr] * 4
+        + [_c_int64, _c_int64, _c_ptr, ctypes.c_size_t, _c_ptr],
+    ),
 }
 
 
@@ -240,6 +265,10 @@ def _stream_of(device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
 
 
+def _ptr(tensor) -> int | None:
+    return None if tensor is None else tensor.data_ptr()
+
+
 class NativeLibrary:
     """The loaded library with its exports bound once."""
 
@@ -265,6 +294,9 @@ class NativeLibrary:
         # scratch sizes by device and dims (a plan each, asked for several times a step)
         self._size = lru_cache(maxsize=1024)(self._workspace_size)
         self._dfa_scratch = lru_cache(maxsize=1024)(self._dfa_scratch_bytes)
+        self._linear_scratch = lru_cache(maxsize=1024)(self._raw["linear_backward_workspace_size"])
+        self._norm_scratch = lru_cache(maxsize=1024)(
+            self._raw["layer_norm_backward_workspace_size"])
         self._bound: dict[str, Callable[..., Any]] = {
             "check_forward": self.check_forward,
             "check_backward": self.check_backward,
@@ -294,6 +326,11 @@ class NativeLibrary:
             "deformable_aggregation_backward_base": self.deformable_aggregation_backward_base,
             "deformable_aggregation_backward": self.deformable_aggregation_backward,
             "ms_deform_attn_scatter_div_grad": self.ms_deform_attn_scatter_div_grad,
+            "linear_forward": self.linear_forward,
+            "linear_checkpoint": self.linear_checkpoint,
+            "linear_backward": self.linear_backward,
+            "layer_norm_forward": self.layer_norm_forward,
+            "layer_norm_backward": self.layer_norm_backward,
             "add_one": self.add_one,
         }
 
@@ -972,6 +1009,144 @@ class NativeLibrary:
         self._dfa_backward("deformable_aggregation_backward_base", mc_ms_feat, spatial_shape,
                            scale_start_index, sampling_location, weights, grad_output,
                            grad_mc_ms_feat, grad_sampling_location, grad_weights)
+
+    # ------------------------------------------------- dense operators ---
+    def _check_all(self, like, dtypes, *named) -> None:
+        """Each (tensor, name, shape) a contiguous tensor on ``like``'s device,
+        None skipped; ``dtypes`` as in :func:`_check`."""
+        for tensor, name, shape in named:
+            if tensor is not None:
+                _check(tensor, name, dtypes, like.device)
+                if shape is not None:
+                    _check_shape(tensor, name, shape)
+
+    def linear_forward(self, input, weight, bias, residual, output, kept, activation: int) -> None:
+        """output = act(input weight^T + bias) + residual; ``kept``: None, relu's
+        bits (uint8) or gelu's pre-activation (the input's dtype)."""
+        _check(input, "input", tuple(_DTYPE_CODES))
+        same = (input.dtype,)
+        if weight is None or weight.dim() != 2 or input.dim() == 0:
+            raise RuntimeError("weight must be 2-D and input at least 1-D")
+        out, cols = weight.shape
+        lead = tuple(input.shape[:-1])
+        rows = math.prod(lead)
+        self._check_all(input, same, (weight, "weight", (out, input.shape[-1])),
+                        (bias, "bias", (out,)), (residual, "residual", (*lead, out)),
+                        (output, "output", (*lead, out)))
+        mask = z = None
+        if kept is not None and activation == 1:
+            self._check_all(input, (torch.uint8,), (kept, "relu_mask", (rows, (out + 7) // 8)))
+            mask = kept.data_ptr()
+        elif kept is not None and activation == 2:
+            self._check_all(input, same, (kept, "pre_activation", (rows, out)))
+            z = kept.data_ptr()
+        self._launch(
+            "linear_forward", input.device,
+            input.data_ptr(), _DTYPE_CODES[input.dtype], weight.data_ptr(), _ptr(bias),
+            _ptr(residual), output.data_ptr(), mask, z, rows, cols, out, activation,
+        )
+
+    def linear_checkpoint(self, input, codes, scales) -> None:
+        """codes [rows, pad32(cols)] int8, scales [rows, pad32(cols) / 32] uint8."""
+        _check(input, "input", tuple(_DTYPE_CODES))
+        if input.dim() != 2:
+            raise RuntimeError("input must be 2-D")
+        rows, cols = input.shape
+        padded = (cols + 31) // 32 * 32
+        self._check_all(input, (torch.int8,), (codes, "codes", (rows, padded)))
+        self._check_all(input, (torch.uint8,), (scales, "scales", (rows, padded // 32)))
+        self._launch("linear_checkpoint", input.device, input.data_ptr(),
+                     _DTYPE_CODES[input.dtype], codes.data_ptr(), scales.data_ptr(), rows, cols)
+
+    def linear_backward(self, grad_output, input, codes, scales, weight, kept, grad_input,
+                        grad_weight, grad_bias, weight_shape, activation: int) -> None:
+        """The gradients that are not None, from ``input`` or its checkpoint
+        (``codes``, ``scales``) and what :meth:`linear_forward` kept."""
+        _check(grad_output, "grad_output", tuple(_DTYPE_CODES))
+        same = (grad_output.dtype,)
+        out, cols = weight_shape
+        lead = tuple(grad_output.shape[:-1])
+        rows = math.prod(lead)
+        padded = (cols + 31) // 32 * 32
+        _check_shape(grad_output, "grad_output", (*lead, out))
+        self._check_all(grad_output, same, (input, "input", (*lead, cols)),
+                        (weight, "weight", (out, cols)), (grad_input, "grad_input", (*lead, cols)),
+                        (grad_weight, "grad_weight", (out, cols)),
+                        (grad_bias, "grad_bias", (out,)))
+        self._check_all(grad_output, (torch.int8,), (codes, "codes", (rows, padded)))
+        self._check_all(grad_output, (torch.uint8,), (scales, "scales", (rows, padded // 32)))
+        mask = z = None
+        if kept is not None and activation == 1:
+            self._check_all(grad_output, (torch.uint8,),
+                            (kept, "relu_mask", (rows, (out + 7) // 8)))
+            mask = kept.data_ptr()
+        elif kept is not None and activation == 2:
+            self._check_all(grad_output, same, (kept, "pre_activation", (rows, out)))
+            z = kept.data_ptr()
+        code = _DTYPE_CODES[grad_output.dtype]
+        nbytes = self._linear_scratch(code, rows, cols, out, activation)
+        workspace = None
+        if nbytes:
+            workspace = torch.empty(nbytes, dtype=torch.uint8, device=grad_output.device)
+        self._launch(
+            "linear_backward", grad_output.device,
+            grad_output.data_ptr(), code, _ptr(input), _ptr(codes), _ptr(scales), _ptr(weight),
+            mask, z, _ptr(grad_input), _ptr(grad_weight), _ptr(grad_bias), rows, cols, out,
+            activation, _ptr(workspace), nbytes,
+        )
+
+    def _norm_weights(self, input, *named):
+        """Checks weight-like tensors; the C-ABI's weight_dtype."""
+        dtype = input.dtype
+        for tensor, name in named:
+            if tensor is not None:
+                dtype = tensor.dtype
+                break
+        allowed = (dtype,) if dtype in (input.dtype, torch.float32) else (input.dtype,)
+        self._check_all(input, allowed,
+                        *((tensor, name, (input.shape[-1],)) for tensor, name in named))
+        return _DTYPE_CODES[dtype]
+
+    def layer_norm_forward(self, input, weight, bias, output, statistics, eps: float) -> None:
+        """output = layer norm of input over its last dimension; ``statistics``:
+        None or float32 [rows, 2] for the backward."""
+        _check(input, "input", tuple(_DTYPE_CODES))
+        if input.dim() == 0:
+            raise RuntimeError("input must be at least 1-D")
+        shape = tuple(input.shape)
+        rows = math.prod(shape[:-1])
+        self._check_all(input, (input.dtype,), (output, "output", shape))
+        self._check_all(input, (torch.float32,), (statistics, "statistics", (rows, 2)))
+        wdtype = self._norm_weights(input, (weight, "weight"), (bias, "bias"))
+        self._launch(
+            "layer_norm_forward", input.device,
+            input.data_ptr(), _DTYPE_CODES[input.dtype], _ptr(weight), _ptr(bias), wdtype,
+            output.data_ptr(), _ptr(statistics), rows, shape[-1], eps,
+        )
+
+    def layer_norm_backward(self, grad_output, input, weight, statistics, grad_input, grad_weight,
+                            grad_bias) -> None:
+        """The gradients that are not None, from the forward's statistics."""
+        _check(input, "input", tuple(_DTYPE_CODES))
+        shape = tuple(input.shape)
+        rows, cols = math.prod(shape[:-1]), shape[-1]
+        self._check_all(input, (input.dtype,), (grad_output, "grad_output", shape),
+                        (grad_input, "grad_input", shape))
+        self._check_all(input, (torch.float32,), (statistics, "statistics", (rows, 2)))
+        wdtype = self._norm_weights(input, (weight, "weight"), (grad_weight, "grad_weight"),
+                                    (grad_bias, "grad_bias"))
+        code = _DTYPE_CODES[input.dtype]
+        nbytes, workspace = 0, None
+        if grad_weight is not None or grad_bias is not None:
+            nbytes = self._norm_scratch(code, rows, cols)
+        if nbytes:
+            workspace = torch.empty(nbytes, dtype=torch.uint8, device=input.device)
+        self._launch(
+            "layer_norm_backward", input.device,
+            grad_output.data_ptr(), code, input.data_ptr(), _ptr(weight), wdtype,
+            statistics.data_ptr(), _ptr(grad_input), _ptr(grad_weight), _ptr(grad_bias), rows,
+            cols, _ptr(workspace), nbytes,
+        )
 
     def add_one(self, value, actual) -> None:
         """Build smoke: actual = value + 1 (float32 device tensors)."""

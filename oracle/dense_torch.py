@@ -1,0 +1,160 @@
+"""Float64 restatement of the layer's dense operators, with error bounds.
+
+``linear`` and ``layer_norm`` with their gradients in float64 from the formulas,
+and the 8-bit checkpoint in exact arithmetic. The bounds are worst cases, element
+by element, of an implementation that sums in float32 in any order and rounds
+each result once: a sum of n products errs by at most (n + 2) 2^-23 times the sum
+of their magnitudes (two float32 roundings of 2^-24 per term), a result by half a
+step of its type more.
+"""
+
+from __future__ import annotations
+
+import math
+
+import torch
+
+SUM_STEP = 2.0**-23
+
+
+def half_step(dtype: torch.dtype) -> float:
+    return torch.finfo(dtype).eps / 2
+
+
+def tiny(dtype: torch.dtype) -> float:
+    """Half a step among the type's subnormal numbers."""
+    return torch.finfo(dtype).smallest_normal * half_step(dtype)
+
+
+def gelu(z):
+    return 0.5 * z * torch.special.erfc(-z * math.sqrt(0.5))
+
+
+def gelu_slope(z):
+    return (0.5 * torch.special.erfc(-z * math.sqrt(0.5))
+            + z * torch.exp(-0.5 * z * z) / math.sqrt(2.0 * math.pi))
+
+
+def checkpoint(x):
+    """(codes, scale bytes, restored values) of a finite or non-finite x [rows, cols]."""
+    dtype = x.dtype
+    low = -24 if dtype == torch.float16 else -126
+    rows, cols = x.shape
+    padded = (cols + 31) // 32 * 32
+    values = torch.zeros((rows, padded), dtype=torch.float64, device=x.device)
+    values[:, :cols] = x.double()
+    blocks = values.view(rows, -1, 32)
+    finite = torch.isfinite(blocks).all(-1, keepdim=True)
+    top = torch.where(finite, blocks, 0.0).abs().amax(-1, keepdim=True)
+    exponent = torch.full_like(top, float(low))
+    # step up from the lowest exponent: no logarithm to round
+    for e in range(low, 123):
+        exponent = torch.where(top > 127.0 * 2.0**e, float(e + 1), exponent)
+    scale = torch.exp2(exponent)
+    codes = torch.round(blocks / scale)
+    past = codes.abs() * scale > torch.finfo(dtype).max
+    codes = torch.where(past, codes.sign() * 63.0, codes)
+    codes = torch.where(finite, codes, 1.0)
+    restored = torch.where(finite, codes * scale, math.nan).view(rows, padded)[:, :cols]
+    scales = torch.where(finite, exponent + 127.0, 255.0).view(rows, -1)
+    return codes.view(rows, padded).to(torch.int8), scales.to(torch.uint8), restored
+
+
+def linear(x, weight, bias, activation, residual, grad=None, kept=None):
+    """([results], [bounds]): y, and with ``grad`` dx, dW, db. ``kept`` [rows, in]
+    float64 replaces x in dW (an 8-bit checkpoint)."""
+    dtype, u, small = x.dtype, half_step(x.dtype), tiny(x.dtype)
+    x, w = x.double(), weight.double()
+    rows, inner = x.shape
+    b = torch.zeros(w.shape[0], dtype=torch.float64, device=x.device)
+    if bias is not None:
+        b = bias.double()
+    z = x @ w.t() + b
+    z_err = (inner + 2) * SUM_STEP * (x.abs() @ w.abs().t() + b.abs())
+    if activation == "relu":
+        y, slope, y_err = z.clamp_min(0.0), (z > 0).double(), z_err
+    elif activation == "gelu":
+        # |slope| < 1.13; erf, two products and a sum: 8 float32 steps of z
+        y, slope = gelu(z), gelu_slope(z)
+        y_err = 1.13 * z_err + 8 * SUM_STEP * z.abs()
+    else:
+        y, slope, y_err = z, torch.ones_like(z), z_err
+    if residual is not None:
+        y = y + residual.double()
+        y_err = y_err + SUM_STEP * y.abs()
+    results, bounds = [y], [y_err * (1 + u) + u * y.abs() + small]
+    if grad is None:
+        return results, bounds
+    g = grad.double()
+    dz = g * slope
+    dz_err = torch.zeros_like(dz)
+    if activation == "gelu":
+        # the kept z is rounded to the type (|slope'| < 0.8), the slope is a float32
+        # function of it, dz is rounded to the type
+        dz_err = g.abs() * (0.8 * (z_err + u * z.abs() + small) + 16 * SUM_STEP)
+        dz_err = dz_err * (1 + u) + u * dz.abs() + small
+    dx = dz @ w
+    dx_err = (dz_err @ w.abs()
+              + (w.shape[0] + 2) * SUM_STEP * ((dz.abs() + dz_err) @ w.abs()))
+    rest = x if kept is None else kept
+    dw = dz.t() @ rest
+    dw_err = (dz_err.t() @ rest.abs()
+              + (rows + 2) * SUM_STEP * ((dz.abs() + dz_err).t() @ rest.abs()))
+    db = dz.sum(0)
+    db_err = dz_err.sum(0) + (rows + 2) * SUM_STEP * (dz.abs() + dz_err).sum(0)
+    for value, err in ((dx, dx_err), (dw, dw_err), (db, db_err)):
+        results.append(value)
+        bounds.append(err * (1 + u) + u * value.abs() + small)
+    return results, bounds
+
+
+def layer_norm(x, weight, bias, eps, grad=None):
+    """([results], [bounds]): y, and with ``grad`` dx, dw, db (of the weight's type).
+
+    With d = x - x0 (x0 the row's first value) every |d| is at most D, the row's
+    largest: d errs by 2^-24 |d|, the mean of d by (n + 2) 2^-23 D, so c by
+    e = (n + 4) 2^-23 D. s errs by a relative (e / sigma)(1 + e / sigma) from c, where
+    sigma = 1 / s, and (n + 8) 2^-23 from its own sums.
+    """
+    dtype, u, small = x.dtype, half_step(x.dtype), tiny(x.dtype)
+    wdtype = weight.dtype if weight is not None else dtype
+    rows, cols = x.shape
+    x = x.double()
+    w = torch.ones(cols, dtype=torch.float64, device=x.device) if weight is None else weight.double()
+    b = torch.zeros_like(w) if bias is None else bias.double()
+    mean = x.mean(-1, keepdim=True)
+    c = x - mean
+    sigma = (c.square().mean(-1, keepdim=True) + eps).sqrt()
+    s = 1.0 / sigma
+    reach = (x - x[:, :1]).abs().amax(-1, keepdim=True)
+    e = (cols + 4) * SUM_STEP * reach
+    s_rel = (e * s) * (1 + e * s) + (cols + 8) * SUM_STEP
+    h = c * s
+    h_err = e * s * (1 + s_rel) + h.abs() * s_rel + SUM_STEP * h.abs()
+    y = h * w + b
+    y_err = h_err * w.abs() + 2 * SUM_STEP * (h.abs() * w.abs() + b.abs())
+    results, bounds = [y], [y_err * (1 + u) + u * y.abs() + small]
+    if grad is None:
+        return results, bounds
+    g = grad.double()
+    v = g * w
+    mv, mh = v.mean(-1, keepdim=True), (v * h).mean(-1, keepdim=True)
+    inner = v - mv - h * mh
+    mv_err = (cols + 4) * SUM_STEP * v.abs().mean(-1, keepdim=True)
+    mh_err = ((v.abs() * h_err).mean(-1, keepdim=True)
+              + (cols + 4) * SUM_STEP * (v * h).abs().mean(-1, keepdim=True))
+    inner_err = (mv_err + h_err * (mh.abs() + mh_err) + h.abs() * mh_err
+                 + 4 * SUM_STEP * (v.abs() + mv.abs() + (h * mh).abs()))
+    dx = s * inner
+    dx_err = s * (1 + s_rel) * inner_err + dx.abs() * (s_rel + SUM_STEP)
+    results.append(dx)
+    bounds.append(dx_err * (1 + u) + u * dx.abs() + small)
+    u, small = half_step(wdtype), tiny(wdtype)
+    dw, db = (g * h).sum(0), g.sum(0)
+    dw_err = ((g.abs() * h_err).sum(0)
+              + (rows + 2) * SUM_STEP * (g.abs() * (h.abs() + h_err)).sum(0))
+    db_err = (rows + 2) * SUM_STEP * g.abs().sum(0)
+    for value, err in ((dw, dw_err), (db, db_err)):
+        results.append(value)
+        bounds.append(err * (1 + u) + u * value.abs() + small)
+    return results, bounds
