@@ -17,19 +17,10 @@ import torch
 import torch.nn.functional as F
 from torch.autograd.function import once_differentiable
 
-from ..runtime.kernel_dispatch import (
-    NATIVE_BACKEND,
-    DispatchReport,
-    explain_dispatch as _explain_dispatch,
-    is_rocm_tensor,
-    record_dispatch_report,
-)
-from ..runtime.native import native_error
-from .multi_scale_deformable_attn import _native_extension
+from .layer_common import DTYPES as _DTYPES
+from .layer_common import check_device, choose_native, require_native
 
 OPERATOR_NAME = "layer_norm"
-
-_DTYPES = (torch.float32, torch.float16, torch.bfloat16)
 
 
 def layer_norm_pytorch(input, weight=None, bias=None, *, eps=1e-5):
@@ -46,52 +37,39 @@ def layer_norm_pytorch(input, weight=None, bias=None, *, eps=1e-5):
 
 class _NativeLayerNormFunction(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, input, weight, bias, eps):
-        ext = _native_extension()
-        if ext is None:
-            raise RuntimeError("muSPACE HIP native library is unavailable")
+    def forward(ctx, input, weight, bias, weight_dtype, eps):
+        ext = require_native()
         rows = math.prod(input.shape[:-1])
         output = torch.empty_like(input)
         stats = torch.empty((rows, 2), dtype=torch.float32, device=input.device)
-        ext.layer_norm_forward(input, weight, bias, output, stats, eps)
-        ctx.weight_dtype = (weight if weight is not None else bias if bias is not None
-                            else input).dtype
+        ext.layer_norm_forward_launch(input, weight, bias, weight_dtype, output, stats, rows, eps)
+        # all that the backward needs to know, looked up here: its thread runs Python slowly
+        ctx.launch = ext.layer_norm_backward_launch
+        ctx.plan = ext.layer_norm_plan(input.dtype, weight_dtype, rows, input.shape[-1])
+        ctx.weight_dtype = weight_dtype
         ctx.save_for_backward(input, weight, stats)
         return output
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, grad_output):
-        ext = _native_extension()
-        if ext is None:
-            raise RuntimeError("muSPACE HIP native library is unavailable")
-        input, weight, stats = ctx.saved_tensors
-        need_input, need_weight, need_bias = ctx.needs_input_grad[:3]
-        cols = input.shape[-1]
-
-        def column_gradient(wanted):
-            if not wanted:
-                return None
-            return torch.empty(cols, dtype=ctx.weight_dtype, device=input.device)
-
-        grad_input = torch.empty_like(input) if need_input else None
-        grad_weight, grad_bias = column_gradient(need_weight), column_gradient(need_bias)
-        ext.layer_norm_backward(grad_output.contiguous(), input, weight, stats, grad_input,
-                                grad_weight, grad_bias)
-        return grad_input, grad_weight, grad_bias, None
+        if torch.is_grad_enabled():  # create_graph: refuses a second differentiation
+            return _layer_norm_backward_once(ctx, grad_output)
+        return _layer_norm_backward(ctx, grad_output)
 
 
-def _report(backend, selected, decision, native_available):
-    record_dispatch_report(
-        DispatchReport(
-            operator=OPERATOR_NAME,
-            requested_backend=backend,
-            selected_backend=selected,
-            device=decision.device,
-            reason=decision.reason,
-            native_available=native_available,
-        )
-    )
+def _layer_norm_backward(ctx, grad_output):
+    input, weight, stats = ctx.saved_tensors
+    need_input, need_weight, need_bias = ctx.needs_input_grad[:3]
+    grad_input = torch.empty_like(input) if need_input else None
+    cols, dtype = input.shape[-1:], ctx.weight_dtype
+    grad_weight = stats.new_empty(cols, dtype=dtype) if need_weight else None
+    grad_bias = stats.new_empty(cols, dtype=dtype) if need_bias else None
+    ctx.launch(grad_output.contiguous(), input, weight, stats, grad_input, grad_weight, grad_bias,
+               ctx.plan)
+    return grad_input, grad_weight, grad_bias, None, None
+
+
+_layer_norm_backward_once = once_differentiable(_layer_norm_backward)
 
 
 def _validate(input, weight, bias, eps) -> None:
@@ -130,25 +108,21 @@ def layer_norm(
     Gradients can be taken once (no gradients of gradients) on the HIP path.
     """
     _validate(input, weight, bias, eps)
-    ext = _native_extension()
-    decision = _explain_dispatch(input, backend=backend, native_available=ext is not None)
-    if decision.backend == "error":
-        _report(backend, "error", decision, ext is not None)
-        detail = native_error() if ext is None and is_rocm_tensor(input) else None
-        raise RuntimeError(f"{decision.reason}: {detail}" if detail else decision.reason)
-    if decision.backend == "reference":
-        _report(backend, "reference", decision, ext is not None)
+    ext = choose_native(OPERATOR_NAME, input, backend)
+    if ext is None:
         return layer_norm_pytorch(input, weight, bias, eps=eps)
+    check_device(input, (weight, "weight"), (bias, "bias"))
     input = input.contiguous()
     weight = None if weight is None else weight.contiguous()
     bias = None if bias is None else bias.contiguous()
-    if torch.is_grad_enabled() and any(
-            t is not None and t.requires_grad for t in (input, weight, bias)):
-        output = _NativeLayerNormFunction.apply(input, weight, bias, eps)
-    else:
-        output = torch.empty_like(input)
-        ext.layer_norm_forward(input, weight, bias, output, None, eps)
-    _report(backend, NATIVE_BACKEND, decision, True)
+    weight_dtype = (weight if weight is not None else bias if bias is not None else input).dtype
+    if torch.is_grad_enabled() and (
+            input.requires_grad or (weight is not None and weight.requires_grad)
+            or (bias is not None and bias.requires_grad)):
+        return _NativeLayerNormFunction.apply(input, weight, bias, weight_dtype, eps)
+    output = torch.empty_like(input)
+    ext.layer_norm_forward_launch(input, weight, bias, weight_dtype, output, None,
+                                  math.prod(input.shape[:-1]), eps)
     return output
 
 

@@ -27,21 +27,14 @@ import torch
 import torch.nn.functional as F
 from torch.autograd.function import once_differentiable
 
-from ..runtime.kernel_dispatch import (
-    NATIVE_BACKEND,
-    DispatchReport,
-    explain_dispatch as _explain_dispatch,
-    is_rocm_tensor,
-    record_dispatch_report,
-)
-from ..runtime.native import native_error
-from .multi_scale_deformable_attn import _native_extension
+from ..runtime.kernel_dispatch import is_rocm_tensor
+from .layer_common import DTYPES as _DTYPES
+from .layer_common import check_device, choose_native, require_native
 
 OPERATOR_NAME = "linear"
 BLOCK = 32  # values of a row that share a scale in an 8-bit checkpoint
 ACTIVATIONS = {None: 0, "relu": 1, "gelu": 2}
 
-_DTYPES = (torch.float32, torch.float16, torch.bfloat16)
 # by type: the smallest scale exponent, and the one whose codes end at 63 since
 # 64 * 2^e is past the type's largest number
 _SCALE_RANGE = {torch.float16: (-24, 10), torch.bfloat16: (-126, 122), torch.float32: (-126, 122)}
@@ -67,12 +60,9 @@ def checkpoint_int8(input: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     rows = math.prod(input.shape[:-1])
     padded = (cols + BLOCK - 1) // BLOCK * BLOCK
     if is_rocm_tensor(input):
-        ext = _native_extension()
-        if ext is None:
-            raise RuntimeError(f"muSPACE HIP native library is unavailable: {native_error()}")
         codes = torch.empty((rows, padded), dtype=torch.int8, device=input.device)
         scales = torch.empty((rows, padded // BLOCK), dtype=torch.uint8, device=input.device)
-        ext.linear_checkpoint(input.contiguous().view(rows, cols), codes, scales)
+        require_native().linear_checkpoint_launch(input.contiguous(), codes, scales, rows, cols)
         return codes, scales
     low, high = _SCALE_RANGE[input.dtype]
     x = F.pad(input.reshape(rows, cols).float(), (0, padded - cols)).view(rows, -1, BLOCK)
@@ -146,71 +136,65 @@ def linear_pytorch(input, weight, bias=None, *, activation=None, residual=None, 
 # ------------------------------------------------------------ native path ---
 
 
-def _forward(ext, input, weight, bias, residual, activation, keep):
+def _forward(ext, input, weight, bias, residual, activation, rows, keep):
     """The output, and what the gradient of the activation needs (``keep``)."""
-    rows = math.prod(input.shape[:-1])
-    features = weight.shape[0]
+    features, cols = weight.shape
     output = input.new_empty((*input.shape[:-1], features))
     kept = None
     if keep and activation == 1:
         kept = torch.empty((rows, (features + 7) // 8), dtype=torch.uint8, device=input.device)
     elif keep and activation == 2:
         kept = input.new_empty((rows, features))
-    ext.linear_forward(input, weight, bias, residual, output, kept, activation)
+    ext.linear_forward_launch(input, weight, bias, residual, output, kept, activation, rows, cols,
+                              features)
     return output, kept
 
 
 class _NativeLinearFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, input, weight, bias, residual, activation, checkpoint):
-        ext = _native_extension()
-        if ext is None:
-            raise RuntimeError("muSPACE HIP native library is unavailable")
-        need_input, need_weight, need_bias = ctx.needs_input_grad[:3]
-        keep = need_input or need_weight or need_bias
-        output, kept = _forward(ext, input, weight, bias, residual, activation, keep)
+        ext = require_native()
+        need_input, need_weight, need_bias, _ = ctx.needs_input_grad[:4]
+        rows = math.prod(input.shape[:-1])
+        features, cols = weight.shape
+        needed = need_input or need_weight or need_bias
+        output, kept = _forward(ext, input, weight, bias, residual, activation, rows, needed)
         codes = scales = None
         if need_weight and checkpoint:
             codes, scales = checkpoint_int8(input)
-        ctx.activation = activation
-        ctx.input_shape = input.shape
-        ctx.weight_shape = weight.shape
+        # all that the backward needs to know, looked up here: its thread runs Python slowly
+        ctx.launch = ext.linear_backward_launch if needed else None
+        ctx.plan = ext.linear_plan(input.dtype, rows, cols, features, activation)
+        ctx.shapes = (input.shape if need_input else None, weight.shape if need_weight else None,
+                      features if need_bias else None)
         ctx.save_for_backward(input if need_weight and not checkpoint else None, codes, scales,
                               weight if need_input else None, kept)
         return output
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, grad_output):
-        need_input, need_weight, need_bias, need_residual = ctx.needs_input_grad[:4]
-        grad_residual = grad_output if need_residual else None
-        if not (need_input or need_weight or need_bias):
-            return None, None, None, grad_residual, None, None
-        ext = _native_extension()
-        if ext is None:
-            raise RuntimeError("muSPACE HIP native library is unavailable")
-        input, codes, scales, weight, kept = ctx.saved_tensors
-        grad = grad_output.contiguous()
-        new = grad.new_empty
-        grad_input = new(ctx.input_shape) if need_input else None
-        grad_weight = new(ctx.weight_shape) if need_weight else None
-        grad_bias = new(ctx.weight_shape[0]) if need_bias else None
-        ext.linear_backward(grad, input, codes, scales, weight, kept, grad_input, grad_weight,
-                            grad_bias, ctx.weight_shape, ctx.activation)
-        return grad_input, grad_weight, grad_bias, grad_residual, None, None
+        if torch.is_grad_enabled():  # create_graph: refuses a second differentiation
+            return _linear_backward_once(ctx, grad_output)
+        return _linear_backward(ctx, grad_output)
 
 
-def _report(backend, selected, decision, native_available):
-    record_dispatch_report(
-        DispatchReport(
-            operator=OPERATOR_NAME,
-            requested_backend=backend,
-            selected_backend=selected,
-            device=decision.device,
-            reason=decision.reason,
-            native_available=native_available,
-        )
-    )
+def _linear_backward(ctx, grad_output):
+    grad_residual = grad_output if ctx.needs_input_grad[3] else None
+    if ctx.launch is None:
+        return None, None, None, grad_residual, None, None
+    input, codes, scales, weight, kept = ctx.saved_tensors
+    grad = grad_output.contiguous()
+    new = grad.new_empty
+    input_shape, weight_shape, bias_shape = ctx.shapes
+    grad_input = None if input_shape is None else new(input_shape)
+    grad_weight = None if weight_shape is None else new(weight_shape)
+    grad_bias = None if bias_shape is None else new(bias_shape)
+    ctx.launch(grad, input, codes, scales, weight, kept, grad_input, grad_weight, grad_bias,
+               ctx.plan)
+    return grad_input, grad_weight, grad_bias, grad_residual, None, None
+
+
+_linear_backward_once = once_differentiable(_linear_backward)
 
 
 def _validate(input, weight, bias, activation, residual, checkpoint) -> None:
@@ -259,28 +243,22 @@ def linear(
     once (no gradients of gradients) on the HIP path.
     """
     _validate(input, weight, bias, activation, residual, checkpoint)
-    ext = _native_extension()
-    decision = _explain_dispatch(input, backend=backend, native_available=ext is not None)
-    if decision.backend == "error":
-        _report(backend, "error", decision, ext is not None)
-        detail = native_error() if ext is None and is_rocm_tensor(input) else None
-        raise RuntimeError(f"{decision.reason}: {detail}" if detail else decision.reason)
-    if decision.backend == "reference":
-        _report(backend, "reference", decision, ext is not None)
+    ext = choose_native(OPERATOR_NAME, input, backend)
+    if ext is None:
         return linear_pytorch(input, weight, bias, activation=activation, residual=residual,
                               checkpoint=checkpoint)
+    check_device(input, (weight, "weight"), (bias, "bias"), (residual, "residual"))
     input, weight = input.contiguous(), weight.contiguous()
     bias = None if bias is None else bias.contiguous()
     residual = None if residual is None else residual.contiguous()
     code = ACTIVATIONS[activation]
-    if torch.is_grad_enabled() and any(
-            t is not None and t.requires_grad for t in (input, weight, bias, residual)):
-        output = _NativeLinearFunction.apply(input, weight, bias, residual, code,
-                                             checkpoint is not None)
-    else:
-        output, _ = _forward(ext, input, weight, bias, residual, code, False)
-    _report(backend, NATIVE_BACKEND, decision, True)
-    return output
+    if torch.is_grad_enabled() and (
+            input.requires_grad or weight.requires_grad
+            or (bias is not None and bias.requires_grad)
+            or (residual is not None and residual.requires_grad)):
+        return _NativeLinearFunction.apply(input, weight, bias, residual, code,
+                                           checkpoint is not None)
+    return _forward(ext, input, weight, bias, residual, code, math.prod(input.shape[:-1]), False)[0]
 
 
 __all__ = ["checkpoint_int8", "checkpoint_restore", "linear", "linear_pytorch"]

@@ -329,8 +329,15 @@ class NativeLibrary:
             "linear_forward": self.linear_forward,
             "linear_checkpoint": self.linear_checkpoint,
             "linear_backward": self.linear_backward,
+            "linear_plan": self.linear_plan,
+            "linear_forward_launch": self.linear_forward_launch,
+            "linear_checkpoint_launch": self.linear_checkpoint_launch,
+            "linear_backward_launch": self.linear_backward_launch,
             "layer_norm_forward": self.layer_norm_forward,
             "layer_norm_backward": self.layer_norm_backward,
+            "layer_norm_plan": self.layer_norm_plan,
+            "layer_norm_forward_launch": self.layer_norm_forward_launch,
+            "layer_norm_backward_launch": self.layer_norm_backward_launch,
             "add_one": self.add_one,
         }
 
@@ -1011,39 +1018,49 @@ class NativeLibrary:
                            grad_mc_ms_feat, grad_sampling_location, grad_weights)
 
     # ------------------------------------------------- dense operators ---
+    # The operators make and check their tensors themselves and launch with plain
+    # addresses (`*_launch`): Python run by the backward's thread costs two to three
+    # times what it costs in the forward's. The tensor-level entries check first.
     def _check_all(self, like, dtypes, *named) -> None:
-        """Each (tensor, name, shape) a contiguous tensor on ``like``'s device,
-        None skipped; ``dtypes`` as in :func:`_check`."""
+        """Each (tensor, name, shape) a contiguous tensor on ``like``'s device with
+        one of ``dtypes``; None skipped."""
         for tensor, name, shape in named:
             if tensor is not None:
                 _check(tensor, name, dtypes, like.device)
-                if shape is not None:
-                    _check_shape(tensor, name, shape)
+                _check_shape(tensor, name, shape)
+
+    def _check_kept(self, like, kept, rows, out, activation) -> None:
+        if activation == 1:
+            self._check_all(like, (torch.uint8,), (kept, "relu_mask", (rows, (out + 7) // 8)))
+        elif activation == 2:
+            self._check_all(like, (like.dtype,), (kept, "pre_activation", (rows, out)))
+        elif kept is not None:
+            raise RuntimeError("nothing is kept without an activation")
 
     def linear_forward(self, input, weight, bias, residual, output, kept, activation: int) -> None:
         """output = act(input weight^T + bias) + residual; ``kept``: None, relu's
         bits (uint8) or gelu's pre-activation (the input's dtype)."""
         _check(input, "input", tuple(_DTYPE_CODES))
-        same = (input.dtype,)
         if weight is None or weight.dim() != 2 or input.dim() == 0:
             raise RuntimeError("weight must be 2-D and input at least 1-D")
         out, cols = weight.shape
         lead = tuple(input.shape[:-1])
         rows = math.prod(lead)
-        self._check_all(input, same, (weight, "weight", (out, input.shape[-1])),
+        self._check_all(input, (input.dtype,), (weight, "weight", (out, input.shape[-1])),
                         (bias, "bias", (out,)), (residual, "residual", (*lead, out)),
                         (output, "output", (*lead, out)))
-        mask = z = None
-        if kept is not None and activation == 1:
-            self._check_all(input, (torch.uint8,), (kept, "relu_mask", (rows, (out + 7) // 8)))
-            mask = kept.data_ptr()
-        elif kept is not None and activation == 2:
-            self._check_all(input, same, (kept, "pre_activation", (rows, out)))
-            z = kept.data_ptr()
+        self._check_kept(input, kept, rows, out, activation)
+        self.linear_forward_launch(input, weight, bias, residual, output, kept, activation, rows,
+                                   cols, out)
+
+    def linear_forward_launch(self, input, weight, bias, residual, output, kept, activation, rows,
+                              cols, out) -> None:
+        kept_ptr = _ptr(kept)
         self._launch(
             "linear_forward", input.device,
             input.data_ptr(), _DTYPE_CODES[input.dtype], weight.data_ptr(), _ptr(bias),
-            _ptr(residual), output.data_ptr(), mask, z, rows, cols, out, activation,
+            _ptr(residual), output.data_ptr(), kept_ptr if activation == 1 else None,
+            kept_ptr if activation == 2 else None, rows, cols, out, activation,
         )
 
     def linear_checkpoint(self, input, codes, scales) -> None:
@@ -1055,6 +1072,9 @@ class NativeLibrary:
         padded = (cols + 31) // 32 * 32
         self._check_all(input, (torch.int8,), (codes, "codes", (rows, padded)))
         self._check_all(input, (torch.uint8,), (scales, "scales", (rows, padded // 32)))
+        self.linear_checkpoint_launch(input, codes, scales, rows, cols)
+
+    def linear_checkpoint_launch(self, input, codes, scales, rows, cols) -> None:
         self._launch("linear_checkpoint", input.device, input.data_ptr(),
                      _DTYPE_CODES[input.dtype], codes.data_ptr(), scales.data_ptr(), rows, cols)
 
@@ -1063,49 +1083,51 @@ class NativeLibrary:
         """The gradients that are not None, from ``input`` or its checkpoint
         (``codes``, ``scales``) and what :meth:`linear_forward` kept."""
         _check(grad_output, "grad_output", tuple(_DTYPE_CODES))
-        same = (grad_output.dtype,)
         out, cols = weight_shape
         lead = tuple(grad_output.shape[:-1])
         rows = math.prod(lead)
         padded = (cols + 31) // 32 * 32
         _check_shape(grad_output, "grad_output", (*lead, out))
-        self._check_all(grad_output, same, (input, "input", (*lead, cols)),
+        self._check_all(grad_output, (grad_output.dtype,), (input, "input", (*lead, cols)),
                         (weight, "weight", (out, cols)), (grad_input, "grad_input", (*lead, cols)),
                         (grad_weight, "grad_weight", (out, cols)),
                         (grad_bias, "grad_bias", (out,)))
         self._check_all(grad_output, (torch.int8,), (codes, "codes", (rows, padded)))
         self._check_all(grad_output, (torch.uint8,), (scales, "scales", (rows, padded // 32)))
-        mask = z = None
-        if kept is not None and activation == 1:
-            self._check_all(grad_output, (torch.uint8,),
-                            (kept, "relu_mask", (rows, (out + 7) // 8)))
-            mask = kept.data_ptr()
-        elif kept is not None and activation == 2:
-            self._check_all(grad_output, same, (kept, "pre_activation", (rows, out)))
-            z = kept.data_ptr()
-        code = _DTYPE_CODES[grad_output.dtype]
-        nbytes = self._linear_scratch(code, rows, cols, out, activation)
+        self._check_kept(grad_output, kept, rows, out, activation)
+        self.linear_backward_launch(
+            grad_output, input, codes, scales, weight, kept, grad_input, grad_weight, grad_bias,
+            self.linear_plan(grad_output.dtype, rows, cols, out, activation))
+
+    def linear_plan(self, dtype, rows, cols, out, activation) -> tuple:
+        """What :meth:`linear_backward_launch` needs besides tensors: the last is
+        the workspace's size."""
+        code = _DTYPE_CODES[dtype]
+        return (code, rows, cols, out, activation,
+                self._linear_scratch(code, rows, cols, out, activation))
+
+    def linear_backward_launch(self, grad_output, input, codes, scales, weight, kept, grad_input,
+                               grad_weight, grad_bias, plan) -> None:
+        code, rows, cols, out, activation, nbytes = plan
         workspace = None
         if nbytes:
             workspace = torch.empty(nbytes, dtype=torch.uint8, device=grad_output.device)
+        kept_ptr = _ptr(kept)
         self._launch(
             "linear_backward", grad_output.device,
             grad_output.data_ptr(), code, _ptr(input), _ptr(codes), _ptr(scales), _ptr(weight),
-            mask, z, _ptr(grad_input), _ptr(grad_weight), _ptr(grad_bias), rows, cols, out,
+            kept_ptr if activation == 1 else None, kept_ptr if activation == 2 else None,
+            _ptr(grad_input), _ptr(grad_weight), _ptr(grad_bias), rows, cols, out,
             activation, _ptr(workspace), nbytes,
         )
 
-    def _norm_weights(self, input, *named):
-        """Checks weight-like tensors; the C-ABI's weight_dtype."""
-        dtype = input.dtype
-        for tensor, name in named:
-            if tensor is not None:
-                dtype = tensor.dtype
-                break
+    def _norm_dtype(self, input, *named):
+        """Checks weight-like tensors; their common dtype (the input's without any)."""
+        dtype = next((t.dtype for t, _ in named if t is not None), input.dtype)
         allowed = (dtype,) if dtype in (input.dtype, torch.float32) else (input.dtype,)
         self._check_all(input, allowed,
                         *((tensor, name, (input.shape[-1],)) for tensor, name in named))
-        return _DTYPE_CODES[dtype]
+        return dtype
 
     def layer_norm_forward(self, input, weight, bias, output, statistics, eps: float) -> None:
         """output = layer norm of input over its last dimension; ``statistics``:
@@ -1117,11 +1139,16 @@ class NativeLibrary:
         rows = math.prod(shape[:-1])
         self._check_all(input, (input.dtype,), (output, "output", shape))
         self._check_all(input, (torch.float32,), (statistics, "statistics", (rows, 2)))
-        wdtype = self._norm_weights(input, (weight, "weight"), (bias, "bias"))
+        dtype = self._norm_dtype(input, (weight, "weight"), (bias, "bias"))
+        self.layer_norm_forward_launch(input, weight, bias, dtype, output, statistics, rows, eps)
+
+    def layer_norm_forward_launch(self, input, weight, bias, weight_dtype, output, statistics,
+                                  rows, eps) -> None:
         self._launch(
             "layer_norm_forward", input.device,
-            input.data_ptr(), _DTYPE_CODES[input.dtype], _ptr(weight), _ptr(bias), wdtype,
-            output.data_ptr(), _ptr(statistics), rows, shape[-1], eps,
+            input.data_ptr(), _DTYPE_CODES[input.dtype], _ptr(weight), _ptr(bias),
+            _DTYPE_CODES[weight_dtype], output.data_ptr(), _ptr(statistics), rows,
+            input.shape[-1], eps,
         )
 
     def layer_norm_backward(self, grad_output, input, weight, statistics, grad_input, grad_weight,
@@ -1129,21 +1156,32 @@ class NativeLibrary:
         """The gradients that are not None, from the forward's statistics."""
         _check(input, "input", tuple(_DTYPE_CODES))
         shape = tuple(input.shape)
-        rows, cols = math.prod(shape[:-1]), shape[-1]
+        rows = math.prod(shape[:-1])
         self._check_all(input, (input.dtype,), (grad_output, "grad_output", shape),
                         (grad_input, "grad_input", shape))
         self._check_all(input, (torch.float32,), (statistics, "statistics", (rows, 2)))
-        wdtype = self._norm_weights(input, (weight, "weight"), (grad_weight, "grad_weight"),
-                                    (grad_bias, "grad_bias"))
-        code = _DTYPE_CODES[input.dtype]
-        nbytes, workspace = 0, None
-        if grad_weight is not None or grad_bias is not None:
-            nbytes = self._norm_scratch(code, rows, cols)
+        dtype = self._norm_dtype(input, (weight, "weight"), (grad_weight, "grad_weight"),
+                                 (grad_bias, "grad_bias"))
+        self.layer_norm_backward_launch(grad_output, input, weight, statistics, grad_input,
+                                        grad_weight, grad_bias,
+                                        self.layer_norm_plan(input.dtype, dtype, rows, shape[-1]))
+
+    def layer_norm_plan(self, dtype, weight_dtype, rows, cols) -> tuple:
+        """What :meth:`layer_norm_backward_launch` needs besides tensors."""
+        code = _DTYPE_CODES[dtype]
+        return code, _DTYPE_CODES[weight_dtype], rows, cols, self._norm_scratch(code, rows, cols)
+
+    def layer_norm_backward_launch(self, grad_output, input, weight, statistics, grad_input,
+                                   grad_weight, grad_bias, plan) -> None:
+        code, weight_code, rows, cols, nbytes = plan
+        workspace = None
+        if grad_weight is None and grad_bias is None:
+            nbytes = 0
         if nbytes:
             workspace = torch.empty(nbytes, dtype=torch.uint8, device=input.device)
         self._launch(
             "layer_norm_backward", input.device,
-            grad_output.data_ptr(), code, input.data_ptr(), _ptr(weight), wdtype,
+            grad_output.data_ptr(), code, input.data_ptr(), _ptr(weight), weight_code,
             statistics.data_ptr(), _ptr(grad_input), _ptr(grad_weight), _ptr(grad_bias), rows,
             cols, _ptr(workspace), nbytes,
         )
