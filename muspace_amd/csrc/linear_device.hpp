@@ -2,18 +2,30 @@
 // pieces of a row ("chunks"), their layouts in LDS and the matrix instructions.
 //
 // A chunk is 16 bytes of a row: 8 values of a 16-bit type or 4 float32 values.
-// A tile of an operand is staged in LDS in one of two layouts, by how the
-// operand lies in memory against the product's summed index k:
+// The matrix cores multiply 16-bit values sixteen times as fast as float32 ones,
+// so float32 operands are multiplied as sums of three bfloat16 numbers, x = x1 +
+// x2 + x3 (split_chunk): each takes the next 8 bits of x, rounded, which leaves
+// |x2| <= 2^-8 |x| and |x3| <= 2^-16 |x|, and x3 what is left of 24 bits exactly.
+// Of the nine products those of planes i + j <= 4 are taken, six; the rest is
+// under 2^-23 |x y| for a product x y, the size of float32's own two roundings, and
+// of random sign. Infinities, NaN and numbers that round to an infinity in bfloat16
+// make such a sum an infinity or NaN: a tile with one in it is multiplied again
+// in float32.
+//
+// A tile of an operand (of one plane) is staged in LDS in one of two layouts, by
+// how the operand lies in memory against the product's summed index k:
 //
 //   along    k is the contiguous index (x and W of x W^T). LDS holds a row of
-//            128 bytes (kStep values of k) per tile row. Chunk c of row r sits in
-//            slot c ^ (r & 7), so that the 8 lanes which an LDS access serves at
-//            a time, 8 rows of one chunk column, touch all banks once.
+//            128 bytes (a plane of float32: 64) per tile row, the step's values of
+//            k. A chunk sits in its slot XOR a key of the row, so that 16 rows of
+//            one chunk column, what an access serves at a time, touch each of the
+//            64 banks once.
 //   across   k is the row index (both operands of dz^T x, W of dz W). LDS holds a
-//            row per k. 16-bit operands are read with the transposing LDS read
-//            (four rows of 16 values per 16 lanes): 32-byte pieces are rotated by
-//            XOR with k, so that the four rows lie in different banks. float32
-//            operands are read a dword a lane, 32 consecutive ones a row.
+//            row per k. 16-bit values are read with the transposing LDS read
+//            (four rows of 16 values per 16 lanes): 32-byte pieces are moved by XOR
+//            with a key of k, so that the four rows' two neighbouring pieces, what
+//            32 lanes read at a time, lie in different banks. float32 values are
+//            read a dword a lane, 32 consecutive ones a row.
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -31,7 +43,7 @@ using msda::to_float;
 
 constexpr int kWave = 64;
 constexpr int kThreads = 256;
-constexpr int kRowBytes = 128;  // of k per tile row and step
+constexpr int kRowBytes = 128;  // of k per row of an operand and step
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
@@ -260,39 +272,55 @@ __device__ __forceinline__ u32x4 decode(const uint32_t (&w)[Piece<T>::kValues / 
   return pack<T>(v);
 }
 
-// ------------------------------------------------------------ LDS layouts ---
+// ----------------------------------------------------------- three planes ---
 
-__device__ __forceinline__ uint32_t along_offset(int row, int chunk) {
-  return row * kRowBytes + ((chunk ^ (row & 7)) << 4);
+__device__ __forceinline__ uint32_t pack_pair(float a, float b) {
+  const __bf16 x = static_cast<__bf16>(a), y = static_cast<__bf16>(b);
+  return static_cast<uint32_t>(__builtin_bit_cast(unsigned short, x)) |
+         static_cast<uint32_t>(__builtin_bit_cast(unsigned short, y)) << 16;
 }
 
-// chunk `c` of row `k` of an across tile of R values a row
-template <typename T, int R>
-__device__ __forceinline__ uint32_t across_offset(int k, int c) {
-  if constexpr (sizeof(T) == 4) {
-    return (k * R + c * 4) * 4;
-  } else {
-    constexpr int kPairs = R / 16;  // 32-byte pieces of a row
-    constexpr int kMask = (kPairs < 8 ? kPairs : 8) - 1;
-    return k * (R * 2) + ((((c >> 1) ^ (k & kMask)) << 1 | (c & 1)) << 4);
+// Four float32 values as kPlanes bfloat16 numbers each, the largest first.
+template <int kPlanes>
+__device__ __forceinline__ void split_chunk(const u32x4 &v, u32x2 (&o)[kPlanes]) {
+#pragma unroll
+  for (int half = 0; half < 2; ++half) {
+    float a = __uint_as_float(v[2 * half]), b = __uint_as_float(v[2 * half + 1]);
+#pragma unroll
+    for (int i = 0; i < kPlanes; ++i) {
+      const uint32_t w = pack_pair(a, b);
+      o[i][half] = w;
+      a -= __uint_as_float(w << 16);  // exact
+      b -= __uint_as_float(w & 0xffff0000u);
+    }
   }
 }
 
-// A lane's part of 32 rows by 8 (float32) or 16 (16-bit) of k: lane l holds row
-// l % 32 and, with h = l / 32, the chunk 2 s + h of a step's 8.
-template <typename T, bool kAlong, int R>
+// ------------------------------------------------------------ LDS layouts ---
+
+// chunk `c` of row `row` of an along tile with rows of kRow bytes
+template <int kRow>
+__device__ __forceinline__ uint32_t along_offset(int row, int c) {
+  const int key = kRow == 128 ? (row >> 1) & 7 : (row >> 2) & 3;
+  return row * kRow + ((c ^ key) << 4);
+}
+
+// chunk `c` of row `k` of an across tile of R 16-bit values a row
+template <int R>
+__device__ __forceinline__ uint32_t across_offset(int k, int c) {
+  // rows of 256 bytes (R = 128): pieces 2 k apart; of 128 bytes: two rows fill the
+  // banks, every second one is moved
+  const int key = R >= 128 ? (k & 3) << 1 : k & 2;
+  return k * (R * 2) + ((((c >> 1) ^ key) << 1 | (c & 1)) << 4);
+}
+
+// A lane's part of 32 rows by 16 of k, 16-bit values: lane l holds row l % 32 and,
+// with h = l / 32, the eight k of the step's chunk 2 s + h.
+template <bool kAlong, int R, int kRow>
 __device__ __forceinline__ u32x4 read_fragment(const char *tile, int row0, int s, int lane) {
   if constexpr (kAlong) {
-    const int row = row0 + (lane & 31);
-    return *reinterpret_cast<const u32x4 *>(tile + along_offset(row, 2 * s + (lane >> 5)));
-  } else if constexpr (sizeof(T) == 4) {
-    u32x4 o;
-    const int k = (2 * s + (lane >> 5)) * 4;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      o[i] = *reinterpret_cast<const uint32_t *>(tile + ((k + i) * R + row0 + (lane & 31)) * 4);
-    }
-    return o;
+    return *reinterpret_cast<const u32x4 *>(
+        tile + along_offset<kRow>(row0 + (lane & 31), 2 * s + (lane >> 5)));
   } else {
     // a group of 16 lanes hands in four k rows of 16 values (lane i: row i / 4,
     // values 4 (i % 4) on) and gets back, lane i, the four k of value i
@@ -301,8 +329,8 @@ __device__ __forceinline__ u32x4 read_fragment(const char *tile, int row0, int s
     const int k = (2 * s + (group >> 1)) * 8 + (i >> 2);
     const int c = (row0 + (group & 1) * 16) / 8 + ((i & 3) >> 1);
     typedef __attribute__((address_space(3))) i16x4 *lds_ptr;
-    const uint32_t o0 = across_offset<T, R>(k, c) + (i & 1) * 8;
-    const uint32_t o1 = across_offset<T, R>(k + 4, c) + (i & 1) * 8;
+    const uint32_t o0 = across_offset<R>(k, c) + (i & 1) * 8;
+    const uint32_t o1 = across_offset<R>(k + 4, c) + (i & 1) * 8;
     const i16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
         (lds_ptr)const_cast<char *>(tile + o0));
     const i16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
@@ -312,6 +340,23 @@ __device__ __forceinline__ u32x4 read_fragment(const char *tile, int row0, int s
 #else
     return u32x4{};
 #endif
+  }
+}
+
+// The same of float32 values: 32 rows by 8 of k, four k a lane.
+template <bool kAlong, int R>
+__device__ __forceinline__ u32x4 read_fragment_f32(const char *tile, int row0, int s, int lane) {
+  if constexpr (kAlong) {
+    return *reinterpret_cast<const u32x4 *>(
+        tile + along_offset<128>(row0 + (lane & 31), 2 * s + (lane >> 5)));
+  } else {
+    u32x4 o;
+    const int k = (2 * s + (lane >> 5)) * 4;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      o[i] = *reinterpret_cast<const uint32_t *>(tile + ((k + i) * R + row0 + (lane & 31)) * 4);
+    }
+    return o;
   }
 }
 

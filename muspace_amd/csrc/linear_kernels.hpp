@@ -9,13 +9,15 @@
 //
 // linear_product: a workgroup of four wavefronts makes a BM x BN tile of the
 // result, each wavefront a quarter. Both operands go through LDS in steps of 128
-// bytes of k, two buffers: the chunks of step i + 1 are in registers on their way
-// while step i is multiplied. Products run on the matrix cores with float32 sums:
-// 32x32x16 for 16-bit types, 32x32x2 for float32. The wavefront multiplies with
-// the result's columns as the matrix instruction's rows, so that a lane holds
-// runs of four columns of a row and the tile goes through LDS in 16-byte pieces
-// into whole 128-byte row segments, where bias, activation, residual and mask
-// are applied once per value.
+// bytes of k; the chunks of step i + 1 are in registers on their way while step i
+// is multiplied. One LDS buffer, not two: a second workgroup more on a CU hides
+// more of the loads than the second buffer did (369900 x 256 -> 256 bf16 114 ->
+// 94 us, 44446 x 256 -> 1024 float32 217 -> 208). The matrix cores multiply 16-bit
+// values (32x32x16), float32 ones as three bfloat16 planes (linear_device.hpp).
+// The wavefront multiplies with the result's columns as the matrix instruction's
+// rows, so that a lane holds runs of four columns of a row and the tile goes
+// through LDS in 16-byte pieces into whole 128-byte row segments, where bias,
+// activation, residual and mask are applied once per value.
 //
 // All sums are in float32 and in a fixed order: results do not change from run to
 // run. Results are rounded once, to the tensors' type.
@@ -200,9 +202,34 @@ struct Loader {
     }
   }
 
+  // LDS bytes of one plane's tile
+  static constexpr int kRow = sizeof(T) == 4 ? 64 : 128;
+  static constexpr int kPlaneBytes = R * kRow;
+  // 8-bit codes need one plane: 7 bits
+  static constexpr int kPlanes = sizeof(T) == 4 ? (kCodes ? 1 : 3) : 1;
+
   __device__ __forceinline__ void put(char *tile, int i, const u32x4 &value) const {
-    const uint32_t at = kAlong ? along_offset(r + 32 * i, c)
-                               : across_offset<T, R>(r + i * kStride, c);
+    if constexpr (sizeof(T) == 4) {
+      u32x2 part[kPlanes];
+      split_chunk<kPlanes>(value, part);
+      const uint32_t at = (kAlong ? along_offset<64>(r + 32 * i, c >> 1)
+                                  : across_offset<R>(r + i * kStride, c >> 1)) +
+                          (c & 1) * 8;
+#pragma unroll
+      for (int e = 0; e < kPlanes; ++e) {
+        *reinterpret_cast<u32x2 *>(tile + e * kPlaneBytes + at) = part[e];
+      }
+    } else {
+      const uint32_t at = kAlong ? along_offset<128>(r + 32 * i, c)
+                                 : across_offset<R>(r + i * kStride, c);
+      *reinterpret_cast<u32x4 *>(tile + at) = value;
+    }
+  }
+
+  // float32 as it is, for the tiles that hold more than bfloat16's range
+  __device__ __forceinline__ void put_f32(char *tile, int i, const u32x4 &value) const {
+    const uint32_t at = kAlong ? along_offset<128>(r + 32 * i, c)
+                               : static_cast<uint32_t>(((r + i * kStride) * R + c * 4) * 4);
     *reinterpret_cast<u32x4 *>(tile + at) = value;
   }
 };
@@ -270,19 +297,27 @@ __device__ __forceinline__ void finish_forward(const Product &a, int64_t row, in
 
 // ------------------------------------------------------------- tile kernel ---
 
+// Two workgroups a CU at least: the loads of one hide behind the products of the
+// other (up to three with the 136 to 168 registers that most variants need; four,
+// at 128 registers, spill).
 template <typename T, Job kJob, int BM, int BN, bool kTight, bool kMask, bool kCodes>
-__global__ __launch_bounds__(kThreads) void linear_product(const Product a) {
+__global__ __launch_bounds__(kThreads, 2) void linear_product(const Product a) {
   constexpr int kV = Piece<T>::kValues;
   constexpr int kStep = Piece<T>::kStep;
+  constexpr bool kF32 = sizeof(T) == 4;
   constexpr bool kPAlong = kJob != Job::kWeight;
   constexpr bool kQAlong = kJob == Job::kForward;
   constexpr int WM = BM / 2, WN = BN / 2;  // a wavefront's quarter
   constexpr int kI = WM / 32, kJ = WN / 32;
-  constexpr int kTileP = BM * kRowBytes, kTileQ = BN * kRowBytes;
-  constexpr int kBuffer = kTileP + kTileQ;
+  using P = Loader<T, kPAlong, BM, kTight, kMask, false>;
+  using Q = Loader<T, kQAlong, BN, kTight, false, kCodes>;
   constexpr int kStageLd = WN + 4;  // floats; the pad spreads rows over the banks
-  static_assert(4 * 32 * kStageLd * 4 <= 2 * kBuffer, "result stage exceeds the tiles' LDS");
-  __shared__ __attribute__((aligned(16))) char lds[2 * kBuffer];
+  constexpr int kTiles = P::kPlanes * P::kPlaneBytes + Q::kPlanes * Q::kPlaneBytes;
+  constexpr int kTilesF32 = kF32 ? (BM + BN) * kRowBytes : 0;
+  constexpr int kStage = 4 * 32 * kStageLd * 4;
+  constexpr int kLds = kStage > kTiles ? (kStage > kTilesF32 ? kStage : kTilesF32)
+                                       : (kTiles > kTilesF32 ? kTiles : kTilesF32);
+  __shared__ __attribute__((aligned(16))) char lds[kLds];
 
   int tile = xcd_order(blockIdx.x, gridDim.x);
   int split = 0;
@@ -296,25 +331,33 @@ __global__ __launch_bounds__(kThreads) void linear_product(const Product a) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int wr = (wave >> 1) * WM, wc = (wave & 1) * WN;
 
-  Loader<T, kPAlong, BM, kTight, kMask, false> p;
-  Loader<T, kQAlong, BN, kTight, false, kCodes> q;
+  P p;
+  Q q;
   p.init(a.p, a.ldp, a.mask, a.mask_ld, row0, a.m, k_end);
   q.init(a.q, a.ldq, a.scales, a.scale_ld, col0, a.n, k_end);
 
   f32x16 acc[kI][kJ];
+  auto clear = [&]() {
 #pragma unroll
-  for (int i = 0; i < kI; ++i) {
+    for (int i = 0; i < kI; ++i) {
 #pragma unroll
-    for (int j = 0; j < kJ; ++j) acc[i][j] = f32x16{};
-  }
+      for (int j = 0; j < kJ; ++j) acc[i][j] = f32x16{};
+    }
+  };
+  clear();
   // kWeight's first tile column also sums dz over its rows: a thread's chunks all
   // lie in one column of chunks
   float sums[kV] = {};
   const bool sum_p = kJob == Job::kWeight && col0 == 0;
 
-  auto put = [&](char *buffer) {
+  char *const tile_p = lds, *const tile_q = lds + P::kPlanes * P::kPlaneBytes;
+  if (k_begin < k_end) {
+    p.fetch(k_begin);
+    q.fetch(k_begin);
+  }
+  for (int k0 = k_begin; k0 < k_end; k0 += kStep) {
 #pragma unroll
-    for (int i = 0; i < p.kCount; ++i) {
+    for (int i = 0; i < P::kCount; ++i) {
       const u32x4 v = p.chunk(i);
       if constexpr (kJob == Job::kWeight) {
         if (sum_p) {
@@ -324,42 +367,91 @@ __global__ __launch_bounds__(kThreads) void linear_product(const Product a) {
           for (int e = 0; e < kV; ++e) sums[e] += f[e];
         }
       }
-      p.put(buffer, i, v);
+      p.put(tile_p, i, v);
     }
 #pragma unroll
-    for (int i = 0; i < q.kCount; ++i) q.put(buffer + kTileP, i, q.chunk(i));
-  };
-
-  if (k_begin < k_end) {
-    p.fetch(k_begin);
-    q.fetch(k_begin);
-    put(lds);
-  }
-  __syncthreads();
-  int at = 0;
-  for (int k0 = k_begin; k0 < k_end; k0 += kStep) {
-    const bool more = k0 + kStep < k_end;
-    if (more) {
+    for (int i = 0; i < Q::kCount; ++i) q.put(tile_q, i, q.chunk(i));
+    __syncthreads();
+    if (k0 + kStep < k_end) {
       p.fetch(k0 + kStep);
       q.fetch(k0 + kStep);
     }
-    const char *tile_p = lds + at, *tile_q = lds + at + kTileP;
 #pragma unroll
-    for (int s = 0; s < 4; ++s) {
-      u32x4 fp[kI], fq[kJ];
+    for (int s = 0; s < P::kRow / 32; ++s) {
+      u32x4 fp[P::kPlanes][kI], fq[Q::kPlanes][kJ];
 #pragma unroll
-      for (int i = 0; i < kI; ++i) fp[i] = read_fragment<T, kPAlong, BM>(tile_p, wr + 32 * i, s, lane);
+      for (int e = 0; e < P::kPlanes; ++e) {
 #pragma unroll
-      for (int j = 0; j < kJ; ++j) fq[j] = read_fragment<T, kQAlong, BN>(tile_q, wc + 32 * j, s, lane);
+        for (int i = 0; i < kI; ++i) {
+          fp[e][i] = read_fragment<kPAlong, BM, P::kRow>(tile_p + e * P::kPlaneBytes, wr + 32 * i,
+                                                         s, lane);
+        }
+      }
 #pragma unroll
-      for (int i = 0; i < kI; ++i) {
+      for (int e = 0; e < Q::kPlanes; ++e) {
 #pragma unroll
-        for (int j = 0; j < kJ; ++j) acc[i][j] = multiply<T>(fq[j], fp[i], acc[i][j]);
+        for (int j = 0; j < kJ; ++j) {
+          fq[e][j] = read_fragment<kQAlong, BN, P::kRow>(tile_q + e * Q::kPlaneBytes, wc + 32 * j,
+                                                         s, lane);
+        }
+      }
+#pragma unroll
+      for (int x = 0; x < P::kPlanes; ++x) {
+#pragma unroll
+        for (int y = 0; y < Q::kPlanes; ++y) {
+          if (x + y > 2) continue;
+#pragma unroll
+          for (int i = 0; i < kI; ++i) {
+#pragma unroll
+            for (int j = 0; j < kJ; ++j) {
+              acc[i][j] = multiply<std::conditional_t<kF32, bf16_t, T>>(fq[y][j], fp[x][i],
+                                                                       acc[i][j]);
+            }
+          }
+        }
       }
     }
-    at ^= kBuffer;
-    if (more) put(lds + at);
     __syncthreads();
+  }
+
+  if constexpr (kF32) {
+    // a sum that is not finite: an infinity, NaN or a number past bfloat16's range
+    // among its values, or an overflow. Then the tile again, in float32.
+    float zero = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kI; ++i) {
+#pragma unroll
+      for (int j = 0; j < kJ; ++j) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) zero = fmaf(acc[i][j][e], 0.0f, zero);
+      }
+    }
+    if (__syncthreads_or(!(zero == 0.0f))) {
+      clear();
+      char *const wide_q = lds + BM * kRowBytes;
+      for (int k0 = k_begin; k0 < k_end; k0 += kStep) {
+        p.fetch(k0);
+        q.fetch(k0);
+#pragma unroll
+        for (int i = 0; i < P::kCount; ++i) p.put_f32(lds, i, p.chunk(i));
+#pragma unroll
+        for (int i = 0; i < Q::kCount; ++i) q.put_f32(wide_q, i, q.chunk(i));
+        __syncthreads();
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+#pragma unroll
+          for (int i = 0; i < kI; ++i) {
+            const u32x4 fp = read_fragment_f32<kPAlong, BM>(lds, wr + 32 * i, s, lane);
+#pragma unroll
+            for (int j = 0; j < kJ; ++j) {
+              const u32x4 fq = read_fragment_f32<kQAlong, BN>(wide_q, wc + 32 * j, s, lane);
+              acc[i][j] = multiply<float>(fq, fp, acc[i][j]);
+            }
+          }
+        }
+        __syncthreads();
+      }
+    }
   }
 
   // the bias gradient: threads of one chunk column add their sums, in thread order

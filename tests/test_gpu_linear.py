@@ -246,6 +246,39 @@ def test_infinities_and_nan_stay_in_their_rows_and_columns(size, dtype):
     assert db[3].isnan() and db[:3].isfinite().all() and db[4:].isfinite().all()
 
 
+@pytest.mark.parametrize("size", [(40, 40, 24), (9000, 72, 136), (257, 203, 131)], ids=str)
+def test_float32_over_its_whole_range(size):
+    """float32 is multiplied as bfloat16 numbers: values past that type's range (finite in
+    float32), infinities and very small values must come out as float32 has them."""
+    rows, inner, outer = size
+    x, w, b, _, g = make(*size, torch.float32, exact=False, seed=4)
+    w = torch.where(w.abs() < 2.0**-6, 2.0**-6, w)
+    top = torch.finfo(torch.float32).max
+    x[3] = 0.0
+    x[3, 5] = top  # rounds to an infinity in bfloat16
+    w[:, 5] = w[:, 5].clamp(-0.5, 0.5)
+    x[4] *= 2.0**-100
+    x[rows - 1, 7] = -math.inf
+    check_rows = [i for i in range(rows) if i != rows - 1]
+    out = linear(x, w, b)
+    results, bounds = dense_torch.linear(x[check_rows], w, b, None, None)
+    assert_within(out[check_rows], results[0], bounds[0], "out")
+    assert torch.equal(out[rows - 1], torch.where(w[:, 7] > 0, -math.inf, math.inf))
+    relu = linear(x, w, b, activation="relu")
+    assert torch.equal(relu, torch.relu(out))
+    # the same of a gradient: dz^T x and dz W in their tiles
+    g[2] = 0.0
+    g[2, 3] = top
+    xs, ws, bs = leaves(*make(*size, torch.float32, exact=False, seed=8)[:3])
+    with torch.no_grad():
+        xs[2].clamp_(-0.4, 0.4)
+        ws[3].clamp_(-0.4, 0.4)
+    grads = torch.autograd.grad(linear(xs, ws, bs), [xs, ws, bs], g)
+    results, bounds = dense_torch.linear(xs.detach(), ws.detach(), bs.detach(), None, None, g)
+    for a, e, t in zip(grads, results[1:], bounds[1:]):
+        assert_within(a, e, t, "gradient")
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_relu_masks_whatever_the_gradient_holds(dtype):
     """Where relu is off, an infinite or NaN gradient counts as zero; a NaN
