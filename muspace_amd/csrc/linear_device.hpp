@@ -215,6 +215,22 @@ __device__ __forceinline__ u32x4 loose_load(const T *p, int left) {
   return o;
 }
 
+// A chunk whose first `skip` values are another's: the rest, moved to the front,
+// zeros behind (skip at or over a chunk's values: zeros).
+template <typename T>
+__device__ __forceinline__ u32x4 drop_front(const u32x4 &v, int skip) {
+  const int bits = skip * 8 * static_cast<int>(sizeof(T));
+  const uint64_t lo = v[0] | static_cast<uint64_t>(v[1]) << 32;
+  const uint64_t hi = v[2] | static_cast<uint64_t>(v[3]) << 32;
+  const int b = bits & 63;
+  const uint64_t hi_down = hi >> b;
+  const uint64_t lo_down = b == 0 ? lo : (lo >> b | hi << (64 - b));
+  const uint64_t o_lo = bits < 64 ? lo_down : (bits < 128 ? hi_down : 0);
+  const uint64_t o_hi = bits < 64 ? hi_down : 0;
+  return u32x4{static_cast<uint32_t>(o_lo), static_cast<uint32_t>(o_lo >> 32),
+               static_cast<uint32_t>(o_hi), static_cast<uint32_t>(o_hi >> 32)};
+}
+
 template <typename T>
 __device__ __forceinline__ void loose_store(T *p, const u32x4 &v, int left) {
   if (left >= Piece<T>::kValues) {

@@ -63,7 +63,12 @@ __device__ __forceinline__ int xcd_order(int id, int count) {
 // --------------------------------------------------------- operand loader ---
 
 // One operand's R rows (of the result) by a step of k: kCount chunks per thread,
-// fetched into registers, then put into LDS.
+// fetched into registers, then put into LDS. Loads are unconditional, so that all of
+// a step's are in flight together. Rows off every alignment (!kTight): a chunk that
+// passes the end of its memory row is read as the row's last 16 bytes and its values
+// are moved to the front when it is used; rows past the operand read its last one,
+// which only marks results that are not stored (past k: zeros). Memory rows shorter
+// than a chunk are read value by value.
 template <typename T, bool kAlong, int R, bool kTight, bool kMask, bool kCodes>
 struct Loader {
   static constexpr int kV = Piece<T>::kValues;
@@ -77,6 +82,9 @@ struct Loader {
   int64_t ld, bytes_ld;
   int row0, rows, k_end;  // first result row, their number in all, end of k
   int r, c;               // thread's first row (along) or k row (across); its chunk
+  int skip;               // !kTight: values of the read chunk that are not its own
+  bool moved, past;       // !kTight, uniform: some chunk has skip > 0, k past its end
+  int k_at;
   u32x4 v[kCount];
   uint32_t side[kCount];  // mask byte or scale byte
 
@@ -125,10 +133,21 @@ struct Loader {
                                static_cast<uint32_t>(sizeof(T));
           v[i] = tight_load(s, inside ? off : kPast);
         }
-      } else {
+      } else if (k_end >= kV) {
+        const int col = min(k0 + c * kV, k_end - kV);
+        skip = k0 + c * kV - col;
+        moved = k0 + kStep > k_end;
+        past = false;
 #pragma unroll
         for (int i = 0; i < kCount; ++i) {
-          const int row = row0 + r + 32 * i;
+          const int64_t row = min(row0 + r + 32 * i, rows - 1);
+          v[i] = reinterpret_cast<const Loose16 *>(ptr + row * ld + col)->v;
+        }
+      } else {
+        moved = past = false;
+#pragma unroll
+        for (int i = 0; i < kCount; ++i) {
+          const int64_t row = row0 + r + 32 * i;
           v[i] = loose_load<T>(ptr + row * ld + k0 + c * kV,
                                row < rows ? k_end - (k0 + c * kV) : 0);
         }
@@ -169,7 +188,19 @@ struct Loader {
                                static_cast<uint32_t>(sizeof(T));
           v[i] = tight_load(s, inside ? off : kPast);
         }
+      } else if (rows >= kV) {
+        const int col = min(row0 + c * kV, rows - kV);
+        skip = row0 + c * kV - col;
+        moved = row0 + R > rows;
+        past = k0 + kStep > k_end;
+        k_at = k0;
+#pragma unroll
+        for (int i = 0; i < kCount; ++i) {
+          const int64_t kr = min(k0 + r + i * kStride, k_end - 1);
+          v[i] = reinterpret_cast<const Loose16 *>(ptr + kr * ld + col)->v;
+        }
       } else {
+        moved = past = false;
 #pragma unroll
         for (int i = 0; i < kCount; ++i) {
           const int64_t kr = k0 + r + i * kStride;
@@ -195,10 +226,14 @@ struct Loader {
       w[0] = v[i][0];
       if constexpr (kV == 8) w[1] = v[i][1];
       return decode<T>(w, scale_value(side[i]));
-    } else if constexpr (kMask) {
-      return keep_bits<T>(v[i], side[i] >> ((c * kV) & 7));
     } else {
-      return v[i];
+      u32x4 o = v[i];
+      if constexpr (!kTight) {
+        if (moved) o = drop_front<T>(o, skip);
+        if (!kAlong && past && k_at + r + i * kStride >= k_end) o = u32x4{0, 0, 0, 0};
+      }
+      if constexpr (kMask) o = keep_bits<T>(o, side[i] >> ((c * kV) & 7));
+      return o;
     }
   }
 
@@ -612,40 +647,57 @@ __global__ __launch_bounds__(kWaves * kWave) void linear_forward_few(const Produ
 
 // ----------------------------------------------------- gradient's last step ---
 
-// dW and db from the parts of k, summed in their order.
+// dW and db from the parts of k: a workgroup takes 32 pieces of four columns (or 32
+// rows of db) with eight threads each, which add every eighth part in order and join
+// in LDS, in order. Reading is all of it: one thread a piece kept too little in
+// flight (512 x 256 in 63 parts 16.6 us, 33 MB).
+constexpr int kSumPieces = 32;
+
 template <typename T>
 __global__ __launch_bounds__(kThreads) void linear_weight_sum(const float *partial,
                                                               const float *bias_partial, T *dw,
                                                               T *db, int m, int n, int splits) {
+  constexpr int kRuns = kThreads / kSumPieces;
+  __shared__ __attribute__((aligned(16))) f32x4 lds[kRuns][kSumPieces];
   const int ld = (n + 7) & ~7, per_row = ld / 4;
-  const int64_t i = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
+  const int x = threadIdx.x % kSumPieces, y = threadIdx.x / kSumPieces;
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * kSumPieces + x;
   const int64_t count = static_cast<int64_t>(m) * per_row;
-  if (i < count) {
+  const bool weight = i < count, bias = !weight && db != nullptr && i - count < m;
+  f32x4 s = {0.0f, 0.0f, 0.0f, 0.0f};
+  if (weight) {
+    const float *src = partial + i * 4;
+    const int64_t stride = static_cast<int64_t>(m) * ld;
+    int u = y;
+    for (; u + 3 * kRuns < splits; u += 4 * kRuns) {
+      f32x4 v[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        v[e] = *reinterpret_cast<const f32x4 *>(src + (u + e * kRuns) * stride);
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s += v[e];
+    }
+    for (; u < splits; u += kRuns) s += *reinterpret_cast<const f32x4 *>(src + u * stride);
+  } else if (bias) {
+    for (int u = y; u < splits; u += kRuns) {
+      s[0] += bias_partial[static_cast<int64_t>(u) * m + (i - count)];
+    }
+  }
+  lds[y][x] = s;
+  __syncthreads();
+  if (y != 0) return;
+#pragma unroll
+  for (int u = 1; u < kRuns; ++u) s += lds[u][x];
+  if (weight) {
     const int64_t row = i / per_row;
     const int col = static_cast<int>(i - row * per_row) * 4;
-    const float *src = partial + row * ld + col;
-    const int64_t stride = static_cast<int64_t>(m) * ld;
-    f32x4 s = {0.0f, 0.0f, 0.0f, 0.0f};
-    int u = 0;
-    for (; u + 8 <= splits; u += 8) {
-      f32x4 v[8];
-#pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = *reinterpret_cast<const f32x4 *>(src + (u + e) * stride);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) s += v[e];
-    }
-    for (; u < splits; ++u) s += *reinterpret_cast<const f32x4 *>(src + u * stride);
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       if (col + e < n) dw[row * n + col + e] = from_float<T>(s[e]);
     }
-    return;
-  }
-  const int64_t row = i - count;
-  if (db != nullptr && row < m) {
-    float s = 0.0f;
-    for (int u = 0; u < splits; ++u) s += bias_partial[static_cast<int64_t>(u) * m + row];
-    db[row] = from_float<T>(s);
+  } else if (bias) {
+    db[i - count] = from_float<T>(s[0]);
   }
 }
 
