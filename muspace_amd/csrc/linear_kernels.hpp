@@ -271,13 +271,38 @@ struct Loader {
 
 // ---------------------------------------------------------------- epilogue ---
 
+// Phi(z), the normal distribution function, and exp(-z^2 / 2). With t = 1 / (1 +
+// 0.35 |z|), the upper tail is exp(-z^2 / 2) t P(t); P, of degree 8, is a least
+// squares fit, reweighted until its relative error was level, 3.2e-8 over |z| <= 14
+// (past that the tail is under float32's normal numbers). The tail is computed
+// itself, without a difference from one, so gelu keeps its relative accuracy for
+// negative z. The library's error function costs two to three times the
+// instructions: gelu was a third of the time of the products it ends.
+__device__ __forceinline__ float normal_cdf(float z, float &density) {
+  const float t = __builtin_amdgcn_rcpf(fmaf(0.35f, fabsf(z), 1.0f));
+  float p = -0.029145927f;
+  p = fmaf(p, t, 0.14397168f);
+  p = fmaf(p, t, -0.25571422f);
+  p = fmaf(p, t, 0.15917413f);
+  p = fmaf(p, t, -0.023109811f);
+  p = fmaf(p, t, 0.10550799f);
+  p = fmaf(p, t, 0.11983287f);
+  p = fmaf(p, t, 0.13986187f);
+  p = fmaf(p, t, 0.13962140f);
+  density = __builtin_amdgcn_exp2f(z * z * -0.72134752f);
+  const float tail = t * p * density;
+  return z < 0.0f ? tail : 1.0f - tail;
+}
+
 __device__ __forceinline__ float gelu(float z) {
-  return 0.5f * z * (1.0f + erff(z * 0.70710678118654752f));
+  float density;
+  return z * normal_cdf(z, density);
 }
 
 __device__ __forceinline__ float gelu_slope(float z) {
-  const float cdf = 0.5f * (1.0f + erff(z * 0.70710678118654752f));
-  return cdf + z * (0.39894228040143268f * expf(-0.5f * z * z));
+  float density;
+  const float cdf = normal_cdf(z, density);
+  return fmaf(z * 0.39894228f, density, cdf);
 }
 
 // `left` values of bias from `p` on
