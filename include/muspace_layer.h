@@ -14,8 +14,9 @@
  *               x [rows, in], weight [out, in], bias [out] or NULL,
  *               residual [rows, out] or NULL, output [rows, out]
  * activation    0 none, 1 relu, 2 gelu (z * Phi(z), by the error function)
- * relu_mask     [rows, ceil(out / 8)] bytes: bit i of byte j is set where the
- *               derivative of relu at z[8 j + i] is one (z > 0, or NaN)
+ * relu_mask     [ceil(out / 64), rows, 8] bytes: bit i of byte j of block c is set
+ *               where the derivative of relu at z[64 c + 8 j + i] is one (z > 0, or
+ *               NaN); bits past out are not read
  * pre_activation [rows, out] z in the tensors' type, kept for gelu's derivative
  * codes, scales an 8-bit checkpoint of x: [rows, pad32(in)] int8 and
  *               [rows, pad32(in) / 32] bytes. 32 values share 2^e, the smallest

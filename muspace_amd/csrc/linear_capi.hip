@@ -207,7 +207,7 @@ int linear_forward(const void *x, int dtype, const void *weight, const void *bia
   a.out = output;
   a.z_out = activation == dense::kGelu ? pre_activation : nullptr;
   a.mask_out = activation == dense::kRelu ? relu_mask : nullptr;
-  a.mask_ld = ceil_div(out_features, 8);
+  a.mask_ld = rows * 8;
   a.act = activation;
   const bool tight =
       in_features % chunk_values(dtype) == 0 && aligned16(x) && aligned16(weight);
@@ -308,7 +308,7 @@ int linear_backward(const void *grad_output, int dtype, const void *x, const int
     a.n = static_cast<int>(in_features);
     a.k = static_cast<int>(out_features);
     a.mask = mask;
-    a.mask_ld = ceil_div(out_features, 8);
+    a.mask_ld = rows * 8;
     a.splits = 1;
     a.out = grad_input;
     const bool tight = whole_out && in_features % v == 0 && aligned16(weight);
@@ -329,7 +329,7 @@ int linear_backward(const void *grad_output, int dtype, const void *x, const int
     a.scales = coded ? scales : nullptr;
     a.scale_ld = a.ldq / 32;
     a.mask = mask;
-    a.mask_ld = ceil_div(out_features, 8);
+    a.mask_ld = rows * 8;
     a.splits = plan.splits;
     a.k_split = plan.k_split;
     a.out = grad_weight;

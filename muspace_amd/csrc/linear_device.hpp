@@ -45,10 +45,13 @@ constexpr int kWave = 64;
 constexpr int kThreads = 256;
 constexpr int kRowBytes = 128;  // of k per row of an operand and step
 
+typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef short i16x4 __attribute__((ext_vector_type(4)));
 typedef short i16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
@@ -109,6 +112,15 @@ __device__ __forceinline__ uint32_t bits_of<__half>(__half v) {
   return __half_as_ushort(v);
 }
 
+// Two values, rounded to nearest even by one conversion instruction (gfx950's; NaN
+// stays NaN).
+__device__ __forceinline__ uint32_t pack_pair_bf16(float a, float b) {
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{a, b}, bf16x2));
+}
+__device__ __forceinline__ uint32_t pack_pair_f16(float a, float b) {
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{a, b}, f16x2));
+}
+
 // round to nearest even, once: the results' only rounding below 32 bits
 template <typename T>
 __device__ __forceinline__ u32x4 pack(const float (&v)[Piece<T>::kValues]);
@@ -122,21 +134,15 @@ __device__ __forceinline__ u32x4 pack<__half>(const float (&v)[8]) {
   u32x4 o;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    o[i] = bits_of(from_float<__half>(v[2 * i])) | bits_of(from_float<__half>(v[2 * i + 1])) << 16;
+    o[i] = pack_pair_f16(v[2 * i], v[2 * i + 1]);
   }
   return o;
 }
 template <>
 __device__ __forceinline__ u32x4 pack<bf16_t>(const float (&v)[8]) {
-  // the conversion instruction of gfx950 rounds to nearest even and keeps NaN
   u32x4 o;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const __bf16 a = static_cast<__bf16>(v[2 * i]);
-    const __bf16 b = static_cast<__bf16>(v[2 * i + 1]);
-    o[i] = static_cast<uint32_t>(__builtin_bit_cast(unsigned short, a)) |
-           static_cast<uint32_t>(__builtin_bit_cast(unsigned short, b)) << 16;
-  }
+  for (int i = 0; i < 4; ++i) o[i] = pack_pair_bf16(v[2 * i], v[2 * i + 1]);
   return o;
 }
 
@@ -290,12 +296,6 @@ __device__ __forceinline__ u32x4 decode(const uint32_t (&w)[Piece<T>::kValues / 
 
 // ----------------------------------------------------------- three planes ---
 
-__device__ __forceinline__ uint32_t pack_pair(float a, float b) {
-  const __bf16 x = static_cast<__bf16>(a), y = static_cast<__bf16>(b);
-  return static_cast<uint32_t>(__builtin_bit_cast(unsigned short, x)) |
-         static_cast<uint32_t>(__builtin_bit_cast(unsigned short, y)) << 16;
-}
-
 // Four float32 values as kPlanes bfloat16 numbers each, the largest first.
 template <int kPlanes>
 __device__ __forceinline__ void split_chunk(const u32x4 &v, u32x2 (&o)[kPlanes]) {
@@ -304,7 +304,7 @@ __device__ __forceinline__ void split_chunk(const u32x4 &v, u32x2 (&o)[kPlanes])
     float a = __uint_as_float(v[2 * half]), b = __uint_as_float(v[2 * half + 1]);
 #pragma unroll
     for (int i = 0; i < kPlanes; ++i) {
-      const uint32_t w = pack_pair(a, b);
+      const uint32_t w = pack_pair_bf16(a, b);
       o[i][half] = w;
       a -= __uint_as_float(w << 16);  // exact
       b -= __uint_as_float(w & 0xffff0000u);

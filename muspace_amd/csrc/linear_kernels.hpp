@@ -37,8 +37,8 @@ struct Product {
   const void *q;         // columns: W, W^T or x
   int64_t ldp, ldq;      // values per row in memory
   int m, n, k;           // result rows, columns; summed index
-  const uint8_t *mask;   // relu's bits for p (0: none), one byte per 8 columns
-  int64_t mask_ld;
+  const uint8_t *mask;   // relu's bits for p (0: none), [blocks of 64 columns][rows][8]
+  int64_t mask_ld;       // bytes of a block of columns: 8 a row
   const uint8_t *scales;  // kWeight with codes: q are codes, a scale byte per 32
   int64_t scale_ld;
   int tiles_n, tiles;    // tiles along n; all tiles of the result
@@ -46,7 +46,7 @@ struct Product {
   // forward
   const void *bias, *residual;
   void *out, *z_out;     // z_out: kept x W^T + b (gelu under training)
-  uint8_t *mask_out;     // kept sign bits (relu under training)
+  uint8_t *mask_out;     // kept sign bits (relu under training), as mask
   int act;
   // kWeight
   float *partial, *bias_partial;  // [splits][m][pad8(n)], [splits][m]
@@ -153,11 +153,11 @@ struct Loader {
         }
       }
       if constexpr (kMask) {
-        const Source s = view(bytes, bytes_ld, row0, k0 / 8, rows);
+        const int col = min(k0 + c * kV, k_end - 1);
+        const uint8_t *b = bytes + (col >> 6) * bytes_ld + ((col >> 3) & 7);
 #pragma unroll
         for (int i = 0; i < kCount; ++i) {
-          side[i] = tight_load_byte(
-              s, static_cast<uint32_t>((r + 32 * i) * bytes_ld) + (c * kV) / 8);
+          side[i] = b[static_cast<int64_t>(min(row0 + r + 32 * i, rows - 1)) * 8];
         }
       }
     } else {
@@ -209,11 +209,11 @@ struct Loader {
         }
       }
       if constexpr (kMask) {
-        const Source s = view(bytes, bytes_ld, k0, row0 / 8, k_end);
+        const int col = min(row0 + c * kV, rows - 1);
+        const uint8_t *b = bytes + (col >> 6) * bytes_ld + ((col >> 3) & 7);
 #pragma unroll
         for (int i = 0; i < kCount; ++i) {
-          side[i] = tight_load_byte(
-              s, static_cast<uint32_t>((r + i * kStride) * bytes_ld) + (c * kV) / 8);
+          side[i] = b[static_cast<int64_t>(min(k0 + r + i * kStride, k_end - 1)) * 8];
         }
       }
     }
@@ -312,6 +312,15 @@ __device__ __forceinline__ void load_bias(const T *p, int left, float (&b)[Piece
   unpack<T>(v, b);
 }
 
+// lane l's value from lane l ^ 1
+__device__ __forceinline__ uint32_t swap_neighbours(uint32_t v) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  return __builtin_amdgcn_mov_dpp(static_cast<int>(v), 0xB1, 0xf, 0xf, true);
+#else
+  return v;
+#endif
+}
+
 // A chunk of the forward's result: z holds x W^T + b. `half`: the lane holds the
 // upper four columns of a mask byte (float32).
 template <typename T>
@@ -328,14 +337,15 @@ __device__ __forceinline__ void finish_forward(const Product &a, int64_t row, in
       z[i] = keep ? z[i] : 0.0f;
     }
     if (a.mask_out != nullptr) {
+      uint8_t *mask = a.mask_out + (col >> 6) * a.mask_ld + row * 8 + ((col >> 3) & 7);
       if constexpr (kV == 4) {
         // lanes l and l ^ 1 hold the two halves of a byte
-        const uint32_t other = __shfl_xor(bits, 1);
+        const uint32_t other = swap_neighbours(bits);
         if ((col & 4) == 0 && left > 0) {
-          a.mask_out[row * a.mask_ld + col / 8] = static_cast<uint8_t>(bits | other << 4);
+          *mask = static_cast<uint8_t>(bits | other << 4);
         }
       } else if (left > 0) {
-        a.mask_out[row * a.mask_ld + col / 8] = static_cast<uint8_t>(bits);
+        *mask = static_cast<uint8_t>(bits);
       }
     }
   } else if (a.act == kGelu) {
@@ -357,11 +367,15 @@ __device__ __forceinline__ void finish_forward(const Product &a, int64_t row, in
 
 // ------------------------------------------------------------- tile kernel ---
 
-// Two workgroups a CU at least: the loads of one hide behind the products of the
-// other (up to three with the 136 to 168 registers that most variants need; four,
-// at 128 registers, spill).
+// Three workgroups a CU where the registers allow it (168 of them): the loads and
+// stores of one hide behind the products of the others. 16-bit products need 136 to
+// 168 by themselves; float32 ones are held to it where rows are whole chunks (44446 x
+// 256 -> 1024, input gradient: 158 us at two, 144 at three, three registers spilled).
+// Four, at 128 registers, spill; the chunks of two steps in registers cost the third
+// workgroup (369900 x 256 -> 256 bf16 94 -> 113 us); tiles of 64 x 128 and 128 x 64
+// read more per product (114 and 104 us).
 template <typename T, Job kJob, int BM, int BN, bool kTight, bool kMask, bool kCodes>
-__global__ __launch_bounds__(kThreads, 2) void linear_product(const Product a) {
+__global__ __launch_bounds__(kThreads, (sizeof(T) == 4 && kTight) ? 3 : 2) void linear_product(const Product a) {
   constexpr int kV = Piece<T>::kValues;
   constexpr int kStep = Piece<T>::kStep;
   constexpr bool kF32 = sizeof(T) == 4;

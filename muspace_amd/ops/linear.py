@@ -142,7 +142,8 @@ def _forward(ext, input, weight, bias, residual, activation, rows, keep):
     output = input.new_empty((*input.shape[:-1], features))
     kept = None
     if keep and activation == 1:
-        kept = torch.empty((rows, (features + 7) // 8), dtype=torch.uint8, device=input.device)
+        kept = torch.empty(((features + 63) // 64, rows, 8), dtype=torch.uint8,
+                           device=input.device)
     elif keep and activation == 2:
         kept = input.new_empty((rows, features))
     ext.linear_forward_launch(input, weight, bias, residual, output, kept, activation, rows, cols,

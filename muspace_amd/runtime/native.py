@@ -1031,7 +1031,7 @@ class NativeLibrary:
 
     def _check_kept(self, like, kept, rows, out, activation) -> None:
         if activation == 1:
-            self._check_all(like, (torch.uint8,), (kept, "relu_mask", (rows, (out + 7) // 8)))
+            self._check_all(like, (torch.uint8,), (kept, "relu_mask", ((out + 63) // 64, rows, 8)))
         elif activation == 2:
             self._check_all(like, (like.dtype,), (kept, "pre_activation", (rows, out)))
         elif kept is not None:
