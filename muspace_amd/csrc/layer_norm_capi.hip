@@ -43,15 +43,15 @@ struct RowPlan {
   int lanes, chunks;
 };
 
+// The least lanes and pieces that hold a row, two rows to a wavefront from 65 to 96
+// pieces (77 pieces as 64 lanes by 2 leave 40% of the slots empty).
 RowPlan plan_row(int dtype, int64_t cols) {
   const int64_t n = ceil_div(cols, dtype == 0 ? 4 : 8);
-  if (n <= 16) return {16, 1};
-  if (n <= 32) return {32, 1};
-  if (n <= 64) return {64, 1};
-  if (n <= 128) return {64, 2};
-  if (n <= 256) return {64, 4};
-  if (n <= 512) return {256, 2};
-  if (n <= 2048) return {256, 8};
+  for (const RowPlan p : {RowPlan{16, 1}, RowPlan{32, 1}, RowPlan{64, 1}, RowPlan{32, 3},
+                          RowPlan{64, 2}, RowPlan{64, 3}, RowPlan{64, 4}, RowPlan{256, 2},
+                          RowPlan{256, 4}, RowPlan{256, 8}}) {
+    if (n <= p.lanes * p.chunks) return p;
+  }
   return {0, 0};
 }
 
@@ -64,10 +64,14 @@ int forward_blocks(const RowPlan &p, int64_t rows) {
   return static_cast<int>(want < most ? want : most);
 }
 
-// Workgroups of the backward; each leaves a row of column sums.
+// Workgroups of the backward; each leaves a row of column sums, so wide rows take
+// fewer: at 256 and 512, 20000 x 1024 bf16 28.6 and 31.5 us, 30021 x 611 float16 37.5
+// and 41.1, but 180000 x 256 bf16 59.1 and 58.0; a workgroup a row, at 512 and 1024,
+// 8000 x 4096 bf16 57 and 71.
 int backward_blocks(const RowPlan &p, int64_t rows) {
   if (p.lanes == 0) return static_cast<int>(rows < 64 ? rows : 64);
-  const int64_t most = p.lanes > 64 ? 1024 : 512, want = ceil_div(rows, rows_at_once(p));
+  const int64_t most = p.lanes <= 64 && p.chunks > 1 ? 256 : 512;
+  const int64_t want = ceil_div(rows, rows_at_once(p));
   return static_cast<int>(want < most ? want : most);
 }
 
@@ -111,16 +115,22 @@ template <typename T, bool kW32, bool kBackward>
 void launch(const RowPlan &p, const Norm &a, int blocks, hipStream_t st) {
   if (p.lanes == 16) {
     launch_full<T, kW32, kBackward, 16, 1>(a, blocks, st);
-  } else if (p.lanes == 32) {
+  } else if (p.lanes == 32 && p.chunks == 1) {
     launch_full<T, kW32, kBackward, 32, 1>(a, blocks, st);
+  } else if (p.lanes == 32) {
+    launch_full<T, kW32, kBackward, 32, 3>(a, blocks, st);
   } else if (p.lanes == 64 && p.chunks == 1) {
     launch_full<T, kW32, kBackward, 64, 1>(a, blocks, st);
   } else if (p.lanes == 64 && p.chunks == 2) {
     launch_full<T, kW32, kBackward, 64, 2>(a, blocks, st);
+  } else if (p.lanes == 64 && p.chunks == 3) {
+    launch_full<T, kW32, kBackward, 64, 3>(a, blocks, st);
   } else if (p.lanes == 64) {
     launch_full<T, kW32, kBackward, 64, 4>(a, blocks, st);
   } else if (p.chunks == 2) {
     launch_rows<T, kW32, kBackward, 256, 2, false>(a, blocks, st);
+  } else if (p.chunks == 4) {
+    launch_rows<T, kW32, kBackward, 256, 4, false>(a, blocks, st);
   } else {
     launch_rows<T, kW32, kBackward, 256, 8, false>(a, blocks, st);
   }

@@ -24,14 +24,38 @@ namespace dense {
 
 constexpr int kNormThreads = 512;
 
+// v plus the value of the lane at XOR kDistance, given that the lanes of each
+// aligned group of kDistance hold the same: moves within the vector unit, where a
+// shuffle would go through LDS and wait.
+template <int kDistance>
+__device__ __forceinline__ float add_across(float v) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  const int i = __float_as_int(v);
+  if constexpr (kDistance <= 8) {
+    // lanes 1 0 3 2, 2 3 0 1, mirrored halves of a row of 16, mirrored row
+    constexpr int kMove = kDistance == 1 ? 0xB1 : kDistance == 2 ? 0x4E
+                          : kDistance == 4 ? 0x141 : 0x140;
+    return v + __int_as_float(__builtin_amdgcn_mov_dpp(i, kMove, 0xf, 0xf, true));
+  } else if constexpr (kDistance == 16) {
+    const u32x2 r = __builtin_bit_cast(u32x2, __builtin_amdgcn_permlane16_swap(i, i, false, false));
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+  } else {
+    const u32x2 r = __builtin_bit_cast(u32x2, __builtin_amdgcn_permlane32_swap(i, i, false, false));
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+  }
+#else
+  return v;
+#endif
+}
+
 // kLanes lanes' sums, the same on all of them
 template <int kLanes, int N>
 __device__ __forceinline__ void group_sum(float (&v)[N], float *lds) {
-  constexpr int kIn = kLanes < kWave ? kLanes : kWave;
 #pragma unroll
-  for (int d = 1; d < kIn; d <<= 1) {
-#pragma unroll
-    for (int i = 0; i < N; ++i) v[i] += __shfl_xor(v[i], d);
+  for (int i = 0; i < N; ++i) {
+    v[i] = add_across<8>(add_across<4>(add_across<2>(add_across<1>(v[i]))));
+    if constexpr (kLanes >= 32) v[i] = add_across<16>(v[i]);
+    if constexpr (kLanes >= 64) v[i] = add_across<32>(v[i]);
   }
   if constexpr (kLanes > kWave) {
     // one row per workgroup: wavefront sums through LDS
@@ -91,6 +115,11 @@ struct NormShape {
   static constexpr int kGroups = kThreads / kLanes;  // rows at a time
 };
 
+// A lane's pieces of a row. All loads are unconditional, so that a row's are in
+// flight together: a piece that passes the row's end is read as the row's last 16
+// bytes and its values are moved to the front when it is used, rows past the last
+// read the last and count as zeros. kFull: the pieces end with the row. Rows shorter
+// than a piece are read value by value.
 template <typename T, int kLanes, int kChunks, bool kFull>
 struct RowPieces {
   static constexpr int kV = Piece<T>::kValues;
@@ -99,11 +128,27 @@ struct RowPieces {
   static __device__ __forceinline__ int left(int cols, int lane, int i) {
     return kFull ? kV : cols - (lane + i * kLanes) * kV;
   }
-  __device__ __forceinline__ void load(const T *row, int cols, int lane, bool any) {
+  __device__ __forceinline__ void load(const T *x, int64_t row, int64_t rows, int cols, int lane) {
+    const T *p = x + min(row, rows - 1) * cols;
+    if (kFull || cols >= kV) {
 #pragma unroll
-    for (int i = 0; i < kChunks; ++i) {
-      v[i] = loose_load<T>(row + (lane + i * kLanes) * kV, any ? left(cols, lane, i) : 0);
+      for (int i = 0; i < kChunks; ++i) {
+        const int col = (lane + i * kLanes) * kV;
+        v[i] = reinterpret_cast<const Loose16 *>(p + (kFull ? col : min(col, cols - kV)))->v;
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < kChunks; ++i) v[i] = loose_load<T>(p, i == 0 && lane == 0 ? cols : 0);
     }
+  }
+  // the piece's values, zeros past the row (and of no row: `any` false)
+  __device__ __forceinline__ void values(int i, int cols, int lane, bool any, float (&o)[kV]) const {
+    u32x4 w = v[i];
+    if (!kFull && cols >= kV) {
+      w = drop_front<T>(w, max((lane + i * kLanes + 1) * kV - cols, 0));
+    }
+    if (!any) w = u32x4{0, 0, 0, 0};
+    unpack<T>(w, o);
   }
 };
 
@@ -111,7 +156,7 @@ template <typename T, bool kW32, int kLanes, int kChunks, bool kFull>
 __global__ __launch_bounds__(NormShape<kLanes>::kThreads) void norm_forward(const Norm a) {
   using Shape = NormShape<kLanes>;
   constexpr int kV = Piece<T>::kValues;
-  constexpr bool kHold = kChunks <= 2;  // weight and bias stay in registers
+  constexpr bool kHold = kChunks <= 3;  // weight and bias stay in registers
   __shared__ float lds[16];
   using Pieces = RowPieces<T, kLanes, kChunks, kFull>;
   const int lane = threadIdx.x % kLanes;
@@ -130,14 +175,14 @@ __global__ __launch_bounds__(NormShape<kLanes>::kThreads) void norm_forward(cons
   const int64_t step = static_cast<int64_t>(gridDim.x) * Shape::kGroups;
   int64_t row = static_cast<int64_t>(blockIdx.x) * Shape::kGroups + threadIdx.x / kLanes;
   Pieces next;
-  next.load(x + row * a.cols, a.cols, lane, row < a.rows);
+  next.load(x, row, a.rows, a.cols, lane);
   // groups of one wavefront walk together: lanes past the last row take part in the
   // sums with zeros
   for (int64_t base = static_cast<int64_t>(blockIdx.x) * Shape::kGroups; base < a.rows;
        base += step, row += step) {
     float v[kChunks][kV];
 #pragma unroll
-    for (int i = 0; i < kChunks; ++i) unpack<T>(next.v[i], v[i]);
+    for (int i = 0; i < kChunks; ++i) next.values(i, a.cols, lane, row < a.rows, v[i]);
     const bool any = row < a.rows;
     float x0;
     if constexpr (kLanes > kWave) {
@@ -145,7 +190,7 @@ __global__ __launch_bounds__(NormShape<kLanes>::kThreads) void norm_forward(cons
     } else {
       x0 = __shfl(v[0][0], 0, kLanes);
     }
-    next.load(x + (row + step) * a.cols, a.cols, lane, row + step < a.rows);
+    next.load(x, row + step, a.rows, a.cols, lane);
     float sum[1] = {0.0f};
 #pragma unroll
     for (int i = 0; i < kChunks; ++i) {
@@ -191,7 +236,7 @@ template <typename T, bool kW32, int kLanes, int kChunks, bool kFull>
 __global__ __launch_bounds__(NormShape<kLanes>::kThreads) void norm_backward(const Norm a) {
   using Shape = NormShape<kLanes>;
   constexpr int kV = Piece<T>::kValues;
-  constexpr bool kHold = kChunks <= 2;
+  constexpr bool kHold = kChunks <= 3;
   constexpr int kCols = kLanes * kChunks * kV;
   using Pieces = RowPieces<T, kLanes, kChunks, kFull>;
   __shared__ float lds[Shape::kGroups > 1 ? Shape::kGroups * kCols : 16];
@@ -213,11 +258,11 @@ __global__ __launch_bounds__(NormShape<kLanes>::kThreads) void norm_backward(con
   Pieces nx, ng;
   float n_mean = 0.0f, n_s = 0.0f;
   auto fetch = [&](int64_t r) {
-    const bool any = r < a.rows;
-    nx.load(x + r * a.cols, a.cols, lane, any);
-    ng.load(g + r * a.cols, a.cols, lane, any);
-    n_mean = any ? a.stats[2 * r] : 0.0f;
-    n_s = any ? a.stats[2 * r + 1] : 0.0f;
+    nx.load(x, r, a.rows, a.cols, lane);
+    ng.load(g, r, a.rows, a.cols, lane);
+    const f32x2 stats = reinterpret_cast<const f32x2 *>(a.stats)[min(r, a.rows - 1)];
+    n_mean = stats[0];
+    n_s = stats[1];
   };
   fetch(row);
   for (int64_t base = static_cast<int64_t>(blockIdx.x) * Shape::kGroups; base < a.rows;
@@ -225,8 +270,8 @@ __global__ __launch_bounds__(NormShape<kLanes>::kThreads) void norm_backward(con
     float h[kChunks][kV], u[kChunks][kV];
 #pragma unroll
     for (int i = 0; i < kChunks; ++i) {
-      unpack<T>(nx.v[i], h[i]);
-      unpack<T>(ng.v[i], u[i]);
+      nx.values(i, a.cols, lane, row < a.rows, h[i]);
+      ng.values(i, a.cols, lane, row < a.rows, u[i]);
     }
     const bool any = row < a.rows;
     const float mean = n_mean, s = n_s;
