@@ -13,6 +13,7 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 from pathlib import Path
 
 PACKAGE_DIR = Path(__file__).resolve().parent
@@ -43,6 +44,10 @@ LIBRARY = PACKAGE_DIR / "native" / "libmuspace_msda.so"
 # loaded by the operators
 PROBE_SOURCES = (PACKAGE_DIR / "csrc" / "probes.hip",)
 PROBE_LIBRARY = PACKAGE_DIR / "native" / "libmuspace_probes.so"
+# autograd nodes of the layer's dense operators: host code against torch's C++ API,
+# no kernels (muspace_amd/runtime/layer_host.py loads it)
+HOST_SOURCES = (PACKAGE_DIR / "csrc" / "layer_host.cpp",)
+HOST_LIBRARY = PACKAGE_DIR / "native" / "muspace_layer_host.so"
 OFFLOAD_ARCH = "gfx950"
 
 # -packed-fp32-ops keeps the compiler from emitting packed fp32 VALU
@@ -77,27 +82,49 @@ def build_command(output: Path, sources=SOURCES) -> list[str]:
     return [hipcc(), *HIPCC_FLAGS, *(str(s) for s in sources), "-o", str(output)]
 
 
-def _compile(library: Path, sources, verbose: bool) -> Path:
+def host_command(output: Path) -> list[str]:
+    """The C++ compiler's command for the host module, with torch's own headers and ABI."""
+    import torch
+    from torch.utils import cpp_extension
+
+    rocm = os.environ.get("ROCM_PATH", "/opt/rocm")
+    includes = [*cpp_extension.include_paths(), sysconfig.get_paths()["include"],
+                f"{rocm}/include"]
+    abi = int(torch._C._GLIBCXX_USE_CXX11_ABI)
+    return [
+        os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared",
+        "-fvisibility=hidden", "-Wall", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
+        f"-D_GLIBCXX_USE_CXX11_ABI={abi}",
+        *(arg for path in includes for arg in ("-isystem", path)),
+        *(str(source) for source in HOST_SOURCES), "-o", str(output),
+        *(f"-L{path}" for path in cpp_extension.library_paths()),
+        "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_hip",
+    ]
+
+
+def _compile(library: Path, command, verbose: bool) -> Path:
+    """Run ``command(output)`` into a file beside ``library``, then move it there."""
     library.parent.mkdir(parents=True, exist_ok=True)
     tmp = library.with_name(library.name + f".tmp{os.getpid()}")
-    cmd = build_command(tmp, sources)
+    cmd = command(tmp)
     if verbose:
         print(" ".join(cmd), flush=True)
     proc = subprocess.run(cmd, capture_output=True, text=True)
     if proc.returncode != 0:
         tmp.unlink(missing_ok=True)
         raise RuntimeError(
-            f"hipcc failed ({proc.returncode}) building {library.name}:\n{proc.stderr[-4000:]}"
+            f"{Path(cmd[0]).name} failed ({proc.returncode}) building {library.name}:\n{proc.stderr[-4000:]}"
         )
     os.replace(tmp, library)
     return library
 
 
 def build(verbose: bool = False) -> Path:
-    """Compile the MSDA library and the probe library (always), each moved
-    into place atomically; returns the MSDA library's path."""
-    _compile(PROBE_LIBRARY, PROBE_SOURCES, verbose)
-    return _compile(LIBRARY, SOURCES, verbose)
+    """Compile the MSDA library, the probe library and the host module (always), each
+    moved into place atomically; returns the MSDA library's path."""
+    _compile(PROBE_LIBRARY, lambda out: build_command(out, PROBE_SOURCES), verbose)
+    _compile(HOST_LIBRARY, host_command, verbose)
+    return _compile(LIBRARY, build_command, verbose)
 
 
 def main(argv: list[str] | None = None) -> int:

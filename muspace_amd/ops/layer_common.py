@@ -1,4 +1,4 @@
-"""What the layer's dense operators share: backend choice, reports and checks."""
+"""What the layer's dense operators share: backend choice and reports."""
 
 from __future__ import annotations
 
@@ -14,24 +14,25 @@ from ..runtime.kernel_dispatch import (
     is_rocm_tensor,
     record_dispatch_report,
 )
-from ..runtime.native import NativeModuleUnavailable, load_native_module, native_error
+from ..runtime.layer_host import layer_host_error, load_layer_host
+from ..runtime.native import NativeModuleUnavailable
 
 DTYPES = (torch.float32, torch.float16, torch.bfloat16)
 
 
-def native_library():
-    """The loaded library (its bound methods, without a lookup by name per call), or None."""
+def _native():
     try:
-        return load_native_module()
+        return load_layer_host()
     except NativeModuleUnavailable:
         return None
 
 
 def require_native():
-    library = native_library()
-    if library is None:
-        raise RuntimeError(f"muSPACE HIP native library is unavailable: {native_error()}")
-    return library
+    """The host module with the operators' autograd nodes; RuntimeError without one."""
+    host = _native()
+    if host is None:
+        raise RuntimeError(f"muSPACE HIP native library is unavailable: {layer_host_error()}")
+    return host
 
 
 @lru_cache(maxsize=64)
@@ -42,27 +43,21 @@ def _native_report(operator: str, backend: str, device: str) -> DispatchReport:
     return DispatchReport(operator, backend, NATIVE_BACKEND, device, reason, True)
 
 
+def report_native(operator: str, input: torch.Tensor, backend: str) -> None:
+    record_dispatch_report(_native_report(operator, backend, input.device.type))
+
+
 def choose_native(operator: str, input: torch.Tensor, backend: str):
-    """The library if the call runs on the HIP kernels, None for the PyTorch path; the
-    choice is reported. Raises where neither may run."""
-    library = native_library()
-    if (library is not None and (backend == "auto" or backend in NATIVE_ALIASES)
+    """The host module if the call runs on the HIP kernels, None (reported) for the
+    PyTorch path. Raises, with a report, where neither may run."""
+    host = _native()
+    if (host is not None and (backend == "auto" or backend in NATIVE_ALIASES)
             and is_rocm_tensor(input)):
-        record_dispatch_report(_native_report(operator, backend, input.device.type))
-        return library
-    decision = explain_dispatch(input, backend=backend, native_available=library is not None)
+        return host
+    decision = explain_dispatch(input, backend=backend, native_available=host is not None)
     record_dispatch_report(DispatchReport(operator, backend, decision.backend, decision.device,
-                                          decision.reason, library is not None))
+                                          decision.reason, host is not None))
     if decision.backend == "error":
-        detail = native_error() if library is None and is_rocm_tensor(input) else None
+        detail = layer_host_error() if host is None and is_rocm_tensor(input) else None
         raise RuntimeError(f"{decision.reason}: {detail}" if detail else decision.reason)
     return None
-
-
-def check_device(input: torch.Tensor, *named) -> None:
-    """Every (tensor, name) on the input's device; None skipped."""
-    device = input.device
-    for tensor, name in named:
-        if tensor is not None and tensor.device != device:
-            raise RuntimeError(f"{name} must be a ROCm device tensor on {device} like the input, "
-                               f"got device {tensor.device}")

@@ -29,7 +29,7 @@ from torch.autograd.function import once_differentiable
 
 from ..runtime.kernel_dispatch import is_rocm_tensor
 from .layer_common import DTYPES as _DTYPES
-from .layer_common import check_device, choose_native, require_native
+from .layer_common import choose_native, report_native, require_native
 
 OPERATOR_NAME = "linear"
 BLOCK = 32  # values of a row that share a scale in an 8-bit checkpoint
@@ -60,10 +60,7 @@ def checkpoint_int8(input: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     rows = math.prod(input.shape[:-1])
     padded = (cols + BLOCK - 1) // BLOCK * BLOCK
     if is_rocm_tensor(input):
-        codes = torch.empty((rows, padded), dtype=torch.int8, device=input.device)
-        scales = torch.empty((rows, padded // BLOCK), dtype=torch.uint8, device=input.device)
-        require_native().linear_checkpoint_launch(input.contiguous(), codes, scales, rows, cols)
-        return codes, scales
+        return require_native().checkpoint(input.detach())
     low, high = _SCALE_RANGE[input.dtype]
     x = F.pad(input.reshape(rows, cols).float(), (0, padded - cols)).view(rows, -1, BLOCK)
     finite = torch.isfinite(x).all(-1, keepdim=True)
@@ -133,69 +130,7 @@ def linear_pytorch(input, weight, bias=None, *, activation=None, residual=None, 
     return out if residual is None else out + residual
 
 
-# ------------------------------------------------------------ native path ---
-
-
-def _forward(ext, input, weight, bias, residual, activation, rows, keep):
-    """The output, and what the gradient of the activation needs (``keep``)."""
-    features, cols = weight.shape
-    output = input.new_empty((*input.shape[:-1], features))
-    kept = None
-    if keep and activation == 1:
-        kept = torch.empty(((features + 63) // 64, rows, 8), dtype=torch.uint8,
-                           device=input.device)
-    elif keep and activation == 2:
-        kept = input.new_empty((rows, features))
-    ext.linear_forward_launch(input, weight, bias, residual, output, kept, activation, rows, cols,
-                              features)
-    return output, kept
-
-
-class _NativeLinearFunction(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, input, weight, bias, residual, activation, checkpoint):
-        ext = require_native()
-        need_input, need_weight, need_bias, _ = ctx.needs_input_grad[:4]
-        rows = math.prod(input.shape[:-1])
-        features, cols = weight.shape
-        needed = need_input or need_weight or need_bias
-        output, kept = _forward(ext, input, weight, bias, residual, activation, rows, needed)
-        codes = scales = None
-        if need_weight and checkpoint:
-            codes, scales = checkpoint_int8(input)
-        # all that the backward needs to know, looked up here: its thread runs Python slowly
-        ctx.launch = ext.linear_backward_launch if needed else None
-        ctx.plan = ext.linear_plan(input.dtype, rows, cols, features, activation)
-        ctx.shapes = (input.shape if need_input else None, weight.shape if need_weight else None,
-                      features if need_bias else None)
-        ctx.save_for_backward(input if need_weight and not checkpoint else None, codes, scales,
-                              weight if need_input else None, kept)
-        return output
-
-    @staticmethod
-    def backward(ctx, grad_output):
-        if torch.is_grad_enabled():  # create_graph: refuses a second differentiation
-            return _linear_backward_once(ctx, grad_output)
-        return _linear_backward(ctx, grad_output)
-
-
-def _linear_backward(ctx, grad_output):
-    grad_residual = grad_output if ctx.needs_input_grad[3] else None
-    if ctx.launch is None:
-        return None, None, None, grad_residual, None, None
-    input, codes, scales, weight, kept = ctx.saved_tensors
-    grad = grad_output.contiguous()
-    new = grad.new_empty
-    input_shape, weight_shape, bias_shape = ctx.shapes
-    grad_input = None if input_shape is None else new(input_shape)
-    grad_weight = None if weight_shape is None else new(weight_shape)
-    grad_bias = None if bias_shape is None else new(bias_shape)
-    ctx.launch(grad, input, codes, scales, weight, kept, grad_input, grad_weight, grad_bias,
-               ctx.plan)
-    return grad_input, grad_weight, grad_bias, grad_residual, None, None
-
-
-_linear_backward_once = once_differentiable(_linear_backward)
+# ---------------------------------------------------------------- operator ---
 
 
 def _validate(input, weight, bias, activation, residual, checkpoint) -> None:
@@ -244,22 +179,14 @@ def linear(
     once (no gradients of gradients) on the HIP path.
     """
     _validate(input, weight, bias, activation, residual, checkpoint)
-    ext = choose_native(OPERATOR_NAME, input, backend)
-    if ext is None:
+    host = choose_native(OPERATOR_NAME, input, backend)
+    if host is None:
         return linear_pytorch(input, weight, bias, activation=activation, residual=residual,
                               checkpoint=checkpoint)
-    check_device(input, (weight, "weight"), (bias, "bias"), (residual, "residual"))
-    input, weight = input.contiguous(), weight.contiguous()
-    bias = None if bias is None else bias.contiguous()
-    residual = None if residual is None else residual.contiguous()
-    code = ACTIVATIONS[activation]
-    if torch.is_grad_enabled() and (
-            input.requires_grad or weight.requires_grad
-            or (bias is not None and bias.requires_grad)
-            or (residual is not None and residual.requires_grad)):
-        return _NativeLinearFunction.apply(input, weight, bias, residual, code,
-                                           checkpoint is not None)
-    return _forward(ext, input, weight, bias, residual, code, math.prod(input.shape[:-1]), False)[0]
+    output = host.linear(input, weight, bias, residual, ACTIVATIONS[activation],
+                         checkpoint is not None)
+    report_native(OPERATOR_NAME, input, backend)
+    return output
 
 
 __all__ = ["checkpoint_int8", "checkpoint_restore", "linear", "linear_pytorch"]

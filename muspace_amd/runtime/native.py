@@ -294,9 +294,6 @@ class NativeLibrary:
         # scratch sizes by device and dims (a plan each, asked for several times a step)
         self._size = lru_cache(maxsize=1024)(self._workspace_size)
         self._dfa_scratch = lru_cache(maxsize=1024)(self._dfa_scratch_bytes)
-        self._linear_scratch = lru_cache(maxsize=1024)(self._raw["linear_backward_workspace_size"])
-        self._norm_scratch = lru_cache(maxsize=1024)(
-            self._raw["layer_norm_backward_workspace_size"])
         self._bound: dict[str, Callable[..., Any]] = {
             "check_forward": self.check_forward,
             "check_backward": self.check_backward,
@@ -329,15 +326,8 @@ class NativeLibrary:
             "linear_forward": self.linear_forward,
             "linear_checkpoint": self.linear_checkpoint,
             "linear_backward": self.linear_backward,
-            "linear_plan": self.linear_plan,
-            "linear_forward_launch": self.linear_forward_launch,
-            "linear_checkpoint_launch": self.linear_checkpoint_launch,
-            "linear_backward_launch": self.linear_backward_launch,
             "layer_norm_forward": self.layer_norm_forward,
             "layer_norm_backward": self.layer_norm_backward,
-            "layer_norm_plan": self.layer_norm_plan,
-            "layer_norm_forward_launch": self.layer_norm_forward_launch,
-            "layer_norm_backward_launch": self.layer_norm_backward_launch,
             "add_one": self.add_one,
         }
 
@@ -1018,9 +1008,8 @@ class NativeLibrary:
                            grad_mc_ms_feat, grad_sampling_location, grad_weights)
 
     # ------------------------------------------------- dense operators ---
-    # The operators make and check their tensors themselves and launch with plain
-    # addresses (`*_launch`): Python run by the backward's thread costs two to three
-    # times what it costs in the forward's. The tensor-level entries check first.
+    # Tensor-level entries of include/muspace_layer.h; the operators themselves launch
+    # from their C++ autograd nodes (runtime/layer_host.py).
     def _check_all(self, like, dtypes, *named) -> None:
         """Each (tensor, name, shape) a contiguous tensor on ``like``'s device with
         one of ``dtypes``; None skipped."""
@@ -1050,11 +1039,6 @@ class NativeLibrary:
                         (bias, "bias", (out,)), (residual, "residual", (*lead, out)),
                         (output, "output", (*lead, out)))
         self._check_kept(input, kept, rows, out, activation)
-        self.linear_forward_launch(input, weight, bias, residual, output, kept, activation, rows,
-                                   cols, out)
-
-    def linear_forward_launch(self, input, weight, bias, residual, output, kept, activation, rows,
-                              cols, out) -> None:
         kept_ptr = _ptr(kept)
         self._launch(
             "linear_forward", input.device,
@@ -1072,9 +1056,6 @@ class NativeLibrary:
         padded = (cols + 31) // 32 * 32
         self._check_all(input, (torch.int8,), (codes, "codes", (rows, padded)))
         self._check_all(input, (torch.uint8,), (scales, "scales", (rows, padded // 32)))
-        self.linear_checkpoint_launch(input, codes, scales, rows, cols)
-
-    def linear_checkpoint_launch(self, input, codes, scales, rows, cols) -> None:
         self._launch("linear_checkpoint", input.device, input.data_ptr(),
                      _DTYPE_CODES[input.dtype], codes.data_ptr(), scales.data_ptr(), rows, cols)
 
@@ -1095,20 +1076,8 @@ class NativeLibrary:
         self._check_all(grad_output, (torch.int8,), (codes, "codes", (rows, padded)))
         self._check_all(grad_output, (torch.uint8,), (scales, "scales", (rows, padded // 32)))
         self._check_kept(grad_output, kept, rows, out, activation)
-        self.linear_backward_launch(
-            grad_output, input, codes, scales, weight, kept, grad_input, grad_weight, grad_bias,
-            self.linear_plan(grad_output.dtype, rows, cols, out, activation))
-
-    def linear_plan(self, dtype, rows, cols, out, activation) -> tuple:
-        """What :meth:`linear_backward_launch` needs besides tensors: the last is
-        the workspace's size."""
-        code = _DTYPE_CODES[dtype]
-        return (code, rows, cols, out, activation,
-                self._linear_scratch(code, rows, cols, out, activation))
-
-    def linear_backward_launch(self, grad_output, input, codes, scales, weight, kept, grad_input,
-                               grad_weight, grad_bias, plan) -> None:
-        code, rows, cols, out, activation, nbytes = plan
+        code = _DTYPE_CODES[grad_output.dtype]
+        nbytes = self._raw["linear_backward_workspace_size"](code, rows, cols, out, activation)
         workspace = None
         if nbytes:
             workspace = torch.empty(nbytes, dtype=torch.uint8, device=grad_output.device)
@@ -1140,15 +1109,10 @@ class NativeLibrary:
         self._check_all(input, (input.dtype,), (output, "output", shape))
         self._check_all(input, (torch.float32,), (statistics, "statistics", (rows, 2)))
         dtype = self._norm_dtype(input, (weight, "weight"), (bias, "bias"))
-        self.layer_norm_forward_launch(input, weight, bias, dtype, output, statistics, rows, eps)
-
-    def layer_norm_forward_launch(self, input, weight, bias, weight_dtype, output, statistics,
-                                  rows, eps) -> None:
         self._launch(
             "layer_norm_forward", input.device,
             input.data_ptr(), _DTYPE_CODES[input.dtype], _ptr(weight), _ptr(bias),
-            _DTYPE_CODES[weight_dtype], output.data_ptr(), _ptr(statistics), rows,
-            input.shape[-1], eps,
+            _DTYPE_CODES[dtype], output.data_ptr(), _ptr(statistics), rows, shape[-1], eps,
         )
 
     def layer_norm_backward(self, grad_output, input, weight, statistics, grad_input, grad_weight,
@@ -1162,18 +1126,8 @@ class NativeLibrary:
         self._check_all(input, (torch.float32,), (statistics, "statistics", (rows, 2)))
         dtype = self._norm_dtype(input, (weight, "weight"), (grad_weight, "grad_weight"),
                                  (grad_bias, "grad_bias"))
-        self.layer_norm_backward_launch(grad_output, input, weight, statistics, grad_input,
-                                        grad_weight, grad_bias,
-                                        self.layer_norm_plan(input.dtype, dtype, rows, shape[-1]))
-
-    def layer_norm_plan(self, dtype, weight_dtype, rows, cols) -> tuple:
-        """What :meth:`layer_norm_backward_launch` needs besides tensors."""
-        code = _DTYPE_CODES[dtype]
-        return code, _DTYPE_CODES[weight_dtype], rows, cols, self._norm_scratch(code, rows, cols)
-
-    def layer_norm_backward_launch(self, grad_output, input, weight, statistics, grad_input,
-                                   grad_weight, grad_bias, plan) -> None:
-        code, weight_code, rows, cols, nbytes = plan
+        code = _DTYPE_CODES[input.dtype]
+        nbytes = self._raw["layer_norm_backward_workspace_size"](code, rows, shape[-1])
         workspace = None
         if grad_weight is None and grad_bias is None:
             nbytes = 0
@@ -1181,9 +1135,9 @@ class NativeLibrary:
             workspace = torch.empty(nbytes, dtype=torch.uint8, device=input.device)
         self._launch(
             "layer_norm_backward", input.device,
-            grad_output.data_ptr(), code, input.data_ptr(), _ptr(weight), weight_code,
+            grad_output.data_ptr(), code, input.data_ptr(), _ptr(weight), _DTYPE_CODES[dtype],
             statistics.data_ptr(), _ptr(grad_input), _ptr(grad_weight), _ptr(grad_bias), rows,
-            cols, _ptr(workspace), nbytes,
+            shape[-1], _ptr(workspace), nbytes,
         )
 
     def add_one(self, value, actual) -> None:
