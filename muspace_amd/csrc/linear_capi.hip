@@ -49,9 +49,22 @@ int chunk_values(int dtype) { return 16 / value_bytes(dtype); }
 int step_values(int dtype) { return dense::kRowBytes / value_bytes(dtype); }
 size_t pad256(size_t n) { return (n + 255) & ~static_cast<size_t>(255); }
 
-// Tiles of 128 x 128 where they give every CU one, else 64 x 64.
+// Tiles of 128 x 128 where they give every two CUs three, else 64 x 64. Forward, 64 and
+// 128: 10000 x 512 -> 256 (158 tiles of 128) bf16 8.7 and 10.7 us, 12000 x 256 -> 512
+// (376) 9.8 and 10.4, float32 26.0 and 26.8; 16000 x 256 -> 512 (500) 11.9 and 11.4,
+// float32 33.4 and 29.1; 24000 x 1024 -> 512 (752) 46 and 35, float32 161 and 137.
 bool large_tiles(int64_t m, int64_t n) {
-  return ceil_div(m, 128) * ceil_div(n, 128) >= kCus;
+  return ceil_div(m, 128) * ceil_div(n, 128) * 2 >= 3 * kCus;
+}
+
+// So few tiles of 64 x 64 that a workgroup for 32 x 32 results, its wavefronts sharing k,
+// is done sooner. With it and in tiles: 300 x 256 -> 256 (20 tiles) bf16 3.6 and 3.9 us,
+// float32 4.4 and 8.5; 900 x 1024 -> 256 (60) 6.5 and 8.1, float32 11.5 and 25.4; 1800 x
+// 256 -> 256 (116) 4.5 and 4.0, float32 6.3 and 8.8; 900 x 256 -> 1024 (240) 6.6 and 4.2,
+// float32 11.2 and 9.6.
+template <typename T>
+bool few_results(int64_t m, int64_t n) {
+  return ceil_div(m, 64) * ceil_div(n, 64) < (sizeof(T) == 4 ? 176 : 96);
 }
 
 struct WeightPlan {
@@ -122,7 +135,7 @@ void launch_few(const Product &a, bool tight, hipStream_t st) {
 
 template <typename T>
 void run_forward(Product a, bool tight, hipStream_t st) {
-  if (ceil_div(a.m, 64) * ceil_div(a.n, 64) < kCus) {
+  if (few_results<T>(a.m, a.n)) {
     a.tiles_n = static_cast<int>(ceil_div(a.n, 32));
     a.tiles = static_cast<int>(ceil_div(a.m, 32)) * a.tiles_n;
     launch_few<T, 4>(a, tight, st);
