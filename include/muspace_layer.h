@@ -6,7 +6,9 @@
  *
  * Tensors are device pointers, dense, row-major, all of one type: float32 (0),
  * float16 (1) or bfloat16 (2), unless noted. Products and statistics are summed
- * in float32, in a fixed order; every result is rounded once, to its type. Any
+ * in float32, in a fixed order; every result is rounded once, to its type. float32
+ * products of many rows read their operands to an absolute 2^-134 (magnitudes under
+ * 2^-109 keep fewer than float32's 24 bits). Any
  * sizes and any alignment of the type are allowed; rows of whole 16-byte pieces
  * on 16-byte boundaries are the fast case.
  *
@@ -24,6 +26,7 @@
  *               the byte is e + 127, or 255 where one of them is an infinity or
  *               NaN: such a block reads back as NaN. code * 2^e is a number of
  *               the tensors' type, so products read back exactly what is kept.
+ *               codes start on an 8-byte boundary.
  *
  * Conventions: launches are ordered on `stream`, on the current device; nothing
  * synchronises or allocates. Return 0 or a MUSPACE_E* code with

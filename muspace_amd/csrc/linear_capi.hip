@@ -237,6 +237,9 @@ int linear_checkpoint(const void *x, int dtype, int8_t *codes, uint8_t *scales, 
   if (x == nullptr || codes == nullptr || scales == nullptr) {
     return fail(MUSPACE_EINVAL, "linear_checkpoint: null tensor pointer");
   }
+  if (reinterpret_cast<uintptr_t>(codes) % 8 != 0) {
+    return fail(MUSPACE_EINVAL, "linear_checkpoint: codes must be 8-byte aligned");
+  }
   const int64_t work = rows * (((in_features + 31) & ~int64_t{31}) / chunk_values(dtype));
   hipStream_t st = static_cast<hipStream_t>(stream);
   by_type(dtype, [&](auto t) {
@@ -277,6 +280,9 @@ int linear_backward(const void *grad_output, int dtype, const void *x, const int
   const bool summed = rows > 0 && out_features > 0;  // dz has values
   if ((codes == nullptr) != (scales == nullptr)) {
     return fail(MUSPACE_EINVAL, "%s: codes and scales come together", fn);
+  }
+  if (reinterpret_cast<uintptr_t>(codes) % 8 != 0) {
+    return fail(MUSPACE_EINVAL, "%s: codes must be 8-byte aligned", fn);
   }
   if (summed &&
       (grad_output == nullptr || (want_input && weight == nullptr) ||

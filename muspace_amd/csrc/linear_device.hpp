@@ -8,7 +8,8 @@
 // |x2| <= 2^-8 |x| and |x3| <= 2^-16 |x|, and x3 what is left of 24 bits exactly.
 // Of the nine products those of planes i + j <= 4 are taken, six; the rest is
 // under 2^-23 |x y| for a product x y, the size of float32's own two roundings, and
-// of random sign. Infinities, NaN and numbers that round to an infinity in bfloat16
+// of random sign. bfloat16's smallest number is 2^-133, so float32 values keep an
+// absolute 2^-134: those under 2^-109 keep fewer than 24 bits. Infinities, NaN and numbers that round to an infinity in bfloat16
 // make such a sum an infinity or NaN: a tile with one in it is multiplied again
 // in float32.
 //

@@ -294,15 +294,18 @@ __device__ __forceinline__ float normal_cdf(float z, float &density) {
   return z < 0.0f ? tail : 1.0f - tail;
 }
 
+// z where the other factor is zero must be finite: infinite pre-activations (or kept ones
+// past float16's range) have the limits' value and slope. NaN stays, in the cdf.
 __device__ __forceinline__ float gelu(float z) {
   float density;
-  return z * normal_cdf(z, density);
+  const float cdf = normal_cdf(z, density);
+  return fmaxf(z, -64.0f) * cdf;
 }
 
 __device__ __forceinline__ float gelu_slope(float z) {
   float density;
   const float cdf = normal_cdf(z, density);
-  return fmaf(z * 0.39894228f, density, cdf);
+  return fmaf(fminf(fmaxf(z, -64.0f), 64.0f) * 0.39894228f, density, cdf);
 }
 
 // `left` values of bias from `p` on
@@ -401,7 +404,7 @@ __global__ __launch_bounds__(kThreads, (sizeof(T) == 4 && kTight) ? 3 : 2) void 
   }
   const int row0 = tile / a.tiles_n * BM, col0 = tile % a.tiles_n * BN;
   const int k_begin = split * a.k_split;
-  const int k_end = kJob == Job::kWeight ? min(a.k, k_begin + a.k_split) : a.k;
+  const int k_end = kJob == Job::kWeight && a.k - k_begin > a.k_split ? k_begin + a.k_split : a.k;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int wr = (wave >> 1) * WM, wc = (wave & 1) * WN;
 

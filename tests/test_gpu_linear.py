@@ -246,6 +246,40 @@ def test_infinities_and_nan_stay_in_their_rows_and_columns(size, dtype):
     assert db[3].isnan() and db[:3].isfinite().all() and db[4:].isfinite().all()
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows", [40, 30000])
+def test_gelu_far_from_zero(rows, dtype):
+    """Pre-activations past float16's range (kept as infinities there) and infinite ones:
+    the limits' values and slopes, not 0 * inf."""
+    x = torch.full((rows, 4), 200.0, device=DEV, dtype=dtype)
+    w = torch.tensor([[200.0] * 4, [-200.0] * 4, [3.0] * 4, [-3.0] * 4, [0.01] * 4], device=DEV).to(dtype)
+    xs, ws = leaves(x, w)
+    out = linear(xs, ws, activation="gelu")
+    g = torch.ones_like(out)
+    dx, dw = torch.autograd.grad(out, [xs, ws], g)
+    assert (out[:, 1] == 0).all() and (out[:, 3] == 0).all()
+    if dtype != torch.float16:
+        assert out.isfinite().all()
+    assert dw[1].eq(0).all() and dw[3].eq(0).all() and dx.isfinite().all()
+    x[5] = math.inf
+    out = linear(x, w, activation="gelu")
+    assert (out[5, [0, 2, 4]] == math.inf).all() and (out[5, [1, 3]] == 0).all()
+    x[5] = math.nan
+    assert linear(x, w, activation="gelu")[5].isnan().all()
+
+
+def test_float32_keeps_an_absolute_precision():
+    """Small float32 values: to 2^-134 each in the product of many rows, exact in few."""
+    for rows, step in ((20000, 2.0**-134), (50, 0.0)):
+        gen = torch.Generator(device=DEV).manual_seed(2)
+        x = torch.randn((rows, 64), generator=gen, device=DEV) * 2.0**-112
+        w = torch.randn((512, 64), generator=gen, device=DEV) * 2.0**90
+        out = linear(x, w)
+        results, bounds = dense_torch.linear(x, w, None, None, None)
+        slack = step * w.double().abs().sum(1)
+        assert_within(out, results[0], bounds[0] + slack, "small")
+
+
 @pytest.mark.parametrize("size", [(40, 40, 24), (9000, 72, 136), (257, 203, 131)], ids=str)
 def test_float32_over_its_whole_range(size):
     """float32 is multiplied as bfloat16 numbers: values past that type's range (finite in
@@ -417,6 +451,64 @@ def test_captured_step_replays(checkpoint):
         got = [t.clone() for t in captured]
         torch.cuda.synchronize()
         for a, e in zip(got, step()):
+            assert torch.equal(a, e)
+
+
+def test_two_graphs_share_a_pool():
+    """Two captured steps in one memory pool, replayed in turn: each has its own workspace
+    while it runs."""
+    x, w, b, _, g = make(20000, 96, 128, torch.bfloat16, seed=1)
+    y, v, c, _, h = make(20000, 128, 64, torch.bfloat16, seed=2)
+    sets = [(leaves(x, w, b), g), (leaves(y, v, c), h)]
+
+    def step(params, grad):
+        out = linear(*params, activation="relu", checkpoint="int8")
+        return [out.detach(), *torch.autograd.grad(out, params, grad)]
+
+    want = [step(*s) for s in sets]
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        for s in sets:
+            step(*s)
+    torch.cuda.current_stream().wait_stream(stream)
+    torch.cuda.synchronize()
+    graphs, results, pool = [], [], None
+    for s in sets:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, pool=pool):
+            results.append(step(*s))
+        pool = graph.pool()
+        graphs.append(graph)
+    for _ in range(3):
+        for graph, result, expected in zip(graphs, results, want):
+            graph.replay()
+            got = [t.clone() for t in result]
+            torch.cuda.synchronize()
+            for a, e in zip(got, expected):
+                assert torch.equal(a, e)
+            step(*sets[0])
+
+
+def test_streams_at_once():
+    """Calls in flight on two streams do not share scratch."""
+    x, w, b, _, g = make(60000, 128, 128, torch.bfloat16, seed=1)
+    xs, ws, bs = leaves(x, w, b)
+
+    def step():
+        return torch.autograd.grad(linear(xs, ws, bs, activation="gelu"), [xs, ws, bs], g)
+
+    want = step()
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = []
+    for _ in range(4):
+        for stream in streams:
+            with torch.cuda.stream(stream):
+                got.append(step())
+    torch.cuda.synchronize()
+    for grads in got:
+        for a, e in zip(grads, want):
             assert torch.equal(a, e)
 
 

@@ -236,6 +236,7 @@ def backward_args(**overrides):
         ({"weight": None}, "null tensor pointer"),
         ({"codes": FAR}, "codes and scales come together"),
         ({"scales": FAR}, "codes and scales come together"),
+        ({"codes": FAR + 4, "scales": FAR}, "8-byte aligned"),
         ({"activation": 1, "mask": None}, "null tensor pointer"),
         ({"activation": 2, "z": None}, "null tensor pointer"),
         ({"activation": 2, "workspace": None}, "workspace"),
@@ -266,6 +267,8 @@ def test_checkpoint_abi_refuses(native_lib):
     fn = native_lib.raw("linear_checkpoint")
     assert fn(FAR, 5, FAR, FAR, 4, 8, None) == 1
     assert fn(FAR, 0, FAR, FAR, -4, 8, None) == 1
+    assert fn(FAR, 0, FAR + 4, FAR, 4, 8, None) == 1
+    assert "8-byte aligned" in native_lib.last_error()
     assert fn(FAR, 0, None, FAR, 4, 8, None) == 1
     assert "null tensor pointer" in native_lib.last_error()
     assert fn(None, 0, None, None, 0, 8, None) == 0
@@ -305,6 +308,43 @@ def test_layer_norm_forward_abi_refuses(native_lib):
     assert fn(None, 0, None, None, 0, FAR, None, 4, 8, 1e-5, None) == 1
     assert "null tensor pointer" in native_lib.last_error()
     assert fn(None, 0, None, None, 0, None, None, 0, 8, 1e-5, None) == 0
+
+
+def test_host_module_missing_is_an_error(monkeypatch, tmp_path):
+    """A device call without the host module raises and says how to build it; CPU calls
+    keep the PyTorch path."""
+    from muspace_amd.ops import layer_common
+    from muspace_amd.runtime import layer_host
+
+    monkeypatch.setattr(layer_host, "module_path", lambda: tmp_path / "missing.so")
+    layer_host.load_layer_host.cache_clear()
+    try:
+        assert "python -m muspace_amd.build" in layer_host.layer_host_error()
+        with pytest.raises(RuntimeError, match="missing from this installation"):
+            layer_common.require_native()
+        monkeypatch.setattr(layer_common, "is_rocm_tensor", lambda t: True)
+        x = torch.zeros(2, 4)
+        monkeypatch.setattr("muspace_amd.runtime.kernel_dispatch.is_rocm_tensor", lambda t: True)
+        with pytest.raises(RuntimeError, match="missing from this installation"):
+            layer_norm(x)
+        assert get_last_dispatch_report().selected_backend == "error"
+    finally:
+        layer_host.load_layer_host.cache_clear()
+    monkeypatch.undo()
+    assert torch.equal(layer_norm(torch.zeros(2, 4)), torch.zeros(2, 4))
+    assert layer_host.load_layer_host() is layer_host.load_layer_host()
+
+
+def test_host_module_binds_every_entry(native_lib):
+    """The host module takes its entry points from the loaded library."""
+    from muspace_amd.runtime import layer_host, native
+
+    assert set(layer_host._BOUND) <= set(native._EXPORTS)
+    host = layer_host.load_layer_host()
+    with pytest.raises(Exception, match="linear_forward|map::at|at"):
+        host.bind({"muspace_last_error": 1})
+    layer_host.load_layer_host.cache_clear()  # a partial bind: load (and bind) anew
+    layer_host.load_layer_host()
 
 
 # ------------------------------------------------------------------ oracle ---
