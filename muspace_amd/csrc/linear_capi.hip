@@ -57,14 +57,17 @@ bool large_tiles(int64_t m, int64_t n) {
   return ceil_div(m, 128) * ceil_div(n, 128) * 2 >= 3 * kCus;
 }
 
-// So few tiles of 64 x 64 that a workgroup for 32 x 32 results, its wavefronts sharing k,
-// is done sooner. With it and in tiles: 300 x 256 -> 256 (20 tiles) bf16 3.6 and 3.9 us,
-// float32 4.4 and 8.5; 900 x 1024 -> 256 (60) 6.5 and 8.1, float32 11.5 and 25.4; 1800 x
-// 256 -> 256 (116) 4.5 and 4.0, float32 6.3 and 8.8; 900 x 256 -> 1024 (240) 6.6 and 4.2,
-// float32 11.2 and 9.6.
+// So few tiles of 64 x 64 that workgroups for 32 x 32 results, whose wavefronts share k,
+// are done sooner. With them and in tiles, forward: 300 x 256 -> 256 (20 tiles) bf16 3.4
+// and 3.8 us, float32 4.3 and 8.5; 1800 x 256 -> 256 (116) 4.0 and 4.0, float32 5.9 and
+// 8.8; 2400 x 256 -> 256 (152) 5.7 and 4.0, float32 8.4 and 8.8; 3000 x 1024 -> 256 (188)
+// 8.7 and 10.5, float32 21 and 26; 4000 x 1024 -> 256 (252) 10.6 and 11.2, float32 26.7
+// and 25.9; 1500 x 1024 -> 1024 (384) 15 and 11.5.
 template <typename T>
-bool few_results(int64_t m, int64_t n) {
-  return ceil_div(m, 64) * ceil_div(n, 64) < (sizeof(T) == 4 ? 176 : 96);
+bool few_results(int64_t m, int64_t n, int64_t k) {
+  const int64_t tiles = ceil_div(m, 64) * ceil_div(n, 64);
+  if (sizeof(T) == 4) return tiles < 208;
+  return tiles < (k >= 1024 ? 256 : 120);
 }
 
 struct WeightPlan {
@@ -124,24 +127,26 @@ void launch_product(Product a, bool large, bool tight, hipStream_t st) {
   }
 }
 
-template <typename T, int kWaves>
-void launch_few(const Product &a, bool tight, hipStream_t st) {
+template <typename T, Job kJob, bool kMask>
+void launch_few(Product a, bool tight, hipStream_t st) {
+  // four and eight: 64 x 2048 -> 2048 bf16 8.7 and 6.6 us, 300 x 256 -> 256 3.3 and 3.4
+  constexpr int kWaves = 8;
+  a.tiles_n = static_cast<int>(ceil_div(a.n, 32));
+  a.tiles = static_cast<int>(ceil_div(a.m, 32)) * a.tiles_n;
   if (tight) {
-    dense::linear_forward_few<T, kWaves, true><<<a.tiles, kWaves * 64, 0, st>>>(a);
+    dense::linear_few<T, kJob, kWaves, true, kMask><<<a.tiles, kWaves * 64, 0, st>>>(a);
   } else {
-    dense::linear_forward_few<T, kWaves, false><<<a.tiles, kWaves * 64, 0, st>>>(a);
+    dense::linear_few<T, kJob, kWaves, false, kMask><<<a.tiles, kWaves * 64, 0, st>>>(a);
   }
 }
 
-template <typename T>
-void run_forward(Product a, bool tight, hipStream_t st) {
-  if (few_results<T>(a.m, a.n)) {
-    a.tiles_n = static_cast<int>(ceil_div(a.n, 32));
-    a.tiles = static_cast<int>(ceil_div(a.m, 32)) * a.tiles_n;
-    launch_few<T, 4>(a, tight, st);
-    return;
+template <typename T, Job kJob, bool kMask>
+void run_rows(const Product &a, bool tight, hipStream_t st) {
+  if (few_results<T>(a.m, a.n, a.k)) {
+    launch_few<T, kJob, kMask>(a, tight, st);
+  } else {
+    launch_product<T, kJob, kMask, false>(a, large_tiles(a.m, a.n), tight, st);
   }
-  launch_product<T, Job::kForward, false, false>(a, large_tiles(a.m, a.n), tight, st);
 }
 
 template <typename T>
@@ -164,16 +169,6 @@ void run_weight(const Product &a, const WeightPlan &plan, bool tight, bool codes
         <<<static_cast<unsigned>(ceil_div(work, dense::kSumPieces)), dense::kThreads, 0, st>>>(
             a.partial, a.bias_partial, static_cast<T *>(dw), static_cast<T *>(db), a.m, a.n,
             plan.splits);
-  }
-}
-
-template <typename T>
-void run_input(const Product &a, bool tight, hipStream_t st) {
-  const bool large = large_tiles(a.m, a.n);
-  if (a.mask != nullptr) {
-    launch_product<T, Job::kInput, true, false>(a, large, tight, st);
-  } else {
-    launch_product<T, Job::kInput, false, false>(a, large, tight, st);
   }
 }
 
@@ -225,7 +220,7 @@ int linear_forward(const void *x, int dtype, const void *weight, const void *bia
   const bool tight =
       in_features % chunk_values(dtype) == 0 && aligned16(x) && aligned16(weight);
   hipStream_t st = static_cast<hipStream_t>(stream);
-  by_type(dtype, [&](auto t) { run_forward<decltype(t)>(a, tight, st); });
+  by_type(dtype, [&](auto t) { run_rows<decltype(t), Job::kForward, false>(a, tight, st); });
   return check_launch("linear_forward");
 }
 
@@ -331,7 +326,13 @@ int linear_backward(const void *grad_output, int dtype, const void *x, const int
     a.splits = 1;
     a.out = grad_input;
     const bool tight = whole_out && in_features % v == 0 && aligned16(weight);
-    by_type(dtype, [&](auto t) { run_input<decltype(t)>(a, tight, st); });
+    by_type(dtype, [&](auto t) {
+      if (mask != nullptr) {
+        run_rows<decltype(t), Job::kInput, true>(a, tight, st);
+      } else {
+        run_rows<decltype(t), Job::kInput, false>(a, tight, st);
+      }
+    });
   }
   if (want_weight || want_bias) {
     const WeightPlan plan = plan_weight(dtype, rows, in_features, out_features);

@@ -326,8 +326,9 @@ __device__ __forceinline__ uint32_t along_offset(int row, int c) {
 template <int R>
 __device__ __forceinline__ uint32_t across_offset(int k, int c) {
   // rows of 256 bytes (R = 128): pieces 2 k apart; of 128 bytes: two rows fill the
-  // banks, every second one is moved
-  const int key = R >= 128 ? (k & 3) << 1 : k & 2;
+  // banks, every second pair is moved; of 64 bytes: the four rows fill them
+  static_assert(R == 32 || R == 64 || R == 128, "a row's pieces are 2, 4 or 8");
+  const int key = R == 128 ? (k & 3) << 1 : R == 64 ? k & 2 : 0;
   return k * (R * 2) + ((((c >> 1) ^ key) << 1 | (c & 1)) << 4);
 }
 

@@ -1,9 +1,9 @@
 // Kernels of the dense layer (include/muspace_layer.h):
 //
-//   y  = act(x W^T + b) + r          linear_product<Job::kForward> / linear_forward_few
+//   y  = act(x W^T + b) + r          linear_product<Job::kForward> or linear_few
 //   dz = g * act'(x W^T + b)         on the fly from a bit mask (relu), or
 //                                    linear_gelu_grad (gelu, from the kept x W^T + b)
-//   dx = dz W                        linear_product<Job::kInput>
+//   dx = dz W                        linear_product<Job::kInput> or linear_few
 //   dW = dz^T x, db = sum of dz      linear_product<Job::kWeight> + linear_weight_sum
 //   x in 8 bits                      linear_checkpoint; read back by kWeight's loader
 //
@@ -62,20 +62,22 @@ __device__ __forceinline__ int xcd_order(int id, int count) {
 
 // --------------------------------------------------------- operand loader ---
 
-// One operand's R rows (of the result) by a step of k: kCount chunks per thread,
-// fetched into registers, then put into LDS. Loads are unconditional, so that all of
+// One operand's R rows (of the result) by a step of k: kCount chunks for each of kTeam
+// threads, fetched into registers, then put into LDS. Loads are unconditional, so that all of
 // a step's are in flight together. Rows off every alignment (!kTight): a chunk that
 // passes the end of its memory row is read as the row's last 16 bytes and its values
 // are moved to the front when it is used; rows past the operand read its last one,
 // which only marks results that are not stored (past k: zeros). Memory rows shorter
 // than a chunk are read value by value.
-template <typename T, bool kAlong, int R, bool kTight, bool kMask, bool kCodes>
+template <typename T, bool kAlong, int R, bool kTight, bool kMask, bool kCodes,
+          int kTeam = kThreads>
 struct Loader {
   static constexpr int kV = Piece<T>::kValues;
   static constexpr int kStep = Piece<T>::kStep;
-  static constexpr int kCount = R / 32;
-  static constexpr int kAcross = R / kV;              // chunks per k row (across)
-  static constexpr int kStride = kThreads / kAcross;  // k rows between a thread's chunks
+  static constexpr int kCount = R * 8 / kTeam;
+  static constexpr int kDown = kTeam / 8;          // rows between a thread's chunks (along)
+  static constexpr int kAcross = R / kV;           // chunks per k row (across)
+  static constexpr int kStride = kTeam / kAcross;  // k rows between a thread's chunks
 
   const T *ptr;
   const uint8_t *bytes;   // mask or scales
@@ -97,7 +99,7 @@ struct Loader {
     row0 = row0_;
     rows = rows_;
     k_end = k_end_;
-    const int t = threadIdx.x;
+    const int t = threadIdx.x % kTeam;
     if constexpr (kAlong) {
       r = t >> 3;
       c = t & 7;
@@ -129,7 +131,7 @@ struct Loader {
         const Source s = view(ptr, ld, row0, k0, rows);
 #pragma unroll
         for (int i = 0; i < kCount; ++i) {
-          const uint32_t off = static_cast<uint32_t>((r + 32 * i) * ld + c * kV) *
+          const uint32_t off = static_cast<uint32_t>((r + kDown * i) * ld + c * kV) *
                                static_cast<uint32_t>(sizeof(T));
           v[i] = tight_load(s, inside ? off : kPast);
         }
@@ -140,14 +142,14 @@ struct Loader {
         past = false;
 #pragma unroll
         for (int i = 0; i < kCount; ++i) {
-          const int64_t row = min(row0 + r + 32 * i, rows - 1);
+          const int64_t row = min(row0 + r + kDown * i, rows - 1);
           v[i] = reinterpret_cast<const Loose16 *>(ptr + row * ld + col)->v;
         }
       } else {
         moved = past = false;
 #pragma unroll
         for (int i = 0; i < kCount; ++i) {
-          const int64_t row = row0 + r + 32 * i;
+          const int64_t row = row0 + r + kDown * i;
           v[i] = loose_load<T>(ptr + row * ld + k0 + c * kV,
                                row < rows ? k_end - (k0 + c * kV) : 0);
         }
@@ -157,7 +159,7 @@ struct Loader {
         const uint8_t *b = bytes + (col >> 6) * bytes_ld + ((col >> 3) & 7);
 #pragma unroll
         for (int i = 0; i < kCount; ++i) {
-          side[i] = b[static_cast<int64_t>(min(row0 + r + 32 * i, rows - 1)) * 8];
+          side[i] = b[static_cast<int64_t>(min(row0 + r + kDown * i, rows - 1)) * 8];
         }
       }
     } else {
@@ -247,7 +249,7 @@ struct Loader {
     if constexpr (sizeof(T) == 4) {
       u32x2 part[kPlanes];
       split_chunk<kPlanes>(value, part);
-      const uint32_t at = (kAlong ? along_offset<64>(r + 32 * i, c >> 1)
+      const uint32_t at = (kAlong ? along_offset<64>(r + kDown * i, c >> 1)
                                   : across_offset<R>(r + i * kStride, c >> 1)) +
                           (c & 1) * 8;
 #pragma unroll
@@ -255,7 +257,7 @@ struct Loader {
         *reinterpret_cast<u32x2 *>(tile + e * kPlaneBytes + at) = part[e];
       }
     } else {
-      const uint32_t at = kAlong ? along_offset<128>(r + 32 * i, c)
+      const uint32_t at = kAlong ? along_offset<128>(r + kDown * i, c)
                                  : across_offset<R>(r + i * kStride, c);
       *reinterpret_cast<u32x4 *>(tile + at) = value;
     }
@@ -263,7 +265,7 @@ struct Loader {
 
   // float32 as it is, for the tiles that hold more than bfloat16's range
   __device__ __forceinline__ void put_f32(char *tile, int i, const u32x4 &value) const {
-    const uint32_t at = kAlong ? along_offset<128>(r + 32 * i, c)
+    const uint32_t at = kAlong ? along_offset<128>(r + kDown * i, c)
                                : static_cast<uint32_t>(((r + i * kStride) * R + c * 4) * 4);
     *reinterpret_cast<u32x4 *>(tile + at) = value;
   }
@@ -336,7 +338,7 @@ __device__ __forceinline__ void finish_forward(const Product &a, int64_t row, in
 #pragma unroll
     for (int i = 0; i < kV; ++i) {
       const bool keep = !(z[i] <= 0.0f);  // NaN stays NaN
-      bits |= (keep && i < left ? 1u : 0u) << i;
+      bits |= (keep ? 1u : 0u) << i;
       z[i] = keep ? z[i] : 0.0f;
     }
     if (a.mask_out != nullptr) {
@@ -616,74 +618,104 @@ __global__ __launch_bounds__(kThreads, (sizeof(T) == 4 && kTight) ? 3 : 2) void 
   }
 }
 
-// ---------------------------------------------------- forward, few results ---
+// ------------------------------------------------------------ few results ---
 
-// A workgroup makes 32 x 32 results with kWaves wavefronts that share k, chunks
-// straight from memory into the matrix instruction: nothing waits for another
-// wavefront until the sums are joined in LDS, in wavefront order.
-template <typename T, int kWaves, bool kTight>
-__global__ __launch_bounds__(kWaves * kWave) void linear_forward_few(const Product a) {
+// kForward and kInput where the tiles would leave most CUs idle: a workgroup makes 32 x
+// 32 results and its kWaves wavefronts take turns at the steps of k, each with its own
+// tiles in LDS, so that none waits for another until the sums are joined, in wavefront
+// order. float32 is multiplied as it is: the time is that of the loads.
+template <typename T, Job kJob, int kWaves, bool kTight, bool kMask>
+__global__ __launch_bounds__(kWaves *kWave) void linear_few(const Product a) {
   constexpr int kV = Piece<T>::kValues;
   constexpr int kStep = Piece<T>::kStep;
+  constexpr bool kF32 = sizeof(T) == 4;
+  constexpr bool kQAlong = kJob == Job::kForward;
+  using P = Loader<T, true, 32, kTight, kMask, false, kWave>;
+  using Q = Loader<T, kQAlong, 32, kTight, false, false, kWave>;
+  constexpr int kTile = 32 * kRowBytes;
   constexpr int kLd = 36;
-  __shared__ __attribute__((aligned(16))) float lds[kWaves][32 * kLd];
+  static_assert(32 * kLd * 4 <= 2 * kTile, "a wavefront's sums exceed its tiles");
+  __shared__ __attribute__((aligned(16))) char lds[kWaves * 2 * kTile];
   const int tile = xcd_order(blockIdx.x, gridDim.x);
   const int row0 = tile / a.tiles_n * 32, col0 = tile % a.tiles_n * 32;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const T *x = static_cast<const T *>(a.p) + static_cast<int64_t>(row0) * a.ldp;
-  const T *w = static_cast<const T *>(a.q) + static_cast<int64_t>(col0) * a.ldq;
-  const int r = lane & 31, h = lane >> 5;
-  const bool row_in = row0 + r < a.m, col_in = col0 + r < a.n;
+  char *const tile_p = lds + wave * 2 * kTile, *const tile_q = tile_p + kTile;
+  P p;
+  Q q;
+  p.init(a.p, a.ldp, a.mask, a.mask_ld, row0, a.m, a.k);
+  q.init(a.q, a.ldq, nullptr, 0, col0, a.n, a.k);
   f32x16 acc = {};
-  for (int k0 = wave * kStep; k0 < a.k; k0 += kWaves * kStep) {
-    u32x4 fp[4], fq[4];
-    if constexpr (kTight) {
-      using L = Loader<T, true, 32, true, false, false>;
-      const Source sp = L::view(x, a.ldp, 0, k0, a.m - row0);
-      const Source sq = L::view(w, a.ldq, 0, k0, a.n - col0);
+  int k0 = wave * kStep;
+  if (k0 < a.k) {
+    p.fetch(k0);
+    q.fetch(k0);
+  }
+  for (; k0 < a.k; k0 += kWaves * kStep) {
 #pragma unroll
-      for (int s = 0; s < 4; ++s) {
-        const int k = (2 * s + h) * kV;
-        const bool inside = k0 + k < a.k;
-        fp[s] = tight_load(sp, inside ? static_cast<uint32_t>((r * a.ldp + k) * sizeof(T)) : kPast);
-        fq[s] = tight_load(sq, inside ? static_cast<uint32_t>((r * a.ldq + k) * sizeof(T)) : kPast);
-      }
-    } else {
-#pragma unroll
-      for (int s = 0; s < 4; ++s) {
-        const int k = k0 + (2 * s + h) * kV;
-        fp[s] = loose_load<T>(x + r * a.ldp + k, row_in ? a.k - k : 0);
-        fq[s] = loose_load<T>(w + r * a.ldq + k, col_in ? a.k - k : 0);
+    for (int i = 0; i < P::kCount; ++i) {
+      if constexpr (kF32) {
+        p.put_f32(tile_p, i, p.chunk(i));
+      } else {
+        p.put(tile_p, i, p.chunk(i));
       }
     }
 #pragma unroll
-    for (int s = 0; s < 4; ++s) acc = multiply<T>(fq[s], fp[s], acc);
+    for (int i = 0; i < Q::kCount; ++i) {
+      if constexpr (kF32) {
+        q.put_f32(tile_q, i, q.chunk(i));
+      } else {
+        q.put(tile_q, i, q.chunk(i));
+      }
+    }
+    wave_lds_sync();
+    if (k0 + kWaves * kStep < a.k) {
+      p.fetch(k0 + kWaves * kStep);
+      q.fetch(k0 + kWaves * kStep);
+    }
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {
+      if constexpr (kF32) {
+        acc = multiply<T>(read_fragment_f32<kQAlong, 32>(tile_q, 0, s, lane),
+                          read_fragment_f32<true, 32>(tile_p, 0, s, lane), acc);
+      } else {
+        acc = multiply<T>(read_fragment<kQAlong, 32, 128>(tile_q, 0, s, lane),
+                          read_fragment<true, 32, 128>(tile_p, 0, s, lane), acc);
+      }
+    }
+    wave_lds_sync();
   }
+  float *const sums = reinterpret_cast<float *>(tile_p);
 #pragma unroll
   for (int g = 0; g < 4; ++g) {
     const f32x4 v = {acc[4 * g], acc[4 * g + 1], acc[4 * g + 2], acc[4 * g + 3]};
-    *reinterpret_cast<f32x4 *>(&lds[wave][r * kLd + 8 * g + 4 * h]) = v;
+    *reinterpret_cast<f32x4 *>(sums + (lane & 31) * kLd + 8 * g + 4 * (lane >> 5)) = v;
   }
   __syncthreads();
   constexpr int kLanes = 32 / kV;
   // whole wavefronts take part (the mask's halves are exchanged between lanes)
   for (int i = threadIdx.x; i < 32 * kLanes; i += kWaves * kWave) {
-    const int chunk = i % kLanes, rr = i / kLanes;
+    const int chunk = i % kLanes, r = i / kLanes;
     const int col = col0 + chunk * kV;
-    const int64_t row = row0 + rr;
+    const int64_t row = row0 + r;
     const int left = row < a.m ? a.n - col : 0;
-    float z[kV], b[kV] = {};
-    if (a.bias != nullptr) load_bias<T>(static_cast<const T *>(a.bias) + col, a.n - col, b);
-#pragma unroll
-    for (int e = 0; e < kV; ++e) z[e] = 0.0f;
+    float z[kV] = {};
 #pragma unroll
     for (int u = 0; u < kWaves; ++u) {
+      const float *src = reinterpret_cast<const float *>(lds + u * 2 * kTile) + r * kLd + chunk * kV;
 #pragma unroll
-      for (int e = 0; e < kV; ++e) z[e] += lds[u][rr * kLd + chunk * kV + e];
+      for (int e = 0; e < kV; ++e) z[e] += src[e];
     }
+    if constexpr (kJob == Job::kForward) {
+      if (a.bias != nullptr) {
+        float b[kV];
+        load_bias<T>(static_cast<const T *>(a.bias) + col, a.n - col, b);
 #pragma unroll
-    for (int e = 0; e < kV; ++e) z[e] += b[e];
-    finish_forward<T>(a, row, col, left, z);
+        for (int e = 0; e < kV; ++e) z[e] += b[e];
+      }
+      finish_forward<T>(a, row, col, left, z);
+    } else {
+      loose_store(static_cast<T *>(a.out) + row * a.n + col, pack<T>(z), left);
+    }
   }
 }
 
