@@ -4,6 +4,7 @@
 
 #include <climits>
 #include <cstdint>
+#include <type_traits>
 
 #include "../../include/muspace_layer.h"
 #include "capi_errors.hpp"
@@ -15,6 +16,7 @@ using capi::check_launch;
 using capi::fail;
 using capi::ok;
 using dense::Job;
+using dense::Kind;
 using dense::Product;
 
 constexpr int64_t kMaxRows = INT_MAX - 256;
@@ -48,6 +50,14 @@ int value_bytes(int dtype) { return dtype == 0 ? 4 : 2; }
 int chunk_values(int dtype) { return 16 / value_bytes(dtype); }
 int step_values(int dtype) { return dense::kRowBytes / value_bytes(dtype); }
 size_t pad256(size_t n) { return (n + 255) & ~static_cast<size_t>(255); }
+
+// gelu's dz in the workspace: rows of whole chunks, and a second tensor for what
+// rounding to 16 bits left
+int dz_tensors(int dtype) { return dtype == 0 ? 1 : 2; }
+int64_t dz_chunks(int dtype, int64_t out) { return ceil_div(out, chunk_values(dtype)); }
+size_t dz_bytes(int dtype, int64_t rows, int64_t out) {
+  return pad256(static_cast<size_t>(rows) * dz_chunks(dtype, out) * 16);
+}
 
 // Tiles of 128 x 128 where they give every two CUs three, else 64 x 64. Forward, 64 and
 // 128: 10000 x 512 -> 256 (158 tiles of 128) bf16 8.7 and 10.7 us, 12000 x 256 -> 512
@@ -102,18 +112,18 @@ size_t partial_bytes(const WeightPlan &p, int64_t in, int64_t out) {
          pad256(static_cast<size_t>(p.splits) * out * 4);
 }
 
-template <typename T, Job kJob, int B, bool kMask, bool kCodes>
+template <typename T, Job kJob, int B, Kind kKind, bool kCodes>
 void launch_tight(const Product &a, int blocks, bool tight, hipStream_t st) {
   if (tight) {
-    dense::linear_product<T, kJob, B, B, true, kMask, kCodes>
+    dense::linear_product<T, kJob, B, B, true, kKind, kCodes>
         <<<blocks, dense::kThreads, 0, st>>>(a);
   } else {
-    dense::linear_product<T, kJob, B, B, false, kMask, kCodes>
+    dense::linear_product<T, kJob, B, B, false, kKind, kCodes>
         <<<blocks, dense::kThreads, 0, st>>>(a);
   }
 }
 
-template <typename T, Job kJob, bool kMask, bool kCodes>
+template <typename T, Job kJob, Kind kKind, bool kCodes>
 void launch_product(Product a, bool large, bool tight, hipStream_t st) {
   const int b = large ? 128 : 64;
   a.tiles_n = static_cast<int>(ceil_div(a.n > 0 ? a.n : 1, b));
@@ -121,48 +131,61 @@ void launch_product(Product a, bool large, bool tight, hipStream_t st) {
   const int blocks = a.tiles * a.splits;
   if (blocks == 0) return;
   if (large) {
-    launch_tight<T, kJob, 128, kMask, kCodes>(a, blocks, tight, st);
+    launch_tight<T, kJob, 128, kKind, kCodes>(a, blocks, tight, st);
   } else {
-    launch_tight<T, kJob, 64, kMask, kCodes>(a, blocks, tight, st);
+    launch_tight<T, kJob, 64, kKind, kCodes>(a, blocks, tight, st);
   }
 }
 
-template <typename T, Job kJob, bool kMask>
+template <typename T, Job kJob, Kind kKind>
 void launch_few(Product a, bool tight, hipStream_t st) {
   // four and eight: 64 x 2048 -> 2048 bf16 8.7 and 6.6 us, 300 x 256 -> 256 3.3 and 3.4
   constexpr int kWaves = 8;
   a.tiles_n = static_cast<int>(ceil_div(a.n, 32));
   a.tiles = static_cast<int>(ceil_div(a.m, 32)) * a.tiles_n;
   if (tight) {
-    dense::linear_few<T, kJob, kWaves, true, kMask><<<a.tiles, kWaves * 64, 0, st>>>(a);
+    dense::linear_few<T, kJob, kWaves, true, kKind><<<a.tiles, kWaves * 64, 0, st>>>(a);
   } else {
-    dense::linear_few<T, kJob, kWaves, false, kMask><<<a.tiles, kWaves * 64, 0, st>>>(a);
+    dense::linear_few<T, kJob, kWaves, false, kKind><<<a.tiles, kWaves * 64, 0, st>>>(a);
   }
 }
 
-template <typename T, Job kJob, bool kMask>
+template <typename T, Job kJob, Kind kKind>
 void run_rows(const Product &a, bool tight, hipStream_t st) {
   if (few_results<T>(a.m, a.n, a.k)) {
-    launch_few<T, kJob, kMask>(a, tight, st);
+    launch_few<T, kJob, kKind>(a, tight, st);
   } else {
-    launch_product<T, kJob, kMask, false>(a, large_tiles(a.m, a.n), tight, st);
+    launch_product<T, kJob, kKind, false>(a, large_tiles(a.m, a.n), tight, st);
   }
+}
+
+// f(the kind of dz that `a` holds, as a type)
+template <typename T, typename F>
+void by_kind(const Product &a, F &&f) {
+  if (a.mask != nullptr) {
+    f(std::integral_constant<Kind, Kind::kMasked>{});
+    return;
+  }
+  if constexpr (sizeof(T) == 2) {
+    if (a.p_rest != nullptr) {
+      f(std::integral_constant<Kind, Kind::kPair>{});
+      return;
+    }
+  }
+  f(std::integral_constant<Kind, Kind::kPlain>{});
 }
 
 template <typename T>
 void run_weight(const Product &a, const WeightPlan &plan, bool tight, bool codes, void *dw, void *db,
                 hipStream_t st) {
-  if (a.mask != nullptr) {
+  by_kind<T>(a, [&](auto kind) {
+    constexpr Kind kKind = decltype(kind)::value;
     if (codes) {
-      launch_product<T, Job::kWeight, true, true>(a, plan.large, tight, st);
+      launch_product<T, Job::kWeight, kKind, true>(a, plan.large, tight, st);
     } else {
-      launch_product<T, Job::kWeight, true, false>(a, plan.large, tight, st);
+      launch_product<T, Job::kWeight, kKind, false>(a, plan.large, tight, st);
     }
-  } else if (codes) {
-    launch_product<T, Job::kWeight, false, true>(a, plan.large, tight, st);
-  } else {
-    launch_product<T, Job::kWeight, false, false>(a, plan.large, tight, st);
-  }
+  });
   if (plan.splits > 1) {
     const int64_t work = static_cast<int64_t>(a.m) * ((a.n + 7) / 8 * 2) + a.m;
     dense::linear_weight_sum<T>
@@ -220,7 +243,7 @@ int linear_forward(const void *x, int dtype, const void *weight, const void *bia
   const bool tight =
       in_features % chunk_values(dtype) == 0 && aligned16(x) && aligned16(weight);
   hipStream_t st = static_cast<hipStream_t>(stream);
-  by_type(dtype, [&](auto t) { run_rows<decltype(t), Job::kForward, false>(a, tight, st); });
+  by_type(dtype, [&](auto t) { run_rows<decltype(t), Job::kForward, Kind::kPlain>(a, tight, st); });
   return check_launch("linear_forward");
 }
 
@@ -255,7 +278,7 @@ size_t linear_backward_workspace_size(int dtype, int64_t rows, int64_t in_featur
   const WeightPlan plan = plan_weight(dtype, rows, in_features, out_features);
   size_t bytes = partial_bytes(plan, in_features, out_features);
   if (activation == dense::kGelu) {
-    bytes += pad256(static_cast<size_t>(rows) * out_features * value_bytes(dtype));
+    bytes += dz_tensors(dtype) * dz_bytes(dtype, rows, out_features);
   }
   return bytes;
 }
@@ -295,28 +318,33 @@ int linear_backward(const void *grad_output, int dtype, const void *x, const int
   }
   hipStream_t st = static_cast<hipStream_t>(stream);
   char *ws = static_cast<char *>(workspace);
-  const void *dz = grad_output;
+  const void *dz = grad_output, *dz_rest = nullptr;
+  const int v = chunk_values(dtype);
+  int64_t dz_ld = out_features;
   if (activation == dense::kGelu && summed) {
-    const int64_t count = rows * out_features;
+    const size_t bytes = dz_bytes(dtype, rows, out_features);
+    if (dz_tensors(dtype) == 2) dz_rest = ws + bytes;
+    dz_ld = dz_chunks(dtype, out_features) * v;
     by_type(dtype, [&](auto t) {
       using T = decltype(t);
       dense::linear_gelu_grad<T>
-          <<<grid_for(ceil_div(count, chunk_values(dtype))), dense::kThreads, 0, st>>>(
+          <<<grid_for(rows * dz_chunks(dtype, out_features)), dense::kThreads, 0, st>>>(
               static_cast<const T *>(grad_output), static_cast<const T *>(pre_activation),
-              reinterpret_cast<T *>(ws), count);
+              reinterpret_cast<T *>(ws), static_cast<T *>(const_cast<void *>(dz_rest)), rows,
+              static_cast<int>(out_features));
     });
     dz = ws;
-    ws += pad256(static_cast<size_t>(count) * value_bytes(dtype));
+    ws += dz_tensors(dtype) * bytes;
   }
-  const int v = chunk_values(dtype);
-  const bool whole_out = out_features % v == 0 && aligned16(dz);
+  const bool whole_out = dz_ld % v == 0 && aligned16(dz);
   const uint8_t *mask = activation == dense::kRelu && summed ? relu_mask : nullptr;
 
   if (want_input) {
     Product a = {};
     a.p = dz;
+    a.p_rest = dz_rest;
     a.q = weight;
-    a.ldp = out_features;
+    a.ldp = dz_ld;
     a.ldq = in_features;
     a.m = static_cast<int>(rows);
     a.n = static_cast<int>(in_features);
@@ -327,18 +355,18 @@ int linear_backward(const void *grad_output, int dtype, const void *x, const int
     a.out = grad_input;
     const bool tight = whole_out && in_features % v == 0 && aligned16(weight);
     by_type(dtype, [&](auto t) {
-      if (mask != nullptr) {
-        run_rows<decltype(t), Job::kInput, true>(a, tight, st);
-      } else {
-        run_rows<decltype(t), Job::kInput, false>(a, tight, st);
-      }
+      using T = decltype(t);
+      by_kind<T>(a, [&](auto kind) {
+        run_rows<T, Job::kInput, decltype(kind)::value>(a, tight, st);
+      });
     });
   }
   if (want_weight || want_bias) {
     const WeightPlan plan = plan_weight(dtype, rows, in_features, out_features);
     Product a = {};
     a.p = dz;
-    a.ldp = out_features;
+    a.p_rest = dz_rest;
+    a.ldp = dz_ld;
     a.m = static_cast<int>(out_features);
     // without a weight gradient: no columns, the first column of tiles sums dz
     a.n = want_weight ? static_cast<int>(in_features) : 0;

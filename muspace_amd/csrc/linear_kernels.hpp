@@ -34,6 +34,7 @@ enum Activation : int { kNone = 0, kRelu = 1, kGelu = 2 };
 
 struct Product {
   const void *p;         // rows of the result: x, dz or dz^T
+  const void *p_rest;    // what rounding left of p (gelu's dz in 16 bits)
   const void *q;         // columns: W, W^T or x
   int64_t ldp, ldq;      // values per row in memory
   int m, n, k;           // result rows, columns; summed index
@@ -69,9 +70,15 @@ __device__ __forceinline__ int xcd_order(int id, int count) {
 // are moved to the front when it is used; rows past the operand read its last one,
 // which only marks results that are not stored (past k: zeros). Memory rows shorter
 // than a chunk are read value by value.
-template <typename T, bool kAlong, int R, bool kTight, bool kMask, bool kCodes,
+// What an operand is besides its values in memory: relu's bits go with it (masked), or a
+// second tensor holds what rounding to 16 bits left of each value (pair: gelu's dz).
+enum class Kind { kPlain, kMasked, kPair };
+
+template <typename T, bool kAlong, int R, bool kTight, Kind kKind, bool kCodes,
           int kTeam = kThreads>
 struct Loader {
+  static constexpr bool kMask = kKind == Kind::kMasked;
+  static constexpr int kLoads = kKind == Kind::kPair && sizeof(T) == 2 ? 2 : 1;
   static constexpr int kV = Piece<T>::kValues;
   static constexpr int kStep = Piece<T>::kStep;
   static constexpr int kCount = R * 8 / kTeam;
@@ -79,7 +86,7 @@ struct Loader {
   static constexpr int kAcross = R / kV;           // chunks per k row (across)
   static constexpr int kStride = kTeam / kAcross;  // k rows between a thread's chunks
 
-  const T *ptr;
+  const T *ptr, *rest;    // rest: the pair's second tensor
   const uint8_t *bytes;   // mask or scales
   int64_t ld, bytes_ld;
   int row0, rows, k_end;  // first result row, their number in all, end of k
@@ -87,12 +94,14 @@ struct Loader {
   int skip;               // !kTight: values of the read chunk that are not its own
   bool moved, past;       // !kTight, uniform: some chunk has skip > 0, k past its end
   int k_at;
-  u32x4 v[kCount];
+  u32x4 v[kLoads][kCount];
   uint32_t side[kCount];  // mask byte or scale byte
 
-  __device__ __forceinline__ void init(const void *src, int64_t ld_, const uint8_t *b,
-                                       int64_t b_ld, int row0_, int rows_, int k_end_) {
+  __device__ __forceinline__ void init(const void *src, const void *rest_, int64_t ld_,
+                                       const uint8_t *b, int64_t b_ld, int row0_, int rows_,
+                                       int k_end_) {
     ptr = static_cast<const T *>(src);
+    rest = static_cast<const T *>(rest_);
     bytes = b;
     ld = ld_;
     bytes_ld = b_ld;
@@ -128,12 +137,15 @@ struct Loader {
     if constexpr (kAlong) {
       const bool inside = k0 + c * kV < k_end;
       if constexpr (kTight) {
-        const Source s = view(ptr, ld, row0, k0, rows);
 #pragma unroll
-        for (int i = 0; i < kCount; ++i) {
-          const uint32_t off = static_cast<uint32_t>((r + kDown * i) * ld + c * kV) *
-                               static_cast<uint32_t>(sizeof(T));
-          v[i] = tight_load(s, inside ? off : kPast);
+        for (int e = 0; e < kLoads; ++e) {
+          const Source s = view(e == 0 ? ptr : rest, ld, row0, k0, rows);
+#pragma unroll
+          for (int i = 0; i < kCount; ++i) {
+            const uint32_t off = static_cast<uint32_t>((r + kDown * i) * ld + c * kV) *
+                                 static_cast<uint32_t>(sizeof(T));
+            v[e][i] = tight_load(s, inside ? off : kPast);
+          }
         }
       } else if (k_end >= kV) {
         const int col = min(k0 + c * kV, k_end - kV);
@@ -142,16 +154,19 @@ struct Loader {
         past = false;
 #pragma unroll
         for (int i = 0; i < kCount; ++i) {
-          const int64_t row = min(row0 + r + kDown * i, rows - 1);
-          v[i] = reinterpret_cast<const Loose16 *>(ptr + row * ld + col)->v;
+          const int64_t at = static_cast<int64_t>(min(row0 + r + kDown * i, rows - 1)) * ld + col;
+          v[0][i] = reinterpret_cast<const Loose16 *>(ptr + at)->v;
+          if (kLoads == 2) v[kLoads - 1][i] = reinterpret_cast<const Loose16 *>(rest + at)->v;
         }
       } else {
         moved = past = false;
 #pragma unroll
         for (int i = 0; i < kCount; ++i) {
           const int64_t row = row0 + r + kDown * i;
-          v[i] = loose_load<T>(ptr + row * ld + k0 + c * kV,
-                               row < rows ? k_end - (k0 + c * kV) : 0);
+          const int64_t at = row * ld + k0 + c * kV;
+          const int left = row < rows ? k_end - (k0 + c * kV) : 0;
+          v[0][i] = loose_load<T>(ptr + at, left);
+          if (kLoads == 2) v[kLoads - 1][i] = loose_load<T>(rest + at, left);
         }
       }
       if constexpr (kMask) {
@@ -174,21 +189,24 @@ struct Loader {
           const uint32_t off = kr * static_cast<uint32_t>(ld) + c * kV;
           if constexpr (kV == 8) {
             const u32x2 w = tight_load8(s, inside ? off : kPast);
-            v[i][0] = w[0];
-            v[i][1] = w[1];
+            v[0][i][0] = w[0];
+            v[0][i][1] = w[1];
           } else {
-            v[i][0] = tight_load4(s, inside ? off : kPast);
+            v[0][i][0] = tight_load4(s, inside ? off : kPast);
           }
           side[i] = tight_load_byte(
               f, inside ? kr * static_cast<uint32_t>(bytes_ld) + (c * kV) / 32 : kPast);
         }
       } else if constexpr (kTight) {
-        const Source s = view(ptr, ld, k0, row0, k_end);
 #pragma unroll
-        for (int i = 0; i < kCount; ++i) {
-          const uint32_t off = static_cast<uint32_t>((r + i * kStride) * ld + c * kV) *
-                               static_cast<uint32_t>(sizeof(T));
-          v[i] = tight_load(s, inside ? off : kPast);
+        for (int e = 0; e < kLoads; ++e) {
+          const Source s = view(e == 0 ? ptr : rest, ld, k0, row0, k_end);
+#pragma unroll
+          for (int i = 0; i < kCount; ++i) {
+            const uint32_t off = static_cast<uint32_t>((r + i * kStride) * ld + c * kV) *
+                                 static_cast<uint32_t>(sizeof(T));
+            v[e][i] = tight_load(s, inside ? off : kPast);
+          }
         }
       } else if (rows >= kV) {
         const int col = min(row0 + c * kV, rows - kV);
@@ -198,16 +216,19 @@ struct Loader {
         k_at = k0;
 #pragma unroll
         for (int i = 0; i < kCount; ++i) {
-          const int64_t kr = min(k0 + r + i * kStride, k_end - 1);
-          v[i] = reinterpret_cast<const Loose16 *>(ptr + kr * ld + col)->v;
+          const int64_t at = static_cast<int64_t>(min(k0 + r + i * kStride, k_end - 1)) * ld + col;
+          v[0][i] = reinterpret_cast<const Loose16 *>(ptr + at)->v;
+          if (kLoads == 2) v[kLoads - 1][i] = reinterpret_cast<const Loose16 *>(rest + at)->v;
         }
       } else {
         moved = past = false;
 #pragma unroll
         for (int i = 0; i < kCount; ++i) {
           const int64_t kr = k0 + r + i * kStride;
-          v[i] = loose_load<T>(ptr + kr * ld + row0 + c * kV,
-                               kr < k_end ? rows - (row0 + c * kV) : 0);
+          const int64_t at = kr * ld + row0 + c * kV;
+          const int left = kr < k_end ? rows - (row0 + c * kV) : 0;
+          v[0][i] = loose_load<T>(ptr + at, left);
+          if (kLoads == 2) v[kLoads - 1][i] = loose_load<T>(rest + at, left);
         }
       }
       if constexpr (kMask) {
@@ -221,15 +242,15 @@ struct Loader {
     }
   }
 
-  // the fetched chunk as the product reads it
-  __device__ __forceinline__ u32x4 chunk(int i) const {
+  // the fetched chunk as the product reads it (`e`: of the pair's second tensor)
+  __device__ __forceinline__ u32x4 chunk(int i, int e = 0) const {
     if constexpr (kCodes) {
       uint32_t w[kV / 4];
-      w[0] = v[i][0];
-      if constexpr (kV == 8) w[1] = v[i][1];
+      w[0] = v[0][i][0];
+      if constexpr (kV == 8) w[1] = v[0][i][1];
       return decode<T>(w, scale_value(side[i]));
     } else {
-      u32x4 o = v[i];
+      u32x4 o = v[e][i];
       if constexpr (!kTight) {
         if (moved) o = drop_front<T>(o, skip);
         if (!kAlong && past && k_at + r + i * kStride >= k_end) o = u32x4{0, 0, 0, 0};
@@ -243,7 +264,7 @@ struct Loader {
   static constexpr int kRow = sizeof(T) == 4 ? 64 : 128;
   static constexpr int kPlaneBytes = R * kRow;
   // 8-bit codes need one plane: 7 bits
-  static constexpr int kPlanes = sizeof(T) == 4 ? (kCodes ? 1 : 3) : 1;
+  static constexpr int kPlanes = sizeof(T) == 4 ? (kCodes ? 1 : 3) : kLoads;
 
   __device__ __forceinline__ void put(char *tile, int i, const u32x4 &value) const {
     if constexpr (sizeof(T) == 4) {
@@ -379,7 +400,7 @@ __device__ __forceinline__ void finish_forward(const Product &a, int64_t row, in
 // Four, at 128 registers, spill; the chunks of two steps in registers cost the third
 // workgroup (369900 x 256 -> 256 bf16 94 -> 113 us); tiles of 64 x 128 and 128 x 64
 // read more per product (114 and 104 us).
-template <typename T, Job kJob, int BM, int BN, bool kTight, bool kMask, bool kCodes>
+template <typename T, Job kJob, int BM, int BN, bool kTight, Kind kKind, bool kCodes>
 __global__ __launch_bounds__(kThreads, (sizeof(T) == 4 && kTight) ? 3 : 2) void linear_product(const Product a) {
   constexpr int kV = Piece<T>::kValues;
   constexpr int kStep = Piece<T>::kStep;
@@ -388,8 +409,9 @@ __global__ __launch_bounds__(kThreads, (sizeof(T) == 4 && kTight) ? 3 : 2) void 
   constexpr bool kQAlong = kJob == Job::kForward;
   constexpr int WM = BM / 2, WN = BN / 2;  // a wavefront's quarter
   constexpr int kI = WM / 32, kJ = WN / 32;
-  using P = Loader<T, kPAlong, BM, kTight, kMask, false>;
-  using Q = Loader<T, kQAlong, BN, kTight, false, kCodes>;
+  // (the pair is this library's own tensor, its rows padded to whole chunks)
+  using P = Loader<T, kPAlong, BM, kTight || kKind == Kind::kPair, kKind, false>;
+  using Q = Loader<T, kQAlong, BN, kTight, Kind::kPlain, kCodes>;
   constexpr int kStageLd = WN + 4;  // floats; the pad spreads rows over the banks
   constexpr int kTiles = P::kPlanes * P::kPlaneBytes + Q::kPlanes * Q::kPlaneBytes;
   constexpr int kTilesF32 = kF32 ? (BM + BN) * kRowBytes : 0;
@@ -412,8 +434,8 @@ __global__ __launch_bounds__(kThreads, (sizeof(T) == 4 && kTight) ? 3 : 2) void 
 
   P p;
   Q q;
-  p.init(a.p, a.ldp, a.mask, a.mask_ld, row0, a.m, k_end);
-  q.init(a.q, a.ldq, a.scales, a.scale_ld, col0, a.n, k_end);
+  p.init(a.p, a.p_rest, a.ldp, a.mask, a.mask_ld, row0, a.m, k_end);
+  q.init(a.q, nullptr, a.ldq, a.scales, a.scale_ld, col0, a.n, k_end);
 
   f32x16 acc[kI][kJ];
   auto clear = [&]() {
@@ -437,16 +459,19 @@ __global__ __launch_bounds__(kThreads, (sizeof(T) == 4 && kTight) ? 3 : 2) void 
   for (int k0 = k_begin; k0 < k_end; k0 += kStep) {
 #pragma unroll
     for (int i = 0; i < P::kCount; ++i) {
-      const u32x4 v = p.chunk(i);
-      if constexpr (kJob == Job::kWeight) {
-        if (sum_p) {
-          float f[kV];
-          unpack<T>(v, f);
 #pragma unroll
-          for (int e = 0; e < kV; ++e) sums[e] += f[e];
+      for (int l = 0; l < P::kLoads; ++l) {
+        const u32x4 v = p.chunk(i, l);
+        if constexpr (kJob == Job::kWeight) {
+          if (sum_p) {
+            float f[kV];
+            unpack<T>(v, f);
+#pragma unroll
+            for (int e = 0; e < kV; ++e) sums[e] += f[e];
+          }
         }
+        p.put(tile_p + l * P::kPlaneBytes, i, v);
       }
-      p.put(tile_p, i, v);
     }
 #pragma unroll
     for (int i = 0; i < Q::kCount; ++i) q.put(tile_q, i, q.chunk(i));
@@ -624,26 +649,27 @@ __global__ __launch_bounds__(kThreads, (sizeof(T) == 4 && kTight) ? 3 : 2) void 
 // 32 results and its kWaves wavefronts take turns at the steps of k, each with its own
 // tiles in LDS, so that none waits for another until the sums are joined, in wavefront
 // order. float32 is multiplied as it is: the time is that of the loads.
-template <typename T, Job kJob, int kWaves, bool kTight, bool kMask>
+template <typename T, Job kJob, int kWaves, bool kTight, Kind kKind>
 __global__ __launch_bounds__(kWaves *kWave) void linear_few(const Product a) {
   constexpr int kV = Piece<T>::kValues;
   constexpr int kStep = Piece<T>::kStep;
   constexpr bool kF32 = sizeof(T) == 4;
   constexpr bool kQAlong = kJob == Job::kForward;
-  using P = Loader<T, true, 32, kTight, kMask, false, kWave>;
-  using Q = Loader<T, kQAlong, 32, kTight, false, false, kWave>;
+  using P = Loader<T, true, 32, kTight || kKind == Kind::kPair, kKind, false, kWave>;
+  using Q = Loader<T, kQAlong, 32, kTight, Kind::kPlain, false, kWave>;
   constexpr int kTile = 32 * kRowBytes;
+  constexpr int kTiles = (P::kLoads + 1) * kTile;  // of a wavefront
   constexpr int kLd = 36;
-  static_assert(32 * kLd * 4 <= 2 * kTile, "a wavefront's sums exceed its tiles");
-  __shared__ __attribute__((aligned(16))) char lds[kWaves * 2 * kTile];
+  static_assert(32 * kLd * 4 <= kTiles, "a wavefront's sums exceed its tiles");
+  __shared__ __attribute__((aligned(16))) char lds[kWaves * kTiles];
   const int tile = xcd_order(blockIdx.x, gridDim.x);
   const int row0 = tile / a.tiles_n * 32, col0 = tile % a.tiles_n * 32;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  char *const tile_p = lds + wave * 2 * kTile, *const tile_q = tile_p + kTile;
+  char *const tile_p = lds + wave * kTiles, *const tile_q = tile_p + P::kLoads * kTile;
   P p;
   Q q;
-  p.init(a.p, a.ldp, a.mask, a.mask_ld, row0, a.m, a.k);
-  q.init(a.q, a.ldq, nullptr, 0, col0, a.n, a.k);
+  p.init(a.p, a.p_rest, a.ldp, a.mask, a.mask_ld, row0, a.m, a.k);
+  q.init(a.q, nullptr, a.ldq, nullptr, 0, col0, a.n, a.k);
   f32x16 acc = {};
   int k0 = wave * kStep;
   if (k0 < a.k) {
@@ -656,7 +682,8 @@ __global__ __launch_bounds__(kWaves *kWave) void linear_few(const Product a) {
       if constexpr (kF32) {
         p.put_f32(tile_p, i, p.chunk(i));
       } else {
-        p.put(tile_p, i, p.chunk(i));
+#pragma unroll
+        for (int l = 0; l < P::kLoads; ++l) p.put(tile_p + l * kTile, i, p.chunk(i, l));
       }
     }
 #pragma unroll
@@ -678,8 +705,11 @@ __global__ __launch_bounds__(kWaves *kWave) void linear_few(const Product a) {
         acc = multiply<T>(read_fragment_f32<kQAlong, 32>(tile_q, 0, s, lane),
                           read_fragment_f32<true, 32>(tile_p, 0, s, lane), acc);
       } else {
-        acc = multiply<T>(read_fragment<kQAlong, 32, 128>(tile_q, 0, s, lane),
-                          read_fragment<true, 32, 128>(tile_p, 0, s, lane), acc);
+        const u32x4 fq = read_fragment<kQAlong, 32, 128>(tile_q, 0, s, lane);
+#pragma unroll
+        for (int l = 0; l < P::kLoads; ++l) {
+          acc = multiply<T>(fq, read_fragment<true, 32, 128>(tile_p + l * kTile, 0, s, lane), acc);
+        }
       }
     }
     wave_lds_sync();
@@ -701,7 +731,7 @@ __global__ __launch_bounds__(kWaves *kWave) void linear_few(const Product a) {
     float z[kV] = {};
 #pragma unroll
     for (int u = 0; u < kWaves; ++u) {
-      const float *src = reinterpret_cast<const float *>(lds + u * 2 * kTile) + r * kLd + chunk * kV;
+      const float *src = reinterpret_cast<const float *>(lds + u * kTiles) + r * kLd + chunk * kV;
 #pragma unroll
       for (int e = 0; e < kV; ++e) z[e] += src[e];
     }
@@ -777,23 +807,58 @@ __global__ __launch_bounds__(kThreads) void linear_weight_sum(const float *parti
 
 // ------------------------------------------------------------- elementwise ---
 
-// dz = g * gelu'(z), z the kept pre-activation. dz is rounded to the tensors'
-// type: it is an operand of two matrix products.
+// i / d and i % d, with the short division where it holds
+__device__ __forceinline__ int64_t divide(int64_t i, int d, int &rest) {
+  if (i < (int64_t{1} << 32)) {
+    const uint32_t n = static_cast<uint32_t>(i), q = n / static_cast<uint32_t>(d);
+    rest = static_cast<int>(n - q * static_cast<uint32_t>(d));
+    return q;
+  }
+  const int64_t q = i / d;
+  rest = static_cast<int>(i - q * d);
+  return q;
+}
+
+// dz = g * gelu'(z), z the kept pre-activation. dz is an operand of two matrix products;
+// in a 16-bit type it is written as two numbers, itself rounded and what the rounding
+// left, which the products add: rounded once, dz would cost the gradients as much
+// precision again as their own rounding does. A dz past the type's range becomes its
+// largest number and the rest. Rows are padded with zeros to whole chunks, which the
+// products then read as if they were aligned, whatever the number of columns.
 template <typename T>
-__global__ __launch_bounds__(kThreads) void linear_gelu_grad(const T *g, const T *z, T *dz,
-                                                             int64_t count) {
+__global__ __launch_bounds__(kThreads) void linear_gelu_grad(const T *g, const T *z, T *dz, T *rest,
+                                                             int64_t rows, int cols) {
   constexpr int kV = Piece<T>::kValues;
-  const int64_t chunks = (count + kV - 1) / kV;
+  constexpr float kLargest = std::is_same_v<T, __half> ? 65504.0f : 3.38953139e38f;
+  const int per_row = (cols + kV - 1) / kV;
+  const int64_t chunks = rows * per_row;
   for (int64_t i = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x; i < chunks;
        i += static_cast<int64_t>(gridDim.x) * kThreads) {
-    const int64_t at = i * kV;
-    const int left = count - at < kV ? static_cast<int>(count - at) : kV;
+    int chunk;
+    const int64_t row = divide(i, per_row, chunk);
+    const int col = chunk * kV;
     float a[kV], b[kV];
-    unpack<T>(loose_load<T>(g + at, left), a);
-    unpack<T>(loose_load<T>(z + at, left), b);
+    unpack<T>(loose_load<T>(g + row * cols + col, cols - col), a);
+    unpack<T>(loose_load<T>(z + row * cols + col, cols - col), b);
 #pragma unroll
     for (int e = 0; e < kV; ++e) a[e] *= gelu_slope(b[e]);
-    loose_store(dz + at, pack<T>(a), left);
+    u32x4 *const to = reinterpret_cast<u32x4 *>(dz) + i;
+    if constexpr (sizeof(T) == 2) {
+      float h[kV];
+#pragma unroll
+      for (int e = 0; e < kV; ++e) {
+        // infinities and NaN stay what they are
+        h[e] = fabsf(a[e]) < INFINITY ? fminf(fmaxf(a[e], -kLargest), kLargest) : a[e];
+      }
+      const u32x4 w = pack<T>(h);
+      *to = w;
+      unpack<T>(w, h);
+#pragma unroll
+      for (int e = 0; e < kV; ++e) a[e] = fabsf(a[e]) < INFINITY ? a[e] - h[e] : 0.0f;
+      reinterpret_cast<u32x4 *>(rest)[i] = pack<T>(a);
+    } else {
+      *to = pack<T>(a);
+    }
   }
 }
 
@@ -817,8 +882,9 @@ __global__ __launch_bounds__(kThreads) void linear_checkpoint(const T *x, uint8_
   // per_row and the launch's stride are multiples of kGroup: a block's lanes stay together
   for (int64_t i = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x; i < chunks;
        i += static_cast<int64_t>(gridDim.x) * kThreads) {
-    const int64_t row = i / per_row;
-    const int col = static_cast<int>(i - row * per_row) * kV;
+    int chunk;
+    const int64_t row = divide(i, per_row, chunk);
+    const int col = chunk * kV;
     float v[kV];
     unpack<T>(loose_load<T>(x + row * cols + col, cols - col), v);
     uint32_t top = 0;

@@ -90,9 +90,9 @@ def linear(x, weight, bias, activation, residual, grad=None, kept=None):
     dz_err = torch.zeros_like(dz)
     if activation == "gelu":
         # the kept z is rounded to the type (|slope'| < 0.8), the slope is a float32
-        # function of it, dz is rounded to the type
+        # function of it, dz is held to twice the type's bits (float32's at most)
         dz_err = g.abs() * (0.8 * (z_err + u * z.abs() + small) + 16 * SUM_STEP)
-        dz_err = dz_err * (1 + u) + u * dz.abs() + small
+        dz_err = dz_err + max(u * u, SUM_STEP) * dz.abs() + small
     dx = dz @ w
     dx_err = (dz_err @ w.abs()
               + (w.shape[0] + 2) * SUM_STEP * ((dz.abs() + dz_err) @ w.abs()))
