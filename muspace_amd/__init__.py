@@ -3,7 +3,9 @@
 The exports mirror the MSDA part of the reference package
 (/root/reference/mu_space/__init__.py:36,54-59): the canonical operator, its
 dispatch explanation and the dispatch-report accessors. ``import muspace_amd
-as mu_space`` gives code written against the reference the same names.
+as mu_space`` gives code written against the reference the same names. Next to
+them stand the dense operators of an attention layer (``linear``, its 8-bit
+checkpoints, ``layer_norm``), which the reference leaves to torch.
 """
 
 from .ops import (

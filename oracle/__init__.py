@@ -21,6 +21,9 @@ Contents
   msda_softmax.py the operator with its weights given as logits (softmax over
                   each query's L*P samples per head, then msda_torch); autograd
                   and a closed-form logit gradient (tests/test_oracle_softmax.py).
+  dense_torch.py  linear (with its 8-bit input checkpoint) and layer norm with their
+                  gradients in float64 from the formulas, and worst-case error bounds
+                  of a float32 implementation (tests/test_layer_operators.py).
 
 How each function is pinned (tests/test_oracle.py)
   * msda_torch vs msda_direct (two independent formulations) at float64;
