@@ -31,7 +31,8 @@
  * Conventions: launches are ordered on `stream`, on the current device; nothing
  * synchronises or allocates. Return 0 or a MUSPACE_E* code with
  * muspace_last_error() set (muspace_msda.h). rows may be 0 (gradients of weight
- * and bias are then zero). in, out at most 2^20; rows below 2^31 - 256.
+ * and bias are then zero). in, out at most 2^20; rows below 2^31 - 256; any
+ * two of them over at most 2^24 tiles of 128 x 128 (MUSPACE_ERANGE otherwise).
  */
 #ifndef MUSPACE_LAYER_H_
 #define MUSPACE_LAYER_H_

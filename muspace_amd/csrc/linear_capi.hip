@@ -35,10 +35,11 @@ int validate(const char *fn, int dtype, int64_t rows, int64_t in, int64_t out, i
     return fail(MUSPACE_EINVAL, "%s: activation must be 0 (none), 1 (relu) or 2 (gelu), got %d",
                 fn, act);
   }
-  // the tiles of the smallest size, over any two of the three dimensions
-  const int64_t r = rows / 32 + 1, i = in / 32 + 1, o = out / 32 + 1;
-  if (rows > kMaxRows || in > kMaxFeatures || out > kMaxFeatures || r * i > INT_MAX ||
-      r * o > INT_MAX) {
+  // a launch holds fewer than 2^32 threads: 2^24 tiles of 128 x 128
+  const int64_t r = rows / 128 + 1, i = in / 128 + 1, o = out / 128 + 1;
+  constexpr int64_t kTiles = 1 << 24;
+  if (rows > kMaxRows || in > kMaxFeatures || out > kMaxFeatures || r * i > kTiles ||
+      r * o > kTiles || i * o > kTiles) {
     return fail(MUSPACE_ERANGE, "%s: dims exceed the kernels' 32-bit indexing", fn);
   }
   return ok();

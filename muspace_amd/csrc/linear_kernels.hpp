@@ -78,7 +78,8 @@ template <typename T, bool kAlong, int R, bool kTight, Kind kKind, bool kCodes,
           int kTeam = kThreads>
 struct Loader {
   static constexpr bool kMask = kKind == Kind::kMasked;
-  static constexpr int kLoads = kKind == Kind::kPair && sizeof(T) == 2 ? 2 : 1;
+  static constexpr int kLoads = kKind == Kind::kPair ? 2 : 1;
+  static_assert(kKind != Kind::kPair || (sizeof(T) == 2 && kTight), "the pair's rows are whole");
   static constexpr int kV = Piece<T>::kValues;
   static constexpr int kStep = Piece<T>::kStep;
   static constexpr int kCount = R * 8 / kTeam;
@@ -154,19 +155,16 @@ struct Loader {
         past = false;
 #pragma unroll
         for (int i = 0; i < kCount; ++i) {
-          const int64_t at = static_cast<int64_t>(min(row0 + r + kDown * i, rows - 1)) * ld + col;
-          v[0][i] = reinterpret_cast<const Loose16 *>(ptr + at)->v;
-          if (kLoads == 2) v[kLoads - 1][i] = reinterpret_cast<const Loose16 *>(rest + at)->v;
+          const int64_t row = min(row0 + r + kDown * i, rows - 1);
+          v[0][i] = reinterpret_cast<const Loose16 *>(ptr + row * ld + col)->v;
         }
       } else {
         moved = past = false;
 #pragma unroll
         for (int i = 0; i < kCount; ++i) {
           const int64_t row = row0 + r + kDown * i;
-          const int64_t at = row * ld + k0 + c * kV;
-          const int left = row < rows ? k_end - (k0 + c * kV) : 0;
-          v[0][i] = loose_load<T>(ptr + at, left);
-          if (kLoads == 2) v[kLoads - 1][i] = loose_load<T>(rest + at, left);
+          v[0][i] = loose_load<T>(ptr + row * ld + k0 + c * kV,
+                                  row < rows ? k_end - (k0 + c * kV) : 0);
         }
       }
       if constexpr (kMask) {
@@ -216,19 +214,16 @@ struct Loader {
         k_at = k0;
 #pragma unroll
         for (int i = 0; i < kCount; ++i) {
-          const int64_t at = static_cast<int64_t>(min(k0 + r + i * kStride, k_end - 1)) * ld + col;
-          v[0][i] = reinterpret_cast<const Loose16 *>(ptr + at)->v;
-          if (kLoads == 2) v[kLoads - 1][i] = reinterpret_cast<const Loose16 *>(rest + at)->v;
+          const int64_t kr = min(k0 + r + i * kStride, k_end - 1);
+          v[0][i] = reinterpret_cast<const Loose16 *>(ptr + kr * ld + col)->v;
         }
       } else {
         moved = past = false;
 #pragma unroll
         for (int i = 0; i < kCount; ++i) {
           const int64_t kr = k0 + r + i * kStride;
-          const int64_t at = kr * ld + row0 + c * kV;
-          const int left = kr < k_end ? rows - (row0 + c * kV) : 0;
-          v[0][i] = loose_load<T>(ptr + at, left);
-          if (kLoads == 2) v[kLoads - 1][i] = loose_load<T>(rest + at, left);
+          v[0][i] = loose_load<T>(ptr + kr * ld + row0 + c * kV,
+                                  kr < k_end ? rows - (row0 + c * kV) : 0);
         }
       }
       if constexpr (kMask) {

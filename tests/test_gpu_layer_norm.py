@@ -209,3 +209,55 @@ def test_refused_on_the_device():
     x, w, b, g = make(8, 16, torch.float32)
     with pytest.raises(RuntimeError, match="weight must be a ROCm device tensor"):
         layer_norm(x, w.cpu(), b.cpu())
+
+
+def test_tensor_level_entries(native_lib):
+    """The library's checked entries on caller-owned tensors give the operator's results."""
+    x, w, b, g = make(300, 200, torch.float16)
+    leaves = [t.clone().requires_grad_() for t in (x, w, b)]
+    want_out = layer_norm(*leaves)
+    want = torch.autograd.grad(want_out, leaves, g)
+    out, stats = torch.empty_like(x), torch.empty((300, 2), dtype=torch.float32, device=DEV)
+    native_lib.layer_norm_forward(x, w, b, out, stats, EPS)
+    assert torch.equal(out, want_out)
+    got = [torch.full_like(t, math.nan) for t in (x, w, b)]
+    native_lib.layer_norm_backward(g, x, w, stats, *got)
+    for a, e in zip(got, want):
+        assert torch.equal(a, e)
+    with pytest.raises(RuntimeError, match="statistics must have shape"):
+        native_lib.layer_norm_forward(x, w, b, out, stats[:5], EPS)
+    with pytest.raises(RuntimeError, match="weight must be float16"):
+        native_lib.layer_norm_forward(x, w.double(), b, out, stats, EPS)
+    with pytest.raises(RuntimeError, match="grad_bias must be float16"):
+        native_lib.layer_norm_backward(g, x, w, stats, None, None, got[2].float())
+
+
+def test_streams_and_captured_steps():
+    """On another stream, and captured and replayed with eager work in between."""
+    x, w, b, g = make(9000, 256, torch.bfloat16)
+    leaves = [t.clone().requires_grad_() for t in (x, w, b)]
+
+    def step():
+        out = layer_norm(*leaves)
+        return [out.detach(), *torch.autograd.grad(out, leaves, g)]
+
+    want = step()
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        got = step()
+    torch.cuda.current_stream().wait_stream(stream)
+    for a, e in zip(got, want):
+        assert torch.equal(a, e)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = step()
+    for replay in range(4):
+        with torch.no_grad():
+            leaves[0].copy_(torch.randn(x.shape, device=DEV) + replay)
+        graph.replay()
+        got = [t.clone() for t in captured]
+        torch.cuda.synchronize()
+        for a, e in zip(got, step()):
+            assert torch.equal(a, e)

@@ -548,3 +548,53 @@ def test_refused_on_the_device():
     grad, = torch.autograd.grad(linear(xs, w, b), [xs], g)
     with pytest.raises(RuntimeError):
         torch.autograd.grad(linear(xs, w, b), [xs], g, create_graph=True)[0].sum().backward()
+
+
+@pytest.mark.parametrize("checkpoint", [False, True])
+@pytest.mark.parametrize("activation", [0, 1, 2])
+def test_tensor_level_entries(native_lib, activation, checkpoint):
+    """The library's checked entries on caller-owned tensors give the operator's results."""
+    x, w, b, r, g = make(700, 96, 72, torch.bfloat16, residual=True)
+    name = {0: None, 1: "relu", 2: "gelu"}[activation]
+    xs, ws, bs = leaves(x, w, b)
+    want_out = linear(xs, ws, bs, activation=name, residual=r,
+                      checkpoint="int8" if checkpoint else None)
+    want = torch.autograd.grad(want_out, [xs, ws, bs], g)
+    kept = {0: None, 1: torch.empty((2, 700, 8), dtype=torch.uint8, device=DEV),
+            2: torch.empty((700, 72), dtype=torch.bfloat16, device=DEV)}[activation]
+    out = torch.empty((700, 72), dtype=torch.bfloat16, device=DEV)
+    native_lib.linear_forward(x, w, b, r, out, kept, activation)
+    assert torch.equal(out, want_out)
+    codes = scales = None
+    if checkpoint:
+        codes = torch.empty((700, 96), dtype=torch.int8, device=DEV)
+        scales = torch.empty((700, 3), dtype=torch.uint8, device=DEV)
+        native_lib.linear_checkpoint(x, codes, scales)
+    got = [torch.full_like(t, math.nan) for t in (x, w, b)]
+    native_lib.linear_backward(g, None if checkpoint else x, codes, scales, w, kept, *got,
+                               (72, 96), activation)
+    for a, e in zip(got, want):
+        assert torch.equal(a, e)
+
+
+def test_tensor_level_entries_refuse(native_lib):
+    x, w, b, r, g = make(8, 16, 12, torch.float16, residual=True)
+    out = torch.empty_like(r)
+    good = dict(input=x, weight=w, bias=b, residual=r, output=out, kept=None, activation=0)
+    for change, message in (
+            ({"weight": w[:, :8]}, "contiguous"),
+            ({"weight": w.float()}, "weight must be float16"),
+            ({"weight": w.cpu()}, "ROCm device tensor"),
+            ({"bias": b[:5].contiguous()}, "bias must have shape"),
+            ({"output": out[:4]}, "output must have shape"),
+            ({"kept": out, "activation": 1}, "relu_mask must be uint8"),
+            ({"kept": out[:3], "activation": 2}, "pre_activation must have shape"),
+            ({"kept": out}, "nothing is kept")):
+        with pytest.raises(RuntimeError, match=message):
+            native_lib.linear_forward(**{**good, **change})
+    with pytest.raises(RuntimeError, match="codes must have shape"):
+        native_lib.linear_checkpoint(x, torch.empty((8, 16), dtype=torch.int8, device=DEV),
+                                     torch.empty((8, 1), dtype=torch.uint8, device=DEV))
+    with pytest.raises(RuntimeError, match="null tensor pointer"):  # neither input nor codes
+        native_lib.linear_backward(g, None, None, None, w, None, torch.empty_like(x),
+                                   torch.empty_like(w), None, (12, 16), 0)

@@ -200,6 +200,8 @@ def forward_args(**overrides):
         ({"rows": 1 << 31}, 2, "32-bit"),
         ({"inner": (1 << 20) + 1}, 2, "32-bit"),
         ({"rows": 1 << 30, "outer": 1 << 20}, 2, "32-bit"),
+        ({"rows": (1 << 31) - 300, "inner": 200}, 2, "32-bit"),
+        ({"inner": 1 << 20, "outer": 1 << 20}, 2, "32-bit"),
         ({"x": None}, 1, "null tensor pointer"),
         ({"weight": None}, 1, "null tensor pointer"),
         ({"output": None}, 1, "null tensor pointer"),
