@@ -7,9 +7,10 @@
 // for every line, and with these operators' few launches that was most of a call
 // (layer norm of 300 x 256, forward and backward: 51 us on one thread, 107 on two).
 //
-// Contract with the callers in muspace_amd/ops: dtypes and shapes are checked
-// there; devices, strides and whether a graph is recorded are seen to here. A C-ABI
-// error becomes std::runtime_error (RuntimeError in Python) with the library's text.
+// Contract with the callers in muspace_amd/ops: tensors whose types or shapes do not
+// belong together give no result, and the caller says which one it is; devices,
+// strides and whether a graph is recorded are seen to here. A C-ABI error becomes
+// std::runtime_error (RuntimeError in Python) with the library's text.
 #include <ATen/ATen.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
@@ -126,6 +127,16 @@ variable_list once(variable_list grads, const char *name) {
   return (*error)(std::move(marked));
 }
 
+bool supported(at::ScalarType type) {
+  return type == at::kFloat || type == at::kHalf || type == at::kBFloat16;
+}
+
+// a given `t` is one row of `size` values of `type`
+bool row_of(const OptTensor &t, int64_t size, at::ScalarType type) {
+  return !t.has_value() || !t->defined() ||
+         (t->dim() == 1 && t->size(0) == size && t->scalar_type() == type);
+}
+
 // ------------------------------------------------------------------ linear ---
 
 std::pair<Tensor, Tensor> checkpoint_of(const Tensor &input) {
@@ -224,8 +235,23 @@ struct LinearFunction : torch::autograd::Function<LinearFunction> {
   }
 };
 
-Tensor linear(const Tensor &input, const Tensor &weight, const OptTensor &bias,
-              const OptTensor &residual, int64_t activation, bool checkpoint) {
+bool linear_fits(const Tensor &input, const Tensor &weight, const OptTensor &bias,
+                 const OptTensor &residual) {
+  const at::ScalarType type = input.scalar_type();
+  if (!supported(type) || input.dim() == 0 || weight.dim() != 2 ||
+      weight.size(1) != input.size(-1) || weight.scalar_type() != type ||
+      !row_of(bias, weight.size(0), type)) {
+    return false;
+  }
+  if (!residual.has_value() || !residual->defined()) return true;
+  const Tensor &r = *residual;
+  return r.scalar_type() == type && r.dim() == input.dim() && r.size(-1) == weight.size(0) &&
+         r.sizes().slice(0, r.dim() - 1) == input.sizes().slice(0, input.dim() - 1);
+}
+
+OptTensor linear(const Tensor &input, const Tensor &weight, const OptTensor &bias,
+                 const OptTensor &residual, int64_t activation, bool checkpoint) {
+  if (!linear_fits(input, weight, bias, residual)) return OptTensor();
   const c10::DeviceGuard guard(input.device());
   const Tensor x = input.contiguous();
   const Tensor w = prepared(weight, x, "weight"), b = prepared(bias, x, "bias"),
@@ -300,7 +326,17 @@ struct LayerNormFunction : torch::autograd::Function<LayerNormFunction> {
   }
 };
 
-Tensor layer_norm(const Tensor &input, const OptTensor &weight, const OptTensor &bias, double eps) {
+bool norm_fits(const Tensor &input, const OptTensor &weight, const OptTensor &bias, double eps) {
+  if (!supported(input.scalar_type()) || input.dim() == 0 || !(eps >= 0.0)) return false;
+  const at::ScalarType type =
+      norm_type(input, weight.value_or(Tensor()), bias.value_or(Tensor()));
+  return (type == at::kFloat || type == input.scalar_type()) &&
+         row_of(weight, input.size(-1), type) && row_of(bias, input.size(-1), type);
+}
+
+OptTensor layer_norm(const Tensor &input, const OptTensor &weight, const OptTensor &bias,
+                     double eps) {
+  if (!norm_fits(input, weight, bias, eps)) return OptTensor();
   const c10::DeviceGuard guard(input.device());
   const Tensor x = input.contiguous();
   const Tensor w = prepared(weight, x, "weight"), b = prepared(bias, x, "bias");

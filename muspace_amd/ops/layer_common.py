@@ -47,17 +47,20 @@ def report_native(operator: str, input: torch.Tensor, backend: str) -> None:
     record_dispatch_report(_native_report(operator, backend, input.device.type))
 
 
-def choose_native(operator: str, input: torch.Tensor, backend: str):
-    """The host module if the call runs on the HIP kernels, None (reported) for the
-    PyTorch path. Raises, with a report, where neither may run."""
+def native_for(input: torch.Tensor, backend: str):
+    """The host module if a call on ``input`` runs on the HIP kernels, else None."""
+    if (backend == "auto" or backend in NATIVE_ALIASES) and is_rocm_tensor(input):
+        return _native()
+    return None
+
+
+def report_other(operator: str, input: torch.Tensor, backend: str) -> None:
+    """Reports the PyTorch path of a call that :func:`native_for` gives no module for;
+    raises, with a report, where that path may not run."""
     host = _native()
-    if (host is not None and (backend == "auto" or backend in NATIVE_ALIASES)
-            and is_rocm_tensor(input)):
-        return host
     decision = explain_dispatch(input, backend=backend, native_available=host is not None)
     record_dispatch_report(DispatchReport(operator, backend, decision.backend, decision.device,
                                           decision.reason, host is not None))
     if decision.backend == "error":
         detail = layer_host_error() if host is None and is_rocm_tensor(input) else None
         raise RuntimeError(f"{decision.reason}: {detail}" if detail else decision.reason)
-    return None

@@ -15,7 +15,7 @@ import torch
 import torch.nn.functional as F
 
 from .layer_common import DTYPES as _DTYPES
-from .layer_common import choose_native, report_native
+from .layer_common import native_for, report_native, report_other
 
 OPERATOR_NAME = "layer_norm"
 
@@ -67,13 +67,16 @@ def layer_norm(
     ``"reference"``. A native failure is raised, not hidden behind the PyTorch path.
     Gradients can be taken once (no gradients of gradients) on the HIP path.
     """
+    host = native_for(input, backend)
+    if host is not None:
+        output = host.layer_norm(input, weight, bias, eps)
+        if output is not None:
+            report_native(OPERATOR_NAME, input, backend)
+            return output
+    # not the HIP kernels' call, or tensors that do not belong together: say which
     _validate(input, weight, bias, eps)
-    host = choose_native(OPERATOR_NAME, input, backend)
-    if host is None:
-        return layer_norm_pytorch(input, weight, bias, eps=eps)
-    output = host.layer_norm(input, weight, bias, eps)
-    report_native(OPERATOR_NAME, input, backend)
-    return output
+    report_other(OPERATOR_NAME, input, backend)
+    return layer_norm_pytorch(input, weight, bias, eps=eps)
 
 
 __all__ = ["layer_norm", "layer_norm_pytorch"]

@@ -29,7 +29,7 @@ from torch.autograd.function import once_differentiable
 
 from ..runtime.kernel_dispatch import is_rocm_tensor
 from .layer_common import DTYPES as _DTYPES
-from .layer_common import choose_native, report_native, require_native
+from .layer_common import native_for, report_native, report_other, require_native
 
 OPERATOR_NAME = "linear"
 BLOCK = 32  # values of a row that share a scale in an 8-bit checkpoint
@@ -178,15 +178,18 @@ def linear(
     failure is raised, not hidden behind the PyTorch path. Gradients can be taken
     once (no gradients of gradients) on the HIP path.
     """
+    host = native_for(input, backend)
+    if host is not None and activation in ACTIVATIONS and checkpoint in (None, "int8"):
+        output = host.linear(input, weight, bias, residual, ACTIVATIONS[activation],
+                             checkpoint is not None)
+        if output is not None:
+            report_native(OPERATOR_NAME, input, backend)
+            return output
+    # not the HIP kernels' call, or tensors that do not belong together: say which
     _validate(input, weight, bias, activation, residual, checkpoint)
-    host = choose_native(OPERATOR_NAME, input, backend)
-    if host is None:
-        return linear_pytorch(input, weight, bias, activation=activation, residual=residual,
-                              checkpoint=checkpoint)
-    output = host.linear(input, weight, bias, residual, ACTIVATIONS[activation],
-                         checkpoint is not None)
-    report_native(OPERATOR_NAME, input, backend)
-    return output
+    report_other(OPERATOR_NAME, input, backend)
+    return linear_pytorch(input, weight, bias, activation=activation, residual=residual,
+                          checkpoint=checkpoint)
 
 
 __all__ = ["checkpoint_int8", "checkpoint_restore", "linear", "linear_pytorch"]

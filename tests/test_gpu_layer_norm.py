@@ -209,6 +209,18 @@ def test_refused_on_the_device():
     x, w, b, g = make(8, 16, torch.float32)
     with pytest.raises(RuntimeError, match="weight must be a ROCm device tensor"):
         layer_norm(x, w.cpu(), b.cpu())
+    for args, kwargs, error, message in (
+            ((x.double(),), {}, TypeError, "input must be"),
+            ((x[0, 0],), {}, ValueError, "at least one dimension"),
+            ((x, w[:3]), {}, ValueError, "weight must be"),
+            ((x, w.half()), {}, TypeError, "weight must be"),
+            ((x.half(), w, b.half()), {}, TypeError, "of one type"),
+            ((x, w, torch.stack([b, b])), {}, ValueError, "bias must be"),
+            ((x, w, b), {"eps": -1.0}, ValueError, "eps"),
+            ((x, w, b), {"backend": "none"}, RuntimeError, "unknown backend")):
+        with pytest.raises(error, match=message):
+            layer_norm(*args, **kwargs)
+    assert torch.equal(layer_norm(x, w, b, backend="musa"), layer_norm(x, w, b))
 
 
 def test_tensor_level_entries(native_lib):

@@ -544,6 +544,27 @@ def test_refused_on_the_device():
         linear(x, w.cpu(), b)
     with pytest.raises(RuntimeError, match="residual must be a ROCm device tensor"):
         linear(x, w, b, residual=r.cpu())
+    for change, error, message in (
+            ({"input": x.double()}, TypeError, "input must be"),
+            ({"input": x[0, 0]}, ValueError, "at least one dimension"),
+            ({"weight": w[:, :8]}, ValueError, "weight must be"),
+            ({"weight": w[0]}, ValueError, "weight must be"),
+            ({"weight": w.half()}, TypeError, "weight must be"),
+            ({"bias": b[:3]}, ValueError, "bias must be"),
+            ({"bias": b.half()}, TypeError, "bias must be"),
+            ({"residual": r[:1]}, ValueError, "residual must have"),
+            ({"residual": r.view(2, 4, 12)}, ValueError, "residual must have"),
+            ({"residual": r.half()}, TypeError, "residual must be"),
+            ({"activation": "silu"}, ValueError, "activation must be"),
+            ({"checkpoint": "fp8"}, ValueError, "checkpoint must be"),
+            ({"backend": "cuda"}, RuntimeError, "unknown backend")):
+        args = {"input": x, "weight": w, "bias": b, "residual": r, **change}
+        with pytest.raises(error, match=message):
+            linear(args.pop("input"), args.pop("weight"), args.pop("bias"), **args)
+    assert torch.equal(linear(x, w, b, backend="hip"), linear(x, w, b))
+    reference = linear(x, w, b, backend="reference")
+    assert get_last_dispatch_report().selected_backend == "reference"
+    torch.testing.assert_close(reference, linear(x, w, b), rtol=1e-5, atol=1e-5)
     xs = x.clone().requires_grad_()
     grad, = torch.autograd.grad(linear(xs, w, b), [xs], g)
     with pytest.raises(RuntimeError):
