@@ -47,12 +47,15 @@ extern "C" {
 #endif
 
 /* relu_mask and pre_activation may be NULL (no gradient wanted); relu_mask is
- * written for activation 1 only, pre_activation for activation 2 only. */
+ * written for activation 1 only, pre_activation for activation 2 only. codes and
+ * scales may both be NULL (no checkpoint); an empty output writes none. */
 MUSPACE_API int linear_forward(const void *x, int dtype, const void *weight, const void *bias,
                                const void *residual, void *output, uint8_t *relu_mask,
-                               void *pre_activation, int64_t rows, int64_t in_features,
-                               int64_t out_features, int activation, void *stream);
+                               void *pre_activation, int8_t *codes, uint8_t *scales, int64_t rows,
+                               int64_t in_features, int64_t out_features, int activation,
+                               void *stream);
 
+/* The checkpoint alone, the same codes as linear_forward's. */
 MUSPACE_API int linear_checkpoint(const void *x, int dtype, int8_t *codes, uint8_t *scales,
                                   int64_t rows, int64_t in_features, void *stream);
 

@@ -139,39 +139,43 @@ bool row_of(const OptTensor &t, int64_t size, at::ScalarType type) {
 
 // ------------------------------------------------------------------ linear ---
 
-std::pair<Tensor, Tensor> checkpoint_of(const Tensor &input) {
-  const int64_t rows = rows_of(input), cols = input.size(-1), padded = (cols + 31) / 32 * 32;
-  Tensor codes = at::empty({rows, padded}, input.options().dtype(at::kChar));
-  Tensor scales = at::empty({rows, padded / 32}, input.options().dtype(at::kByte));
-  check(api.linear_checkpoint(input.data_ptr(), code_of(input.scalar_type(), "input"),
-                              static_cast<int8_t *>(codes.data_ptr()),
-                              static_cast<uint8_t *>(scales.data_ptr()), rows, cols,
-                              stream_of(input)),
-        "linear_checkpoint");
-  return {codes, scales};
+// room for the 8-bit checkpoint of `input`: codes and scales
+std::pair<Tensor, Tensor> checkpoint_like(const Tensor &input) {
+  const int64_t rows = rows_of(input), padded = (input.size(-1) + 31) / 32 * 32;
+  return {at::empty({rows, padded}, input.options().dtype(at::kChar)),
+          at::empty({rows, padded / 32}, input.options().dtype(at::kByte))};
 }
 
-// The output, and what the activation's gradient needs where `keep` asks for it.
-std::pair<Tensor, Tensor> linear_run(const Tensor &input, const Tensor &weight, const Tensor &bias,
-                                     const Tensor &residual, int64_t activation, bool keep) {
+struct Kept {
+  Tensor activation;     // relu's bits or gelu's pre-activation
+  Tensor codes, scales;  // the input's checkpoint
+};
+
+// The output; with `keep`, what the gradients need besides tensors that are there.
+Tensor linear_run(const Tensor &input, const Tensor &weight, const Tensor &bias,
+                  const Tensor &residual, int64_t activation, bool keep, bool checkpoint,
+                  Kept *kept) {
   const int64_t rows = rows_of(input), cols = weight.size(1), out = weight.size(0);
   auto shape = input.sizes().vec();
   shape.back() = out;
   Tensor output = at::empty(shape, input.options());
-  Tensor kept;
+  Tensor aside, codes, scales;
   if (keep && activation == 1) {
-    kept = at::empty({(out + 63) / 64, rows, 8}, input.options().dtype(at::kByte));
+    aside = at::empty({(out + 63) / 64, rows, 8}, input.options().dtype(at::kByte));
   } else if (keep && activation == 2) {
-    kept = at::empty({rows, out}, input.options());
+    aside = at::empty({rows, out}, input.options());
   }
+  if (checkpoint) std::tie(codes, scales) = checkpoint_like(input);
   check(api.linear_forward(
             input.data_ptr(), code_of(input.scalar_type(), "input"), weight.data_ptr(),
             pointer(bias), pointer(residual), output.data_ptr(),
-            activation == 1 ? static_cast<uint8_t *>(pointer(kept)) : nullptr,
-            activation == 2 ? pointer(kept) : nullptr, rows, cols, out,
+            activation == 1 ? static_cast<uint8_t *>(pointer(aside)) : nullptr,
+            activation == 2 ? pointer(aside) : nullptr, static_cast<int8_t *>(pointer(codes)),
+            static_cast<uint8_t *>(pointer(scales)), rows, cols, out,
             static_cast<int>(activation), stream_of(input)),
         "linear_forward");
-  return {output, kept};
+  if (kept != nullptr) *kept = {aside, codes, scales};
+  return output;
 }
 
 struct LinearFunction : torch::autograd::Function<LinearFunction> {
@@ -180,12 +184,12 @@ struct LinearFunction : torch::autograd::Function<LinearFunction> {
                         bool checkpoint) {
     const Tensor b = bias.value_or(Tensor()), r = residual.value_or(Tensor());
     const bool need_input = input.requires_grad(), need_weight = weight.requires_grad();
-    auto [output, kept] = linear_run(input, weight, b, r, activation,
-                                     need_input || need_weight || wants_grad(b));
-    Tensor codes, scales;
-    if (need_weight && checkpoint) std::tie(codes, scales) = checkpoint_of(input);
-    ctx->save_for_backward({need_weight && !checkpoint ? input : Tensor(), codes, scales,
-                            need_input ? weight : Tensor(), kept});
+    Kept kept;
+    Tensor output = linear_run(input, weight, b, r, activation,
+                               need_input || need_weight || wants_grad(b),
+                               need_weight && checkpoint, &kept);
+    ctx->save_for_backward({need_weight && !checkpoint ? input : Tensor(), kept.codes, kept.scales,
+                            need_input ? weight : Tensor(), kept.activation});
     ctx->saved_data["input"] = input.sizes();
     ctx->saved_data["weight"] = weight.sizes();
     ctx->saved_data["activation"] = activation;
@@ -260,12 +264,19 @@ OptTensor linear(const Tensor &input, const Tensor &weight, const OptTensor &bia
       (wants_grad(x) || wants_grad(w) || wants_grad(b) || wants_grad(r))) {
     return LinearFunction::apply(x, w, opt(b), opt(r), activation, checkpoint);
   }
-  return linear_run(x, w, b, r, activation, false).first;
+  return linear_run(x, w, b, r, activation, false, false, nullptr);
 }
 
 std::pair<Tensor, Tensor> checkpoint(const Tensor &input) {
   const c10::DeviceGuard guard(input.device());
-  return checkpoint_of(input.contiguous());
+  const Tensor x = input.contiguous();
+  auto kept = checkpoint_like(x);
+  check(api.linear_checkpoint(x.data_ptr(), code_of(x.scalar_type(), "input"),
+                              static_cast<int8_t *>(kept.first.data_ptr()),
+                              static_cast<uint8_t *>(kept.second.data_ptr()), rows_of(x),
+                              x.size(-1), stream_of(x)),
+        "linear_checkpoint");
+  return kept;
 }
 
 // -------------------------------------------------------------- layer norm ---

@@ -218,13 +218,19 @@ extern "C" {
 
 int linear_forward(const void *x, int dtype, const void *weight, const void *bias,
                    const void *residual, void *output, uint8_t *relu_mask, void *pre_activation,
-                   int64_t rows, int64_t in_features, int64_t out_features, int activation,
-                   void *stream) {
+                   int8_t *codes, uint8_t *scales, int64_t rows, int64_t in_features,
+                   int64_t out_features, int activation, void *stream) {
   int rc = validate("linear_forward", dtype, rows, in_features, out_features, activation);
   if (rc != MUSPACE_OK) return rc;
   if (rows == 0 || out_features == 0) return ok();
   if (output == nullptr || (in_features > 0 && (x == nullptr || weight == nullptr))) {
     return fail(MUSPACE_EINVAL, "linear_forward: null tensor pointer");
+  }
+  if ((codes == nullptr) != (scales == nullptr)) {
+    return fail(MUSPACE_EINVAL, "linear_forward: codes and scales come together");
+  }
+  if (reinterpret_cast<uintptr_t>(codes) % 8 != 0) {
+    return fail(MUSPACE_EINVAL, "linear_forward: codes must be 8-byte aligned");
   }
   Product a = {};
   a.p = x;
@@ -241,10 +247,18 @@ int linear_forward(const void *x, int dtype, const void *weight, const void *bia
   a.mask_out = activation == dense::kRelu ? relu_mask : nullptr;
   a.mask_ld = rows * 8;
   a.act = activation;
+  a.codes = reinterpret_cast<uint8_t *>(codes);
+  a.code_scales = scales;
   const bool tight =
       in_features % chunk_values(dtype) == 0 && aligned16(x) && aligned16(weight);
   hipStream_t st = static_cast<hipStream_t>(stream);
-  by_type(dtype, [&](auto t) { run_rows<decltype(t), Job::kForward, Kind::kPlain>(a, tight, st); });
+  by_type(dtype, [&](auto t) {
+    if (codes != nullptr) {
+      run_rows<decltype(t), Job::kForward, Kind::kKept>(a, tight, st);
+    } else {
+      run_rows<decltype(t), Job::kForward, Kind::kPlain>(a, tight, st);
+    }
+  });
   return check_launch("linear_forward");
 }
 

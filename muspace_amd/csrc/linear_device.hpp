@@ -295,6 +295,68 @@ __device__ __forceinline__ u32x4 decode(const uint32_t (&w)[Piece<T>::kValues / 
   return pack<T>(v);
 }
 
+// lane l's value from lane l ^ kDistance, where the lanes of each aligned group of
+// kDistance hold the same (1 and 2: any values)
+template <int kDistance>
+__device__ __forceinline__ uint32_t from_lane(uint32_t v) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  // lanes 1 0 3 2; 2 3 0 1; a mirrored half row of 8
+  constexpr int kMove = kDistance == 1 ? 0xB1 : kDistance == 2 ? 0x4E : 0x141;
+  return __builtin_amdgcn_mov_dpp(static_cast<int>(v), kMove, 0xf, 0xf, true);
+#else
+  return v;
+#endif
+}
+
+// A chunk's codes and its block's scale byte. The 32 / kV neighbouring lanes that hold a
+// block's chunks call it together. A block shares 2^e, the smallest power of two with 127 *
+// 2^e >= its largest magnitude; a code is the nearest integer to x / 2^e (ties to even).
+// The byte is e + 127, or 255 for a block with an infinity or NaN. e stays where 2^e is a
+// normal number (and, for float16, a float16 number), and codes end at 63 where 64 * 2^e is
+// past the type's range, so that every code * 2^e is a number of the type.
+template <typename T>
+__device__ __forceinline__ uint32_t encode(const float (&v)[Piece<T>::kValues],
+                                           uint32_t (&w)[Piece<T>::kValues / 4]) {
+  constexpr int kV = Piece<T>::kValues;
+  constexpr bool kHalf = std::is_same_v<T, __half>;
+  constexpr int kLow = kHalf ? 127 - 24 : 1, kHigh = kHalf ? 127 + 10 : 127 + 122;
+  uint32_t top = 0;
+#pragma unroll
+  for (int e = 0; e < kV; ++e) top = max(top, __float_as_uint(v[e]) & 0x7fffffffu);
+  top = max(top, from_lane<1>(top));
+  top = max(top, from_lane<2>(top));
+  if constexpr (kV == 4) top = max(top, from_lane<4>(top));
+  const bool finite = top < 0x7f800000u;
+  // 127 * 2^e reaches top = 1.f * 2^E from E - 6 on, one later if 1.f > 127 / 64
+  const int s = max(kLow, static_cast<int>(top >> 23) - 6 + ((top & 0x7fffffu) > 0x7e0000u));
+  const float inverse = __uint_as_float(static_cast<uint32_t>(254 - s) << 23);
+  const float limit = s >= kHigh ? 63.0f : 127.0f;
+#pragma unroll
+  for (int i = 0; i < kV / 4; ++i) w[i] = 0;
+#pragma unroll
+  for (int e = 0; e < kV; ++e) {
+    float q = rintf(v[e] * inverse);
+    q = finite ? fminf(fmaxf(q, -limit), limit) : 1.0f;  // 1 * NaN reads back as NaN
+    w[e / 4] |= (static_cast<uint32_t>(static_cast<int>(q)) & 0xffu) << (8 * (e & 3));
+  }
+  return finite ? static_cast<uint32_t>(s) : 255u;
+}
+
+// The chunk at `col` of a row's checkpoint: codes [rows][padded], scales [rows][padded / 32].
+template <typename T>
+__device__ __forceinline__ void keep_codes(uint8_t *codes, uint8_t *scales, int64_t row, int col,
+                                           int padded,
+                                           const uint32_t (&w)[Piece<T>::kValues / 4],
+                                           uint32_t scale) {
+  uint8_t *to = codes + row * padded + col;
+  if constexpr (Piece<T>::kValues == 8) {
+    *reinterpret_cast<u32x2 *>(to) = u32x2{w[0], w[1]};
+  } else {
+    *reinterpret_cast<uint32_t *>(to) = w[0];
+  }
+  if (col % 32 == 0) scales[row * (padded / 32) + col / 32] = static_cast<uint8_t>(scale);
+}
+
 // ----------------------------------------------------------- three planes ---
 
 // Four float32 values as kPlanes bfloat16 numbers each, the largest first.

@@ -49,6 +49,7 @@ struct Product {
   void *out, *z_out;     // z_out: kept x W^T + b (gelu under training)
   uint8_t *mask_out;     // kept sign bits (relu under training), as mask
   int act;
+  uint8_t *codes, *code_scales;  // Kind::kKept: the checkpoint of x
   // kWeight
   float *partial, *bias_partial;  // [splits][m][pad8(n)], [splits][m]
   void *bias_out;                 // splits == 1: db (0: none)
@@ -71,8 +72,9 @@ __device__ __forceinline__ int xcd_order(int id, int count) {
 // which only marks results that are not stored (past k: zeros). Memory rows shorter
 // than a chunk are read value by value.
 // What an operand is besides its values in memory: relu's bits go with it (masked), or a
-// second tensor holds what rounding to 16 bits left of each value (pair: gelu's dz).
-enum class Kind { kPlain, kMasked, kPair };
+// second tensor holds what rounding to 16 bits left of each value (pair: gelu's dz), or
+// its 8-bit checkpoint is written as it is read (kept: the forward's x).
+enum class Kind { kPlain, kMasked, kPair, kKept };
 
 template <typename T, bool kAlong, int R, bool kTight, Kind kKind, bool kCodes,
           int kTeam = kThreads>
@@ -279,6 +281,17 @@ struct Loader {
     }
   }
 
+  // the checkpoint of a fetched chunk (along): every lane of a row's takes part
+  __device__ __forceinline__ void keep(uint8_t *codes, uint8_t *scales, int k0, int i,
+                                       const u32x4 &value) const {
+    float f[kV];
+    unpack<T>(value, f);
+    uint32_t w[kV / 4];
+    const uint32_t scale = encode<T>(f, w);
+    const int row = row0 + r + kDown * i, col = k0 + c * kV, padded = (k_end + 31) & ~31;
+    if (row < rows && col < padded) keep_codes<T>(codes, scales, row, col, padded, w, scale);
+  }
+
   // float32 as it is, for the tiles that hold more than bfloat16's range
   __device__ __forceinline__ void put_f32(char *tile, int i, const u32x4 &value) const {
     const uint32_t at = kAlong ? along_offset<128>(r + kDown * i, c)
@@ -333,15 +346,6 @@ __device__ __forceinline__ void load_bias(const T *p, int left, float (&b)[Piece
   unpack<T>(v, b);
 }
 
-// lane l's value from lane l ^ 1
-__device__ __forceinline__ uint32_t swap_neighbours(uint32_t v) {
-#if defined(__HIP_DEVICE_COMPILE__)
-  return __builtin_amdgcn_mov_dpp(static_cast<int>(v), 0xB1, 0xf, 0xf, true);
-#else
-  return v;
-#endif
-}
-
 // A chunk of the forward's result: z holds x W^T + b. `half`: the lane holds the
 // upper four columns of a mask byte (float32).
 template <typename T>
@@ -361,7 +365,7 @@ __device__ __forceinline__ void finish_forward(const Product &a, int64_t row, in
       uint8_t *mask = a.mask_out + (col >> 6) * a.mask_ld + row * 8 + ((col >> 3) & 7);
       if constexpr (kV == 4) {
         // lanes l and l ^ 1 hold the two halves of a byte
-        const uint32_t other = swap_neighbours(bits);
+        const uint32_t other = from_lane<1>(bits);
         if ((col & 4) == 0 && left > 0) {
           *mask = static_cast<uint8_t>(bits | other << 4);
         }
@@ -446,6 +450,9 @@ __global__ __launch_bounds__(kThreads, (sizeof(T) == 4 && kTight) ? 3 : 2) void 
   float sums[kV] = {};
   const bool sum_p = kJob == Job::kWeight && col0 == 0;
 
+  // the checkpoint's rows are shared out among the first columns of tiles
+  const int keepers = min(a.tiles_n, static_cast<int>(P::kCount)), keeper = tile % a.tiles_n;
+
   char *const tile_p = lds, *const tile_q = lds + P::kPlanes * P::kPlaneBytes;
   if (k_begin < k_end) {
     p.fetch(k_begin);
@@ -464,6 +471,9 @@ __global__ __launch_bounds__(kThreads, (sizeof(T) == 4 && kTight) ? 3 : 2) void 
 #pragma unroll
             for (int e = 0; e < kV; ++e) sums[e] += f[e];
           }
+        }
+        if constexpr (kKind == Kind::kKept) {
+          if (i % keepers == keeper) p.keep(a.codes, a.code_scales, k0, i, v);
         }
         p.put(tile_p + l * P::kPlaneBytes, i, v);
       }
@@ -665,6 +675,7 @@ __global__ __launch_bounds__(kWaves *kWave) void linear_few(const Product a) {
   Q q;
   p.init(a.p, a.p_rest, a.ldp, a.mask, a.mask_ld, row0, a.m, a.k);
   q.init(a.q, nullptr, a.ldq, nullptr, 0, col0, a.n, a.k);
+  const int keepers = min(a.tiles_n, static_cast<int>(P::kCount)), keeper = tile % a.tiles_n;
   f32x16 acc = {};
   int k0 = wave * kStep;
   if (k0 < a.k) {
@@ -674,6 +685,9 @@ __global__ __launch_bounds__(kWaves *kWave) void linear_few(const Product a) {
   for (; k0 < a.k; k0 += kWaves * kStep) {
 #pragma unroll
     for (int i = 0; i < P::kCount; ++i) {
+      if constexpr (kKind == Kind::kKept) {
+        if (i % keepers == keeper) p.keep(a.codes, a.code_scales, k0, i, p.chunk(i));
+      }
       if constexpr (kF32) {
         p.put_f32(tile_p, i, p.chunk(i));
       } else {
@@ -857,24 +871,15 @@ __global__ __launch_bounds__(kThreads) void linear_gelu_grad(const T *g, const T
   }
 }
 
-// x in 8 bits. A block of 32 values of a row shares 2^e, the smallest power of two
-// with 127 * 2^e >= its largest magnitude; a code is the nearest integer to
-// x / 2^e (ties to even). codes [rows][pad32(cols)], zero past cols; scales
-// [rows][pad32(cols) / 32] hold e + 127, or 255 for a block with an infinity or
-// NaN. e stays where 2^e is a normal number (and, for float16, a float16 number),
-// and codes end at 63 where 64 * 2^e is past the type's range, so that every
-// code * 2^e is a number of the type.
+// x in 8 bits: codes [rows][pad32(cols)], zero past cols, and scales (encode).
 template <typename T>
 __global__ __launch_bounds__(kThreads) void linear_checkpoint(const T *x, uint8_t *codes,
                                                               uint8_t *scales, int64_t rows,
                                                               int cols) {
   constexpr int kV = Piece<T>::kValues;
-  constexpr int kGroup = 32 / kV;  // lanes per block of 32
-  constexpr bool kHalf = std::is_same_v<T, __half>;
-  constexpr uint32_t kLow = kHalf ? 127 - 24 : 1, kHigh = kHalf ? 127 + 10 : 127 + 122;
   const int padded = (cols + 31) & ~31, per_row = padded / kV;
   const int64_t chunks = rows * per_row;
-  // per_row and the launch's stride are multiples of kGroup: a block's lanes stay together
+  // per_row and the launch's stride are multiples of a block's lanes: they stay together
   for (int64_t i = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x; i < chunks;
        i += static_cast<int64_t>(gridDim.x) * kThreads) {
     int chunk;
@@ -882,32 +887,9 @@ __global__ __launch_bounds__(kThreads) void linear_checkpoint(const T *x, uint8_
     const int col = chunk * kV;
     float v[kV];
     unpack<T>(loose_load<T>(x + row * cols + col, cols - col), v);
-    uint32_t top = 0;
-#pragma unroll
-    for (int e = 0; e < kV; ++e) top = max(top, __float_as_uint(v[e]) & 0x7fffffffu);
-#pragma unroll
-    for (int d = 1; d < kGroup; d <<= 1) top = max(top, static_cast<uint32_t>(__shfl_xor(top, d)));
-    const bool finite = top < 0x7f800000u;
-    const int s0 = static_cast<int>(top >> 23) - 6 + ((top & 0x7fffffu) > 0x7e0000u ? 1 : 0);
-    const uint32_t s = s0 < static_cast<int>(kLow) ? kLow : static_cast<uint32_t>(s0);
-    const float inverse = __uint_as_float((254u - s) << 23);
-    const float limit = s >= kHigh ? 63.0f : 127.0f;
-    uint32_t w[kV / 4] = {};
-#pragma unroll
-    for (int e = 0; e < kV; ++e) {
-      float q = rintf(v[e] * inverse);
-      q = finite ? fminf(fmaxf(q, -limit), limit) : 1.0f;  // 1 * NaN reads back as NaN
-      w[e / 4] |= (static_cast<uint32_t>(static_cast<int>(q)) & 0xffu) << (8 * (e & 3));
-    }
-    uint8_t *to = codes + row * padded + col;
-    if constexpr (kV == 8) {
-      *reinterpret_cast<u32x2 *>(to) = u32x2{w[0], w[1]};
-    } else {
-      *reinterpret_cast<uint32_t *>(to) = w[0];
-    }
-    if (col % 32 == 0) {
-      scales[row * (padded / 32) + col / 32] = static_cast<uint8_t>(finite ? s : 255u);
-    }
+    uint32_t w[kV / 4];
+    const uint32_t scale = encode<T>(v, w);
+    keep_codes<T>(codes, scales, row, col, padded, w, scale);
   }
 }
 

@@ -148,7 +148,7 @@ _EXPORTS: dict[str, tuple[Any, list[Any]]] = {
     ),
     # include/muspace_layer.h
     "linear_forward": (
-        _c_int, [_c_ptr, _c_int] + [_c_ptr] * 6 + [_c_int64] * 3 + [_c_int, _c_ptr]
+        _c_int, [_c_ptr, _c_int] + [_c_ptr] * 8 + [_c_int64] * 3 + [_c_int, _c_ptr]
     ),
     "linear_checkpoint": (
         _c_int, [_c_ptr, _c_int, _c_ptr, _c_ptr, _c_int64, _c_int64, _c_ptr]
@@ -1026,9 +1026,16 @@ class NativeLibrary:
         elif kept is not None:
             raise RuntimeError("nothing is kept without an activation")
 
-    def linear_forward(self, input, weight, bias, residual, output, kept, activation: int) -> None:
+    def _check_codes(self, like, codes, scales, rows, cols) -> None:
+        padded = (cols + 31) // 32 * 32
+        self._check_all(like, (torch.int8,), (codes, "codes", (rows, padded)))
+        self._check_all(like, (torch.uint8,), (scales, "scales", (rows, padded // 32)))
+
+    def linear_forward(self, input, weight, bias, residual, output, kept, activation: int,
+                       codes=None, scales=None) -> None:
         """output = act(input weight^T + bias) + residual; ``kept``: None, relu's
-        bits (uint8) or gelu's pre-activation (the input's dtype)."""
+        bits (uint8) or gelu's pre-activation (the input's dtype); ``codes`` and
+        ``scales``: None or the input's 8-bit checkpoint."""
         _check(input, "input", tuple(_DTYPE_CODES))
         if weight is None or weight.dim() != 2 or input.dim() == 0:
             raise RuntimeError("weight must be 2-D and input at least 1-D")
@@ -1039,12 +1046,14 @@ class NativeLibrary:
                         (bias, "bias", (out,)), (residual, "residual", (*lead, out)),
                         (output, "output", (*lead, out)))
         self._check_kept(input, kept, rows, out, activation)
+        self._check_codes(input, codes, scales, rows, cols)
         kept_ptr = _ptr(kept)
         self._launch(
             "linear_forward", input.device,
             input.data_ptr(), _DTYPE_CODES[input.dtype], weight.data_ptr(), _ptr(bias),
             _ptr(residual), output.data_ptr(), kept_ptr if activation == 1 else None,
-            kept_ptr if activation == 2 else None, rows, cols, out, activation,
+            kept_ptr if activation == 2 else None, _ptr(codes), _ptr(scales), rows, cols, out,
+            activation,
         )
 
     def linear_checkpoint(self, input, codes, scales) -> None:
@@ -1053,9 +1062,7 @@ class NativeLibrary:
         if input.dim() != 2:
             raise RuntimeError("input must be 2-D")
         rows, cols = input.shape
-        padded = (cols + 31) // 32 * 32
-        self._check_all(input, (torch.int8,), (codes, "codes", (rows, padded)))
-        self._check_all(input, (torch.uint8,), (scales, "scales", (rows, padded // 32)))
+        self._check_codes(input, codes, scales, rows, cols)
         self._launch("linear_checkpoint", input.device, input.data_ptr(),
                      _DTYPE_CODES[input.dtype], codes.data_ptr(), scales.data_ptr(), rows, cols)
 
@@ -1067,14 +1074,12 @@ class NativeLibrary:
         out, cols = weight_shape
         lead = tuple(grad_output.shape[:-1])
         rows = math.prod(lead)
-        padded = (cols + 31) // 32 * 32
         _check_shape(grad_output, "grad_output", (*lead, out))
         self._check_all(grad_output, (grad_output.dtype,), (input, "input", (*lead, cols)),
                         (weight, "weight", (out, cols)), (grad_input, "grad_input", (*lead, cols)),
                         (grad_weight, "grad_weight", (out, cols)),
                         (grad_bias, "grad_bias", (out,)))
-        self._check_all(grad_output, (torch.int8,), (codes, "codes", (rows, padded)))
-        self._check_all(grad_output, (torch.uint8,), (scales, "scales", (rows, padded // 32)))
+        self._check_codes(grad_output, codes, scales, rows, cols)
         self._check_kept(grad_output, kept, rows, out, activation)
         code = _DTYPE_CODES[grad_output.dtype]
         nbytes = self._raw["linear_backward_workspace_size"](code, rows, cols, out, activation)

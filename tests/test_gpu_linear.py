@@ -156,6 +156,31 @@ def test_checkpoint_codes_are_exact(cols, dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("size", [(1, 1, 1), (5, 31, 9), (70, 64, 40), (300, 100, 64),
+                                  (9000, 203, 136), (20011, 96, 512), (50001, 200, 260)], ids=str)
+def test_checkpoint_of_the_forward_is_the_checkpoint_alone(native_lib, size, dtype):
+    """The forward's kernels write the checkpoint as they read the input: the same bytes,
+    every one of them, and the same output."""
+    rows, inner, outer = size
+    x, w, b, _, _ = make(*size, dtype, exact=False)
+    gen = torch.Generator(device=DEV).manual_seed(3)
+    x *= torch.exp2(torch.randint(-8, 8, (rows, 1), generator=gen, device=DEV).float()).to(dtype)
+    x[0] = 0.0
+    if rows > 2:
+        x[1, inner - 1], x[2, 0] = math.inf, math.nan
+    padded = (inner + 31) // 32 * 32
+    codes = torch.full((rows + 1, padded), 99, dtype=torch.int8, device=DEV)
+    scales = torch.full((rows + 1, padded // 32), 99, dtype=torch.uint8, device=DEV)
+    out, plain = (torch.empty((rows, outer), dtype=dtype, device=DEV) for _ in range(2))
+    native_lib.linear_forward(x, w, b, None, out, None, 0, codes[:rows], scales[:rows])
+    native_lib.linear_forward(x, w, b, None, plain, None, 0)
+    assert torch.equal(out.view(torch.uint8), plain.view(torch.uint8))
+    want = checkpoint_int8(x)
+    assert torch.equal(codes[:rows], want[0]) and torch.equal(scales[:rows], want[1])
+    assert codes[rows].eq(99).all() and scales[rows].eq(99).all()  # rows behind: as they were
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 def test_empty(dtype):
     for rows, inner, outer in ((0, 16, 8), (5, 16, 0), (5, 0, 8), (0, 0, 8)):
         x, w, b, r, g = make(rows, inner, outer, dtype, residual=True)
@@ -584,13 +609,12 @@ def test_tensor_level_entries(native_lib, activation, checkpoint):
     kept = {0: None, 1: torch.empty((2, 700, 8), dtype=torch.uint8, device=DEV),
             2: torch.empty((700, 72), dtype=torch.bfloat16, device=DEV)}[activation]
     out = torch.empty((700, 72), dtype=torch.bfloat16, device=DEV)
-    native_lib.linear_forward(x, w, b, r, out, kept, activation)
-    assert torch.equal(out, want_out)
     codes = scales = None
     if checkpoint:
         codes = torch.empty((700, 96), dtype=torch.int8, device=DEV)
         scales = torch.empty((700, 3), dtype=torch.uint8, device=DEV)
-        native_lib.linear_checkpoint(x, codes, scales)
+    native_lib.linear_forward(x, w, b, r, out, kept, activation, codes, scales)
+    assert torch.equal(out, want_out)
     got = [torch.full_like(t, math.nan) for t in (x, w, b)]
     native_lib.linear_backward(g, None if checkpoint else x, codes, scales, w, kept, *got,
                                (72, 96), activation)

@@ -184,7 +184,7 @@ FAR = 1 << 12
 
 def forward_args(**overrides):
     args = dict(x=FAR, dtype=0, weight=FAR, bias=None, residual=None, output=FAR, mask=None,
-                z=None, rows=4, inner=8, outer=8, activation=0, stream=None)
+                z=None, codes=None, scales=None, rows=4, inner=8, outer=8, activation=0, stream=None)
     args.update(overrides)
     return list(args.values())
 
@@ -205,6 +205,9 @@ def forward_args(**overrides):
         ({"x": None}, 1, "null tensor pointer"),
         ({"weight": None}, 1, "null tensor pointer"),
         ({"output": None}, 1, "null tensor pointer"),
+        ({"codes": FAR}, 1, "codes and scales come together"),
+        ({"scales": FAR}, 1, "codes and scales come together"),
+        ({"codes": FAR + 2, "scales": FAR}, 1, "8-byte aligned"),
     ],
 )
 def test_linear_forward_abi_refuses(native_lib, overrides, code, message):
