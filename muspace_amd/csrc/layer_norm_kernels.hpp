@@ -24,30 +24,6 @@ namespace dense {
 
 constexpr int kNormThreads = 512;
 
-// v plus the value of the lane at XOR kDistance, given that the lanes of each
-// aligned group of kDistance hold the same: moves within the vector unit, where a
-// shuffle would go through LDS and wait.
-template <int kDistance>
-__device__ __forceinline__ float add_across(float v) {
-#if defined(__HIP_DEVICE_COMPILE__)
-  const int i = __float_as_int(v);
-  if constexpr (kDistance <= 8) {
-    // lanes 1 0 3 2, 2 3 0 1, mirrored halves of a row of 16, mirrored row
-    constexpr int kMove = kDistance == 1 ? 0xB1 : kDistance == 2 ? 0x4E
-                          : kDistance == 4 ? 0x141 : 0x140;
-    return v + __int_as_float(__builtin_amdgcn_mov_dpp(i, kMove, 0xf, 0xf, true));
-  } else if constexpr (kDistance == 16) {
-    const u32x2 r = __builtin_bit_cast(u32x2, __builtin_amdgcn_permlane16_swap(i, i, false, false));
-    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
-  } else {
-    const u32x2 r = __builtin_bit_cast(u32x2, __builtin_amdgcn_permlane32_swap(i, i, false, false));
-    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
-  }
-#else
-  return v;
-#endif
-}
-
 // kLanes lanes' sums, the same on all of them
 template <int kLanes, int N>
 __device__ __forceinline__ void group_sum(float (&v)[N], float *lds) {

@@ -160,6 +160,50 @@ void run_rows(const Product &a, bool tight, hipStream_t st) {
   }
 }
 
+// Rows that the vector unit multiplies while W is read. linear_few and linear_vector, us,
+// at one row, and at the most here (8 of float32, 4 of 16 bits):
+//   float32   256 -> 256    4.1  2.1    4.2  3.1      bfloat16    3.3  2.3    3.3  2.9
+//            2048 -> 2048  15.1  4.3   15.2  6.9                  6.0  2.7    6.0  3.7
+//            4096 -> 16384  117   47    117   79                 54.7 23.9   54.8 32.7
+//             203 -> 611    4.5  2.2    4.6  3.2                  3.6  2.4    3.8  3.0
+// Eight 16-bit rows were no gain (256 -> 256 3.3 3.5, 2048 -> 2048 6.0 5.5).
+template <typename T>
+bool few_rows(int64_t rows) {
+  return rows <= (sizeof(T) == 4 ? 8 : 4);
+}
+
+template <typename T, int kRows, int kCols>
+void launch_vector(const Product &a, hipStream_t st) {
+  dense::linear_vector<T, kRows, kCols>
+      <<<static_cast<int>(ceil_div(a.n, 8)), 8 / kCols * 64, 0, st>>>(a);
+}
+
+template <typename T>
+void run_vector(const Product &a, hipStream_t st) {
+  if (a.m == 1) {
+    launch_vector<T, 1, 1>(a, st);
+  } else if (a.m == 2) {
+    launch_vector<T, 2, 1>(a, st);
+  } else if (a.m <= 4) {
+    launch_vector<T, 4, 2>(a, st);
+  } else if constexpr (sizeof(T) == 4) {
+    launch_vector<T, 8, 2>(a, st);
+  }
+}
+
+int grid_for(int64_t work) {
+  const int64_t b = ceil_div(work, dense::kThreads);
+  return static_cast<int>(b > 65536 ? 65536 : (b < 1 ? 1 : b));
+}
+
+template <typename T>
+void run_checkpoint(const void *x, uint8_t *codes, uint8_t *scales, int64_t rows,
+                    int64_t in_features, hipStream_t st) {
+  const int64_t work = rows * (((in_features + 31) & ~int64_t{31}) / dense::Piece<T>::kValues);
+  dense::linear_checkpoint<T><<<grid_for(work), dense::kThreads, 0, st>>>(
+      static_cast<const T *>(x), codes, scales, rows, static_cast<int>(in_features));
+}
+
 // f(the kind of dz that `a` holds, as a type)
 template <typename T, typename F>
 void by_kind(const Product &a, F &&f) {
@@ -194,11 +238,6 @@ void run_weight(const Product &a, const WeightPlan &plan, bool tight, bool codes
             a.partial, a.bias_partial, static_cast<T *>(dw), static_cast<T *>(db), a.m, a.n,
             plan.splits);
   }
-}
-
-int grid_for(int64_t work) {
-  const int64_t b = ceil_div(work, dense::kThreads);
-  return static_cast<int>(b > 65536 ? 65536 : (b < 1 ? 1 : b));
 }
 
 template <typename F>
@@ -253,10 +292,16 @@ int linear_forward(const void *x, int dtype, const void *weight, const void *bia
       in_features % chunk_values(dtype) == 0 && aligned16(x) && aligned16(weight);
   hipStream_t st = static_cast<hipStream_t>(stream);
   by_type(dtype, [&](auto t) {
+    using T = decltype(t);
+    if (few_rows<T>(a.m)) {
+      if (codes != nullptr && a.k > 0) run_checkpoint<T>(x, a.codes, scales, rows, a.k, st);
+      run_vector<T>(a, st);
+      return;
+    }
     if (codes != nullptr) {
-      run_rows<decltype(t), Job::kForward, Kind::kKept>(a, tight, st);
+      run_rows<T, Job::kForward, Kind::kKept>(a, tight, st);
     } else {
-      run_rows<decltype(t), Job::kForward, Kind::kPlain>(a, tight, st);
+      run_rows<T, Job::kForward, Kind::kPlain>(a, tight, st);
     }
   });
   return check_launch("linear_forward");
@@ -273,13 +318,10 @@ int linear_checkpoint(const void *x, int dtype, int8_t *codes, uint8_t *scales, 
   if (reinterpret_cast<uintptr_t>(codes) % 8 != 0) {
     return fail(MUSPACE_EINVAL, "linear_checkpoint: codes must be 8-byte aligned");
   }
-  const int64_t work = rows * (((in_features + 31) & ~int64_t{31}) / chunk_values(dtype));
   hipStream_t st = static_cast<hipStream_t>(stream);
   by_type(dtype, [&](auto t) {
-    using T = decltype(t);
-    dense::linear_checkpoint<T><<<grid_for(work), dense::kThreads, 0, st>>>(
-        static_cast<const T *>(x), reinterpret_cast<uint8_t *>(codes), scales, rows,
-        static_cast<int>(in_features));
+    run_checkpoint<decltype(t)>(x, reinterpret_cast<uint8_t *>(codes), scales, rows,
+                                in_features, st);
   });
   return check_launch("linear_checkpoint");
 }

@@ -1,11 +1,13 @@
 // Kernels of the dense layer (include/muspace_layer.h):
 //
-//   y  = act(x W^T + b) + r          linear_product<Job::kForward> or linear_few
+//   y  = act(x W^T + b) + r          linear_product<Job::kForward>, linear_few or
+//                                    linear_vector
 //   dz = g * act'(x W^T + b)         on the fly from a bit mask (relu), or
 //                                    linear_gelu_grad (gelu, from the kept x W^T + b)
 //   dx = dz W                        linear_product<Job::kInput> or linear_few
 //   dW = dz^T x, db = sum of dz      linear_product<Job::kWeight> + linear_weight_sum
-//   x in 8 bits                      linear_checkpoint; read back by kWeight's loader
+//   x in 8 bits                      written by the forward as it reads x (Kind::kKept), or
+//                                    linear_checkpoint; read back by kWeight's loader
 //
 // linear_product: a workgroup of four wavefronts makes a BM x BN tile of the
 // result, each wavefront a quarter. Both operands go through LDS in steps of 128
@@ -395,7 +397,8 @@ __device__ __forceinline__ void finish_forward(const Product &a, int64_t row, in
 // Three workgroups a CU where the registers allow it (168 of them): the loads and
 // stores of one hide behind the products of the others. 16-bit products need 136 to
 // 168 by themselves; float32 ones are held to it where rows are whole chunks (44446 x
-// 256 -> 1024, input gradient: 158 us at two, 144 at three, three registers spilled).
+// 256 -> 1024, input gradient: 158 us at two, 144 at three; the masked gradient
+// spills four registers, the forward that keeps its input eight).
 // Four, at 128 registers, spill; the chunks of two steps in registers cost the third
 // workgroup (369900 x 256 -> 256 bf16 94 -> 113 us); tiles of 64 x 128 and 128 x 64
 // read more per product (114 and 104 us).
@@ -450,7 +453,9 @@ __global__ __launch_bounds__(kThreads, (sizeof(T) == 4 && kTight) ? 3 : 2) void 
   float sums[kV] = {};
   const bool sum_p = kJob == Job::kWeight && col0 == 0;
 
-  // the checkpoint's rows are shared out among the first columns of tiles
+  // The checkpoint's rows are shared out among the first columns of tiles. 40000 x 256 -> 512
+  // bf16: a launch of its own and the plain forward 7.7 + 23.7 us, all rows with the first
+  // column 32.8, shared 26.5; 1800 x 1024 -> 256 float32: 4.2 + 15.3 us, shared 18.1.
   const int keepers = min(a.tiles_n, static_cast<int>(P::kCount)), keeper = tile % a.tiles_n;
 
   char *const tile_p = lds, *const tile_q = lds + P::kPlanes * P::kPlaneBytes;
@@ -756,6 +761,111 @@ __global__ __launch_bounds__(kWaves *kWave) void linear_few(const Product a) {
       loose_store(static_cast<T *>(a.out) + row * a.n + col, pack<T>(z), left);
     }
   }
+}
+
+// --------------------------------------------------------- a row or a few ---
+
+// The forward of up to kRows rows: reading W is all of it, and it takes many loads in
+// flight on many CUs, not matrix cores that would multiply 32 rows. A wavefront takes
+// kCols rows of W whole, its lanes 16 bytes of each at a time, multiplies them with the
+// rows of x (in the caches after the first wavefront) on the vector unit and sums over its
+// lanes. A workgroup makes eight columns, a byte of the mask.
+template <typename T, int kRows, int kCols>
+__global__ __launch_bounds__(8 / kCols *kWave) void linear_vector(const Product a) {
+  constexpr int kV = Piece<T>::kValues;
+  constexpr int kAhead = 4;  // of a lane's chunks, in flight together
+  constexpr int kSpan = kWave * kV;
+  constexpr int kLanes = 8 / kV;  // of a result row, at the end
+  static_assert(kRows * kLanes <= kWave && kRows * kCols <= kWave, "one wavefront ends it");
+  __shared__ __attribute__((aligned(16))) float lds[kRows * 8];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int first = blockIdx.x * 8, col0 = first + wave * kCols;
+  const T *w[kCols], *x[kRows];
+#pragma unroll
+  for (int c = 0; c < kCols; ++c) {
+    w[c] = static_cast<const T *>(a.q) + min(col0 + c, a.n - 1) * a.ldq;
+  }
+#pragma unroll
+  for (int m = 0; m < kRows; ++m) x[m] = static_cast<const T *>(a.p) + min(m, a.m - 1) * a.ldp;
+  const int col = first + lane % kLanes * kV, row = lane / kLanes;
+  float bias[kV] = {};
+  if (wave == 0 && a.bias != nullptr) {
+    load_bias<T>(static_cast<const T *>(a.bias) + col, a.n - col, bias);
+  }
+  float sum[kRows][kCols] = {};
+  // the products of one chunk each, but for the first `drop` values
+  auto add = [&](const u32x4(&wv)[kCols], const u32x4(&xv)[kRows], int drop) {
+    float f[kCols][kV];
+#pragma unroll
+    for (int c = 0; c < kCols; ++c) {
+      unpack<T>(wv[c], f[c]);
+#pragma unroll
+      for (int e = 0; e < kV; ++e) f[c][e] = e < drop ? 0.0f : f[c][e];
+    }
+#pragma unroll
+    for (int m = 0; m < kRows; ++m) {
+      float g[kV];
+      unpack<T>(xv[m], g);
+#pragma unroll
+      for (int e = 0; e < kV; ++e) g[e] = e < drop ? 0.0f : g[e];
+#pragma unroll
+      for (int c = 0; c < kCols; ++c) {
+#pragma unroll
+        for (int e = 0; e < kV; ++e) sum[m][c] = fmaf(g[e], f[c][e], sum[m][c]);
+      }
+    }
+  };
+  int k0 = lane * kV;
+  for (; k0 - lane * kV + kAhead * kSpan <= a.k; k0 += kAhead * kSpan) {
+    u32x4 wv[kAhead][kCols], xv[kAhead][kRows];
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      const int k = k0 + i * kSpan;
+#pragma unroll
+      for (int c = 0; c < kCols; ++c) wv[i][c] = reinterpret_cast<const Loose16 *>(w[c] + k)->v;
+#pragma unroll
+      for (int m = 0; m < kRows; ++m) xv[i][m] = reinterpret_cast<const Loose16 *>(x[m] + k)->v;
+    }
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) add(wv[i], xv[i], 0);
+  }
+  for (; k0 < a.k; k0 += kSpan) {
+    u32x4 wv[kCols], xv[kRows];
+    if (a.k >= kV) {
+      // a chunk that passes the end: the rows' last 16 bytes, less what came before
+      const int k = min(k0, a.k - kV);
+#pragma unroll
+      for (int c = 0; c < kCols; ++c) wv[c] = reinterpret_cast<const Loose16 *>(w[c] + k)->v;
+#pragma unroll
+      for (int m = 0; m < kRows; ++m) xv[m] = reinterpret_cast<const Loose16 *>(x[m] + k)->v;
+      add(wv, xv, k0 - k);
+    } else {
+#pragma unroll
+      for (int c = 0; c < kCols; ++c) wv[c] = loose_load<T>(w[c], a.k);
+#pragma unroll
+      for (int m = 0; m < kRows; ++m) xv[m] = loose_load<T>(x[m], a.k);
+      add(wv, xv, 0);
+    }
+  }
+  float mine = 0.0f;
+#pragma unroll
+  for (int m = 0; m < kRows; ++m) {
+#pragma unroll
+    for (int c = 0; c < kCols; ++c) {
+      float v = sum[m][c];
+      v = add_across<8>(add_across<4>(add_across<2>(add_across<1>(v))));
+      v = add_across<32>(add_across<16>(v));
+      if (lane == m * kCols + c && col0 + c < a.n) mine = v;
+    }
+  }
+  if (lane < kRows * kCols) lds[lane / kCols * 8 + wave * kCols + lane % kCols] = mine;
+  __syncthreads();
+  if (wave != 0) return;
+  float z[kV];
+#pragma unroll
+  for (int e = 0; e < kV; ++e) z[e] = lds[min(row, kRows - 1) * 8 + col - first + e] + bias[e];
+  // the whole wavefront: the mask's halves are exchanged between lanes
+  finish_forward<T>(a, row, col, row < min(kRows, a.m) ? a.n - col : 0, z);
 }
 
 // ----------------------------------------------------- gradient's last step ---

@@ -156,6 +156,46 @@ def test_checkpoint_codes_are_exact(cols, dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows", [1, 2, 3, 4, 5, 7, 8, 9])
+@pytest.mark.parametrize(
+    ("inner", "outer", "activation"),
+    [(3, 5, "relu"), (8, 1, None), (9, 130, "relu"), (203, 611, "gelu"), (512, 64, "relu"),
+     (1027, 70, "relu"), (2048, 24, "gelu"), (4112, 33, None)], ids=str)
+def test_few_rows(rows, inner, outer, activation, dtype):
+    check(*make(rows, inner, outer, dtype, residual=True), activation)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("inner", [3, 64, 203, 2051])
+def test_few_rows_at_any_address(inner, dtype):
+    """The values around each tensor are NaN and must not be read into a result; NaN and
+    infinity inside mark their row (x) or column (W) alone."""
+    x, w, b, r, g = make(3, inner, 37, dtype, residual=True)
+
+    def shifted(t):
+        buffer = torch.full((t.numel() + 9,), math.nan, dtype=t.dtype, device=DEV)
+        view = buffer[1:1 + t.numel()].view(t.shape)
+        view.copy_(t)
+        return view
+
+    xs, ws, bs, rs = (shifted(t) for t in (x, w, b, r))
+    results, bounds = dense_torch.linear(x, w, b, "relu", r, g)
+    clean = linear(xs, ws, bs, activation="relu", residual=rs)
+    assert_within(clean, results[0], bounds[0], "shifted")
+    xs[1, inner - 1] = math.nan
+    ws[36, 0] = math.nan
+    out = linear(xs, ws, bs, activation="relu", residual=rs)
+    assert out[1].isnan().all() and out[:, 36].isnan().all()
+    assert torch.equal(out[::2, :36], clean[::2, :36])
+
+
+def test_one_row_and_most_columns():
+    """The most columns that a call takes, every product one value of W: exact."""
+    w = torch.arange(1 << 20, device=DEV, dtype=torch.int32).to(torch.float32)[:, None]
+    assert torch.equal(linear(torch.full((1, 1), 0.5, device=DEV), w), 0.5 * w.t())
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("size", [(1, 1, 1), (5, 31, 9), (70, 64, 40), (300, 100, 64),
                                   (9000, 203, 136), (20011, 96, 512), (50001, 200, 260)], ids=str)
 def test_checkpoint_of_the_forward_is_the_checkpoint_alone(native_lib, size, dtype):
