@@ -19,7 +19,9 @@
  * relu_mask     [ceil(out / 64), rows, 8] bytes: bit i of byte j of block c is set
  *               where the derivative of relu at z[64 c + 8 j + i] is one (z > 0, or
  *               NaN); bits past out are not read
- * pre_activation [rows, out] z in the tensors' type, kept for gelu's derivative
+ * pre_activation [rows, out] what is kept of z for gelu, an element of the tensors' size
+ *               each: the derivative there, a float32 number or a 16-bit code (the
+ *               library's own, within 2^-16, small ones within a relative 2^-11)
  * codes, scales an 8-bit checkpoint of x: [rows, pad32(in)] int8 and
  *               [rows, pad32(in) / 32] bytes. 32 values share 2^e, the smallest
  *               power of two with 127 * 2^e at or over their largest magnitude;

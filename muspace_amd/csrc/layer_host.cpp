@@ -147,7 +147,7 @@ std::pair<Tensor, Tensor> checkpoint_like(const Tensor &input) {
 }
 
 struct Kept {
-  Tensor activation;     // relu's bits or gelu's pre-activation
+  Tensor activation;     // relu's bits or gelu's derivatives
   Tensor codes, scales;  // the input's checkpoint
 };
 

@@ -282,7 +282,7 @@ int linear_forward(const void *x, int dtype, const void *weight, const void *bia
   a.bias = bias;
   a.residual = residual;
   a.out = output;
-  a.z_out = activation == dense::kGelu ? pre_activation : nullptr;
+  a.slope_out = activation == dense::kGelu ? pre_activation : nullptr;
   a.mask_out = activation == dense::kRelu ? relu_mask : nullptr;
   a.mask_ld = rows * 8;
   a.act = activation;

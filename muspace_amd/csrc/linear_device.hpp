@@ -357,6 +357,59 @@ __device__ __forceinline__ void keep_codes(uint8_t *codes, uint8_t *scales, int6
   if (col % 32 == 0) scales[row * (padded / 32) + col / 32] = static_cast<uint8_t>(scale);
 }
 
+// ---------------------------------------------------------- gelu's slope ---
+
+// What gelu's backward needs of a pre-activation is the derivative there, and it lies in
+// [-0.129, 1.129]: sixteen bits hold it closer than they hold z. From 2^-5 on a code counts
+// steps of 2^-15 (an error of 2^-16 at most; rounding z would cost up to 2^-9.6 in bfloat16,
+// 2^-12.6 in float16), below that it is the float16 number, which keeps the relative
+// accuracy of the tails. float32 keeps the derivative itself.
+constexpr uint32_t kTailCodes = 0x2800u;               // float16 numbers under 2^-5
+constexpr uint32_t kZeroStep = 2 * kTailCodes + 4230u;  // code of step 0; steps from -4229 on
+constexpr uint32_t kSlopeNan = 0xffffu;
+
+__device__ __forceinline__ uint32_t slope_code(float s) {
+  const uint32_t tail = __half_as_ushort(__float2half(fabsf(s)));
+  const uint32_t step = kZeroStep + static_cast<uint32_t>(static_cast<int>(rintf(s * 32768.0f)));
+  const uint32_t code = tail < kTailCodes ? tail + (s < 0.0f ? kTailCodes : 0u) : step;
+  return s == s ? code : kSlopeNan;
+}
+
+__device__ __forceinline__ float slope_value(uint32_t code) {
+  const bool below = code >= kTailCodes;
+  const float tail = __half2float(__ushort_as_half(
+      static_cast<unsigned short>(below ? code - kTailCodes : code)));
+  const float step = static_cast<float>(static_cast<int>(code) - static_cast<int>(kZeroStep)) *
+                     0x1p-15f;
+  const float s = code >= 2 * kTailCodes ? step : below ? -tail : tail;
+  return code == kSlopeNan ? __uint_as_float(0x7fc00000u) : s;
+}
+
+// A chunk of derivatives as it is kept.
+template <typename T>
+__device__ __forceinline__ u32x4 pack_slopes(const float (&s)[Piece<T>::kValues]) {
+  if constexpr (sizeof(T) == 4) {
+    return pack<T>(s);
+  } else {
+    u32x4 o;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) o[i] = slope_code(s[2 * i]) | slope_code(s[2 * i + 1]) << 16;
+    return o;
+  }
+}
+template <typename T>
+__device__ __forceinline__ void unpack_slopes(const u32x4 &v, float (&s)[Piece<T>::kValues]) {
+  if constexpr (sizeof(T) == 4) {
+    unpack<T>(v, s);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      s[2 * i] = slope_value(v[i] & 0xffffu);
+      s[2 * i + 1] = slope_value(v[i] >> 16);
+    }
+  }
+}
+
 // ----------------------------------------------------------- three planes ---
 
 // Four float32 values as kPlanes bfloat16 numbers each, the largest first.

@@ -3,7 +3,7 @@
 //   y  = act(x W^T + b) + r          linear_product<Job::kForward>, linear_few or
 //                                    linear_vector
 //   dz = g * act'(x W^T + b)         on the fly from a bit mask (relu), or
-//                                    linear_gelu_grad (gelu, from the kept x W^T + b)
+//                                    linear_gelu_grad (gelu, from the kept derivative)
 //   dx = dz W                        linear_product<Job::kInput> or linear_few
 //   dW = dz^T x, db = sum of dz      linear_product<Job::kWeight> + linear_weight_sum
 //   x in 8 bits                      written by the forward as it reads x (Kind::kKept), or
@@ -48,7 +48,7 @@ struct Product {
   int splits, k_split;   // kWeight: parts of k, steps' values in each
   // forward
   const void *bias, *residual;
-  void *out, *z_out;     // z_out: kept x W^T + b (gelu under training)
+  void *out, *slope_out;  // slope_out: kept derivative (gelu under training)
   uint8_t *mask_out;     // kept sign bits (relu under training), as mask
   int act;
   uint8_t *codes, *code_scales;  // Kind::kKept: the checkpoint of x
@@ -327,18 +327,14 @@ __device__ __forceinline__ float normal_cdf(float z, float &density) {
   return z < 0.0f ? tail : 1.0f - tail;
 }
 
-// z where the other factor is zero must be finite: infinite pre-activations (or kept ones
-// past float16's range) have the limits' value and slope. NaN stays, in the cdf.
-__device__ __forceinline__ float gelu(float z) {
+// gelu and its derivative. z where the other factor is zero must be finite: infinite
+// pre-activations have the limits' value and slope. NaN stays, in the cdf.
+__device__ __forceinline__ float gelu(float z, float &slope) {
   float density;
   const float cdf = normal_cdf(z, density);
-  return fmaxf(z, -64.0f) * cdf;
-}
-
-__device__ __forceinline__ float gelu_slope(float z) {
-  float density;
-  const float cdf = normal_cdf(z, density);
-  return fmaf(fminf(fmaxf(z, -64.0f), 64.0f) * 0.39894228f, density, cdf);
+  const float low = fmaxf(z, -64.0f);
+  slope = fmaf(fminf(low, 64.0f) * 0.39894228f, density, cdf);
+  return low * cdf;
 }
 
 // `left` values of bias from `p` on
@@ -376,11 +372,12 @@ __device__ __forceinline__ void finish_forward(const Product &a, int64_t row, in
       }
     }
   } else if (a.act == kGelu) {
-    if (a.z_out != nullptr && left > 0) {
-      loose_store(static_cast<T *>(a.z_out) + at, pack<T>(z), left);
-    }
+    float slope[kV];
 #pragma unroll
-    for (int i = 0; i < kV; ++i) z[i] = gelu(z[i]);
+    for (int i = 0; i < kV; ++i) z[i] = gelu(z[i], slope[i]);
+    if (a.slope_out != nullptr && left > 0) {
+      loose_store(static_cast<T *>(a.slope_out) + at, pack_slopes<T>(slope), left);
+    }
   }
   if (left <= 0) return;
   if (a.residual != nullptr) {
@@ -938,15 +935,15 @@ __device__ __forceinline__ int64_t divide(int64_t i, int d, int &rest) {
   return q;
 }
 
-// dz = g * gelu'(z), z the kept pre-activation. dz is an operand of two matrix products;
+// dz = g * gelu'(z), the derivative as the forward kept it. dz is an operand of two matrix products;
 // in a 16-bit type it is written as two numbers, itself rounded and what the rounding
 // left, which the products add: rounded once, dz would cost the gradients as much
 // precision again as their own rounding does. A dz past the type's range becomes its
 // largest number and the rest. Rows are padded with zeros to whole chunks, which the
 // products then read as if they were aligned, whatever the number of columns.
 template <typename T>
-__global__ __launch_bounds__(kThreads) void linear_gelu_grad(const T *g, const T *z, T *dz, T *rest,
-                                                             int64_t rows, int cols) {
+__global__ __launch_bounds__(kThreads) void linear_gelu_grad(const T *g, const T *slope, T *dz,
+                                                             T *rest, int64_t rows, int cols) {
   constexpr int kV = Piece<T>::kValues;
   constexpr float kLargest = std::is_same_v<T, __half> ? 65504.0f : 3.38953139e38f;
   const int per_row = (cols + kV - 1) / kV;
@@ -958,9 +955,9 @@ __global__ __launch_bounds__(kThreads) void linear_gelu_grad(const T *g, const T
     const int col = chunk * kV;
     float a[kV], b[kV];
     unpack<T>(loose_load<T>(g + row * cols + col, cols - col), a);
-    unpack<T>(loose_load<T>(z + row * cols + col, cols - col), b);
+    unpack_slopes<T>(loose_load<T>(slope + row * cols + col, cols - col), b);
 #pragma unroll
-    for (int e = 0; e < kV; ++e) a[e] *= gelu_slope(b[e]);
+    for (int e = 0; e < kV; ++e) a[e] *= b[e];
     u32x4 *const to = reinterpret_cast<u32x4 *>(dz) + i;
     if constexpr (sizeof(T) == 2) {
       float h[kV];

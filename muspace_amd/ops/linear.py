@@ -8,7 +8,7 @@ a bias, sometimes an activation, often the layer's input:
 
 ``linear`` computes this in one kernel, on the matrix cores with float32 sums,
 rounded once. Its backward recomputes nothing and keeps little: relu keeps one
-bit per value (not the output), gelu the pre-activation, and the input either
+bit per value (not the output), gelu its derivative in the type's size, and the input either
 as it is or, with ``checkpoint="int8"``, in 8 bits: blocks of 32 values share a
 power of two, and the weight's gradient is the product with exactly the values
 that were kept (``checkpoint_int8``, ``checkpoint_restore``). Such a call keeps

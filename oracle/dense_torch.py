@@ -35,6 +35,16 @@ def gelu_slope(z):
             + z * torch.exp(-0.5 * z * z) / math.sqrt(2.0 * math.pi))
 
 
+def kept_slope_error(slope, dtype):
+    """Of gelu's derivatives of up to these magnitudes as a backward keeps them: float32
+    rounds them; 16 bits hold steps of 2^-15 from 2^-5 on, below that float16 numbers
+    (subnormal under 2^-14, in steps of 2^-24)."""
+    if dtype == torch.float32:
+        return 2.0**-24 * slope
+    return torch.where(slope < 2.0**-5, torch.maximum(2.0**-11 * slope, slope.new_tensor(2.0**-25)),
+                       slope.new_tensor(2.0**-16))
+
+
 def checkpoint(x):
     """(codes, scale bytes, restored values) of a finite or non-finite x [rows, cols]."""
     dtype = x.dtype
@@ -89,9 +99,10 @@ def linear(x, weight, bias, activation, residual, grad=None, kept=None):
     dz = g * slope
     dz_err = torch.zeros_like(dz)
     if activation == "gelu":
-        # the kept z is rounded to the type (|slope'| < 0.8), the slope is a float32
-        # function of it, dz is held to twice the type's bits (float32's at most)
-        dz_err = g.abs() * (0.8 * (z_err + u * z.abs() + small) + 16 * SUM_STEP)
+        # the slope (|slope'| < 0.8) is a float32 function of z and kept in the type's size;
+        # dz is held to twice the type's bits (float32's at most)
+        slope_err = 0.8 * z_err + 16 * SUM_STEP
+        dz_err = g.abs() * (slope_err + kept_slope_error(slope.abs() + slope_err, dtype))
         dz_err = dz_err + max(u * u, SUM_STEP) * dz.abs() + small
     dx = dz @ w
     dx_err = (dz_err @ w.abs()

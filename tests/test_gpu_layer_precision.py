@@ -1,0 +1,100 @@
+"""What the dense operators' results may lose besides their one rounding, on the GPU
+against float64: root mean squares over whole tensors, where a bound per element would
+have to allow the worst order of a sum."""
+
+import math
+
+import pytest
+import torch
+
+from muspace_amd import linear
+from oracle import dense_torch
+
+pytestmark = pytest.mark.gpu
+
+DEV = "cuda"
+
+
+def normal(gen, *shape):
+    return torch.randn(shape, generator=gen, device=DEV)
+
+
+def rms(t):
+    return float(t.double().square().mean().sqrt())
+
+
+# ------------------------------------------------------------ gelu's slope ---
+
+
+def slope_values(codes):
+    """The derivatives that 16-bit codes stand for: float16 numbers under 2^-5 (the negative
+    ones after the positive), then steps of 2^-15, then NaN."""
+    c = codes.to(torch.int64) & 0xFFFF
+    tails = 0x2800
+    bits = torch.where(c < tails, c, c - tails).clamp(0, tails - 1)
+    tail = bits.to(torch.int16).view(torch.float16).double()
+    tail = torch.where(c < tails, tail, -tail)
+    step = (c - (2 * tails + 4230)).double() * 2.0**-15
+    return torch.where(c < 2 * tails, tail, torch.where(c == 0xFFFF, math.nan, step))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+def test_kept_slopes(native_lib, dtype):
+    """Every kept derivative against the exact one, tails and crossings of zero included."""
+    z = torch.cat([torch.linspace(-14.0, 14.0, 20001, device=DEV),
+                   torch.linspace(-0.76, -0.74, 401, device=DEV),
+                   torch.tensor([0.0, -0.0, 300.0, -300.0, math.inf, -math.inf, math.nan],
+                                device=DEV)]).to(dtype)
+    rows = z.numel()
+    w = torch.ones((1, 1), dtype=dtype, device=DEV)
+    out, kept = (torch.empty((rows, 1), dtype=dtype, device=DEV) for _ in range(2))
+    native_lib.linear_forward(z.view(rows, 1), w, None, None, out, kept, 2)
+    kept = kept.view(rows)
+    values = kept.double() if dtype == torch.float32 else slope_values(kept.view(torch.int16))
+    assert values[-1].isnan() and values[-7:-1].tolist() == [0.5, 0.5, 1.0, 0.0, 1.0, 0.0]
+    values, exact = values[:-7], dense_torch.gelu_slope(z[:-7].double())
+    # z is exact here. Relative to each term, z Phi' and Phi, the float32 evaluation of
+    # exp(-z^2 / 2) errs by the roundings of z^2, of log2(e) / 2 and of their product, which
+    # add up to 3 2^-24 z^2 / 2; 20 covers the other roundings. exp(-z^2 / 2) under the normal
+    # numbers, 2^-126, may be zero: that moves z Phi' by less than |z| 2^-126 and Phi by less
+    # than 2^-126.
+    zd = z[:-7].double()
+    density = torch.exp(-0.5 * zd * zd) / math.sqrt(2.0 * math.pi)
+    terms = (zd * density).abs() + 0.5 * torch.special.erfc(-zd * math.sqrt(0.5))
+    computed = terms * (20 + 1.5 * zd * zd) * 2.0**-24
+    bound = computed + dense_torch.kept_slope_error(exact.abs() + computed, dtype)
+    assert ((values - exact).abs() <= bound + (1 + zd.abs()) * 2.0**-126).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("size", [(6000, 203, 611), (5000, 256, 512), (70, 96, 64)], ids=str)
+def test_gelu_gradients_err_by_their_rounding(size, dtype):
+    """The gradients' error is that of the formula in float32, rounded once: what is kept of
+    the pre-activation in 16 bits adds less than 2%. A kept derivative is off by 2^-15 /
+    sqrt(12) = 8.8e-6 (root mean square; smaller ones by less), dz as two numbers of a
+    16-bit type by at most 2^-16 relative. Errors of single terms are independent, so
+    that the products' relative error is of that size against dz's root mean square of
+    about 0.6: under 2e-5, while the results' own rounding is 2e-4 in float16 and 1.6e-3
+    in bfloat16. Squares add: under 1% more."""
+    rows, inner, outer = size
+    gen = torch.Generator(device=DEV).manual_seed(7)
+    x = normal(gen, rows, inner).to(dtype)
+    w = (normal(gen, outer, inner) / math.sqrt(inner)).to(dtype)
+    b = (0.1 * normal(gen, outer)).to(dtype)
+    g = normal(gen, rows, outer).to(dtype)
+    leaves = [t.clone().requires_grad_() for t in (x, w, b)]
+    grads = torch.autograd.grad(linear(*leaves, activation="gelu"), leaves, g)
+
+    def formula(kind):
+        xs, ws, bs, gs = (t.to(kind) for t in (x, w, b, g))
+        z = xs @ ws.t() + bs
+        dz = gs * (0.5 * torch.special.erfc(-z * math.sqrt(0.5))
+                   + z * torch.exp(-0.5 * z * z) / math.sqrt(2.0 * math.pi))
+        return dz @ ws, dz.t() @ xs, dz.sum(0)
+
+    for name, got, plain, exact in zip(("grad_input", "grad_weight", "grad_bias"), grads,
+                                       formula(torch.float32), formula(torch.float64)):
+        if got.numel() < 4096:
+            continue  # too few roundings for their root mean square to be known to 2%
+        ratio = rms(got.double() - exact) / rms(plain.to(dtype).double() - exact)
+        assert ratio <= 1.02, (name, ratio)
