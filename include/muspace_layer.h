@@ -82,7 +82,8 @@ MUSPACE_API int linear_backward(const void *grad_output, int dtype, const void *
  *   c = x - mean(x);  s = 1 / sqrt(mean(c^2) + eps);  output = c s weight + bias
  * x, output [rows, cols]; weight, bias [cols] of weight_dtype (dtype or float32),
  * each may be NULL (ones, zeros). statistics [rows, 2] float32 or NULL: the mean
- * as an offset from the row's first value, and s; the backward reads them. */
+ * as an offset from the row's first value, and s; or, where the mean is nearer to
+ * zero, the mean itself and -s. The backward reads them. */
 MUSPACE_API int layer_norm_forward(const void *x, int dtype, const void *weight, const void *bias,
                                    int weight_dtype, void *output, float *statistics, int64_t rows,
                                    int64_t cols, float eps, void *stream);

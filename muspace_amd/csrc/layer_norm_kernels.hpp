@@ -9,10 +9,15 @@
 // kChunks 16-byte pieces at a stride of kLanes; a wavefront holds several short
 // rows. Wavefronts walk the rows with the next row's pieces on their way.
 //
-// The mean is taken of x - x0, x0 the row's first value: rows far from zero lose
-// nothing to the sum, and a constant row gives c = 0 exactly. |x0 - mean| is at
-// most sqrt(cols) standard deviations, so the shift itself costs no accuracy.
-// Kept for the backward: the mean's offset from x0, and s.
+// The mean is held as an offset from a base, the row's first value x0 or zero, the
+// nearer of the two: c = (x - base) - offset. Rows far from zero, where float32 has
+// few bits for a mean, are then as exact as the differences of their values, a
+// constant row gives c = 0 exactly, and a first value far from the others (a channel
+// of large activation) does not set the size at which they are rounded. A first
+// reduction sums x - x0, which finds base and offset to a few roundings of the row's
+// reach; the second sums c and c^2 together, and the mean of c corrects the offset (and
+// the variance). Kept for the backward: the offset, and s, negative where the base
+// is zero.
 //
 // The backward keeps each column's sums in registers over its rows; workgroups
 // leave one row of sums each, and norm_sum_columns adds them in workgroup order.
@@ -78,12 +83,41 @@ __device__ __forceinline__ void load_weight(const void *p, int col, int left,
 struct Norm {
   const void *x, *weight, *bias, *grad;
   void *out;
-  float *stats;        // [rows][2]: mean - x0, s
+  float *stats;        // [rows][2]: offset, s or -s (keep_centre)
   float *partial;      // [workgroups][2][cols]
   int64_t rows;
   int cols;
   float eps;
 };
+
+// What is subtracted from a row's values: the base, then the offset.
+struct Centre {
+  float base, offset;
+};
+
+// from the first sum; an infinity or NaN ends in the offset, and with it in every value
+__device__ __forceinline__ Centre find_centre(float x0, float mean_from_x0) {
+  const float mean = x0 + mean_from_x0;
+  return fabsf(mean_from_x0) < fabsf(mean) ? Centre{x0, mean_from_x0} : Centre{0.0f, mean};
+}
+
+// s from the second sums, of c and c^2, whose mean goes to the offset. (fma: an infinite
+// sum of squares stays one, whatever the mean's square.)
+__device__ __forceinline__ float correct_centre(Centre &centre, const float (&sums)[2], float inv,
+                                                float eps) {
+  const float rest = sums[0] * inv;
+  centre.offset += rest;
+  return 1.0f / sqrtf(fmaxf(fmaf(-rest, rest, sums[1] * inv), 0.0f) + eps);
+}
+
+__device__ __forceinline__ void keep_centre(float *stats, float x0, const Centre &centre, float s) {
+  stats[0] = centre.offset;
+  stats[1] = centre.base == x0 ? s : -s;
+}
+
+__device__ __forceinline__ Centre kept_centre(float x0, float offset, float s) {
+  return Centre{__float_as_uint(s) >> 31 ? 0.0f : x0, offset};
+}
 
 template <int kLanes>
 struct NormShape {
@@ -172,27 +206,26 @@ __global__ __launch_bounds__(NormShape<kLanes>::kThreads) void norm_forward(cons
     for (int i = 0; i < kChunks; ++i) {
 #pragma unroll
       for (int e = 0; e < kV; ++e) {
-        v[i][e] = kFull || e < Pieces::left(a.cols, lane, i) ? v[i][e] - x0 : 0.0f;
-        sum[0] += v[i][e];
+        sum[0] += kFull || e < Pieces::left(a.cols, lane, i) ? v[i][e] - x0 : 0.0f;
       }
     }
     group_sum<kLanes, 1>(sum, lds);
-    const float mean = sum[0] * inv;
-    float square[1] = {0.0f};
+    Centre centre = find_centre(x0, sum[0] * inv);
+    float sums[2] = {0.0f, 0.0f};
 #pragma unroll
     for (int i = 0; i < kChunks; ++i) {
 #pragma unroll
       for (int e = 0; e < kV; ++e) {
-        v[i][e] = kFull || e < Pieces::left(a.cols, lane, i) ? v[i][e] - mean : 0.0f;
-        square[0] += v[i][e] * v[i][e];
+        v[i][e] -= centre.base;
+        const float c =
+            kFull || e < Pieces::left(a.cols, lane, i) ? v[i][e] - centre.offset : 0.0f;
+        sums[0] += c;
+        sums[1] += c * c;
       }
     }
-    group_sum<kLanes, 1>(square, lds);
-    const float s = 1.0f / sqrtf(square[0] * inv + a.eps);
-    if (a.stats != nullptr && any && lane == 0) {
-      a.stats[2 * row] = mean;
-      a.stats[2 * row + 1] = s;
-    }
+    group_sum<kLanes, 2>(sums, lds);
+    const float s = correct_centre(centre, sums, inv, a.eps);
+    if (a.stats != nullptr && any && lane == 0) keep_centre(a.stats + 2 * row, x0, centre, s);
 #pragma unroll
     for (int i = 0; i < kChunks; ++i) {
       const int col = (lane + i * kLanes) * kV;
@@ -201,7 +234,9 @@ __global__ __launch_bounds__(NormShape<kLanes>::kThreads) void norm_forward(cons
         load_weight<T, kW32>(a.bias, col, a.cols - col, b[i], 0.0f);
       }
 #pragma unroll
-      for (int e = 0; e < kV; ++e) v[i][e] = v[i][e] * s * w[i][e] + b[i][e];
+      for (int e = 0; e < kV; ++e) {
+        v[i][e] = (v[i][e] - centre.offset) * s * w[i][e] + b[i][e];
+      }
       loose_store(out + row * a.cols + col, pack<T>(v[i]),
                   any ? Pieces::left(a.cols, lane, i) : 0);
     }
@@ -232,12 +267,12 @@ __global__ __launch_bounds__(NormShape<kLanes>::kThreads) void norm_backward(con
   const int64_t step = static_cast<int64_t>(gridDim.x) * Shape::kGroups;
   int64_t row = static_cast<int64_t>(blockIdx.x) * Shape::kGroups + group;
   Pieces nx, ng;
-  float n_mean = 0.0f, n_s = 0.0f;
+  float n_offset = 0.0f, n_s = 0.0f;
   auto fetch = [&](int64_t r) {
     nx.load(x, r, a.rows, a.cols, lane);
     ng.load(g, r, a.rows, a.cols, lane);
     const f32x2 stats = reinterpret_cast<const f32x2 *>(a.stats)[min(r, a.rows - 1)];
-    n_mean = stats[0];
+    n_offset = stats[0];
     n_s = stats[1];
   };
   fetch(row);
@@ -250,13 +285,14 @@ __global__ __launch_bounds__(NormShape<kLanes>::kThreads) void norm_backward(con
       ng.values(i, a.cols, lane, row < a.rows, u[i]);
     }
     const bool any = row < a.rows;
-    const float mean = n_mean, s = n_s;
+    const float s = fabsf(n_s);
     float x0;
     if constexpr (kLanes > kWave) {
       x0 = to_float(x[row * a.cols]);
     } else {
       x0 = __shfl(h[0][0], 0, kLanes);
     }
+    const Centre centre = kept_centre(x0, n_offset, n_s);
     fetch(row + step);
     float sum[2] = {0.0f, 0.0f};
 #pragma unroll
@@ -268,7 +304,9 @@ __global__ __launch_bounds__(NormShape<kLanes>::kThreads) void norm_backward(con
 #pragma unroll
       for (int e = 0; e < kV; ++e) {
         // the operations of the forward, so that h is the forward's own
-        h[i][e] = kFull || e < Pieces::left(a.cols, lane, i) ? (h[i][e] - x0 - mean) * s : 0.0f;
+        h[i][e] = kFull || e < Pieces::left(a.cols, lane, i)
+                      ? (h[i][e] - centre.base - centre.offset) * s
+                      : 0.0f;
         dw[i][e] += u[i][e] * h[i][e];
         db[i][e] += u[i][e];
         u[i][e] *= w[i][e];
@@ -346,30 +384,30 @@ __global__ __launch_bounds__(256) void norm_forward_long(const Norm a) {
       for (int e = 0; e < kV; ++e) sum[0] += col + e < a.cols ? v[e] - x0 : 0.0f;
     }
     group_sum<256, 1>(sum, lds);
-    const float mean = sum[0] * inv;
-    float square[1] = {0.0f};
+    Centre centre = find_centre(x0, sum[0] * inv);
+    float sums[2] = {0.0f, 0.0f};
     for (int col = threadIdx.x * kV; col < a.cols; col += 256 * kV) {
       float v[kV];
       unpack<T>(loose_load<T>(x + col, a.cols - col), v);
 #pragma unroll
       for (int e = 0; e < kV; ++e) {
-        const float c = col + e < a.cols ? v[e] - x0 - mean : 0.0f;
-        square[0] += c * c;
+        const float c = col + e < a.cols ? v[e] - centre.base - centre.offset : 0.0f;
+        sums[0] += c;
+        sums[1] += c * c;
       }
     }
-    group_sum<256, 1>(square, lds);
-    const float s = 1.0f / sqrtf(square[0] * inv + a.eps);
-    if (a.stats != nullptr && threadIdx.x == 0) {
-      a.stats[2 * row] = mean;
-      a.stats[2 * row + 1] = s;
-    }
+    group_sum<256, 2>(sums, lds);
+    const float s = correct_centre(centre, sums, inv, a.eps);
+    if (a.stats != nullptr && threadIdx.x == 0) keep_centre(a.stats + 2 * row, x0, centre, s);
     for (int col = threadIdx.x * kV; col < a.cols; col += 256 * kV) {
       float v[kV], w[kV], b[kV];
       unpack<T>(loose_load<T>(x + col, a.cols - col), v);
       load_weight<T, kW32>(a.weight, col, a.cols - col, w, 1.0f);
       load_weight<T, kW32>(a.bias, col, a.cols - col, b, 0.0f);
 #pragma unroll
-      for (int e = 0; e < kV; ++e) v[e] = (v[e] - x0 - mean) * s * w[e] + b[e];
+      for (int e = 0; e < kV; ++e) {
+        v[e] = (v[e] - centre.base - centre.offset) * s * w[e] + b[e];
+      }
       loose_store(out + col, pack<T>(v), a.cols - col);
     }
   }
@@ -384,7 +422,8 @@ __global__ __launch_bounds__(256) void norm_backward_long(const Norm a) {
     const T *x = static_cast<const T *>(a.x) + row * a.cols;
     const T *g = static_cast<const T *>(a.grad) + row * a.cols;
     T *dx = static_cast<T *>(a.out) + row * a.cols;
-    const float x0 = to_float(x[0]), mean = a.stats[2 * row], s = a.stats[2 * row + 1];
+    const float kept_s = a.stats[2 * row + 1], s = fabsf(kept_s);
+    const Centre centre = kept_centre(to_float(x[0]), a.stats[2 * row], kept_s);
     float sum[2] = {0.0f, 0.0f};
     for (int pass = 0; pass < 2; ++pass) {
       for (int col = threadIdx.x * kV; col < a.cols; col += 256 * kV) {
@@ -394,7 +433,7 @@ __global__ __launch_bounds__(256) void norm_backward_long(const Norm a) {
         load_weight<T, kW32>(a.weight, col, a.cols - col, w, 1.0f);
 #pragma unroll
         for (int e = 0; e < kV; ++e) {
-          h[e] = (h[e] - x0 - mean) * s;
+          h[e] = (h[e] - centre.base - centre.offset) * s;
           u[e] *= w[e];
           if (pass == 0) {
             sum[0] += col + e < a.cols ? u[e] : 0.0f;
@@ -425,13 +464,14 @@ __global__ __launch_bounds__(256) void norm_columns_long(const Norm a) {
   for (int64_t row = blockIdx.y; row < a.rows; row += gridDim.y) {
     const T *x = static_cast<const T *>(a.x) + row * a.cols;
     const T *g = static_cast<const T *>(a.grad) + row * a.cols;
-    const float x0 = to_float(x[0]), mean = a.stats[2 * row], s = a.stats[2 * row + 1];
+    const float kept_s = a.stats[2 * row + 1], s = fabsf(kept_s);
+    const Centre centre = kept_centre(to_float(x[0]), a.stats[2 * row], kept_s);
     float h[kV], u[kV];
     unpack<T>(loose_load<T>(x + col, left), h);
     unpack<T>(loose_load<T>(g + col, left), u);
 #pragma unroll
     for (int e = 0; e < kV; ++e) {
-      dw[e] += u[e] * ((h[e] - x0 - mean) * s);
+      dw[e] += u[e] * ((h[e] - centre.base - centre.offset) * s);
       db[e] += u[e];
     }
   }

@@ -122,10 +122,13 @@ def linear(x, weight, bias, activation, residual, grad=None, kept=None):
 def layer_norm(x, weight, bias, eps, grad=None):
     """([results], [bounds]): y, and with ``grad`` dx, dw, db (of the weight's type).
 
-    With d = x - x0 (x0 the row's first value) every |d| is at most D, the row's
-    largest: d errs by 2^-24 |d|, the mean of d by (n + 2) 2^-23 D, so c by
-    e = (n + 4) 2^-23 D. s errs by a relative (e / sigma)(1 + e / sigma) from c, where
-    sigma = 1 / s, and (n + 8) 2^-23 from its own sums.
+    The bounds are of a two-pass form whose sums over a row have at most D additions on
+    any value's way (a part of the row per lane, then a tree), D = 64 + cols / 256. c = (x -
+    base) - offset, base + offset the mean and |offset| <= min(|mean|, |mean - x0|), x0
+    the row's first value. x - base, the offset and c round once each, and the offset
+    is corrected by the mean of c, so that c errs by e = 2^-24 (2 |c| + 2 |offset| + D mean|c|),
+    whatever the row's largest value. s errs by a relative mean(|c| e) / sigma^2 from
+    c (sigma = 1 / s) and (D + 8) 2^-24 from its own sums and operations.
     """
     dtype, u, small = x.dtype, half_step(x.dtype), tiny(x.dtype)
     wdtype = weight.dtype if weight is not None else dtype
@@ -137,9 +140,10 @@ def layer_norm(x, weight, bias, eps, grad=None):
     c = x - mean
     sigma = (c.square().mean(-1, keepdim=True) + eps).sqrt()
     s = 1.0 / sigma
-    reach = (x - x[:, :1]).abs().amax(-1, keepdim=True)
-    e = (cols + 4) * SUM_STEP * reach
-    s_rel = (e * s) * (1 + e * s) + (cols + 8) * SUM_STEP
+    step, depth = SUM_STEP / 2, 64 + cols // 256
+    offset = torch.minimum(mean.abs(), (mean - x[:, :1]).abs())
+    e = step * (2 * c.abs() + 2 * offset + depth * c.abs().mean(-1, keepdim=True)) * (1 + 2.0**-10)
+    s_rel = (c.abs() * e + e * e).mean(-1, keepdim=True) * s * s + (depth + 8) * step
     h = c * s
     h_err = e * s * (1 + s_rel) + h.abs() * s_rel + SUM_STEP * h.abs()
     y = h * w + b
@@ -151,9 +155,9 @@ def layer_norm(x, weight, bias, eps, grad=None):
     v = g * w
     mv, mh = v.mean(-1, keepdim=True), (v * h).mean(-1, keepdim=True)
     inner = v - mv - h * mh
-    mv_err = (cols + 4) * SUM_STEP * v.abs().mean(-1, keepdim=True)
+    mv_err = (depth + 4) * step * v.abs().mean(-1, keepdim=True)
     mh_err = ((v.abs() * h_err).mean(-1, keepdim=True)
-              + (cols + 4) * SUM_STEP * (v * h).abs().mean(-1, keepdim=True))
+              + (depth + 4) * step * (v * h).abs().mean(-1, keepdim=True))
     inner_err = (mv_err + h_err * (mh.abs() + mh_err) + h.abs() * mh_err
                  + 4 * SUM_STEP * (v.abs() + mv.abs() + (h * mh).abs()))
     dx = s * inner

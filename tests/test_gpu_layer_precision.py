@@ -7,7 +7,7 @@ import math
 import pytest
 import torch
 
-from muspace_amd import linear
+from muspace_amd import layer_norm, linear
 from oracle import dense_torch
 
 pytestmark = pytest.mark.gpu
@@ -98,3 +98,80 @@ def test_gelu_gradients_err_by_their_rounding(size, dtype):
             continue  # too few roundings for their root mean square to be known to 2%
         ratio = rms(got.double() - exact) / rms(plain.to(dtype).double() - exact)
         assert ratio <= 1.02, (name, ratio)
+
+
+# -------------------------------------------------------------- layer norm ---
+
+
+def plain_norm(x, w, b, eps, g, kind):
+    """(y, dx, dw, db) in two passes over x in the floating-point type ``kind``."""
+    x, w, b, g = (t.to(kind) for t in (x, w, b, g))
+    c = x - x.mean(-1, keepdim=True)
+    s = 1.0 / torch.sqrt((c * c).mean(-1, keepdim=True) + eps)
+    h, u = c * s, g * w
+    dx = s * (u - u.mean(-1, keepdim=True) - h * (u * h).mean(-1, keepdim=True))
+    return h * w + b, dx, (g * h).sum(0), g.sum(0)
+
+
+@pytest.mark.parametrize("far", [0.0, 50.0], ids=["around_zero", "far_from_zero"])
+@pytest.mark.parametrize("at", [0, 1, -1], ids=["first", "second", "last"])
+@pytest.mark.parametrize("size", [10.0, 1e3, 1e5], ids=str)
+@pytest.mark.parametrize("cols", [64, 256, 611, 1024, 4096, 20000])
+def test_norm_of_rows_with_a_large_channel(cols, size, at, far):
+    """A channel far from the others, wherever it lies, costs their results nothing: the
+    error is that of the two-pass formula in float32. Both round each value's difference from
+    the mean, and the mean, to float32; three times the plain error allows for the few
+    roundings more of a sum in another order."""
+    gen = torch.Generator(device=DEV).manual_seed(5)
+    rows = 400
+    x = normal(gen, rows, cols) + far
+    x[:, at] = size * (1.0 + 0.1 * normal(gen, rows))
+    w, b = 1.0 + 0.2 * normal(gen, cols), 0.01 * normal(gen, cols)
+    g = normal(gen, rows, cols)
+    leaves = [t.clone().requires_grad_() for t in (x, w, b)]
+    out = layer_norm(*leaves)
+    got = [out.detach(), *torch.autograd.grad(out, leaves, g)]
+    others = [i for i in range(cols) if i != at % cols]
+    exact = plain_norm(x, w, b, 1e-5, g, torch.float64)
+    plain = plain_norm(x, w, b, 1e-5, g, torch.float32)
+    for name, a, p, e in zip(("out", "grad_input", "grad_weight"), got, plain, exact):
+        mine, theirs = (rms((t.double() - e)[..., others]) for t in (a, p))
+        assert mine <= 3 * theirs, (name, mine / theirs)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("cols", [8, 100, 256, 1000, 4096, 20000])
+def test_norm_of_constant_and_nearly_constant_rows(cols, dtype):
+    """Constant rows of any size give the bias itself and gradients without NaN; a step of
+    one value's last bit is seen as such."""
+    gen = torch.Generator(device=DEV).manual_seed(6)
+    info = torch.finfo(dtype)
+    levels = torch.tensor([0.0, 3.3, -1000.0, info.max / 4, -info.max / 4, info.tiny], device=DEV)
+    x = levels[:, None].expand(-1, cols).to(dtype)
+    w, b = ((1.0 + 0.2 * normal(gen, cols)).to(dtype) for _ in range(2))
+    xs = x.clone().requires_grad_()
+    out = layer_norm(xs, w, b)
+    assert torch.equal(out, b.expand_as(out))
+    assert torch.autograd.grad(out, [xs], torch.ones_like(out))[0].isfinite().all()
+    # rows of 1 with one value 1 + eps, first or last: h = sqrt(cols - 1) there and
+    # -1 / sqrt(cols - 1) elsewhere, without eps
+    near = torch.ones((2, cols), dtype=dtype, device=DEV)
+    near[0, 0] = near[1, -1] = 1.0 + info.eps
+    out = layer_norm(near, eps=0.0).double()
+    expected = torch.full((2, cols), -1.0 / math.sqrt(cols - 1), dtype=torch.float64, device=DEV)
+    expected[0, 0] = expected[1, -1] = math.sqrt(cols - 1)
+    # each sum over the row errs by 2^-24 an addition on a value's way. In the first row the
+    # others' mean lies eps from x0, and rounds by 2^-24 of that, as what is left of it
+    # does: against sigma = eps / sqrt(cols), 2 sqrt(cols) 2^-24.
+    slack = info.eps / 2 + (80 + cols / 128) * 2.0**-24
+    bound = slack * expected.abs() + slack / math.sqrt(cols)
+    bound[0] += 2 * math.sqrt(cols) * 2.0**-24
+    assert ((out - expected).abs() <= bound).all()
+
+
+def test_norm_of_values_whose_squares_overflow():
+    """As in the formula: an infinite variance gives zeros, not values of any size."""
+    gen = torch.Generator(device=DEV).manual_seed(7)
+    x = 1e30 * normal(gen, 5, 300)
+    out = layer_norm(x)
+    assert torch.equal(out, torch.zeros_like(out))
