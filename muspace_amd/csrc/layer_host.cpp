@@ -13,10 +13,12 @@
 // std::runtime_error (RuntimeError in Python) with the library's text.
 #include <ATen/ATen.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPStream.h>
 #include <pybind11/stl.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/csrc/utils/pybind.h>
 
 #include <optional>
@@ -135,6 +137,18 @@ bool supported(at::ScalarType type) {
 bool row_of(const OptTensor &t, int64_t size, at::ScalarType type) {
   return !t.has_value() || !t->defined() ||
          (t->dim() == 1 && t->size(0) == size && t->scalar_type() == type);
+}
+
+// Kernels fill tensors that torch has only seen allocated. A tracer would record the
+// allocation alone, and a module traced so would answer with uninitialised memory.
+void refuse_tracing(const char *name) {
+  using Modes = c10::impl::TorchDispatchModeTLS;
+  using Key = c10::impl::TorchDispatchModeKey;
+  if (torch::jit::tracer::isTracing() || Modes::get_mode(Key::PROXY).has_value() ||
+      Modes::get_mode(Key::FUNCTIONAL).has_value() || Modes::get_mode(Key::FAKE).has_value()) {
+    throw std::runtime_error(std::string(name) +
+                             ": HIP kernels cannot be traced (the PyTorch path can)");
+  }
 }
 
 // ------------------------------------------------------------------ linear ---
@@ -256,6 +270,7 @@ bool linear_fits(const Tensor &input, const Tensor &weight, const OptTensor &bia
 OptTensor linear(const Tensor &input, const Tensor &weight, const OptTensor &bias,
                  const OptTensor &residual, int64_t activation, bool checkpoint) {
   if (!linear_fits(input, weight, bias, residual)) return OptTensor();
+  refuse_tracing("linear");
   const c10::DeviceGuard guard(input.device());
   const Tensor x = input.contiguous();
   const Tensor w = prepared(weight, x, "weight"), b = prepared(bias, x, "bias"),
@@ -268,6 +283,7 @@ OptTensor linear(const Tensor &input, const Tensor &weight, const OptTensor &bia
 }
 
 std::pair<Tensor, Tensor> checkpoint(const Tensor &input) {
+  refuse_tracing("checkpoint_int8");
   const c10::DeviceGuard guard(input.device());
   const Tensor x = input.contiguous();
   auto kept = checkpoint_like(x);
@@ -348,6 +364,7 @@ bool norm_fits(const Tensor &input, const OptTensor &weight, const OptTensor &bi
 OptTensor layer_norm(const Tensor &input, const OptTensor &weight, const OptTensor &bias,
                      double eps) {
   if (!norm_fits(input, weight, bias, eps)) return OptTensor();
+  refuse_tracing("layer_norm");
   const c10::DeviceGuard guard(input.device());
   const Tensor x = input.contiguous();
   const Tensor w = prepared(weight, x, "weight"), b = prepared(bias, x, "bias");
