@@ -12,6 +12,7 @@
 // strides and whether a graph is recorded are seen to here. A C-ABI error becomes
 // std::runtime_error (RuntimeError in Python) with the library's text.
 #include <ATen/ATen.h>
+#include <c10/core/AutogradState.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPStream.h>
@@ -151,6 +152,17 @@ void refuse_tracing(const char *name) {
   }
 }
 
+// Forward-mode derivatives are not there, and must not be dropped.
+void refuse_tangents(const char *name, std::initializer_list<const Tensor *> tensors) {
+  if (!c10::AutogradState::get_tls_state().get_fw_grad_mode()) return;
+  for (const Tensor *t : tensors) {
+    if (t->defined() && t->_fw_grad(/*level=*/0).defined()) {
+      throw std::runtime_error(std::string(name) + ": the HIP path has no forward-mode "
+                               "derivatives (the PyTorch path has)");
+    }
+  }
+}
+
 // ------------------------------------------------------------------ linear ---
 
 // room for the 8-bit checkpoint of `input`: codes and scales
@@ -275,6 +287,7 @@ OptTensor linear(const Tensor &input, const Tensor &weight, const OptTensor &bia
   const Tensor x = input.contiguous();
   const Tensor w = prepared(weight, x, "weight"), b = prepared(bias, x, "bias"),
                r = prepared(residual, x, "residual");
+  refuse_tangents("linear", {&x, &w, &b, &r});
   if (at::GradMode::is_enabled() &&
       (wants_grad(x) || wants_grad(w) || wants_grad(b) || wants_grad(r))) {
     return LinearFunction::apply(x, w, opt(b), opt(r), activation, checkpoint);
@@ -368,6 +381,7 @@ OptTensor layer_norm(const Tensor &input, const OptTensor &weight, const OptTens
   const c10::DeviceGuard guard(input.device());
   const Tensor x = input.contiguous();
   const Tensor w = prepared(weight, x, "weight"), b = prepared(bias, x, "bias");
+  refuse_tangents("layer_norm", {&x, &w, &b});
   if (at::GradMode::is_enabled() && (wants_grad(x) || wants_grad(w) || wants_grad(b))) {
     return LayerNormFunction::apply(x, opt(w), opt(b), eps);
   }

@@ -1,7 +1,9 @@
-"""Ways to call the dense operators on the GPU besides the plain ones."""
+"""Ways to call the dense operators on the GPU besides the plain ones: traced, with
+forward-mode derivatives, and of tensors in unusual states."""
 
 import pytest
 import torch
+import torch.autograd.forward_ad as forward_ad
 from torch.fx.experimental.proxy_tensor import make_fx
 
 from muspace_amd import checkpoint_int8, layer_norm, linear
@@ -22,15 +24,34 @@ def calls():
 
 @pytest.mark.parametrize("graph", [False, True])
 @pytest.mark.parametrize("which", ["linear", "checkpointed", "layer_norm"])
-def test_tracing_is_refused(which, graph):
+def test_tracing_and_forward_mode_are_refused(which, graph):
     call = calls()[which]
     x = torch.randn((3, 8), device=DEV, requires_grad=graph)
     for trace in (lambda: torch.jit.trace(call, (x,)), lambda: make_fx(call)(x.detach())):
         with pytest.raises(RuntimeError, match="HIP kernels cannot be traced"):
             trace()
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(x, torch.ones_like(x))
+        with pytest.raises(RuntimeError, match="no forward-mode derivatives"):
+            call(dual)
+    # a tensor without a tangent, and where forward mode is off
     assert call(x).isfinite().all()
     with pytest.raises(RuntimeError, match="HIP kernels cannot be traced"):
         torch.jit.trace(lambda t: checkpoint_int8(t)[0], (x.detach(),))
+
+
+def test_a_weight_with_a_tangent_is_refused():
+    x, w = torch.randn((3, 8), device=DEV), torch.randn((4, 8), device=DEV)
+    b, r = torch.randn(4, device=DEV), torch.randn((3, 4), device=DEV)
+    with forward_ad.dual_level():
+        for i in range(1, 4):
+            given = [x, w, b, r]
+            given[i] = forward_ad.make_dual(given[i], torch.ones_like(given[i]))
+            with pytest.raises(RuntimeError, match="linear: the HIP path has no forward-mode"):
+                linear(*given[:3], residual=given[3])
+        scale = torch.ones(8, device=DEV)
+        with pytest.raises(RuntimeError, match="layer_norm: the HIP path has no forward-mode"):
+            layer_norm(x, scale, forward_ad.make_dual(scale, scale))
 
 
 def test_the_reference_backend_is_traced_on_the_device():

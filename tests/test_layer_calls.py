@@ -3,12 +3,13 @@ itself refuses them before anything runs."""
 
 import pytest
 import torch
+import torch.autograd.forward_ad as forward_ad
 from torch.fx.experimental.proxy_tensor import make_fx
 
 from muspace_amd import layer_norm, linear
 from muspace_amd.runtime.layer_host import load_layer_host
 
-# ----------------------------------------------------------------- tracing ---
+# ------------------------------------------------- tracing, forward mode ---
 
 
 def host_calls():
@@ -32,8 +33,27 @@ def test_host_refuses_to_be_traced(which, graph):
         make_fx(call)(x.detach())
 
 
-def test_the_pytorch_path_is_traced():
+@pytest.mark.parametrize("which", range(3))
+@pytest.mark.parametrize("graph", [False, True])
+def test_host_refuses_forward_mode(which, graph):
+    name, call = host_calls()[which]
+    x = torch.randn(3, 8, requires_grad=graph)
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(x, torch.ones(3, 8))
+        with pytest.raises(RuntimeError, match=f"{name}: the HIP path has no forward-mode"):
+            call(dual)
+        # the same of a view that is copied first
+        dual = forward_ad.make_dual(torch.randn(8, 3), torch.ones(8, 3)).t()
+        with pytest.raises(RuntimeError, match=f"{name}: the HIP path has no forward-mode"):
+            call(dual)
+
+
+def test_the_pytorch_path_is_traced_and_has_forward_mode():
     x, w = torch.randn(3, 8), torch.randn(4, 8)
     traced = torch.jit.trace(lambda t: layer_norm(linear(t, w, activation="relu")), (x,))
     y = torch.randn(3, 8)
     torch.testing.assert_close(traced(y), layer_norm(linear(y, w, activation="relu")))
+    with forward_ad.dual_level():
+        out = linear(forward_ad.make_dual(x, torch.ones(3, 8)), w)
+        torch.testing.assert_close(forward_ad.unpack_dual(out).tangent,
+                                   torch.ones(3, 8) @ w.t())
