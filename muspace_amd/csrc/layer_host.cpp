@@ -96,7 +96,15 @@ int64_t rows_of(const Tensor &t) {
   return rows;
 }
 
-// `t` on the input's device and contiguous; undefined where absent
+// `t` with its values in memory as they are, row by row: a view may also be one that
+// is read with its sign changed (the imaginary part of a conjugate), which a
+// contiguous tensor keeps.
+Tensor dense(const Tensor &t) {
+  const Tensor c = t.contiguous();
+  return c.is_neg() ? c.resolve_neg() : c;
+}
+
+// `t` on the input's device and dense; undefined where absent
 Tensor prepared(const OptTensor &t, const Tensor &input, const char *name) {
   if (!t.has_value() || !t->defined()) return Tensor();
   if (t->device() != input.device()) {
@@ -104,7 +112,7 @@ Tensor prepared(const OptTensor &t, const Tensor &input, const char *name) {
                              input.device().str() + " like the input, got device " +
                              t->device().str());
   }
-  return t->contiguous();
+  return dense(*t);
 }
 
 bool wants_grad(const Tensor &t) { return t.defined() && t.requires_grad(); }
@@ -239,7 +247,7 @@ struct LinearFunction : torch::autograd::Function<LinearFunction> {
       const auto shape = ctx->saved_data["input"].toIntVector();
       const auto wshape = ctx->saved_data["weight"].toIntVector();
       const int activation = static_cast<int>(ctx->saved_data["activation"].toInt());
-      const Tensor g = grads[0].contiguous();
+      const Tensor g = dense(grads[0]);
       const c10::DeviceGuard guard(g.device());
       const int64_t cols = wshape[1], out = wshape[0];
       int64_t rows = 1;
@@ -284,7 +292,7 @@ OptTensor linear(const Tensor &input, const Tensor &weight, const OptTensor &bia
   if (!linear_fits(input, weight, bias, residual)) return OptTensor();
   refuse_tracing("linear");
   const c10::DeviceGuard guard(input.device());
-  const Tensor x = input.contiguous();
+  const Tensor x = dense(input);
   const Tensor w = prepared(weight, x, "weight"), b = prepared(bias, x, "bias"),
                r = prepared(residual, x, "residual");
   refuse_tangents("linear", {&x, &w, &b, &r});
@@ -298,7 +306,7 @@ OptTensor linear(const Tensor &input, const Tensor &weight, const OptTensor &bia
 std::pair<Tensor, Tensor> checkpoint(const Tensor &input) {
   refuse_tracing("checkpoint_int8");
   const c10::DeviceGuard guard(input.device());
-  const Tensor x = input.contiguous();
+  const Tensor x = dense(input);
   auto kept = checkpoint_like(x);
   check(api.linear_checkpoint(x.data_ptr(), code_of(x.scalar_type(), "input"),
                               static_cast<int8_t *>(kept.first.data_ptr()),
@@ -342,7 +350,7 @@ struct LayerNormFunction : torch::autograd::Function<LayerNormFunction> {
     const variable_list saved = ctx->get_saved_variables();
     const Tensor &x = saved[0], &weight = saved[1], &stats = saved[2];
     const auto type = static_cast<at::ScalarType>(ctx->saved_data["type"].toInt());
-    const Tensor g = grads[0].contiguous();
+    const Tensor g = dense(grads[0]);
     const c10::DeviceGuard guard(x.device());
     const int64_t rows = rows_of(x), cols = x.size(-1);
     Tensor grad_input, grad_weight, grad_bias;
@@ -379,7 +387,7 @@ OptTensor layer_norm(const Tensor &input, const OptTensor &weight, const OptTens
   if (!norm_fits(input, weight, bias, eps)) return OptTensor();
   refuse_tracing("layer_norm");
   const c10::DeviceGuard guard(input.device());
-  const Tensor x = input.contiguous();
+  const Tensor x = dense(input);
   const Tensor w = prepared(weight, x, "weight"), b = prepared(bias, x, "bias");
   refuse_tangents("layer_norm", {&x, &w, &b});
   if (at::GradMode::is_enabled() && (wants_grad(x) || wants_grad(w) || wants_grad(b))) {

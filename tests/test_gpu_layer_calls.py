@@ -59,3 +59,34 @@ def test_the_reference_backend_is_traced_on_the_device():
     traced = torch.jit.trace(lambda t: linear(t, w, backend="reference"), (x,))
     y = torch.randn((3, 8), device=DEV)
     torch.testing.assert_close(traced(y), linear(y, w, backend="reference"))
+
+
+@pytest.mark.parametrize("shape", [(1, 1), (5, 8)])
+def test_views_read_with_their_sign_changed(shape):
+    """A contiguous view of another tensor's negative (of one value: the imaginary part of a
+    conjugate) counts with its own values, as an input and as a gradient."""
+    gen = torch.Generator(device=DEV).manual_seed(2)
+    rows, cols = shape
+
+    def negated(*sizes):
+        if sizes == (1, 1):
+            view = torch.randn(sizes, generator=gen, dtype=torch.complex64, device=DEV).conj().imag
+        else:
+            view = torch._neg_view(torch.randn(sizes, generator=gen, device=DEV))
+        assert view.is_neg() and view.is_contiguous()
+        return view
+
+    x, w, r, g = negated(rows, cols), negated(3, cols), negated(rows, 3), negated(rows, 3)
+    h = negated(rows, cols)
+
+    def results(tensors, grads):
+        xs, ws, rs = (t.detach().requires_grad_() for t in tensors)
+        y = linear(xs, ws, residual=rs)
+        n = layer_norm(xs, ws[0])
+        return [y.detach(), n.detach(), *torch.autograd.grad(y, [xs, ws], grads[0]),
+                *torch.autograd.grad(n, [xs, ws], grads[1]), *checkpoint_int8(xs)]
+
+    mine = results((x, w, r), (g, h))
+    plain = results([t.resolve_neg() for t in (x, w, r)], [t.resolve_neg() for t in (g, h)])
+    for a, e in zip(mine, plain):
+        assert torch.equal(a, e)
