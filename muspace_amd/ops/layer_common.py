@@ -35,6 +35,14 @@ def require_native():
     return host
 
 
+def runs_native(input: torch.Tensor) -> bool:
+    """Whether ``backend="auto"`` takes the HIP kernels for ``input`` (or raises without
+    them), not the PyTorch path."""
+    if not is_rocm_tensor(input):
+        return False
+    return explain_dispatch(input, native_available=_native() is not None).backend != "reference"
+
+
 @lru_cache(maxsize=64)
 def _native_report(operator: str, backend: str, device: str) -> DispatchReport:
     # reports of one operator's native calls are equal and immutable: one is enough

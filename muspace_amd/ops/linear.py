@@ -27,9 +27,8 @@ import torch
 import torch.nn.functional as F
 from torch.autograd.function import once_differentiable
 
-from ..runtime.kernel_dispatch import is_rocm_tensor
 from .layer_common import DTYPES as _DTYPES
-from .layer_common import native_for, report_native, report_other, require_native
+from .layer_common import native_for, report_native, report_other, require_native, runs_native
 
 OPERATOR_NAME = "linear"
 BLOCK = 32  # values of a row that share a scale in an 8-bit checkpoint
@@ -41,6 +40,26 @@ _SCALE_RANGE = {torch.float16: (-24, 10), torch.bfloat16: (-126, 122), torch.flo
 
 
 # ------------------------------------------------------------- checkpoints ---
+
+
+def _checkpoint_pytorch(input: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """``checkpoint_int8`` in PyTorch operations, on any device."""
+    cols = input.shape[-1]
+    rows = math.prod(input.shape[:-1])
+    padded = (cols + BLOCK - 1) // BLOCK * BLOCK
+    low, high = _SCALE_RANGE[input.dtype]
+    x = F.pad(input.reshape(rows, cols).float(), (0, padded - cols)).view(rows, -1, BLOCK)
+    finite = torch.isfinite(x).all(-1, keepdim=True)
+    mantissa, exponent = torch.frexp(torch.where(finite, x, 0.0).abs().amax(-1, keepdim=True))
+    exponent = (exponent - 7 + (mantissa > 127.0 / 128.0).int()).clamp_min(low)
+    exponent = torch.where(mantissa == 0, low, exponent)  # a block of zeros
+    limit = torch.where(exponent >= high, 63.0, 127.0)
+    # 2^-e from its bits (a power function may be off by its last one, which would show at
+    # ties): e is in [-126, 122]
+    codes = (x * ((127 - exponent) << 23).view(torch.float32)).round()
+    codes = torch.where(finite, torch.minimum(torch.maximum(codes, -limit), limit), 1.0)
+    scales = torch.where(finite, exponent + 127, 255)
+    return codes.view(rows, padded).to(torch.int8), scales.view(rows, -1).to(torch.uint8)
 
 
 def checkpoint_int8(input: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
@@ -56,24 +75,9 @@ def checkpoint_int8(input: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
         raise TypeError("input must be float16, bfloat16 or float32")
     if input.dim() == 0:
         raise ValueError("input must have at least one dimension")
-    cols = input.shape[-1]
-    rows = math.prod(input.shape[:-1])
-    padded = (cols + BLOCK - 1) // BLOCK * BLOCK
-    if is_rocm_tensor(input):
+    if runs_native(input):
         return require_native().checkpoint(input.detach())
-    low, high = _SCALE_RANGE[input.dtype]
-    x = F.pad(input.reshape(rows, cols).float(), (0, padded - cols)).view(rows, -1, BLOCK)
-    finite = torch.isfinite(x).all(-1, keepdim=True)
-    mantissa, exponent = torch.frexp(torch.where(finite, x, 0.0).abs().amax(-1, keepdim=True))
-    exponent = (exponent - 7 + (mantissa > 127.0 / 128.0).int()).clamp_min(low)
-    exponent = torch.where(mantissa == 0, low, exponent)  # a block of zeros
-    limit = torch.where(exponent >= high, 63.0, 127.0)
-    # two factors: 2^-e alone leaves float32's range of normal numbers
-    half = exponent // 2
-    codes = torch.ldexp(torch.ldexp(x, -half), half - exponent).round()
-    codes = torch.where(finite, torch.minimum(torch.maximum(codes, -limit), limit), 1.0)
-    scales = torch.where(finite, exponent + 127, 255)
-    return codes.view(rows, padded).to(torch.int8), scales.view(rows, -1).to(torch.uint8)
+    return _checkpoint_pytorch(input.detach())
 
 
 def checkpoint_restore(codes: torch.Tensor, scales: torch.Tensor, cols: int,
@@ -106,7 +110,7 @@ class _CheckpointedInput(torch.autograd.Function):
     @staticmethod
     def forward(ctx, input, weight):
         ctx.shape, ctx.dtype = input.shape, input.dtype
-        ctx.save_for_backward(weight, *checkpoint_int8(input))
+        ctx.save_for_backward(weight, *_checkpoint_pytorch(input))
         return F.linear(input, weight)
 
     @staticmethod

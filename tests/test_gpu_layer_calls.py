@@ -1,12 +1,17 @@
 """Ways to call the dense operators on the GPU besides the plain ones: traced, with
 forward-mode derivatives, and of tensors in unusual states."""
 
+import importlib
+import math
+
 import pytest
 import torch
 import torch.autograd.forward_ad as forward_ad
 from torch.fx.experimental.proxy_tensor import make_fx
 
 from muspace_amd import checkpoint_int8, layer_norm, linear
+
+linear_module = importlib.import_module("muspace_amd.ops.linear")  # (the package has the function)
 
 pytestmark = pytest.mark.gpu
 
@@ -90,3 +95,30 @@ def test_views_read_with_their_sign_changed(shape):
     plain = results([t.resolve_neg() for t in (x, w, r)], [t.resolve_neg() for t in (g, h)])
     for a, e in zip(mine, plain):
         assert torch.equal(a, e)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+def test_the_reference_backend_launches_no_kernel_of_the_library(dtype, monkeypatch):
+    """A checkpointed call too; its codes on the device are the kernels' codes."""
+    gen = torch.Generator(device=DEV).manual_seed(3)
+    x = torch.randn((60, 100), generator=gen, device=DEV)
+    x *= torch.exp2(torch.randint(-40, 12, (60, 1), generator=gen, device=DEV).float())
+    x = x.to(dtype)
+    info = torch.finfo(dtype)
+    x[0], x[1], x[2], x[3] = 0.0, info.max, info.smallest_normal / 4, -63.5
+    x[4, 7], x[5, 99] = math.inf, math.nan
+    w = torch.randn((12, 100), generator=gen, device=DEV).to(dtype)
+    codes, scales = checkpoint_int8(x)
+
+    def refuse(*args):
+        raise AssertionError("the HIP library is called")
+
+    monkeypatch.setattr(linear_module, "require_native", refuse)
+    xs, ws = x.clone().requires_grad_(), w.clone().requires_grad_()
+    out = linear(xs, ws, checkpoint="int8", backend="reference")
+    dx, dw = torch.autograd.grad(out, [xs, ws], torch.ones_like(out))
+    # (float16's largest number and 59 others may add up to an infinity)
+    assert dw[:, :32].isnan().all() and dw[:, 96:].isnan().all() and not dw[:, 32:96].isnan().any()
+    assert dx.isfinite().all()
+    mine = linear_module._checkpoint_pytorch(x)
+    assert torch.equal(mine[0], codes) and torch.equal(mine[1], scales)

@@ -1,13 +1,17 @@
-"""Calls of the dense operators that only a part of torch sees, on the CPU: the host module
-itself refuses them before anything runs."""
+"""Calls of the dense operators that are not the plain ones, on the CPU: what the host module
+refuses before anything runs, and what the PyTorch path does in its place."""
+
+import importlib
 
 import pytest
 import torch
 import torch.autograd.forward_ad as forward_ad
 from torch.fx.experimental.proxy_tensor import make_fx
 
-from muspace_amd import layer_norm, linear
+from muspace_amd import checkpoint_int8, get_last_dispatch_report, layer_norm, linear
 from muspace_amd.runtime.layer_host import load_layer_host
+
+linear_module = importlib.import_module("muspace_amd.ops.linear")  # (the package has the function)
 
 # ------------------------------------------------- tracing, forward mode ---
 
@@ -57,3 +61,50 @@ def test_the_pytorch_path_is_traced_and_has_forward_mode():
         out = linear(forward_ad.make_dual(x, torch.ones(3, 8)), w)
         torch.testing.assert_close(forward_ad.unpack_dual(out).tangent,
                                    torch.ones(3, 8) @ w.t())
+
+
+# ------------------------------------------------------- the PyTorch path ---
+
+
+@pytest.fixture
+def device_without_library(monkeypatch, tmp_path):
+    """CPU tensors count as ROCm tensors, and the host module is missing."""
+    from muspace_amd.ops import layer_common
+    from muspace_amd.runtime import kernel_dispatch, layer_host
+
+    monkeypatch.setattr(layer_host, "module_path", lambda: tmp_path / "missing.so")
+    monkeypatch.setattr(layer_common, "is_rocm_tensor", lambda t: True)
+    monkeypatch.setattr(kernel_dispatch, "is_rocm_tensor", lambda t: True)
+    if hasattr(linear_module, "is_rocm_tensor"):
+        monkeypatch.setattr(linear_module, "is_rocm_tensor", lambda t: True)
+    layer_host.load_layer_host.cache_clear()
+    yield
+    layer_host.load_layer_host.cache_clear()
+
+
+def checkpointed_step(**kwargs):
+    gen = torch.Generator().manual_seed(4)
+    x, w = torch.randn((6, 40), generator=gen), torch.randn((5, 40), generator=gen)
+    xs, ws = x.clone().requires_grad_(), w.clone().requires_grad_()
+    out = linear(xs, ws, checkpoint="int8", **kwargs)
+    return [out.detach(), *torch.autograd.grad(out.square().sum(), [xs, ws]), *checkpoint_int8(x)]
+
+
+def test_the_fallback_has_checkpoints(device_without_library, monkeypatch):
+    """Where a missing library degrades to the PyTorch path, a checkpointed call does too."""
+    with pytest.raises(RuntimeError, match="missing from this installation"):
+        linear(torch.zeros(2, 4), torch.zeros(3, 4), checkpoint="int8")
+    with pytest.raises(RuntimeError, match="missing from this installation"):
+        checkpoint_int8(torch.zeros(2, 4))
+    monkeypatch.setenv("MUSPACE_AUTO_FALLBACK", "1")
+    got = checkpointed_step()
+    assert get_last_dispatch_report().selected_backend == "reference"
+    monkeypatch.undo()
+    for a, e in zip(got, checkpointed_step()):
+        assert torch.equal(a, e)
+
+
+def test_the_reference_backend_needs_no_library(device_without_library):
+    checkpointed = linear(torch.ones(2, 40, requires_grad=True), torch.ones(3, 40),
+                          checkpoint="int8", backend="reference")
+    assert torch.equal(checkpointed, torch.full((2, 3), 40.0))
