@@ -2,7 +2,7 @@
 
 from __future__ import annotations
 
-from functools import lru_cache
+from functools import lru_cache, wraps
 
 import torch
 
@@ -41,6 +41,21 @@ def runs_native(input: torch.Tensor) -> bool:
     if not is_rocm_tensor(input):
         return False
     return explain_dispatch(input, native_available=_native() is not None).backend != "reference"
+
+
+def in_the_tensors_type(function):
+    """A PyTorch path that computes in its tensors' type, as the kernels do: autocast, which
+    would choose another, is off within it."""
+
+    @wraps(function)
+    def call(input, *args, **kwargs):
+        device = input.device.type
+        if not torch.amp.is_autocast_available(device) or not torch.is_autocast_enabled(device):
+            return function(input, *args, **kwargs)
+        with torch.autocast(device, enabled=False):
+            return function(input, *args, **kwargs)
+
+    return call
 
 
 @lru_cache(maxsize=64)

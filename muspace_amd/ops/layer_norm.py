@@ -15,11 +15,12 @@ import torch
 import torch.nn.functional as F
 
 from .layer_common import DTYPES as _DTYPES
-from .layer_common import native_for, report_native, report_other
+from .layer_common import in_the_tensors_type, native_for, report_native, report_other
 
 OPERATOR_NAME = "layer_norm"
 
 
+@in_the_tensors_type
 def layer_norm_pytorch(input, weight=None, bias=None, *, eps=1e-5):
     """``layer_norm`` in PyTorch operations, on any device."""
     if weight is None or weight.dtype == input.dtype:

@@ -28,7 +28,14 @@ import torch.nn.functional as F
 from torch.autograd.function import once_differentiable
 
 from .layer_common import DTYPES as _DTYPES
-from .layer_common import native_for, report_native, report_other, require_native, runs_native
+from .layer_common import (
+    in_the_tensors_type,
+    native_for,
+    report_native,
+    report_other,
+    require_native,
+    runs_native,
+)
 
 OPERATOR_NAME = "linear"
 BLOCK = 32  # values of a row that share a scale in an 8-bit checkpoint
@@ -122,6 +129,7 @@ class _CheckpointedInput(torch.autograd.Function):
         return grad @ weight, flat.t() @ kept
 
 
+@in_the_tensors_type
 def linear_pytorch(input, weight, bias=None, *, activation=None, residual=None, checkpoint=None):
     """``linear`` in PyTorch operations, on any device."""
     if checkpoint is None:

@@ -3,6 +3,7 @@ forward-mode derivatives, and of tensors in unusual states."""
 
 import importlib
 import math
+from contextlib import nullcontext
 
 import pytest
 import torch
@@ -122,3 +123,23 @@ def test_the_reference_backend_launches_no_kernel_of_the_library(dtype, monkeypa
     assert dx.isfinite().all()
     mine = linear_module._checkpoint_pytorch(x)
     assert torch.equal(mine[0], codes) and torch.equal(mine[1], scales)
+
+
+@pytest.mark.parametrize("backend", ["auto", "reference"])
+@pytest.mark.parametrize("checkpoint", [None, "int8"])
+def test_autocast_changes_nothing(checkpoint, backend):
+    gen = torch.Generator(device=DEV).manual_seed(5)
+    x, w, b = (torch.randn(s, generator=gen, device=DEV) for s in ((60, 40), (24, 40), (24,)))
+
+    def step(dtype, mode):
+        leaves = [t.to(dtype, copy=True).requires_grad_() for t in (x, w, b)]
+        with mode:
+            out = linear(*leaves, activation="gelu", checkpoint=checkpoint, backend=backend)
+            norm = layer_norm(out, leaves[2].float(), leaves[2].float(), backend=backend)
+        # torch asks for backward passes outside of autocast
+        return [out, norm, *torch.autograd.grad(norm.sum() + out.sum(), leaves)]
+
+    for dtype in (torch.float32, torch.bfloat16):
+        want = step(dtype, nullcontext())
+        for a, e in zip(step(dtype, torch.autocast("cuda", dtype=torch.float16)), want):
+            assert a.dtype == dtype and torch.equal(a, e)

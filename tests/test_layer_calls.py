@@ -2,6 +2,7 @@
 refuses before anything runs, and what the PyTorch path does in its place."""
 
 import importlib
+from contextlib import nullcontext
 
 import pytest
 import torch
@@ -108,3 +109,30 @@ def test_the_reference_backend_needs_no_library(device_without_library):
     checkpointed = linear(torch.ones(2, 40, requires_grad=True), torch.ones(3, 40),
                           checkpoint="int8", backend="reference")
     assert torch.equal(checkpointed, torch.full((2, 3), 40.0))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("checkpoint", [None, "int8"])
+def test_autocast_does_not_reach_the_pytorch_path(checkpoint, dtype):
+    """Results and gradients are of the tensors' type, the same as without autocast."""
+    gen = torch.Generator().manual_seed(5)
+    x, w, b = (torch.randn(s, generator=gen).to(dtype) for s in ((6, 40), (5, 40), (5,)))
+
+    def step(mode):
+        leaves = [t.clone().requires_grad_() for t in (x, w, b)]
+        with mode:
+            out = linear(*leaves, activation="gelu", checkpoint=checkpoint)
+            norm = layer_norm(out, leaves[2], leaves[2])
+            plain = layer_norm(out)
+        # torch asks for backward passes outside of autocast
+        return [out, norm, plain, *torch.autograd.grad(norm.sum() + out.sum(), leaves)]
+
+    want = step(nullcontext())
+    for other in (torch.bfloat16, torch.float16):
+        for a, e in zip(step(torch.autocast("cpu", dtype=other)), want):
+            assert a.dtype == dtype and torch.equal(a, e)
+
+
+def test_the_pytorch_path_takes_devices_without_autocast():
+    x, w = torch.empty((3, 8), device="meta"), torch.empty((4, 8), device="meta")
+    assert layer_norm(linear(x, w)).shape == (3, 4)
