@@ -56,7 +56,7 @@
 extern "C" {
 #endif
 
-#define MUSPACE_MSDA_ABI_VERSION 6
+#define MUSPACE_MSDA_ABI_VERSION 7
 
 /* the library is built with -fvisibility=hidden; only these symbols export */
 #if defined(__GNUC__)
@@ -380,8 +380,9 @@ MUSPACE_API int add_one(const float *x, float *y, int64_t n, void *stream);
  * (/root/reference/csrc/ffi/tensor_utils.hpp:13-38). */
 MUSPACE_API const char *muspace_last_error(void);
 
-/* MUSPACE_MSDA_ABI_VERSION of the loaded library. No reference counterpart:
- * lets the Python loader refuse a stale library. */
+/* MUSPACE_MSDA_ABI_VERSION of the loaded library; it counts every change of a signature
+ * or of what a buffer holds, in all of the library's headers. No reference
+ * counterpart: lets the Python loaders refuse a stale library or host module. */
 MUSPACE_API int muspace_abi_version(void);
 
 #ifdef __cplusplus

@@ -400,6 +400,8 @@ OptTensor layer_norm(const Tensor &input, const OptTensor &weight, const OptTens
 
 PYBIND11_MODULE(muspace_layer_host, m) {
   namespace py = pybind11;
+  // of the headers that this module's calls are compiled from
+  m.attr("abi_version") = MUSPACE_MSDA_ABI_VERSION;
   m.def("bind", &bind);
   m.def("linear", &linear, py::call_guard<py::gil_scoped_release>());
   m.def("checkpoint", &checkpoint, py::call_guard<py::gil_scoped_release>());

@@ -2,7 +2,9 @@
 
 The module holds the operators' autograd nodes (C++ against torch's API) and no
 kernel; it launches through the C-ABI of ``libmuspace_msda.so``, whose addresses are
-handed to it here, after that library's own checks (exports, ABI version).
+handed to it here, after that library's own checks (exports, ABI version) and the
+check that the module was compiled from the same version's headers: it calls those
+addresses by the headers' signatures.
 """
 
 from __future__ import annotations
@@ -14,7 +16,7 @@ from importlib.resources import files
 from importlib.util import module_from_spec, spec_from_loader
 from pathlib import Path
 
-from .native import NativeModuleUnavailable, load_native_module
+from .native import ABI_VERSION, NativeModuleUnavailable, load_native_module
 
 MODULE_NAME = "muspace_layer_host"
 _BOUND = (
@@ -43,6 +45,12 @@ def load_layer_host():
         loader.exec_module(module)
     except ImportError as exc:
         raise NativeModuleUnavailable(f"unable to load muSPACE host module {path}: {exc}") from exc
+    version = getattr(module, "abi_version", None)
+    if version != ABI_VERSION:
+        raise NativeModuleUnavailable(
+            f"muSPACE host module {path} has ABI version {version}, expected {ABI_VERSION}; "
+            "rebuild it with `python -m muspace_amd.build`"
+        )
     module.bind({name: ctypes.cast(library.raw(name), ctypes.c_void_p).value for name in _BOUND})
     return module
 

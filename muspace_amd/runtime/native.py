@@ -28,7 +28,7 @@ from typing import Any, Callable
 import torch
 
 LIBRARY_RELPATH = "native/libmuspace_msda.so"
-ABI_VERSION = 6
+ABI_VERSION = 7
 
 DTYPE_F32, DTYPE_F16, DTYPE_BF16 = 0, 1, 2
 

@@ -10,6 +10,7 @@ import torch.autograd.forward_ad as forward_ad
 from torch.fx.experimental.proxy_tensor import make_fx
 
 from muspace_amd import checkpoint_int8, get_last_dispatch_report, layer_norm, linear
+from muspace_amd.runtime import native
 from muspace_amd.runtime.layer_host import load_layer_host
 
 linear_module = importlib.import_module("muspace_amd.ops.linear")  # (the package has the function)
@@ -136,3 +137,30 @@ def test_autocast_does_not_reach_the_pytorch_path(checkpoint, dtype):
 def test_the_pytorch_path_takes_devices_without_autocast():
     x, w = torch.empty((3, 8), device="meta"), torch.empty((4, 8), device="meta")
     assert layer_norm(linear(x, w)).shape == (3, 4)
+
+
+# --------------------------------------------------------- the host module ---
+
+
+@pytest.mark.parametrize("version", [None, 5, 999])
+def test_a_host_module_of_other_headers_is_refused(version, monkeypatch):
+    """The module calls bare addresses by the signatures it was compiled with: one from before
+    a change of a signature (without the attribute, or of another version) does not bind."""
+    import types
+
+    from muspace_amd.runtime import layer_host
+
+    stale = types.SimpleNamespace(bind=lambda addresses: pytest.fail("bound"))
+    if version is not None:
+        stale.abi_version = version
+    monkeypatch.setattr(layer_host, "module_from_spec", lambda spec: stale)
+    monkeypatch.setattr(layer_host.ExtensionFileLoader, "exec_module", lambda self, module: None)
+    layer_host.load_layer_host.cache_clear()
+    try:
+        with pytest.raises(native.NativeModuleUnavailable,
+                           match=f"has ABI version {version}, expected {native.ABI_VERSION}; rebuild"):
+            layer_host.load_layer_host()
+    finally:
+        monkeypatch.undo()
+        layer_host.load_layer_host.cache_clear()
+    assert layer_host.load_layer_host().abi_version == native.ABI_VERSION
