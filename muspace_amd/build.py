@@ -121,10 +121,13 @@ def _compile(library: Path, command, verbose: bool) -> Path:
 
 def build(verbose: bool = False) -> Path:
     """Compile the MSDA library, the probe library and the host module (always), each
-    moved into place atomically; returns the MSDA library's path."""
+    moved into place atomically; returns the MSDA library's path. The host module comes
+    last: without a C++ compiler or torch's headers it is the only one that fails, and
+    only the operators it holds are not there."""
+    _compile(LIBRARY, build_command, verbose)
     _compile(PROBE_LIBRARY, lambda out: build_command(out, PROBE_SOURCES), verbose)
     _compile(HOST_LIBRARY, host_command, verbose)
-    return _compile(LIBRARY, build_command, verbose)
+    return LIBRARY
 
 
 def main(argv: list[str] | None = None) -> int:

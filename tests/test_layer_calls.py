@@ -164,3 +164,19 @@ def test_a_host_module_of_other_headers_is_refused(version, monkeypatch):
         monkeypatch.undo()
         layer_host.load_layer_host.cache_clear()
     assert layer_host.load_layer_host().abi_version == native.ABI_VERSION
+
+
+def test_the_libraries_are_built_without_a_host_compiler(monkeypatch, tmp_path):
+    """What the host module's build needs besides hipcc is not needed by the others."""
+    from muspace_amd import build
+
+    for name in ("LIBRARY", "PROBE_LIBRARY", "HOST_LIBRARY"):
+        monkeypatch.setattr(build, name, tmp_path / getattr(build, name).name)
+    monkeypatch.setattr(build, "build_command", lambda out, *sources: ["touch", str(out)])
+    monkeypatch.setattr(build, "host_command", lambda out: ["false"])
+    with pytest.raises(RuntimeError, match="building muspace_layer_host.so"):
+        build.build()
+    assert build.LIBRARY.is_file() and build.PROBE_LIBRARY.is_file()
+    assert not build.HOST_LIBRARY.exists()
+    monkeypatch.setattr(build, "host_command", lambda out: ["touch", str(out)])
+    assert build.build() == build.LIBRARY and build.HOST_LIBRARY.is_file()
