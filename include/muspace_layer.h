@@ -61,9 +61,14 @@ MUSPACE_API int linear_forward(const void *x, int dtype, const void *weight, con
 MUSPACE_API int linear_checkpoint(const void *x, int dtype, int8_t *codes, uint8_t *scales,
                                   int64_t rows, int64_t in_features, void *stream);
 
-/* Bytes of workspace of linear_backward (256-byte aligned; 0: none needed). */
+/* Bytes of workspace of linear_backward (256-byte aligned; 0: none needed): enough for
+ * any set of gradients; _for: for those whose flag is not 0. */
 MUSPACE_API size_t linear_backward_workspace_size(int dtype, int64_t rows, int64_t in_features,
                                                   int64_t out_features, int activation);
+MUSPACE_API size_t linear_backward_workspace_size_for(int dtype, int64_t rows, int64_t in_features,
+                                                      int64_t out_features, int activation,
+                                                      int want_input, int want_weight,
+                                                      int want_bias);
 
 /* dz = grad_output * act'(z); grad_input = dz weight; grad_weight = dz^T x;
  * grad_bias = sum of dz over rows. A NULL gradient is not computed. x is needed

@@ -40,7 +40,7 @@ struct Api {
   decltype(&::muspace_last_error) last_error = nullptr;
   decltype(&::linear_forward) linear_forward = nullptr;
   decltype(&::linear_checkpoint) linear_checkpoint = nullptr;
-  decltype(&::linear_backward_workspace_size) linear_workspace = nullptr;
+  decltype(&::linear_backward_workspace_size_for) linear_workspace = nullptr;
   decltype(&::linear_backward) linear_backward = nullptr;
   decltype(&::layer_norm_forward) norm_forward = nullptr;
   decltype(&::layer_norm_backward_workspace_size) norm_workspace = nullptr;
@@ -56,7 +56,7 @@ void bind(const std::map<std::string, std::uintptr_t> &addresses) {
   bind_one(api.last_error, addresses, "muspace_last_error");
   bind_one(api.linear_forward, addresses, "linear_forward");
   bind_one(api.linear_checkpoint, addresses, "linear_checkpoint");
-  bind_one(api.linear_workspace, addresses, "linear_backward_workspace_size");
+  bind_one(api.linear_workspace, addresses, "linear_backward_workspace_size_for");
   bind_one(api.linear_backward, addresses, "linear_backward");
   bind_one(api.norm_forward, addresses, "layer_norm_forward");
   bind_one(api.norm_workspace, addresses, "layer_norm_backward_workspace_size");
@@ -256,7 +256,8 @@ struct LinearFunction : torch::autograd::Function<LinearFunction> {
       if (need_weight) grad_weight = at::empty(wshape, g.options());
       if (need_bias) grad_bias = at::empty({out}, g.options());
       const int code = code_of(g.scalar_type(), "grad_output");
-      const size_t bytes = api.linear_workspace(code, rows, cols, out, activation);
+      const size_t bytes = api.linear_workspace(code, rows, cols, out, activation, need_input,
+                                                 need_weight, need_bias);
       const Tensor workspace = scratch(bytes, g);
       check(api.linear_backward(
                 g.data_ptr(), code, pointer(x), static_cast<const int8_t *>(pointer(codes)),

@@ -106,11 +106,31 @@ WeightPlan plan_weight(int dtype, int64_t rows, int64_t in, int64_t out) {
   return p;
 }
 
-size_t partial_bytes(const WeightPlan &p, int64_t in, int64_t out) {
-  if (p.splits == 1) return 0;
+// gradients that are asked for and have values
+struct Wanted {
+  bool input, weight, bias;
+  Wanted(bool input_, bool weight_, bool bias_, int64_t rows, int64_t in, int64_t out)
+      : input(input_ && rows > 0 && in > 0), weight(weight_ && in > 0 && out > 0),
+        bias(bias_ && out > 0) {}
+  bool any() const { return input || weight || bias; }
+};
+
+// The parts' sums: the weight's, then the bias's.
+size_t weight_partial_bytes(const WeightPlan &p, const Wanted &want, int64_t in, int64_t out) {
+  if (p.splits == 1 || !want.weight) return 0;
   const size_t ld = static_cast<size_t>((in + 7) & ~int64_t{7});
-  return pad256(static_cast<size_t>(p.splits) * out * ld * 4) +
-         pad256(static_cast<size_t>(p.splits) * out * 4);
+  return pad256(static_cast<size_t>(p.splits) * out * ld * 4);
+}
+size_t bias_partial_bytes(const WeightPlan &p, const Wanted &want, int64_t out) {
+  return p.splits == 1 || !want.bias ? 0 : pad256(static_cast<size_t>(p.splits) * out * 4);
+}
+
+size_t workspace_bytes_of(int dtype, const Wanted &want, int64_t rows, int64_t in, int64_t out,
+                          int activation) {
+  const WeightPlan plan = plan_weight(dtype, rows, in, out);
+  size_t bytes = weight_partial_bytes(plan, want, in, out) + bias_partial_bytes(plan, want, out);
+  if (activation == dense::kGelu && want.any()) bytes += dz_tensors(dtype) * dz_bytes(dtype, rows, out);
+  return bytes;
 }
 
 template <typename T, Job kJob, int B, Kind kKind, bool kCodes>
@@ -326,18 +346,22 @@ int linear_checkpoint(const void *x, int dtype, int8_t *codes, uint8_t *scales, 
   return check_launch("linear_checkpoint");
 }
 
-size_t linear_backward_workspace_size(int dtype, int64_t rows, int64_t in_features,
-                                      int64_t out_features, int activation) {
+size_t linear_backward_workspace_size_for(int dtype, int64_t rows, int64_t in_features,
+                                          int64_t out_features, int activation, int want_input,
+                                          int want_weight, int want_bias) {
   if (validate("linear_backward_workspace_size", dtype, rows, in_features, out_features,
                activation) != MUSPACE_OK) {
     return 0;
   }
-  const WeightPlan plan = plan_weight(dtype, rows, in_features, out_features);
-  size_t bytes = partial_bytes(plan, in_features, out_features);
-  if (activation == dense::kGelu) {
-    bytes += dz_tensors(dtype) * dz_bytes(dtype, rows, out_features);
-  }
-  return bytes;
+  const Wanted want(want_input != 0, want_weight != 0, want_bias != 0, rows, in_features,
+                    out_features);
+  return workspace_bytes_of(dtype, want, rows, in_features, out_features, activation);
+}
+
+size_t linear_backward_workspace_size(int dtype, int64_t rows, int64_t in_features,
+                                      int64_t out_features, int activation) {
+  return linear_backward_workspace_size_for(dtype, rows, in_features, out_features, activation, 1,
+                                            1, 1);
 }
 
 int linear_backward(const void *grad_output, int dtype, const void *x, const int8_t *codes,
@@ -348,10 +372,9 @@ int linear_backward(const void *grad_output, int dtype, const void *x, const int
   const char *fn = "linear_backward";
   int rc = validate(fn, dtype, rows, in_features, out_features, activation);
   if (rc != MUSPACE_OK) return rc;
-  const bool want_input = grad_input != nullptr && rows > 0 && in_features > 0;
-  const bool want_weight = grad_weight != nullptr && in_features > 0 && out_features > 0;
-  const bool want_bias = grad_bias != nullptr && out_features > 0;
-  if (!want_input && !want_weight && !want_bias) return ok();
+  const Wanted want(grad_input != nullptr, grad_weight != nullptr, grad_bias != nullptr, rows,
+                    in_features, out_features);
+  if (!want.any()) return ok();
   const bool summed = rows > 0 && out_features > 0;  // dz has values
   if ((codes == nullptr) != (scales == nullptr)) {
     return fail(MUSPACE_EINVAL, "%s: codes and scales come together", fn);
@@ -360,14 +383,14 @@ int linear_backward(const void *grad_output, int dtype, const void *x, const int
     return fail(MUSPACE_EINVAL, "%s: codes must be 8-byte aligned", fn);
   }
   if (summed &&
-      (grad_output == nullptr || (want_input && weight == nullptr) ||
-       (want_weight && x == nullptr && codes == nullptr) ||
+      (grad_output == nullptr || (want.input && weight == nullptr) ||
+       (want.weight && x == nullptr && codes == nullptr) ||
        (activation == dense::kRelu && relu_mask == nullptr) ||
        (activation == dense::kGelu && pre_activation == nullptr))) {
     return fail(MUSPACE_EINVAL, "%s: null tensor pointer", fn);
   }
   const size_t need =
-      linear_backward_workspace_size(dtype, rows, in_features, out_features, activation);
+      workspace_bytes_of(dtype, want, rows, in_features, out_features, activation);
   if (need > 0 && (workspace == nullptr || workspace_bytes < need ||
                    reinterpret_cast<uintptr_t>(workspace) % 256 != 0)) {
     return fail(MUSPACE_EINVAL, "%s: needs a 256-byte aligned workspace of %zu bytes, got %zu", fn,
@@ -396,7 +419,7 @@ int linear_backward(const void *grad_output, int dtype, const void *x, const int
   const bool whole_out = dz_ld % v == 0 && aligned16(dz);
   const uint8_t *mask = activation == dense::kRelu && summed ? relu_mask : nullptr;
 
-  if (want_input) {
+  if (want.input) {
     Product a = {};
     a.p = dz;
     a.p_rest = dz_rest;
@@ -418,7 +441,7 @@ int linear_backward(const void *grad_output, int dtype, const void *x, const int
       });
     });
   }
-  if (want_weight || want_bias) {
+  if (want.weight || want.bias) {
     const WeightPlan plan = plan_weight(dtype, rows, in_features, out_features);
     Product a = {};
     a.p = dz;
@@ -426,9 +449,9 @@ int linear_backward(const void *grad_output, int dtype, const void *x, const int
     a.ldp = dz_ld;
     a.m = static_cast<int>(out_features);
     // without a weight gradient: no columns, the first column of tiles sums dz
-    a.n = want_weight ? static_cast<int>(in_features) : 0;
+    a.n = want.weight ? static_cast<int>(in_features) : 0;
     a.k = static_cast<int>(rows);
-    const bool coded = want_weight && codes != nullptr;
+    const bool coded = want.weight && codes != nullptr;
     a.q = coded ? static_cast<const void *>(codes) : x;
     a.ldq = coded ? (in_features + 31) & ~int64_t{31} : in_features;
     a.scales = coded ? scales : nullptr;
@@ -439,19 +462,18 @@ int linear_backward(const void *grad_output, int dtype, const void *x, const int
     a.k_split = plan.k_split;
     a.out = grad_weight;
     if (plan.splits > 1) {
-      a.partial = reinterpret_cast<float *>(ws);
-      if (want_bias) {
-        const size_t ld = static_cast<size_t>((in_features + 7) & ~int64_t{7});
+      a.partial = reinterpret_cast<float *>(ws);  // (without a weight gradient: not written)
+      if (want.bias) {
         a.bias_partial = reinterpret_cast<float *>(
-            ws + pad256(static_cast<size_t>(plan.splits) * out_features * ld * 4));
+            ws + weight_partial_bytes(plan, want, in_features, out_features));
       }
-    } else if (want_bias) {
+    } else if (want.bias) {
       a.bias_out = grad_bias;
     }
     const bool tight =
-        whole_out && (!want_weight || coded || (in_features % v == 0 && aligned16(x)));
+        whole_out && (!want.weight || coded || (in_features % v == 0 && aligned16(x)));
     by_type(dtype, [&](auto t) {
-      run_weight<decltype(t)>(a, plan, tight, coded, grad_weight, want_bias ? grad_bias : nullptr,
+      run_weight<decltype(t)>(a, plan, tight, coded, grad_weight, want.bias ? grad_bias : nullptr,
                               st);
     });
   }

@@ -21,7 +21,7 @@ from .native import ABI_VERSION, NativeModuleUnavailable, load_native_module
 MODULE_NAME = "muspace_layer_host"
 _BOUND = (
     "muspace_last_error", "linear_forward", "linear_checkpoint",
-    "linear_backward_workspace_size", "linear_backward", "layer_norm_forward",
+    "linear_backward_workspace_size_for", "linear_backward", "layer_norm_forward",
     "layer_norm_backward_workspace_size", "layer_norm_backward",
 )
 

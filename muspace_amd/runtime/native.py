@@ -154,6 +154,9 @@ _EXPORTS: dict[str, tuple[Any, list[Any]]] = {
         _c_int, [_c_ptr, _c_int, _c_ptr, _c_ptr, _c_int64, _c_int64, _c_ptr]
     ),
     "linear_backward_workspace_size": (ctypes.c_size_t, [_c_int] + [_c_int64] * 3 + [_c_int]),
+    "linear_backward_workspace_size_for": (
+        ctypes.c_size_t, [_c_int] + [_c_int64] * 3 + [_c_int] * 4
+    ),
     "linear_backward": (
         _c_int,
         [_c_ptr, _c_int] + [_c_ptr] * 9 + [_c_int64] * 3
@@ -1082,7 +1085,9 @@ class NativeLibrary:
         self._check_codes(grad_output, codes, scales, rows, cols)
         self._check_kept(grad_output, kept, rows, out, activation)
         code = _DTYPE_CODES[grad_output.dtype]
-        nbytes = self._raw["linear_backward_workspace_size"](code, rows, cols, out, activation)
+        nbytes = self._raw["linear_backward_workspace_size_for"](
+            code, rows, cols, out, activation, grad_input is not None, grad_weight is not None,
+            grad_bias is not None)
         workspace = None
         if nbytes:
             workspace = torch.empty(nbytes, dtype=torch.uint8, device=grad_output.device)

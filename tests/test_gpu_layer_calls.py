@@ -143,3 +143,34 @@ def test_autocast_changes_nothing(checkpoint, backend):
         want = step(dtype, nullcontext())
         for a, e in zip(step(dtype, torch.autocast("cuda", dtype=torch.float16)), want):
             assert a.dtype == dtype and torch.equal(a, e)
+
+
+@pytest.mark.parametrize("activation", [None, "relu", "gelu"])
+@pytest.mark.parametrize("which", [(0,), (1,), (2,), (0, 2), (1, 2), (0, 1, 2)], ids=str)
+def test_a_backward_allocates_for_the_wanted_gradients(which, activation):
+    """A frozen weight's partial sums (33 MB here) are not allocated; every set of gradients
+    equals the same ones of the whole set."""
+    gen = torch.Generator(device=DEV).manual_seed(6)
+    rows, inner, outer = 40000, 512, 256
+    x, w, b, g = (torch.randn(s, generator=gen, device=DEV).bfloat16()
+                  for s in ((rows, inner), (outer, inner), (outer,), (rows, outer)))
+
+    def step(which):
+        leaves = [t.detach() for t in (x, w, b)]
+        for i in which:
+            leaves[i] = leaves[i].clone().requires_grad_()
+        out = linear(*leaves, activation=activation)
+        torch.cuda.synchronize()
+        torch.cuda.reset_peak_memory_stats()
+        before = torch.cuda.memory_allocated()
+        grads = torch.autograd.grad(out, [leaves[i] for i in which], g)
+        return grads, torch.cuda.max_memory_allocated() - before
+
+    every, _ = step((0, 1, 2))
+    grads, peak = step(which)
+    for i, grad in zip(which, grads):
+        assert torch.equal(grad, every[i])
+    room = sum(t.numel() * 2 for t in grads) + 4 * 64 * outer * (inner * (1 in which) + 1)
+    if activation == "gelu":
+        room += 2 * rows * outer * 2
+    assert peak <= room + (1 << 20)

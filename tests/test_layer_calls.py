@@ -180,3 +180,24 @@ def test_the_libraries_are_built_without_a_host_compiler(monkeypatch, tmp_path):
     assert not build.HOST_LIBRARY.exists()
     monkeypatch.setattr(build, "host_command", lambda out: ["touch", str(out)])
     assert build.build() == build.LIBRARY and build.HOST_LIBRARY.is_file()
+
+
+# ----------------------------------------------------------- the workspace ---
+
+
+def test_the_workspace_is_that_of_the_wanted_gradients(native_lib):
+    every = native_lib.raw("linear_backward_workspace_size")
+    size = native_lib.raw("linear_backward_workspace_size_for")
+    dims = (2, 80000, 512, 256)
+    # 8 tiles of 128 x 128, for two workgroups on each of 256 CUs: 64 parts of 1250 steps, 20
+    # steps each, which makes 63
+    splits = 63
+    weight, bias = splits * 256 * 512 * 4, splits * 256 * 4
+    assert every(*dims, 0) == size(*dims, 0, 1, 1, 1) == weight + bias
+    assert size(*dims, 0, 1, 0, 0) == size(*dims, 0, 0, 0, 0) == 0
+    assert size(*dims, 0, 0, 1, 0) == size(*dims, 1, 1, 1, 0) == weight
+    assert size(*dims, 0, 0, 0, 1) == size(*dims, 1, 1, 0, 1) == bias
+    dz = 2 * 80000 * 256 * 2  # gelu's, for any of them
+    assert size(*dims, 2, 1, 0, 0) == dz and size(*dims, 2, 0, 0, 1) == dz + bias
+    assert size(*dims, 2, 0, 0, 0) == 0 and every(*dims, 2) == dz + weight + bias
+    assert size(9, 80000, 512, 256, 0, 1, 1, 1) == 0
