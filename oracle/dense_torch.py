@@ -26,6 +26,16 @@ def tiny(dtype: torch.dtype) -> float:
     return torch.finfo(dtype).smallest_normal * half_step(dtype)
 
 
+def product_rms(k: int) -> float:
+    """What the error of a float32 product of k random terms of either sign may be, as root
+    mean squares over the result and relative to the result's own. A rounding errs by 0.4
+    2^-24 of the partial sum; after i terms that is sqrt(i / k) of the result. Three planes
+    take six products a term, each rounded into the sum at the worst: 0.4 2^-24 sqrt(6 k
+    / 2). The parts of a long sum are added apart: 1024 terms at the most count. 4 2^-24
+    are for the operands' planes, the parts' sum and the result."""
+    return 2.0**-24 * (0.7 * math.sqrt(min(k, 1024)) + 4)
+
+
 def gelu(z):
     return 0.5 * z * torch.special.erfc(-z * math.sqrt(0.5))
 

@@ -23,6 +23,30 @@ def rms(t):
     return float(t.double().square().mean().sqrt())
 
 
+# ------------------------------------------------------ float32 products ---
+
+
+@pytest.mark.parametrize(
+    "size", [(9000, 72, 136), (20000, 64, 512), (9001, 203, 611), (6000, 520, 1030), (44446, 256, 96),
+             (300, 256, 256), (1800, 1024, 256), (3, 203, 611), (1, 2048, 512)], ids=str)
+@pytest.mark.parametrize("residual", [False, True])
+def test_float32_products_have_float32_errors(size, residual):
+    """Values with all their bits, in the kernels of many rows, of few results and of few rows:
+    root mean squares, which two bfloat16 planes in place of three would exceed."""
+    rows, inner, outer = size
+    gen = torch.Generator(device=DEV).manual_seed(8)
+    x, w, g = normal(gen, rows, inner), normal(gen, outer, inner), normal(gen, rows, outer)
+    r = normal(gen, rows, outer) if residual else None
+    xs, ws = x.clone().requires_grad_(), w.clone().requires_grad_()
+    out = linear(xs, ws, residual=r)
+    dx, dw = torch.autograd.grad(out, [xs, ws], g)
+    y = x.double() @ w.double().t()
+    for name, got, exact, k in (("out", out.detach(), y if r is None else y + r, inner),
+                                ("grad_input", dx, g.double() @ w.double(), outer),
+                                ("grad_weight", dw, g.double().t() @ x.double(), rows)):
+        assert rms(got.double() - exact) <= dense_torch.product_rms(k) * rms(exact), name
+
+
 # ------------------------------------------------------------ gelu's slope ---
 
 

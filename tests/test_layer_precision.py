@@ -6,6 +6,46 @@ import torch
 
 from oracle import dense_torch
 
+# ----------------------------------------------------- float32 products ---
+
+
+def planes(x, count):
+    """x as the sum of ``count`` bfloat16 numbers, the largest first, each in float32."""
+    out = []
+    for _ in range(count):
+        out.append(x.bfloat16().float())
+        x = x - out[-1]
+    return out
+
+
+def product_model(x, w, count=3, most=2):
+    """x w^T from the products of planes i and j (from 0) with i + j <= most."""
+    total = torch.zeros(x.shape[0], w.shape[0])
+    for i, a in enumerate(planes(x, count)):
+        for j, b in enumerate(planes(w, count)):
+            if i + j <= most:
+                total = total + a @ b.t()
+    return total
+
+
+def relative_rms(got, exact):
+    return float((got.double() - exact).square().mean().sqrt() / exact.square().mean().sqrt())
+
+
+@pytest.mark.parametrize("inner", [32, 256, 1024])
+def test_product_bound_holds_for_three_planes_and_rejects_two(inner):
+    gen = torch.Generator().manual_seed(2)
+    x, w = torch.randn((400, inner), generator=gen), torch.randn((300, inner), generator=gen)
+    exact = x.double() @ w.double().t()
+    limit = dense_torch.product_rms(inner)
+    assert relative_rms(product_model(x, w), exact) <= limit
+    # two planes, all four of their products; the third planes without their products with
+    # the first; one operand in two planes
+    assert relative_rms(product_model(x, w, count=2), exact) > limit
+    assert relative_rms(product_model(x, w, most=1), exact) > limit
+    assert relative_rms(product_model(sum(planes(x, 2)), w), exact) > limit
+
+
 # ------------------------------------------------------------- layer norm ---
 
 
