@@ -174,3 +174,57 @@ def test_a_backward_allocates_for_the_wanted_gradients(which, activation):
     if activation == "gelu":
         room += 2 * rows * outer * 2
     assert peak <= room + (1 << 20)
+
+
+def block(x, w, v, scale, checkpoint):
+    hidden = linear(layer_norm(x, scale, scale), w, activation="gelu", checkpoint=checkpoint)
+    return linear(hidden, v, residual=x, checkpoint=checkpoint)
+
+
+@pytest.mark.parametrize("last", ["linear", "layer_norm"])
+@pytest.mark.parametrize("checkpoint", [None, "int8"])
+def test_recomputed_and_offloaded_blocks(checkpoint, last):
+    """A block under torch.utils.checkpoint (which ends its second forward by an exception from
+    the last tensor kept) and with its kept tensors in host memory equals the plain one."""
+    from torch.utils.checkpoint import checkpoint as recomputed
+
+    gen = torch.Generator(device=DEV).manual_seed(7)
+    shapes = ((500, 64), (128, 64), (64, 128), (64,))
+    tensors = [torch.randn(s, generator=gen, device=DEV).bfloat16() for s in shapes]
+    g = torch.randn((500, 64), generator=gen, device=DEV).bfloat16()
+
+    def function(x, w, v, scale):
+        out = block(x, w, v, scale, checkpoint)
+        return out if last == "linear" else layer_norm(out, scale)
+
+    def step(call):
+        leaves = [t.clone().requires_grad_() for t in tensors]
+        out = call(*leaves)
+        return [out.detach(), *torch.autograd.grad(out, leaves, g)]
+
+    want = step(function)
+    with torch.autograd.graph.save_on_cpu():
+        offloaded = step(function)
+    for got in (step(lambda *leaves: recomputed(function, *leaves, use_reentrant=False)), offloaded):
+        for a, e in zip(got, want):
+            assert torch.equal(a, e)
+    leaves = [t.clone().requires_grad_() for t in tensors]
+    recomputed(function, *leaves, use_reentrant=True).backward(g)
+    for a, e in zip(leaves, want[1:]):
+        assert torch.equal(a.grad, e)
+
+
+def test_what_cannot_be_read_is_refused():
+    """Batched tensors (vmap, gradients taken in a batch) and tensors of torch.func's
+    transforms have no memory of their own: an error, not an answer."""
+    x, w = torch.randn((3, 5, 8), device=DEV), torch.randn((4, 8), device=DEV)
+    with pytest.raises(RuntimeError):
+        torch.func.vmap(lambda t: linear(t, w))(x)
+    with pytest.raises(RuntimeError):
+        torch.func.grad(lambda t: layer_norm(t).sum())(x)
+    with pytest.raises(RuntimeError):
+        torch.func.jvp(lambda t: linear(t, w), (x,), (x,))
+    xs = x.clone().requires_grad_()
+    out = linear(xs, w)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(out, [xs], torch.ones((2, *out.shape), device=DEV), is_grads_batched=True)
