@@ -9,9 +9,9 @@
 // Of the nine products those of planes i + j <= 4 are taken, six; the rest is
 // under 2^-23 |x y| for a product x y, the size of float32's own two roundings, and
 // of random sign. bfloat16's smallest number is 2^-133, so float32 values keep an
-// absolute 2^-134: those under 2^-109 keep fewer than 24 bits. Infinities, NaN and numbers that round to an infinity in bfloat16
-// make such a sum an infinity or NaN: a tile with one in it is multiplied again
-// in float32.
+// absolute 2^-134: those under 2^-109 keep fewer than 24 bits. Infinities, NaN and
+// numbers that round to an infinity in bfloat16 make such a sum an infinity or NaN: a
+// tile with one in it is multiplied again in float32.
 //
 // A tile of an operand (of one plane) is staged in LDS in one of two layouts, by
 // how the operand lies in memory against the product's summed index k:
@@ -69,9 +69,6 @@ struct Piece {
 // addresses, the packed type tells the compiler so.
 struct __attribute__((packed, aligned(2))) Loose16 {
   u32x4 v;
-};
-struct __attribute__((packed, aligned(2))) Loose8 {
-  u32x2 v;
 };
 
 template <typename T>
@@ -152,8 +149,9 @@ __device__ __forceinline__ u32x4 pack<bf16_t>(const float (&v)[8]) {
 // Loads of one operand's chunks. kTight: every chunk starts on a 16-byte
 // boundary and a row's length is a whole number of chunks; the loads are then
 // unconditional buffer loads, whose range check returns zeros past the operand.
-// Otherwise rows start anywhere: a chunk inside its row is one load at its own
-// alignment, the last one of a row value by value.
+// Otherwise rows start anywhere: every chunk is one load at its own alignment, a row's
+// last as the row's last 16 bytes, whose values drop_front moves to the front; only
+// rows shorter than a chunk are read value by value (loose_load).
 struct Source {
   const char *base;   // first byte of the step's window (uniform)
   uint32_t bytes;     // of the window: what lies beyond reads as zero

@@ -90,6 +90,16 @@ def test_kept_slopes(native_lib, dtype):
     assert ((values - exact).abs() <= bound + (1 + zd.abs()) * 2.0**-126).all()
 
 
+def test_gelu_keeps_the_digits_of_its_tails():
+    """float32: relative to gelu's own value, however far below zero; the roundings of
+    exp(-z^2 / 2) as above, 20 for the others."""
+    z = torch.linspace(-13.0, 3.0, 30001, device=DEV)
+    out = linear(z[:, None], torch.ones((1, 1), device=DEV), activation="gelu")[:, 0].double()
+    zd = z.double()
+    exact = dense_torch.gelu(zd)
+    assert ((out - exact).abs() <= exact.abs() * (20 + 1.5 * zd * zd) * 2.0**-24 + 2.0**-126).all()
+
+
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
 @pytest.mark.parametrize("size", [(6000, 203, 611), (5000, 256, 512), (70, 96, 64)], ids=str)
 def test_gelu_gradients_err_by_their_rounding(size, dtype):
