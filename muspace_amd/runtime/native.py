@@ -1037,7 +1037,7 @@ class NativeLibrary:
     def linear_forward(self, input, weight, bias, residual, output, kept, activation: int,
                        codes=None, scales=None) -> None:
         """output = act(input weight^T + bias) + residual; ``kept``: None, relu's
-        bits (uint8) or gelu's pre-activation (the input's dtype); ``codes`` and
+        bits (uint8) or gelu's derivatives (the input's dtype); ``codes`` and
         ``scales``: None or the input's 8-bit checkpoint."""
         _check(input, "input", tuple(_DTYPE_CODES))
         if weight is None or weight.dim() != 2 or input.dim() == 0:
