@@ -55,7 +55,8 @@ def _checkpoint_pytorch(input: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor
     rows = math.prod(input.shape[:-1])
     padded = (cols + BLOCK - 1) // BLOCK * BLOCK
     low, high = _SCALE_RANGE[input.dtype]
-    x = F.pad(input.reshape(rows, cols).float(), (0, padded - cols)).view(rows, -1, BLOCK)
+    x = F.pad(input.reshape(rows, cols).float(), (0, padded - cols))
+    x = x.view(rows, padded // BLOCK, BLOCK)
     finite = torch.isfinite(x).all(-1, keepdim=True)
     mantissa, exponent = torch.frexp(torch.where(finite, x, 0.0).abs().amax(-1, keepdim=True))
     exponent = (exponent - 7 + (mantissa > 127.0 / 128.0).int()).clamp_min(low)
@@ -66,7 +67,7 @@ def _checkpoint_pytorch(input: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor
     codes = (x * ((127 - exponent) << 23).view(torch.float32)).round()
     codes = torch.where(finite, torch.minimum(torch.maximum(codes, -limit), limit), 1.0)
     scales = torch.where(finite, exponent + 127, 255)
-    return codes.view(rows, padded).to(torch.int8), scales.view(rows, -1).to(torch.uint8)
+    return codes.view(rows, padded).to(torch.int8), scales.squeeze(-1).to(torch.uint8)
 
 
 def checkpoint_int8(input: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
@@ -91,13 +92,13 @@ def checkpoint_restore(codes: torch.Tensor, scales: torch.Tensor, cols: int,
                        dtype: torch.dtype) -> torch.Tensor:
     """The values an 8-bit checkpoint stands for, ``[rows, cols]`` in ``dtype``
     (exact: a code times its power of two is a number of the type)."""
-    rows = codes.shape[0]
+    rows, padded = codes.shape
     exponent = scales.to(torch.int32) - 127
     # 2^e straight from its bits: e is in [-126, 122]
     factor = ((exponent + 127).clamp(1, 254) << 23).view(torch.float32)
     factor = torch.where(scales == 255, math.nan, factor)
-    values = codes.view(rows, -1, BLOCK).float() * factor.unsqueeze(-1)
-    return values.view(rows, -1)[:, :cols].to(dtype)
+    values = codes.view(rows, padded // BLOCK, BLOCK).float() * factor.unsqueeze(-1)
+    return values.view(rows, padded)[:, :cols].to(dtype)
 
 
 # ---------------------------------------------------------- PyTorch path ---
@@ -125,7 +126,7 @@ class _CheckpointedInput(torch.autograd.Function):
     def backward(ctx, grad):
         weight, codes, scales = ctx.saved_tensors
         kept = checkpoint_restore(codes, scales, ctx.shape[-1], ctx.dtype)
-        flat = grad.reshape(-1, grad.shape[-1])
+        flat = grad.reshape(kept.shape[0], grad.shape[-1])
         return grad @ weight, flat.t() @ kept
 
 

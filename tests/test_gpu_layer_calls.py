@@ -10,7 +10,7 @@ import torch
 import torch.autograd.forward_ad as forward_ad
 from torch.fx.experimental.proxy_tensor import make_fx
 
-from muspace_amd import checkpoint_int8, layer_norm, linear
+from muspace_amd import checkpoint_int8, checkpoint_restore, layer_norm, linear
 
 linear_module = importlib.import_module("muspace_amd.ops.linear")  # (the package has the function)
 
@@ -228,3 +228,20 @@ def test_what_cannot_be_read_is_refused():
     out = linear(xs, w)
     with pytest.raises(RuntimeError):
         torch.autograd.grad(out, [xs], torch.ones((2, *out.shape), device=DEV), is_grads_batched=True)
+
+
+@pytest.mark.parametrize("backend", ["auto", "reference"])
+@pytest.mark.parametrize(("shape", "outer"), [((0, 40), 6), ((2, 0, 5), 6), ((0, 0), 6), ((3, 0), 6),
+                                              ((0,), 6), ((3, 40), 0), ((0, 40), 0), ((40,), 6)], ids=str)
+def test_empty_checkpointed_calls(shape, outer, backend):
+    x = torch.ones(shape, device=DEV, requires_grad=True)
+    w, b = (torch.ones(s, device=DEV, requires_grad=True) for s in ((outer, shape[-1]), (outer,)))
+    out = linear(x, w, b, activation="gelu", checkpoint="int8", backend=backend)
+    assert out.shape == (*shape[:-1], outer)
+    dx, dw, db = torch.autograd.grad(out, [x, w, b], torch.ones_like(out))
+    assert dx.shape == shape and dw.shape == w.shape and db.shape == b.shape
+    if 0 in shape:
+        assert not dw.any() and not dx.any()
+    codes, scales = checkpoint_int8(x)
+    restored = checkpoint_restore(codes, scales, shape[-1], torch.float32)
+    assert torch.equal(restored, x.detach().reshape(restored.shape))

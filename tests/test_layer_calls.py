@@ -2,6 +2,7 @@
 refuses before anything runs, and what the PyTorch path does in its place."""
 
 import importlib
+import math
 from contextlib import nullcontext
 
 import pytest
@@ -9,7 +10,13 @@ import torch
 import torch.autograd.forward_ad as forward_ad
 from torch.fx.experimental.proxy_tensor import make_fx
 
-from muspace_amd import checkpoint_int8, get_last_dispatch_report, layer_norm, linear
+from muspace_amd import (
+    checkpoint_int8,
+    checkpoint_restore,
+    get_last_dispatch_report,
+    layer_norm,
+    linear,
+)
 from muspace_amd.runtime import native
 from muspace_amd.runtime.layer_host import load_layer_host
 
@@ -132,6 +139,29 @@ def test_autocast_does_not_reach_the_pytorch_path(checkpoint, dtype):
     for other in (torch.bfloat16, torch.float16):
         for a, e in zip(step(torch.autocast("cpu", dtype=other)), want):
             assert a.dtype == dtype and torch.equal(a, e)
+
+
+EMPTY = [((0, 40), 6), ((2, 0, 5), 6), ((0, 0), 6), ((3, 0), 6), ((0,), 6), ((3, 40), 0), ((0, 40), 0),
+         ((40,), 6)]
+
+
+@pytest.mark.parametrize("checkpoint", [None, "int8"])
+@pytest.mark.parametrize(("shape", "outer"), EMPTY, ids=str)
+def test_empty_calls_of_the_pytorch_path(shape, outer, checkpoint):
+    x = torch.ones(shape, requires_grad=True)
+    w, b = (torch.ones(s, requires_grad=True) for s in ((outer, shape[-1]), (outer,)))
+    out = linear(x, w, b, activation="gelu", checkpoint=checkpoint)
+    assert out.shape == (*shape[:-1], outer)
+    dx, dw, db = torch.autograd.grad(out, [x, w, b], torch.ones_like(out))
+    rows = math.prod(shape[:-1])
+    assert dx.shape == shape and dw.shape == w.shape and db.shape == b.shape
+    if 0 in shape:
+        assert not dw.any() and not dx.any()
+    codes, scales = checkpoint_int8(x)
+    blocks = (shape[-1] + 31) // 32
+    assert codes.shape == (rows, 32 * blocks) and scales.shape == (rows, blocks)
+    assert torch.equal(checkpoint_restore(codes, scales, shape[-1], torch.float32),
+                       x.detach().reshape(rows, shape[-1]))
 
 
 def test_the_pytorch_path_takes_devices_without_autocast():
