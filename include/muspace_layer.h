@@ -1,8 +1,9 @@
 /*
  * C-ABI of the dense operators around deformable attention in an encoder or
  * decoder layer: the linear layer with its epilogue and gradients, its 8-bit
- * input checkpoint, and layer norm with its gradients. Part of
- * `libmuspace_msda.so`, MI355X (gfx950).
+ * input checkpoint, layer norm with its gradients, dropout, and the sum of a block
+ * with the residual stream and the norm after it. Part of `libmuspace_msda.so`,
+ * MI355X (gfx950).
  *
  * Tensors are device pointers, dense, row-major, all of one type: float32 (0),
  * float16 (1) or bfloat16 (2), unless noted. Products and statistics are summed
@@ -104,6 +105,52 @@ MUSPACE_API int layer_norm_backward(const void *grad_output, int dtype, const vo
                                     void *grad_input, void *grad_weight, void *grad_bias,
                                     int64_t rows, int64_t cols, void *workspace,
                                     size_t workspace_bytes, void *stream);
+
+/* dropout: output = kept ? x / (1 - p) : 0, plus residual (or NULL), over `count`
+ * elements. Element i is kept if word i % 4 of Philox4x32-10 at counter (i / 4, offset)
+ * (64 bits each, low words first) under the key `seed` is at or over p 2^32, to the
+ * nearest. device_seed, where not NULL, is read by the kernel in place of seed: a
+ * captured call whose seed changes draws another mask. The gradient of x is the same
+ * call on output's gradient, without residual; the residual's is output's own. */
+MUSPACE_API int dropout_forward(const void *x, int dtype, const void *residual, void *output,
+                                int64_t count, double p, uint64_t seed,
+                                const int64_t *device_seed, uint64_t offset, void *stream);
+
+/* The sum of a block with the residual stream, and the norm after it:
+ *   y = post_norm(block) (post_norm -1 none: the block; 0 layer, 1 rms)
+ *   stream_values = residual_scale residual + gate dropout(y)
+ *   output = norm(stream_values as stored)   (norm 0 layer, 1 rms)
+ * block, residual, output, stream_values [rows, cols]; weight, bias, gate, post_weight,
+ * post_bias [cols] of weight_dtype (dtype or float32), each may be NULL (ones; biases
+ * zeros). The rms norm is x / sqrt(mean(x^2) + eps) weight + bias. dropout is that of
+ * dropout_forward over the tensor's elements, p 0 for none. stream_values, statistics
+ * and post_statistics ([rows, 2] float32, as layer norm's, for the backward) may be
+ * NULL. */
+MUSPACE_API int residual_norm_forward(const void *block, int dtype, const void *residual,
+                                      const void *weight, const void *bias, const void *gate,
+                                      const void *post_weight, const void *post_bias,
+                                      int weight_dtype, void *output, void *stream_values,
+                                      float *statistics, float *post_statistics, int64_t rows,
+                                      int64_t cols, int norm, int post_norm, float eps,
+                                      float residual_scale, double p, uint64_t seed,
+                                      const int64_t *device_seed, uint64_t offset, void *stream);
+
+/* Bytes of workspace of residual_norm_backward (16-byte aligned) for `sums` of the five
+ * gradients of weights. */
+MUSPACE_API size_t residual_norm_backward_workspace_size(int dtype, int64_t rows, int64_t cols,
+                                                         int sums);
+
+/* The gradients from those of output and stream_values (NULL: zeros). A NULL gradient
+ * is not computed. block is read where there is a post norm or grad_gate is wanted, and
+ * may be NULL otherwise; p, seed, device_seed's value and offset are the forward's. */
+MUSPACE_API int residual_norm_backward(
+    const void *grad_output, const void *grad_stream, int dtype, const void *block,
+    const void *stream_values, const void *weight, const void *gate, const void *post_weight,
+    const void *post_bias, int weight_dtype, const float *statistics, const float *post_statistics,
+    void *grad_block, void *grad_residual, void *grad_weight, void *grad_bias, void *grad_gate,
+    void *grad_post_weight, void *grad_post_bias, int64_t rows, int64_t cols, int norm,
+    int post_norm, float residual_scale, double p, uint64_t seed, const int64_t *device_seed,
+    uint64_t offset, void *workspace, size_t workspace_bytes, void *stream);
 
 #ifdef __cplusplus
 }

@@ -5,12 +5,13 @@ The exports mirror the MSDA part of the reference package
 dispatch explanation and the dispatch-report accessors. ``import muspace_amd
 as mu_space`` gives code written against the reference the same names. Next to
 them stand the dense operators of an attention layer (``linear``, its 8-bit
-checkpoints, ``layer_norm``), which the reference leaves to torch.
+checkpoints, ``layer_norm``, ``dropout``, ``residual_norm``), which the reference leaves to torch.
 """
 
 from .ops import (
     checkpoint_int8,
     checkpoint_restore,
+    dropout,
     explain_dispatch,
     layer_norm,
     linear,
@@ -19,6 +20,7 @@ from .ops import (
     multi_scale_deformable_attn_pytorch_compat,
     multi_scale_deformable_attn_scatter_div,
     multi_scale_deformable_attn_softmax,
+    residual_norm,
 )
 from .runtime.kernel_dispatch import (
     DispatchDecision,
@@ -37,6 +39,7 @@ __all__ = [
     "checkpoint_int8",
     "checkpoint_restore",
     "clear_dispatch_report",
+    "dropout",
     "explain_dispatch",
     "get_dispatch_reports",
     "get_last_dispatch_report",
@@ -47,4 +50,5 @@ __all__ = [
     "multi_scale_deformable_attn_pytorch_compat",
     "multi_scale_deformable_attn_scatter_div",
     "multi_scale_deformable_attn_softmax",
+    "residual_norm",
 ]

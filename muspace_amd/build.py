@@ -23,6 +23,7 @@ SOURCES = (
     PACKAGE_DIR / "csrc" / "dfa_capi.hip",
     PACKAGE_DIR / "csrc" / "linear_capi.hip",
     PACKAGE_DIR / "csrc" / "layer_norm_capi.hip",
+    PACKAGE_DIR / "csrc" / "residual_norm_capi.hip",
 )
 DEPENDS = (
     PACKAGE_DIR / "csrc" / "capi_errors.hpp",
@@ -35,6 +36,8 @@ DEPENDS = (
     PACKAGE_DIR / "csrc" / "linear_device.hpp",
     PACKAGE_DIR / "csrc" / "linear_kernels.hpp",
     PACKAGE_DIR / "csrc" / "layer_norm_kernels.hpp",
+    PACKAGE_DIR / "csrc" / "dropout_device.hpp",
+    PACKAGE_DIR / "csrc" / "residual_norm_kernels.hpp",
     REPO_DIR / "include" / "muspace_msda.h",
     REPO_DIR / "include" / "muspace_dfa.h",
     REPO_DIR / "include" / "muspace_layer.h",
@@ -46,7 +49,10 @@ PROBE_SOURCES = (PACKAGE_DIR / "csrc" / "probes.hip",)
 PROBE_LIBRARY = PACKAGE_DIR / "native" / "libmuspace_probes.so"
 # autograd nodes of the layer's dense operators: host code against torch's C++ API,
 # no kernels (muspace_amd/runtime/layer_host.py loads it)
-HOST_SOURCES = (PACKAGE_DIR / "csrc" / "layer_host.cpp",)
+HOST_SOURCES = (
+    PACKAGE_DIR / "csrc" / "layer_host.cpp",
+    PACKAGE_DIR / "csrc" / "layer_host_block.cpp",
+)
 HOST_LIBRARY = PACKAGE_DIR / "native" / "muspace_layer_host.so"
 OFFLOAD_ARCH = "gfx950"
 

@@ -1,0 +1,699 @@
+// The end of a block of an encoder or decoder layer and the start of the next
+// (include/muspace_layer.h):
+//
+//   y      = post_norm(block), or the block's output itself
+//   stream = residual_scale residual + gate dropout(y)
+//   output = norm(stream)
+//
+// and its gradients: with h = norm's unit row, s its factor and g = d output,
+//   u  = g w;  ds = d stream + s (u - mean(u) - h mean(u h))
+//   d residual = residual_scale ds;  dw = sum of g h, db = sum of g
+//   dt = ds kept / (1 - p);  d gate = sum of dt y;  dy = dt gate
+//   d block = dy, or the post norm's s' (v - mean(v) - h' mean(v h')), v = dy w'
+// The rms norm is the same without means. Memory-bound: each tensor is read and written
+// once, rows in registers over the reductions as in layer norm (layer_norm_kernels.hpp,
+// whose statistics these are); the dropout's mask is computed in both directions
+// (dropout_device.hpp).
+//
+// `output` is the norm of the stream as it is stored, rounded to the tensors' type: the
+// backward keeps the stream alone and differentiates exactly what the forward
+// computed, and a stream read back gives the same norm. (With the norm of the unrounded
+// sum the backward would have to keep the block and the residual in its place, one
+// tensor more to keep and to read of five.)
+#pragma once
+
+#include "dropout_device.hpp"
+#include "layer_norm_kernels.hpp"
+
+namespace dense {
+
+enum Norms : int { kNoNorm = -1, kLayerNorm = 0, kRmsNorm = 1 };
+
+constexpr int kSums = 5;  // dw, db, d gate, d post weight, d post bias
+
+struct Residual {
+  const void *block, *residual, *weight, *bias, *gate, *post_weight, *post_bias;
+  const void *grad_out, *grad_stream, *stream_in;
+  void *out, *stream;              // forward
+  void *d_block, *d_residual;      // backward
+  float *stats, *post_stats;       // [rows][2] each, as layer norm's
+  float *partial;                  // [workgroups][sums][cols]
+  float *row_sums;                 // rows of any length: [rows][4] for the column sums
+  int slot[kSums];                 // a column sum's place in `partial` (-1: not wanted)
+  int sums;                        // of them
+  int64_t rows;
+  int cols;
+  float eps, scale;                // residual_scale
+  int w32, norm, post;             // weights are float32; Norms
+  Drop drop;
+};
+
+// a piece of a weight, `none` without one
+template <typename T>
+__device__ __forceinline__ void load_vector(const void *p, int w32, int col, int left,
+                                            float (&w)[Piece<T>::kValues], float none) {
+  if (w32) {
+    load_weight<T, sizeof(T) == 2>(p, col, left, w, none);
+  } else {
+    load_weight<T, false>(p, col, left, w, none);
+  }
+}
+
+// 0 beyond a row's values, so that sums may take whole pieces
+template <bool kFull>
+__device__ __forceinline__ float inside(float v, int e, int left) {
+  return kFull || e < left ? v : 0.0f;
+}
+
+// Workgroups of 512 threads, kLanes of them a row, a 16-byte piece each: rows of up to
+// 512 pieces. Short rows share a wavefront, long ones take several and join their sums
+// in LDS.
+constexpr int kRowThreads = 512;
+constexpr int kTeamLds = 2 * (kRowThreads / kWave);  // floats of team_sum
+
+// kLanes lanes' sums, the same on all of them (every thread of the workgroup calls it)
+template <int kLanes, int N>
+__device__ __forceinline__ void team_sum(float (&v)[N], float *lds) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    v[i] = add_across<8>(add_across<4>(add_across<2>(add_across<1>(v[i]))));
+    if constexpr (kLanes >= 32) v[i] = add_across<16>(v[i]);
+    if constexpr (kLanes >= 64) v[i] = add_across<32>(v[i]);
+  }
+  if constexpr (kLanes > kWave) {
+    const int wave = threadIdx.x / kWave, first = threadIdx.x / kLanes * (kLanes / kWave);
+    __syncthreads();
+    if (threadIdx.x % kWave == 0) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) lds[wave * N + i] = v[i];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      v[i] = 0.0f;
+#pragma unroll
+      for (int u = 0; u < kLanes / kWave; ++u) v[i] += lds[(first + u) * N + i];
+    }
+  }
+}
+
+// a row's first value, on all of its lanes
+template <int kLanes>
+__device__ __forceinline__ float first_value(float v, float *lds) {
+  if constexpr (kLanes <= kWave) {
+    return __shfl(v, 0, kLanes);
+  } else {
+    __syncthreads();
+    if (threadIdx.x % kLanes == 0) lds[threadIdx.x / kLanes] = v;
+    __syncthreads();
+    return lds[threadIdx.x / kLanes];
+  }
+}
+
+// Centre and factor of a row in registers. `v` keeps its values; `x0` is the first.
+template <int kLanes, bool kFull, int kV>
+__device__ __forceinline__ float row_statistics(const float (&v)[kV], int cols, int lane,
+                                                float x0, int norm, float inv, float eps,
+                                                float *lds, Centre &centre) {
+  float sums[2] = {0.0f, 0.0f};
+  centre = Centre{0.0f, 0.0f};
+  if (norm == kLayerNorm) {
+    float sum[1] = {0.0f};
+    const int left = cols - lane * kV;
+#pragma unroll
+    for (int e = 0; e < kV; ++e) sum[0] += inside<kFull>(v[e] - x0, e, left);
+    team_sum<kLanes, 1>(sum, lds);
+    centre = find_centre(x0, sum[0] * inv);
+  }
+  const int left = cols - lane * kV;
+#pragma unroll
+  for (int e = 0; e < kV; ++e) {
+    const float c = inside<kFull>(v[e] - centre.base - centre.offset, e, left);
+    sums[0] += c;
+    sums[1] += c * c;
+  }
+  team_sum<kLanes, 2>(sums, lds);
+  if (norm == kRmsNorm) return 1.0f / sqrtf(sums[1] * inv + eps);
+  return correct_centre(centre, sums, inv, eps);
+}
+
+template <typename T, int kLanes, bool kFull, bool kPost>
+__global__ __launch_bounds__(kRowThreads) void residual_forward(const Residual a) {
+  constexpr int kGroups = kRowThreads / kLanes;  // rows at a time
+  constexpr int kV = Piece<T>::kValues;
+  using Pieces = RowPieces<T, kLanes, 1, kFull>;
+  __shared__ float lds[kTeamLds];
+  const int lane = threadIdx.x % kLanes;
+  const T *block = static_cast<const T *>(a.block), *residual = static_cast<const T *>(a.residual);
+  const float inv = 1.0f / static_cast<float>(a.cols);
+  const uint64_t seed = seed_of(a.drop);
+  float w[kV], b[kV], gate[kV], pw[kV], pb[kV];
+  const int col = lane * kV, left = Pieces::left(a.cols, lane, 0);
+  load_vector<T>(a.weight, a.w32, col, left, w, 1.0f);
+  load_vector<T>(a.bias, a.w32, col, left, b, 0.0f);
+  load_vector<T>(a.gate, a.w32, col, left, gate, 1.0f);
+  if constexpr (kPost) {
+    load_vector<T>(a.post_weight, a.w32, col, left, pw, 1.0f);
+    load_vector<T>(a.post_bias, a.w32, col, left, pb, 0.0f);
+  }
+  const int64_t step = static_cast<int64_t>(gridDim.x) * kGroups;
+  int64_t row = static_cast<int64_t>(blockIdx.x) * kGroups + threadIdx.x / kLanes;
+  Pieces next_y, next_r;
+  next_y.load(block, row, a.rows, a.cols, lane);
+  next_r.load(residual, row, a.rows, a.cols, lane);
+  // groups of one workgroup walk together: past the last row they sum zeros
+  for (int64_t base = static_cast<int64_t>(blockIdx.x) * kGroups; base < a.rows;
+       base += step, row += step) {
+    const bool any = row < a.rows;
+    float y[kV], v[kV];
+    next_y.values(0, a.cols, lane, any, y);
+    next_r.values(0, a.cols, lane, any, v);
+    next_y.load(block, row + step, a.rows, a.cols, lane);
+    next_r.load(residual, row + step, a.rows, a.cols, lane);
+    Centre centre;
+    if constexpr (kPost) {
+      const float x0 = first_value<kLanes>(y[0], lds);
+      const float s = row_statistics<kLanes, kFull>(y, a.cols, lane, x0, a.post, inv, a.eps, lds,
+                                                    centre);
+      if (a.post_stats != nullptr && any && lane == 0) {
+        keep_centre(a.post_stats + 2 * row, x0, centre, s);
+      }
+#pragma unroll
+      for (int e = 0; e < kV; ++e) {
+        y[e] = (y[e] - centre.base - centre.offset) * s * pw[e] + pb[e];
+      }
+    }
+    if (a.drop.on) {
+      const uint32_t bits = kept_bits<kV>(a.drop, seed, row * a.cols + col);
+#pragma unroll
+      for (int e = 0; e < kV; ++e) y[e] = (bits >> e) & 1u ? y[e] * a.drop.scale : 0.0f;
+    }
+#pragma unroll
+    for (int e = 0; e < kV; ++e) v[e] = fmaf(a.scale, v[e], gate[e] * y[e]);
+    const u32x4 stored = pack<T>(v);
+    if (a.stream != nullptr) {
+      loose_store(static_cast<T *>(a.stream) + row * a.cols + col, stored, any ? left : 0);
+    }
+    unpack<T>(stored, v);
+    const float x0 = first_value<kLanes>(v[0], lds);
+    const float s = row_statistics<kLanes, kFull>(v, a.cols, lane, x0, a.norm, inv, a.eps, lds,
+                                                  centre);
+    if (a.stats != nullptr && any && lane == 0) keep_centre(a.stats + 2 * row, x0, centre, s);
+#pragma unroll
+    for (int e = 0; e < kV; ++e) {
+      v[e] = (v[e] - centre.base - centre.offset) * s * w[e] + b[e];
+    }
+    loose_store(static_cast<T *>(a.out) + row * a.cols + col, pack<T>(v), any ? left : 0);
+  }
+}
+
+// kBlock: the block's output is read again, for a post norm or the gate's gradient.
+template <typename T, int kLanes, bool kFull, bool kBlock>
+__global__ __launch_bounds__(kRowThreads) void residual_backward(const Residual a) {
+  constexpr int kGroups = kRowThreads / kLanes;  // rows at a time
+  constexpr int kV = Piece<T>::kValues;
+  constexpr int kCols = kLanes * kV;
+  constexpr int kMine = kBlock ? kSums : 2;
+  using Pieces = RowPieces<T, kLanes, 1, kFull>;
+  __shared__ float lds[kGroups > 1 ? kGroups * kCols : kTeamLds];
+  const int lane = threadIdx.x % kLanes, group = threadIdx.x / kLanes;
+  const T *stream = static_cast<const T *>(a.stream_in), *block = static_cast<const T *>(a.block);
+  const T *go = static_cast<const T *>(a.grad_out), *gs = static_cast<const T *>(a.grad_stream);
+  const float inv = 1.0f / static_cast<float>(a.cols);
+  const uint64_t seed = seed_of(a.drop);
+  float w[kV], gate[kV], pw[kV], pb[kV];
+  const int col = lane * kV, left = Pieces::left(a.cols, lane, 0);
+  load_vector<T>(a.weight, a.w32, col, left, w, 1.0f);
+  load_vector<T>(a.gate, a.w32, col, left, gate, 1.0f);
+  if constexpr (kBlock) {
+    load_vector<T>(a.post_weight, a.w32, col, left, pw, 1.0f);
+    load_vector<T>(a.post_bias, a.w32, col, left, pb, 0.0f);
+  }
+  float sum[kMine][kV] = {};
+  const int64_t step = static_cast<int64_t>(gridDim.x) * kGroups;
+  int64_t row = static_cast<int64_t>(blockIdx.x) * kGroups + group;
+  Pieces n_stream, n_go = {}, n_gs = {}, n_block;
+  f32x2 n_stats = {0.0f, 0.0f}, n_post = {0.0f, 0.0f};
+  auto fetch = [&](int64_t r) {
+    const int64_t at = min(r, a.rows - 1);
+    n_stream.load(stream, r, a.rows, a.cols, lane);
+    if (go != nullptr) n_go.load(go, r, a.rows, a.cols, lane);
+    if (gs != nullptr) n_gs.load(gs, r, a.rows, a.cols, lane);
+    n_stats = reinterpret_cast<const f32x2 *>(a.stats)[at];
+    if constexpr (kBlock) {
+      n_block.load(block, r, a.rows, a.cols, lane);
+      if (a.post != kNoNorm) n_post = reinterpret_cast<const f32x2 *>(a.post_stats)[at];
+    }
+  };
+  fetch(row);
+  for (int64_t base = static_cast<int64_t>(blockIdx.x) * kGroups; base < a.rows;
+       base += step, row += step) {
+    const bool any = row < a.rows;
+    float h[kV], u[kV], ds[kV], y[kV];
+    n_stream.values(0, a.cols, lane, any, h);
+    n_go.values(0, a.cols, lane, any && go != nullptr, u);
+    n_gs.values(0, a.cols, lane, any && gs != nullptr, ds);
+    if constexpr (kBlock) n_block.values(0, a.cols, lane, any, y);
+    const f32x2 stats = n_stats, post = n_post;
+    fetch(row + step);
+    const float x0 = first_value<kLanes>(h[0], lds);
+    const Centre centre = kept_centre(x0, stats[0], stats[1]);
+    const float s = fabsf(stats[1]);
+    float along[2] = {0.0f, 0.0f};
+#pragma unroll
+    for (int e = 0; e < kV; ++e) {
+      // the operations of the forward, so that h is the forward's own
+      h[e] = inside<kFull>((h[e] - centre.base - centre.offset) * s, e, left);
+      sum[0][e] += u[e] * h[e];
+      sum[1][e] += u[e];
+      u[e] *= w[e];
+      along[0] += u[e];
+      along[1] += u[e] * h[e];
+    }
+    // (without a gradient of the output both are zero, and rows that have no statistics
+    // to speak of, of infinities, do not reach the stream's gradient)
+    if (go != nullptr) {
+      team_sum<kLanes, 2>(along, lds);
+      const float mu = a.norm == kLayerNorm ? along[0] * inv : 0.0f, mh = along[1] * inv;
+#pragma unroll
+      for (int e = 0; e < kV; ++e) ds[e] += s * (u[e] - mu - h[e] * mh);
+    }
+    float p0 = 0.0f;
+    if constexpr (kBlock) p0 = first_value<kLanes>(y[0], lds);
+    const Centre centre_p = kept_centre(p0, post[0], post[1]);
+    const float sp = fabsf(post[1]);
+    float across[2] = {0.0f, 0.0f};
+    const int64_t at = row * a.cols + col;
+    if (a.d_residual != nullptr) {
+      float r[kV];
+#pragma unroll
+      for (int e = 0; e < kV; ++e) r[e] = a.scale * ds[e];
+      loose_store(static_cast<T *>(a.d_residual) + at, pack<T>(r), any ? left : 0);
+    }
+    // (no bits past the last row)
+    const uint32_t bits = !any ? 0u : a.drop.on ? kept_bits<kV>(a.drop, seed, at) : ~0u;
+#pragma unroll
+    for (int e = 0; e < kV; ++e) {
+      const bool kept = (bits >> e) & 1u;
+      const float dt = kept ? ds[e] * a.drop.scale : 0.0f;
+      float dy = kept ? dt * gate[e] : 0.0f;
+      if constexpr (kBlock) {
+        dy = inside<kFull>(dy, e, left);
+        float unit = y[e];
+        if (a.post != kNoNorm) unit = (unit - centre_p.base - centre_p.offset) * sp;
+        unit = inside<kFull>(unit, e, left);
+        // with a post norm y is its result, otherwise the block's output
+        const float value = a.post != kNoNorm ? unit * pw[e] + pb[e] : unit;
+        sum[2][e] += kept && (kFull || e < left) ? dt * value : 0.0f;
+        sum[3][e] += dy * unit;
+        sum[4][e] += dy;
+        if (a.post != kNoNorm) dy *= pw[e];
+        across[0] += dy;
+        across[1] += dy * unit;
+        y[e] = unit;
+      }
+      ds[e] = dy;
+    }
+    if (a.d_block == nullptr) continue;
+    if constexpr (kBlock) {
+      if (a.post != kNoNorm) {
+        team_sum<kLanes, 2>(across, lds);
+        const float mv = a.post == kLayerNorm ? across[0] * inv : 0.0f, mh = across[1] * inv;
+#pragma unroll
+        for (int e = 0; e < kV; ++e) ds[e] = sp * (ds[e] - mv - y[e] * mh);
+      }
+    }
+    loose_store(static_cast<T *>(a.d_block) + at, pack<T>(ds), any ? left : 0);
+  }
+  if (a.partial == nullptr) return;
+  float *to = a.partial + static_cast<int64_t>(blockIdx.x) * a.sums * a.cols;
+#pragma unroll
+  for (int k = 0; k < kMine; ++k) {
+    if (a.slot[k] < 0) continue;
+    float *dst = to + static_cast<int64_t>(a.slot[k]) * a.cols;
+    if constexpr (kGroups == 1) {
+#pragma unroll
+      for (int e = 0; e < kV; ++e) {
+        if (col + e < a.cols) dst[col + e] = sum[k][e];
+      }
+    } else {
+      __syncthreads();
+#pragma unroll
+      for (int e = 0; e < kV; e += 4) {
+        const f32x4 v = {sum[k][e], sum[k][e + 1], sum[k][e + 2], sum[k][e + 3]};
+        *reinterpret_cast<f32x4 *>(lds + group * kCols + col + e) = v;
+      }
+      __syncthreads();
+      for (int c = threadIdx.x; c < a.cols; c += kRowThreads) {
+        float total = 0.0f;
+#pragma unroll
+        for (int q = 0; q < kGroups; ++q) total += lds[q * kCols + c];
+        dst[c] = total;
+      }
+    }
+  }
+}
+
+// --------------------------------------------------- rows of any length ---
+
+// A workgroup per row, its values computed from memory in every pass over it.
+constexpr int kLongThreads = 256;
+constexpr int kLongLds = 2 * (kLongThreads / kWave);  // floats of team_sum
+
+template <typename T, typename F>
+__device__ __forceinline__ void over_row(int cols, F &&f) {
+  constexpr int kV = Piece<T>::kValues;
+  for (int col = threadIdx.x * kV; col < cols; col += kLongThreads * kV) f(col, cols - col);
+}
+
+// Centre and factor of a row whose pieces `values(col, left, v)` gives.
+template <typename T, typename F>
+__device__ __forceinline__ float long_statistics(int cols, float x0, int norm, float inv, float eps,
+                                                 float *lds, Centre &centre, F &&values) {
+  constexpr int kV = Piece<T>::kValues;
+  float sums[2] = {0.0f, 0.0f};
+  centre = Centre{0.0f, 0.0f};
+  if (norm == kLayerNorm) {
+    float sum[1] = {0.0f};
+    over_row<T>(cols, [&](int col, int left) {
+      float v[kV];
+      values(col, left, v);
+#pragma unroll
+      for (int e = 0; e < kV; ++e) sum[0] += e < left ? v[e] - x0 : 0.0f;
+    });
+    team_sum<kLongThreads, 1>(sum, lds);
+    centre = find_centre(x0, sum[0] * inv);
+  }
+  over_row<T>(cols, [&](int col, int left) {
+    float v[kV];
+    values(col, left, v);
+#pragma unroll
+    for (int e = 0; e < kV; ++e) {
+      const float c = e < left ? v[e] - centre.base - centre.offset : 0.0f;
+      sums[0] += c;
+      sums[1] += c * c;
+    }
+  });
+  team_sum<kLongThreads, 2>(sums, lds);
+  if (norm == kRmsNorm) return 1.0f / sqrtf(sums[1] * inv + eps);
+  return correct_centre(centre, sums, inv, eps);
+}
+
+template <typename T>
+__global__ __launch_bounds__(kLongThreads) void residual_forward_long(const Residual a) {
+  constexpr int kV = Piece<T>::kValues;
+  __shared__ float lds[kLongLds];
+  const float inv = 1.0f / static_cast<float>(a.cols);
+  const uint64_t seed = seed_of(a.drop);
+  for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+    const T *block = static_cast<const T *>(a.block) + row * a.cols;
+    const T *residual = static_cast<const T *>(a.residual) + row * a.cols;
+    Centre centre_p = {0.0f, 0.0f};
+    float sp = 1.0f;
+    if (a.post != kNoNorm) {
+      const float p0 = to_float(block[0]);
+      sp = long_statistics<T>(a.cols, p0, a.post, inv, a.eps, lds, centre_p,
+                              [&](int col, int left, float(&v)[kV]) {
+                                unpack<T>(loose_load<T>(block + col, left), v);
+                              });
+      if (a.post_stats != nullptr && threadIdx.x == 0) {
+        keep_centre(a.post_stats + 2 * row, p0, centre_p, sp);
+      }
+    }
+    // the stream's piece as it is stored
+    auto stream = [&](int col, int left, float(&v)[kV]) {
+      float y[kV], gate[kV];
+      unpack<T>(loose_load<T>(block + col, left), y);
+      unpack<T>(loose_load<T>(residual + col, left), v);
+      load_vector<T>(a.gate, a.w32, col, left, gate, 1.0f);
+      if (a.post != kNoNorm) {
+        float pw[kV], pb[kV];
+        load_vector<T>(a.post_weight, a.w32, col, left, pw, 1.0f);
+        load_vector<T>(a.post_bias, a.w32, col, left, pb, 0.0f);
+#pragma unroll
+        for (int e = 0; e < kV; ++e) {
+          y[e] = (y[e] - centre_p.base - centre_p.offset) * sp * pw[e] + pb[e];
+        }
+      }
+      if (a.drop.on) {
+        const uint32_t bits = kept_bits<kV>(a.drop, seed, row * a.cols + col);
+#pragma unroll
+        for (int e = 0; e < kV; ++e) y[e] = (bits >> e) & 1u ? y[e] * a.drop.scale : 0.0f;
+      }
+#pragma unroll
+      for (int e = 0; e < kV; ++e) v[e] = fmaf(a.scale, v[e], gate[e] * y[e]);
+      unpack<T>(pack<T>(v), v);
+    };
+    float v0[kV] = {};
+    if (threadIdx.x == 0) stream(0, a.cols, v0);
+    const float x0 = first_value<kLongThreads>(v0[0], lds);
+    Centre centre;
+    const float s = long_statistics<T>(a.cols, x0, a.norm, inv, a.eps, lds, centre, stream);
+    if (a.stats != nullptr && threadIdx.x == 0) keep_centre(a.stats + 2 * row, x0, centre, s);
+    over_row<T>(a.cols, [&](int col, int left) {
+      float v[kV], w[kV], b[kV];
+      stream(col, left, v);
+      if (a.stream != nullptr) {
+        loose_store(static_cast<T *>(a.stream) + row * a.cols + col, pack<T>(v), left);
+      }
+      load_vector<T>(a.weight, a.w32, col, left, w, 1.0f);
+      load_vector<T>(a.bias, a.w32, col, left, b, 0.0f);
+#pragma unroll
+      for (int e = 0; e < kV; ++e) {
+        v[e] = (v[e] - centre.base - centre.offset) * s * w[e] + b[e];
+      }
+      loose_store(static_cast<T *>(a.out) + row * a.cols + col, pack<T>(v), left);
+    });
+  }
+}
+
+// A row's piece in the backward, given the means of u and u h.
+template <typename T>
+struct LongRow {
+  static constexpr int kV = Piece<T>::kValues;
+  Centre centre, centre_p;
+  float s, sp;
+
+  __device__ __forceinline__ void open(const Residual &a, int64_t row) {
+    const float k = a.stats[2 * row + 1];
+    s = fabsf(k);
+    centre = kept_centre(to_float(static_cast<const T *>(a.stream_in)[row * a.cols]),
+                         a.stats[2 * row], k);
+    centre_p = Centre{0.0f, 0.0f};
+    sp = 1.0f;
+    if (a.post != kNoNorm) {
+      const float kp = a.post_stats[2 * row + 1];
+      sp = fabsf(kp);
+      centre_p = kept_centre(to_float(static_cast<const T *>(a.block)[row * a.cols]),
+                             a.post_stats[2 * row], kp);
+    }
+  }
+  // h and g of the norm
+  __device__ __forceinline__ void unit(const Residual &a, int64_t row, int col, int left,
+                                       float (&h)[kV], float (&g)[kV]) const {
+    const int64_t at = row * a.cols + col;
+    unpack<T>(loose_load<T>(static_cast<const T *>(a.stream_in) + at, left), h);
+    unpack<T>(loose_load<T>(static_cast<const T *>(a.grad_out) + at, a.grad_out != nullptr ? left : 0),
+              g);
+#pragma unroll
+    for (int e = 0; e < kV; ++e) {
+      h[e] = e < left ? (h[e] - centre.base - centre.offset) * s : 0.0f;
+    }
+  }
+  // the stream's gradient
+  __device__ __forceinline__ void stream_grad(const Residual &a, int64_t row, int col, int left,
+                                              float mu, float mh, const float (&h)[kV],
+                                              const float (&g)[kV], float (&ds)[kV]) const {
+    const int64_t at = row * a.cols + col;
+    unpack<T>(loose_load<T>(static_cast<const T *>(a.grad_stream) + at,
+                            a.grad_stream != nullptr ? left : 0), ds);
+    if (a.grad_out == nullptr) return;
+    float w[kV];
+    load_vector<T>(a.weight, a.w32, col, left, w, 1.0f);
+#pragma unroll
+    for (int e = 0; e < kV; ++e) ds[e] += s * (g[e] * w[e] - mu - h[e] * mh);
+  }
+  // from ds: dy, the post norm's unit row (or the block's output) and what the gate
+  // multiplies
+  __device__ __forceinline__ void block_grad(const Residual &a, uint64_t seed, int64_t row, int col,
+                                             int left, const float (&ds)[kV], float (&dy)[kV],
+                                             float (&unit)[kV], float (&gated)[kV]) const {
+    const int64_t at = row * a.cols + col;
+    const uint32_t bits = a.drop.on ? kept_bits<kV>(a.drop, seed, at) : ~0u;
+    float gate[kV];
+    load_vector<T>(a.gate, a.w32, col, left, gate, 1.0f);
+    unpack<T>(loose_load<T>(static_cast<const T *>(a.block) + at, a.block != nullptr ? left : 0),
+              unit);
+    float pw[kV], pb[kV];
+    load_vector<T>(a.post_weight, a.w32, col, left, pw, 1.0f);
+    load_vector<T>(a.post_bias, a.w32, col, left, pb, 0.0f);
+#pragma unroll
+    for (int e = 0; e < kV; ++e) {
+      const bool kept = ((bits >> e) & 1u) && e < left;
+      const float dt = kept ? ds[e] * a.drop.scale : 0.0f;
+      dy[e] = kept ? dt * gate[e] : 0.0f;
+      float value = unit[e];
+      if (a.post != kNoNorm) {
+        unit[e] = e < left ? (unit[e] - centre_p.base - centre_p.offset) * sp : 0.0f;
+        value = unit[e] * pw[e] + pb[e];
+      }
+      gated[e] = kept ? dt * value : 0.0f;
+    }
+  }
+};
+
+template <typename T>
+__global__ __launch_bounds__(kLongThreads) void residual_backward_long(const Residual a) {
+  constexpr int kV = Piece<T>::kValues;
+  __shared__ float lds[kLongLds];
+  const float inv = 1.0f / static_cast<float>(a.cols);
+  const uint64_t seed = seed_of(a.drop);
+  for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+    LongRow<T> r;
+    r.open(a, row);
+    float mean[2] = {0.0f, 0.0f}, mean_p[2] = {0.0f, 0.0f};
+    if (a.grad_out != nullptr) {
+      over_row<T>(a.cols, [&](int col, int left) {
+        float h[kV], g[kV], w[kV];
+        r.unit(a, row, col, left, h, g);
+        load_vector<T>(a.weight, a.w32, col, left, w, 1.0f);
+#pragma unroll
+        for (int e = 0; e < kV; ++e) {
+          mean[0] += g[e] * w[e];
+          mean[1] += g[e] * w[e] * h[e];
+        }
+      });
+      team_sum<kLongThreads, 2>(mean, lds);
+      mean[0] = a.norm == kLayerNorm ? mean[0] * inv : 0.0f;
+      mean[1] *= inv;
+    }
+    if (a.row_sums != nullptr && threadIdx.x == 0) {
+      a.row_sums[2 * row] = mean[0];
+      a.row_sums[2 * row + 1] = mean[1];
+    }
+    auto block_grad = [&](int col, int left, float(&ds)[kV], float(&dy)[kV], float(&unit)[kV]) {
+      float h[kV], g[kV], gated[kV];
+      r.unit(a, row, col, left, h, g);
+      r.stream_grad(a, row, col, left, mean[0], mean[1], h, g, ds);
+      r.block_grad(a, seed, row, col, left, ds, dy, unit, gated);
+      if (a.post != kNoNorm) {
+        float pw[kV];
+        load_vector<T>(a.post_weight, a.w32, col, left, pw, 1.0f);
+#pragma unroll
+        for (int e = 0; e < kV; ++e) dy[e] *= pw[e];
+      }
+    };
+    if (a.post != kNoNorm && a.d_block != nullptr) {
+      over_row<T>(a.cols, [&](int col, int left) {
+        float ds[kV], dy[kV], unit[kV];
+        block_grad(col, left, ds, dy, unit);
+#pragma unroll
+        for (int e = 0; e < kV; ++e) {
+          mean_p[0] += dy[e];
+          mean_p[1] += dy[e] * unit[e];
+        }
+      });
+      team_sum<kLongThreads, 2>(mean_p, lds);
+      mean_p[0] = a.post == kLayerNorm ? mean_p[0] * inv : 0.0f;
+      mean_p[1] *= inv;
+    }
+    over_row<T>(a.cols, [&](int col, int left) {
+      float ds[kV], dy[kV], unit[kV];
+      block_grad(col, left, ds, dy, unit);
+      const int64_t at = row * a.cols + col;
+      if (a.d_block != nullptr) {
+        if (a.post != kNoNorm) {
+#pragma unroll
+          for (int e = 0; e < kV; ++e) dy[e] = r.sp * (dy[e] - mean_p[0] - unit[e] * mean_p[1]);
+        }
+        loose_store(static_cast<T *>(a.d_block) + at, pack<T>(dy), left);
+      }
+      if (a.d_residual != nullptr) {
+#pragma unroll
+        for (int e = 0; e < kV; ++e) ds[e] *= a.scale;
+        loose_store(static_cast<T *>(a.d_residual) + at, pack<T>(ds), left);
+      }
+    });
+  }
+}
+
+// Column sums of long rows, after residual_backward_long: a thread per piece of columns,
+// blockIdx.y a run of rows.
+template <typename T>
+__global__ __launch_bounds__(kLongThreads) void residual_columns_long(const Residual a) {
+  constexpr int kV = Piece<T>::kValues;
+  const int col = (blockIdx.x * kLongThreads + threadIdx.x) * kV;
+  if (col >= a.cols) return;
+  const int left = a.cols - col;
+  const uint64_t seed = seed_of(a.drop);
+  float sum[kSums][kV] = {};
+  for (int64_t row = blockIdx.y; row < a.rows; row += gridDim.y) {
+    LongRow<T> r;
+    r.open(a, row);
+    float h[kV], g[kV];
+    r.unit(a, row, col, left, h, g);
+#pragma unroll
+    for (int e = 0; e < kV; ++e) {
+      sum[0][e] += g[e] * h[e];
+      sum[1][e] += g[e];
+    }
+    if (a.slot[2] < 0 && a.slot[3] < 0 && a.slot[4] < 0) continue;
+    float ds[kV], dy[kV], unit[kV], gated[kV];
+    r.stream_grad(a, row, col, left, a.row_sums[2 * row], a.row_sums[2 * row + 1], h, g, ds);
+    r.block_grad(a, seed, row, col, left, ds, dy, unit, gated);
+#pragma unroll
+    for (int e = 0; e < kV; ++e) {
+      sum[2][e] += gated[e];
+      sum[3][e] += dy[e] * unit[e];
+      sum[4][e] += dy[e];
+    }
+  }
+  float *to = a.partial + static_cast<int64_t>(blockIdx.y) * a.sums * a.cols;
+#pragma unroll
+  for (int k = 0; k < kSums; ++k) {
+    if (a.slot[k] < 0) continue;
+    float *dst = to + static_cast<int64_t>(a.slot[k]) * a.cols + col;
+#pragma unroll
+    for (int e = 0; e < kV; ++e) {
+      if (e < left) dst[e] = sum[k][e];
+    }
+  }
+}
+
+struct SumTargets {
+  void *to[kSums];  // by place in `partial`
+};
+
+// The workgroups' rows of sums, added in order: 16 columns by 16 runs of rows a
+// workgroup, runs joined in LDS.
+template <typename W>
+__global__ __launch_bounds__(256) void residual_sum_columns(const float *partial, int parts,
+                                                            int cols, int sums, SumTargets out) {
+  __shared__ float lds[16][17];
+  const int x = threadIdx.x & 15, y = threadIdx.x >> 4;
+  const int64_t ld = static_cast<int64_t>(sums) * cols;
+  const int64_t col = static_cast<int64_t>(blockIdx.x) * 16 + x;
+  float total = 0.0f;
+  if (col < ld) {
+    const float *src = partial + col;
+    int p = y;
+    for (; p + 7 * 16 < parts; p += 8 * 16) {
+      float v[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = src[(p + 16 * e) * ld];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) total += v[e];
+    }
+    for (; p < parts; p += 16) total += src[p * ld];
+  }
+  lds[y][x] = total;
+  __syncthreads();
+  if (y != 0 || col >= ld) return;
+  total = 0.0f;
+#pragma unroll
+  for (int e = 0; e < 16; ++e) total += lds[e][x];
+  const int k = static_cast<int>(col / cols);
+  static_cast<W *>(out.to[k])[col - static_cast<int64_t>(k) * cols] = from_float<W>(total);
+}
+
+}  // namespace dense

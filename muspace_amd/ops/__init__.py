@@ -15,8 +15,10 @@ from .deformable_aggregation import (
     deformable_aggregation_reference,
     feature_maps_format,
 )
+from .dropout import dropout, dropout_pytorch
 from .layer_norm import layer_norm, layer_norm_pytorch
 from .linear import checkpoint_int8, checkpoint_restore, linear, linear_pytorch
+from .residual_norm import residual_norm, residual_norm_pytorch
 
 __all__ = [
     "attention_softmax",
@@ -25,6 +27,8 @@ __all__ = [
     "deformable_aggregation",
     "deformable_aggregation_function",
     "deformable_aggregation_reference",
+    "dropout",
+    "dropout_pytorch",
     "feature_maps_format",
     "explain_dispatch",
     "layer_norm",
@@ -37,4 +41,6 @@ __all__ = [
     "multi_scale_deformable_attn_pytorch_compat",
     "multi_scale_deformable_attn_scatter_div",
     "multi_scale_deformable_attn_softmax",
+    "residual_norm",
+    "residual_norm_pytorch",
 ]

@@ -3,6 +3,7 @@
 from __future__ import annotations
 
 from functools import lru_cache, wraps
+from inspect import signature
 
 import torch
 
@@ -47,13 +48,15 @@ def in_the_tensors_type(function):
     """A PyTorch path that computes in its tensors' type, as the kernels do: autocast, which
     would choose another, is off within it."""
 
+    first = next(iter(signature(function).parameters))
+
     @wraps(function)
-    def call(input, *args, **kwargs):
-        device = input.device.type
+    def call(*args, **kwargs):
+        device = (args[0] if args else kwargs[first]).device.type
         if not torch.amp.is_autocast_available(device) or not torch.is_autocast_enabled(device):
-            return function(input, *args, **kwargs)
+            return function(*args, **kwargs)
         with torch.autocast(device, enabled=False):
-            return function(input, *args, **kwargs)
+            return function(*args, **kwargs)
 
     return call
 

@@ -28,7 +28,7 @@ from typing import Any, Callable
 import torch
 
 LIBRARY_RELPATH = "native/libmuspace_msda.so"
-ABI_VERSION = 7
+ABI_VERSION = 8
 
 DTYPE_F32, DTYPE_F16, DTYPE_BF16 = 0, 1, 2
 
@@ -172,6 +172,26 @@ _EXPORTS: dict[str, tuple[Any, list[Any]]] = {
         _c_int,
         [_c_ptr, _c_int, _c_ptr, _c_ptr, _c_int] + [_c_ptr] * 4
         + [_c_int64, _c_int64, _c_ptr, ctypes.c_size_t, _c_ptr],
+    ),
+    "dropout_forward": (
+        _c_int,
+        [_c_ptr, _c_int, _c_ptr, _c_ptr, _c_int64, ctypes.c_double, ctypes.c_uint64, _c_ptr,
+         ctypes.c_uint64, _c_ptr],
+    ),
+    "residual_norm_forward": (
+        _c_int,
+        [_c_ptr, _c_int] + [_c_ptr] * 6 + [_c_int] + [_c_ptr] * 4 + [_c_int64, _c_int64, _c_int,
+         _c_int, ctypes.c_float, ctypes.c_float, ctypes.c_double, ctypes.c_uint64, _c_ptr,
+         ctypes.c_uint64, _c_ptr],
+    ),
+    "residual_norm_backward_workspace_size": (
+        ctypes.c_size_t, [_c_int, _c_int64, _c_int64, _c_int]
+    ),
+    "residual_norm_backward": (
+        _c_int,
+        [_c_ptr, _c_ptr, _c_int] + [_c_ptr] * 6 + [_c_int] + [_c_ptr] * 9
+        + [_c_int64, _c_int64, _c_int, _c_int, ctypes.c_float, ctypes.c_double, ctypes.c_uint64,
+           _c_ptr, ctypes.c_uint64, _c_ptr, ctypes.c_size_t, _c_ptr],
     ),
 }
 
