@@ -1,7 +1,7 @@
 /*
  * C-ABI of the dense operators around deformable attention in an encoder or
  * decoder layer: the linear layer with its epilogue and gradients, its 8-bit
- * input checkpoint, layer norm with its gradients, dropout, and the sum of a block
+ * input checkpoint, the gated layer, layer norm with its gradients, dropout, and the sum of a block
  * with the residual stream and the norm after it. Part of `libmuspace_msda.so`,
  * MI355X (gfx950).
  *
@@ -83,6 +83,33 @@ MUSPACE_API int linear_backward(const void *grad_output, int dtype, const void *
                                 int64_t rows, int64_t in_features, int64_t out_features,
                                 int activation, void *workspace, size_t workspace_bytes,
                                 void *stream);
+
+/* The gated layer: weight [2 hidden, in] holds the gate's rows, then the others' (bias
+ * [2 hidden] or NULL the same); with a and u the two halves of x weight^T + bias,
+ *   output = act(a) u   [rows, hidden]
+ * activation: 0 none, 1 relu, 2 gelu, 3 silu (a / (1 + exp(-a))), 4 sigmoid. */
+MUSPACE_API int gated_linear_forward(const void *x, int dtype, const void *weight,
+                                     const void *bias, void *output, int64_t rows,
+                                     int64_t in_features, int64_t hidden_features, int activation,
+                                     void *stream);
+
+/* Bytes of workspace of gated_linear_backward (256-byte aligned) for the gradients whose
+ * flag is not 0. */
+MUSPACE_API size_t gated_linear_backward_workspace_size(int dtype, int64_t rows,
+                                                        int64_t in_features,
+                                                        int64_t hidden_features, int want_input,
+                                                        int want_weight, int want_bias);
+
+/* a and u are computed again; da = grad_output u act'(a) and du = grad_output act(a) are
+ * rounded to the tensors' type (past its range: to infinities); grad_input = [da du]
+ * weight, grad_weight = [da du]^T x, grad_bias their sums over the rows. A NULL gradient
+ * is not computed; x, weight and bias are needed for any. Outputs are overwritten. */
+MUSPACE_API int gated_linear_backward(const void *grad_output, int dtype, const void *x,
+                                      const void *weight, const void *bias, void *grad_input,
+                                      void *grad_weight, void *grad_bias, int64_t rows,
+                                      int64_t in_features, int64_t hidden_features,
+                                      int activation, void *workspace, size_t workspace_bytes,
+                                      void *stream);
 
 /* layer norm over the last dimension:
  *   c = x - mean(x);  s = 1 / sqrt(mean(c^2) + eps);  output = c s weight + bias

@@ -5,7 +5,7 @@ The exports mirror the MSDA part of the reference package
 dispatch explanation and the dispatch-report accessors. ``import muspace_amd
 as mu_space`` gives code written against the reference the same names. Next to
 them stand the dense operators of an attention layer (``linear``, its 8-bit
-checkpoints, ``layer_norm``, ``dropout``, ``residual_norm``), which the reference leaves to torch.
+checkpoints, ``gated_linear``, ``layer_norm``, ``dropout``, ``residual_norm``), which the reference leaves to torch.
 """
 
 from .ops import (
@@ -13,6 +13,7 @@ from .ops import (
     checkpoint_restore,
     dropout,
     explain_dispatch,
+    gated_linear,
     layer_norm,
     linear,
     multi_scale_deformable_attn,
@@ -41,6 +42,7 @@ __all__ = [
     "clear_dispatch_report",
     "dropout",
     "explain_dispatch",
+    "gated_linear",
     "get_dispatch_reports",
     "get_last_dispatch_report",
     "layer_norm",

@@ -36,6 +36,9 @@ struct Api {
   decltype(&::layer_norm_forward) norm_forward = nullptr;
   decltype(&::layer_norm_backward_workspace_size) norm_workspace = nullptr;
   decltype(&::layer_norm_backward) norm_backward = nullptr;
+  decltype(&::gated_linear_forward) gated_forward = nullptr;
+  decltype(&::gated_linear_backward_workspace_size) gated_workspace = nullptr;
+  decltype(&::gated_linear_backward) gated_backward = nullptr;
   decltype(&::dropout_forward) dropout_forward = nullptr;
   decltype(&::residual_norm_forward) residual_forward = nullptr;
   decltype(&::residual_norm_backward_workspace_size) residual_workspace = nullptr;

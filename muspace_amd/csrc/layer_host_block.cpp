@@ -1,5 +1,5 @@
-// Autograd nodes of what stands around the products of a layer's blocks: dropout and
-// the residual norm. The contract is that of layer_host.cpp.
+// Autograd nodes of a layer's blocks besides linear and layer norm: the gated layer,
+// dropout and the residual norm. The contract is that of layer_host.cpp.
 #include <pybind11/stl.h>
 
 #include <cmath>
@@ -10,6 +10,73 @@
 namespace {
 
 using namespace layer_host;
+
+// ------------------------------------------------------------ gated linear ---
+
+Tensor gated_run(const Tensor &input, const Tensor &weight, const Tensor &bias,
+                 int64_t activation) {
+  auto shape = input.sizes().vec();
+  shape.back() = weight.size(0) / 2;
+  Tensor output = at::empty(shape, input.options());
+  check(api.gated_forward(input.data_ptr(), code_of(input.scalar_type(), "input"),
+                          weight.data_ptr(), pointer(bias), output.data_ptr(), rows_of(input),
+                          weight.size(1), weight.size(0) / 2, static_cast<int>(activation),
+                          stream_of(input)),
+        "gated_linear_forward");
+  return output;
+}
+
+struct GatedFunction : torch::autograd::Function<GatedFunction> {
+  static Tensor forward(AutogradContext *ctx, const Tensor &input, const Tensor &weight,
+                        const OptTensor &bias, int64_t activation) {
+    // every gradient needs both halves of the product, which are computed again
+    ctx->save_for_backward({input, weight, bias.value_or(Tensor())});
+    ctx->saved_data["activation"] = activation;
+    return gated_run(input, weight, bias.value_or(Tensor()), activation);
+  }
+
+  static variable_list backward(AutogradContext *ctx, variable_list grads) {
+    const variable_list saved = ctx->get_saved_variables();
+    const Tensor &x = saved[0], &weight = saved[1], &bias = saved[2];
+    const Tensor g = dense(grads[0]);
+    const c10::DeviceGuard guard(g.device());
+    const int64_t rows = rows_of(x), cols = weight.size(1), hidden = weight.size(0) / 2;
+    Tensor grad_input, grad_weight, grad_bias;
+    if (ctx->needs_input_grad(0)) grad_input = at::empty(x.sizes(), x.options());
+    if (ctx->needs_input_grad(1)) grad_weight = at::empty(weight.sizes(), x.options());
+    if (bias.defined() && ctx->needs_input_grad(2)) {
+      grad_bias = at::empty(bias.sizes(), x.options());
+    }
+    const int code = code_of(x.scalar_type(), "input");
+    const size_t bytes = api.gated_workspace(code, rows, cols, hidden, grad_input.defined(),
+                                             grad_weight.defined(), grad_bias.defined());
+    const Tensor workspace = scratch(bytes, x);
+    check(api.gated_backward(g.data_ptr(), code, x.data_ptr(), weight.data_ptr(), pointer(bias),
+                             pointer(grad_input), pointer(grad_weight), pointer(grad_bias), rows,
+                             cols, hidden, static_cast<int>(ctx->saved_data["activation"].toInt()),
+                             pointer(workspace), bytes, stream_of(x)),
+          "gated_linear_backward");
+    return once({grad_input, grad_weight, grad_bias, Tensor()}, "gated_linear");
+  }
+};
+
+OptTensor gated_linear(const Tensor &input, const Tensor &weight, const OptTensor &bias,
+                       int64_t activation) {
+  const at::ScalarType type = input.scalar_type();
+  if (!supported(type) || input.dim() == 0 || weight.dim() != 2 || weight.size(0) % 2 != 0 ||
+      weight.size(1) != input.size(-1) || weight.scalar_type() != type ||
+      !row_of(bias, weight.size(0), type)) {
+    return OptTensor();
+  }
+  refuse_tracing("gated_linear");
+  const c10::DeviceGuard guard(input.device());
+  const Tensor x = dense(input), w = prepared(weight, x, "weight"), b = prepared(bias, x, "bias");
+  refuse_tangents("gated_linear", {&x, &w, &b});
+  if (at::GradMode::is_enabled() && (wants_grad(x) || wants_grad(w) || wants_grad(b))) {
+    return GatedFunction::apply(x, w, opt(b), activation);
+  }
+  return gated_run(x, w, b, activation);
+}
 
 // ----------------------------------------------------------------- dropout ---
 
@@ -273,6 +340,7 @@ namespace layer_host {
 
 void define_block(pybind11::module_ &m) {
   namespace py = pybind11;
+  m.def("gated_linear", &gated_linear, py::call_guard<py::gil_scoped_release>());
   m.def("dropout", &dropout, py::call_guard<py::gil_scoped_release>());
   m.def("residual_norm", &residual_norm, py::call_guard<py::gil_scoped_release>());
 }

@@ -23,17 +23,13 @@ constexpr int64_t kMaxRows = INT_MAX - 256;
 constexpr int64_t kMaxFeatures = 1 << 20;
 constexpr int kCus = 256;
 
-int validate(const char *fn, int dtype, int64_t rows, int64_t in, int64_t out, int act) {
+int validate(const char *fn, int dtype, int64_t rows, int64_t in, int64_t out) {
   if (dtype < 0 || dtype > 2) {
     return fail(MUSPACE_EINVAL, "%s: tensors must be float32, float16 or bfloat16", fn);
   }
   if (rows < 0 || in < 0 || out < 0) {
     return fail(MUSPACE_EINVAL, "%s: invalid dims rows=%lld in_features=%lld out_features=%lld",
                 fn, (long long)rows, (long long)in, (long long)out);
-  }
-  if (act < dense::kNone || act > dense::kGelu) {
-    return fail(MUSPACE_EINVAL, "%s: activation must be 0 (none), 1 (relu) or 2 (gelu), got %d",
-                fn, act);
   }
   // a launch holds fewer than 2^32 threads: 2^24 tiles of 128 x 128
   const int64_t r = rows / 128 + 1, i = in / 128 + 1, o = out / 128 + 1;
@@ -43,6 +39,30 @@ int validate(const char *fn, int dtype, int64_t rows, int64_t in, int64_t out, i
     return fail(MUSPACE_ERANGE, "%s: dims exceed the kernels' 32-bit indexing", fn);
   }
   return ok();
+}
+
+int validate(const char *fn, int dtype, int64_t rows, int64_t in, int64_t out, int act) {
+  const int rc = validate(fn, dtype, rows, in, out);
+  if (rc == MUSPACE_EINVAL) return rc;
+  if (act < dense::kNone || act > dense::kGelu) {
+    return fail(MUSPACE_EINVAL, "%s: activation must be 0 (none), 1 (relu) or 2 (gelu), got %d",
+                fn, act);
+  }
+  return rc;
+}
+
+// of the gated layer: [Wg; Wu] is a weight of 2 hidden rows
+int validate_gated(const char *fn, int dtype, int64_t rows, int64_t in, int64_t hidden, int act) {
+  const int rc = validate(fn, dtype, rows, in,
+                          hidden > kMaxFeatures ? kMaxFeatures + 1 : 2 * hidden);
+  if (rc == MUSPACE_EINVAL) return rc;
+  if (act < dense::kNone || act > dense::kSigmoid) {
+    return fail(MUSPACE_EINVAL,
+                "%s: activation must be 0 (none), 1 (relu), 2 (gelu), 3 (silu) or 4 (sigmoid), "
+                "got %d",
+                fn, act);
+  }
+  return rc;
 }
 
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
@@ -147,7 +167,7 @@ void launch_tight(const Product &a, int blocks, bool tight, hipStream_t st) {
 template <typename T, Job kJob, Kind kKind, bool kCodes>
 void launch_product(Product a, bool large, bool tight, hipStream_t st) {
   const int b = large ? 128 : 64;
-  a.tiles_n = static_cast<int>(ceil_div(a.n > 0 ? a.n : 1, b));
+  a.tiles_n = static_cast<int>(ceil_div(a.n > 0 ? a.n : 1, dense::gated(kJob) ? b / 2 : b));
   a.tiles = static_cast<int>(ceil_div(a.m, b)) * a.tiles_n;
   const int blocks = a.tiles * a.splits;
   if (blocks == 0) return;
@@ -162,7 +182,7 @@ template <typename T, Job kJob, Kind kKind>
 void launch_few(Product a, bool tight, hipStream_t st) {
   // four and eight: 64 x 2048 -> 2048 bf16 8.7 and 6.6 us, 300 x 256 -> 256 3.3 and 3.4
   constexpr int kWaves = 8;
-  a.tiles_n = static_cast<int>(ceil_div(a.n, 32));
+  a.tiles_n = static_cast<int>(ceil_div(a.n, dense::gated(kJob) ? 16 : 32));
   a.tiles = static_cast<int>(ceil_div(a.m, 32)) * a.tiles_n;
   if (tight) {
     dense::linear_few<T, kJob, kWaves, true, kKind><<<a.tiles, kWaves * 64, 0, st>>>(a);
@@ -173,10 +193,11 @@ void launch_few(Product a, bool tight, hipStream_t st) {
 
 template <typename T, Job kJob, Kind kKind>
 void run_rows(const Product &a, bool tight, hipStream_t st) {
-  if (few_results<T>(a.m, a.n, a.k)) {
+  const int64_t columns = dense::gated(kJob) ? 2 * int64_t{a.n} : a.n;
+  if (few_results<T>(a.m, columns, a.k)) {
     launch_few<T, kJob, kKind>(a, tight, st);
   } else {
-    launch_product<T, kJob, kKind, false>(a, large_tiles(a.m, a.n), tight, st);
+    launch_product<T, kJob, kKind, false>(a, large_tiles(a.m, columns), tight, st);
   }
 }
 
@@ -192,24 +213,26 @@ bool few_rows(int64_t rows) {
   return rows <= (sizeof(T) == 4 ? 8 : 4);
 }
 
-template <typename T, int kRows, int kCols>
+template <typename T, Job kJob, int kRows, int kCols>
 void launch_vector(const Product &a, hipStream_t st) {
-  dense::linear_vector<T, kRows, kCols>
+  dense::linear_vector<T, kJob, kRows, kCols>
       <<<static_cast<int>(ceil_div(a.n, 8)), 8 / kCols * 64, 0, st>>>(a);
 }
 
-template <typename T>
+template <typename T, Job kJob>
 void run_vector(const Product &a, hipStream_t st) {
+  constexpr int kCols = dense::gated(kJob) ? 1 : 2;  // rows of (either half of) W
   if (a.m == 1) {
-    launch_vector<T, 1, 1>(a, st);
+    launch_vector<T, kJob, 1, 1>(a, st);
   } else if (a.m == 2) {
-    launch_vector<T, 2, 1>(a, st);
+    launch_vector<T, kJob, 2, 1>(a, st);
   } else if (a.m <= 4) {
-    launch_vector<T, 4, 2>(a, st);
+    launch_vector<T, kJob, 4, kCols>(a, st);
   } else if constexpr (sizeof(T) == 4) {
-    launch_vector<T, 8, 2>(a, st);
+    launch_vector<T, kJob, 8, kCols>(a, st);
   }
 }
+
 
 int grid_for(int64_t work) {
   const int64_t b = ceil_div(work, dense::kThreads);
@@ -271,6 +294,115 @@ void by_type(int dtype, F &&f) {
   }
 }
 
+template <Job kJob>
+void run_gated(int dtype, const Product &a, bool tight, hipStream_t st) {
+  by_type(dtype, [&](auto t) {
+    using T = decltype(t);
+    if (few_rows<T>(a.m)) {
+      run_vector<T, kJob>(a, st);
+    } else {
+      run_rows<T, kJob, Kind::kPlain>(a, tight, st);
+    }
+  });
+}
+
+Product gated_product(const void *x, const void *weight, const void *bias, int64_t rows, int64_t in,
+                      int64_t hidden, int act, void *out) {
+  Product a = {};
+  a.p = x;
+  a.q = weight;
+  a.ldp = a.ldq = in;
+  a.m = static_cast<int>(rows);
+  a.n = static_cast<int>(hidden);
+  a.k = static_cast<int>(in);
+  a.splits = 1;
+  a.bias = bias;
+  a.out = out;
+  a.act = act;
+  return a;
+}
+
+bool gated_tight(int dtype, const void *x, const void *weight, int64_t in) {
+  return in % chunk_values(dtype) == 0 && aligned16(x) && aligned16(weight);
+}
+
+// What the gradients' products read: dz [rows, ld] (and what rounding left of it), relu's
+// mask over it, x or its codes, the weight.
+struct Gradients {
+  const void *dz, *dz_rest;
+  int64_t dz_ld;
+  const uint8_t *mask;
+  const void *x;
+  const int8_t *codes;
+  const uint8_t *scales;
+  const void *weight;
+  void *input, *weight_out, *bias;
+  int64_t rows, in, out;
+};
+
+// dx = dz W, dW = dz^T x and db; `ws`: the parts' sums.
+void run_gradients(int dtype, const Gradients &g, const Wanted &want, char *ws, hipStream_t st) {
+  const int v = chunk_values(dtype);
+  const bool whole_out = g.dz_ld % v == 0 && aligned16(g.dz);
+  if (want.input) {
+    Product a = {};
+    a.p = g.dz;
+    a.p_rest = g.dz_rest;
+    a.q = g.weight;
+    a.ldp = g.dz_ld;
+    a.ldq = g.in;
+    a.m = static_cast<int>(g.rows);
+    a.n = static_cast<int>(g.in);
+    a.k = static_cast<int>(g.out);
+    a.mask = g.mask;
+    a.mask_ld = g.rows * 8;
+    a.splits = 1;
+    a.out = g.input;
+    const bool tight = whole_out && g.in % v == 0 && aligned16(g.weight);
+    by_type(dtype, [&](auto t) {
+      using T = decltype(t);
+      by_kind<T>(a, [&](auto kind) {
+        run_rows<T, Job::kInput, decltype(kind)::value>(a, tight, st);
+      });
+    });
+  }
+  if (want.weight || want.bias) {
+    const WeightPlan plan = plan_weight(dtype, g.rows, g.in, g.out);
+    Product a = {};
+    a.p = g.dz;
+    a.p_rest = g.dz_rest;
+    a.ldp = g.dz_ld;
+    a.m = static_cast<int>(g.out);
+    // without a weight gradient: no columns, the first column of tiles sums dz
+    a.n = want.weight ? static_cast<int>(g.in) : 0;
+    a.k = static_cast<int>(g.rows);
+    const bool coded = want.weight && g.codes != nullptr;
+    a.q = coded ? static_cast<const void *>(g.codes) : g.x;
+    a.ldq = coded ? (g.in + 31) & ~int64_t{31} : g.in;
+    a.scales = coded ? g.scales : nullptr;
+    a.scale_ld = a.ldq / 32;
+    a.mask = g.mask;
+    a.mask_ld = g.rows * 8;
+    a.splits = plan.splits;
+    a.k_split = plan.k_split;
+    a.out = g.weight_out;
+    if (plan.splits > 1) {
+      a.partial = reinterpret_cast<float *>(ws);  // (without a weight gradient: not written)
+      if (want.bias) {
+        a.bias_partial =
+            reinterpret_cast<float *>(ws + weight_partial_bytes(plan, want, g.in, g.out));
+      }
+    } else if (want.bias) {
+      a.bias_out = g.bias;
+    }
+    const bool tight = whole_out && (!want.weight || coded || (g.in % v == 0 && aligned16(g.x)));
+    by_type(dtype, [&](auto t) {
+      run_weight<decltype(t)>(a, plan, tight, coded, g.weight_out, want.bias ? g.bias : nullptr,
+                              st);
+    });
+  }
+}
+
 }  // namespace
 
 extern "C" {
@@ -315,7 +447,7 @@ int linear_forward(const void *x, int dtype, const void *weight, const void *bia
     using T = decltype(t);
     if (few_rows<T>(a.m)) {
       if (codes != nullptr && a.k > 0) run_checkpoint<T>(x, a.codes, scales, rows, a.k, st);
-      run_vector<T>(a, st);
+      run_vector<T, Job::kForward>(a, st);
       return;
     }
     if (codes != nullptr) {
@@ -416,67 +548,78 @@ int linear_backward(const void *grad_output, int dtype, const void *x, const int
     dz = ws;
     ws += dz_tensors(dtype) * bytes;
   }
-  const bool whole_out = dz_ld % v == 0 && aligned16(dz);
-  const uint8_t *mask = activation == dense::kRelu && summed ? relu_mask : nullptr;
+  const Gradients g = {dz, dz_rest, dz_ld,
+                       activation == dense::kRelu && summed ? relu_mask : nullptr, x, codes, scales,
+                       weight, grad_input, grad_weight, grad_bias, rows, in_features, out_features};
+  run_gradients(dtype, g, want, ws, st);
+  return check_launch(fn);
+}
 
-  if (want.input) {
-    Product a = {};
-    a.p = dz;
-    a.p_rest = dz_rest;
-    a.q = weight;
-    a.ldp = dz_ld;
-    a.ldq = in_features;
-    a.m = static_cast<int>(rows);
-    a.n = static_cast<int>(in_features);
-    a.k = static_cast<int>(out_features);
-    a.mask = mask;
-    a.mask_ld = rows * 8;
-    a.splits = 1;
-    a.out = grad_input;
-    const bool tight = whole_out && in_features % v == 0 && aligned16(weight);
-    by_type(dtype, [&](auto t) {
-      using T = decltype(t);
-      by_kind<T>(a, [&](auto kind) {
-        run_rows<T, Job::kInput, decltype(kind)::value>(a, tight, st);
-      });
-    });
+int gated_linear_forward(const void *x, int dtype, const void *weight, const void *bias,
+                         void *output, int64_t rows, int64_t in_features, int64_t hidden_features,
+                         int activation, void *stream) {
+  const char *fn = "gated_linear_forward";
+  const int rc = validate_gated(fn, dtype, rows, in_features, hidden_features, activation);
+  if (rc != MUSPACE_OK) return rc;
+  if (rows == 0 || hidden_features == 0) return ok();
+  if (output == nullptr || (in_features > 0 && (x == nullptr || weight == nullptr))) {
+    return fail(MUSPACE_EINVAL, "%s: null tensor pointer", fn);
   }
-  if (want.weight || want.bias) {
-    const WeightPlan plan = plan_weight(dtype, rows, in_features, out_features);
-    Product a = {};
-    a.p = dz;
-    a.p_rest = dz_rest;
-    a.ldp = dz_ld;
-    a.m = static_cast<int>(out_features);
-    // without a weight gradient: no columns, the first column of tiles sums dz
-    a.n = want.weight ? static_cast<int>(in_features) : 0;
-    a.k = static_cast<int>(rows);
-    const bool coded = want.weight && codes != nullptr;
-    a.q = coded ? static_cast<const void *>(codes) : x;
-    a.ldq = coded ? (in_features + 31) & ~int64_t{31} : in_features;
-    a.scales = coded ? scales : nullptr;
-    a.scale_ld = a.ldq / 32;
-    a.mask = mask;
-    a.mask_ld = rows * 8;
-    a.splits = plan.splits;
-    a.k_split = plan.k_split;
-    a.out = grad_weight;
-    if (plan.splits > 1) {
-      a.partial = reinterpret_cast<float *>(ws);  // (without a weight gradient: not written)
-      if (want.bias) {
-        a.bias_partial = reinterpret_cast<float *>(
-            ws + weight_partial_bytes(plan, want, in_features, out_features));
-      }
-    } else if (want.bias) {
-      a.bias_out = grad_bias;
-    }
-    const bool tight =
-        whole_out && (!want.weight || coded || (in_features % v == 0 && aligned16(x)));
-    by_type(dtype, [&](auto t) {
-      run_weight<decltype(t)>(a, plan, tight, coded, grad_weight, want.bias ? grad_bias : nullptr,
-                              st);
-    });
+  const Product a = gated_product(x, weight, bias, rows, in_features, hidden_features, activation,
+                                  output);
+  run_gated<Job::kGated>(dtype, a, gated_tight(dtype, x, weight, in_features),
+                         static_cast<hipStream_t>(stream));
+  return check_launch(fn);
+}
+
+size_t gated_linear_backward_workspace_size(int dtype, int64_t rows, int64_t in_features,
+                                            int64_t hidden_features, int want_input,
+                                            int want_weight, int want_bias) {
+  if (validate_gated("gated_linear_backward_workspace_size", dtype, rows, in_features,
+                     hidden_features, 0) != MUSPACE_OK) {
+    return 0;
   }
+  const Wanted want(want_input != 0, want_weight != 0, want_bias != 0, rows, in_features,
+                    2 * hidden_features);
+  if (!want.any()) return 0;
+  return dz_bytes(dtype, rows, 2 * hidden_features) +
+         workspace_bytes_of(dtype, want, rows, in_features, 2 * hidden_features, dense::kNone);
+}
+
+int gated_linear_backward(const void *grad_output, int dtype, const void *x, const void *weight,
+                          const void *bias, void *grad_input, void *grad_weight, void *grad_bias,
+                          int64_t rows, int64_t in_features, int64_t hidden_features,
+                          int activation, void *workspace, size_t workspace_bytes, void *stream) {
+  const char *fn = "gated_linear_backward";
+  const int rc = validate_gated(fn, dtype, rows, in_features, hidden_features, activation);
+  if (rc != MUSPACE_OK) return rc;
+  const int64_t out = 2 * hidden_features;
+  const Wanted want(grad_input != nullptr, grad_weight != nullptr, grad_bias != nullptr, rows,
+                    in_features, out);
+  if (!want.any()) return ok();
+  const bool summed = rows > 0 && out > 0;  // dz has values
+  if (summed && (grad_output == nullptr ||
+                 (in_features > 0 && (x == nullptr || weight == nullptr)))) {
+    return fail(MUSPACE_EINVAL, "%s: null tensor pointer", fn);
+  }
+  const size_t need = gated_linear_backward_workspace_size(
+      dtype, rows, in_features, hidden_features, want.input, want.weight, want.bias);
+  if (need > 0 && (workspace == nullptr || workspace_bytes < need ||
+                   reinterpret_cast<uintptr_t>(workspace) % 256 != 0)) {
+    return fail(MUSPACE_EINVAL, "%s: needs a 256-byte aligned workspace of %zu bytes, got %zu", fn,
+                need, workspace == nullptr ? size_t{0} : workspace_bytes);
+  }
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  char *ws = static_cast<char *>(workspace);
+  Product a = gated_product(x, weight, bias, rows, in_features, hidden_features, activation, ws);
+  a.grad = grad_output;
+  a.ldz = dz_chunks(dtype, out) * chunk_values(dtype);
+  if (summed) {
+    run_gated<Job::kGatedGrad>(dtype, a, gated_tight(dtype, x, weight, in_features), st);
+  }
+  const Gradients g = {ws, nullptr, a.ldz, nullptr, x, nullptr, nullptr, weight, grad_input,
+                       grad_weight, grad_bias, rows, in_features, out};
+  run_gradients(dtype, g, want, ws + dz_bytes(dtype, rows, out), st);
   return check_launch(fn);
 }
 

@@ -9,6 +9,15 @@
 //   x in 8 bits                      written by the forward as it reads x (Kind::kKept), or
 //                                    linear_checkpoint; read back by kWeight's loader
 //
+// The gated layer, W = [Wg; Wu], a = x Wg^T + bg, u = x Wu^T + bu:
+//
+//   y  = act(a) u                    the same three kernels, Job::kGated
+//   da = g u act'(a), du = g act(a)  Job::kGatedGrad: a and u multiplied again
+//   dx = [da du] W, dW = [da du]^T x, db as above, from [da du] in memory
+//
+// A tile's rows of W are half Wg's and half Wu's, of the same results, 16 or 32 of each in
+// turn, so that a wavefront holds a and u of a result and neither is ever written.
+//
 // linear_product: a workgroup of four wavefronts makes a BM x BN tile of the
 // result, each wavefront a quarter. Both operands go through LDS in steps of 128
 // bytes of k; the chunks of step i + 1 are in registers on their way while step i
@@ -31,8 +40,11 @@
 
 namespace dense {
 
-enum class Job { kForward, kInput, kWeight };
-enum Activation : int { kNone = 0, kRelu = 1, kGelu = 2 };
+enum class Job { kForward, kInput, kWeight, kGated, kGatedGrad };
+// (silu and sigmoid: the gated layer's alone)
+enum Activation : int { kNone = 0, kRelu = 1, kGelu = 2, kSilu = 3, kSigmoid = 4 };
+
+constexpr bool gated(Job job) { return job == Job::kGated || job == Job::kGatedGrad; }
 
 struct Product {
   const void *p;         // rows of the result: x, dz or dz^T
@@ -52,6 +64,9 @@ struct Product {
   uint8_t *mask_out;     // kept sign bits (relu under training), as mask
   int act;
   uint8_t *codes, *code_scales;  // Kind::kKept: the checkpoint of x
+  // kGatedGrad: g [m, n]; out is [m, ldz], da, du and zeros up to whole chunks
+  const void *grad;
+  int64_t ldz;
   // kWeight
   float *partial, *bias_partial;  // [splits][m][pad8(n)], [splits][m]
   void *bias_out;                 // splits == 1: db (0: none)
@@ -75,8 +90,9 @@ __device__ __forceinline__ int xcd_order(int id, int count) {
 // than a chunk are read value by value.
 // What an operand is besides its values in memory: relu's bits go with it (masked), or a
 // second tensor holds what rounding to 16 bits left of each value (pair: gelu's dz), or
-// its 8-bit checkpoint is written as it is read (kept: the forward's x).
-enum class Kind { kPlain, kMasked, kPair, kKept };
+// its 8-bit checkpoint is written as it is read (kept: the forward's x), or it is the gated
+// layer's weight, half of its R rows from either half (`rows` is the rows of one).
+enum class Kind { kPlain, kMasked, kPair, kKept, kGated };
 
 template <typename T, bool kAlong, int R, bool kTight, Kind kKind, bool kCodes,
           int kTeam = kThreads>
@@ -90,6 +106,19 @@ struct Loader {
   static constexpr int kDown = kTeam / 8;          // rows between a thread's chunks (along)
   static constexpr int kAcross = R / kV;           // chunks per k row (across)
   static constexpr int kStride = kTeam / kAcross;  // k rows between a thread's chunks
+  static constexpr bool kGated = kKind == Kind::kGated;
+  static_assert(!kGated || kAlong, "the gated weight is read along k");
+
+  // of chunk i (along): its row, counted from row0, of the operand or of its half; the
+  // tile's row that it is put into
+  __device__ __forceinline__ int line(int i) const { return r + kDown * (kGated ? i >> 1 : i); }
+  __device__ __forceinline__ int slot(int i) const {
+    if constexpr (!kGated) return line(i);
+    constexpr int kRun = R == 128 ? 32 : 16;  // half a wavefront's columns
+    return line(i) / kRun * 2 * kRun + (i & 1) * kRun + line(i) % kRun;
+  }
+  // rows of memory before chunk i's half
+  __device__ __forceinline__ int64_t half(int i) const { return kGated && (i & 1) ? rows : 0; }
 
   const T *ptr, *rest;    // rest: the pair's second tensor
   const uint8_t *bytes;   // mask or scales
@@ -145,11 +174,12 @@ struct Loader {
 #pragma unroll
         for (int e = 0; e < kLoads; ++e) {
           const Source s = view(e == 0 ? ptr : rest, ld, row0, k0, rows);
+          const Source up = kGated ? view(ptr + rows * ld, ld, row0, k0, rows) : s;
 #pragma unroll
           for (int i = 0; i < kCount; ++i) {
-            const uint32_t off = static_cast<uint32_t>((r + kDown * i) * ld + c * kV) *
+            const uint32_t off = static_cast<uint32_t>(line(i) * ld + c * kV) *
                                  static_cast<uint32_t>(sizeof(T));
-            v[e][i] = tight_load(s, inside ? off : kPast);
+            v[e][i] = tight_load(kGated && (i & 1) ? up : s, inside ? off : kPast);
           }
         }
       } else if (k_end >= kV) {
@@ -159,15 +189,15 @@ struct Loader {
         past = false;
 #pragma unroll
         for (int i = 0; i < kCount; ++i) {
-          const int64_t row = min(row0 + r + kDown * i, rows - 1);
+          const int64_t row = min(row0 + line(i), rows - 1) + half(i);
           v[0][i] = reinterpret_cast<const Loose16 *>(ptr + row * ld + col)->v;
         }
       } else {
         moved = past = false;
 #pragma unroll
         for (int i = 0; i < kCount; ++i) {
-          const int64_t row = row0 + r + kDown * i;
-          v[0][i] = loose_load<T>(ptr + row * ld + k0 + c * kV,
+          const int64_t row = row0 + line(i);
+          v[0][i] = loose_load<T>(ptr + (row + half(i)) * ld + k0 + c * kV,
                                   row < rows ? k_end - (k0 + c * kV) : 0);
         }
       }
@@ -269,7 +299,7 @@ struct Loader {
     if constexpr (sizeof(T) == 4) {
       u32x2 part[kPlanes];
       split_chunk<kPlanes>(value, part);
-      const uint32_t at = (kAlong ? along_offset<64>(r + kDown * i, c >> 1)
+      const uint32_t at = (kAlong ? along_offset<64>(slot(i), c >> 1)
                                   : across_offset<R>(r + i * kStride, c >> 1)) +
                           (c & 1) * 8;
 #pragma unroll
@@ -277,7 +307,7 @@ struct Loader {
         *reinterpret_cast<u32x2 *>(tile + e * kPlaneBytes + at) = part[e];
       }
     } else {
-      const uint32_t at = kAlong ? along_offset<128>(r + kDown * i, c)
+      const uint32_t at = kAlong ? along_offset<128>(slot(i), c)
                                  : across_offset<R>(r + i * kStride, c);
       *reinterpret_cast<u32x4 *>(tile + at) = value;
     }
@@ -296,7 +326,7 @@ struct Loader {
 
   // float32 as it is, for the tiles that hold more than bfloat16's range
   __device__ __forceinline__ void put_f32(char *tile, int i, const u32x4 &value) const {
-    const uint32_t at = kAlong ? along_offset<128>(r + kDown * i, c)
+    const uint32_t at = kAlong ? along_offset<128>(slot(i), c)
                                : static_cast<uint32_t>(((r + i * kStride) * R + c * 4) * 4);
     *reinterpret_cast<u32x4 *>(tile + at) = value;
   }
@@ -391,6 +421,91 @@ __device__ __forceinline__ void finish_forward(const Product &a, int64_t row, in
   loose_store(static_cast<T *>(a.out) + at, pack<T>(z), left);
 }
 
+// The logistic function and one less it, from exp(-|z|), which has no overflow: both
+// keep their relative accuracy, 4e-7 (the exponent's product is carried to twice
+// float32's bits, rcp rounds to one step).
+__device__ __forceinline__ float logistic(float z, float &other) {
+  // (past 128 exp is zero; an infinity would be subtracted from itself, NaN stays)
+  const float m = fabsf(z) > 128.0f ? -128.0f : -fabsf(z), p = m * 1.44269504f;
+  const float rest = fmaf(m, 1.44269504f, -p) + m * 1.92596300e-8f;
+  const float power = __builtin_amdgcn_exp2f(p);
+  const float e = fmaf(power * rest, 0.69314718f, power);
+  const float large = __builtin_amdgcn_rcpf(1.0f + e), small = e * large;
+  // (!(z < 0): NaN stays in both)
+  other = z < 0.0f ? large : small;
+  return z < 0.0f ? small : large;
+}
+
+// The gate's activation and its derivative; infinities have the limits' values.
+__device__ __forceinline__ float gate_of(int act, float z, float &slope) {
+  if (act == kSilu || act == kSigmoid) {
+    float other;
+    const float s = logistic(z, other);
+    if (act == kSigmoid) {
+      slope = s * other;
+      return s;
+    }
+    const float low = fmaxf(z, -128.0f);  // past it the other factor is zero
+    slope = s * fmaf(fminf(low, 128.0f), other, 1.0f);
+    return low * s;
+  }
+  if (act == kGelu) return gelu(z, slope);
+  if (act == kRelu) {
+    const bool keep = !(z <= 0.0f);  // NaN stays NaN
+    slope = keep ? 1.0f : 0.0f;
+    return keep ? z : 0.0f;
+  }
+  slope = 1.0f;
+  return z;
+}
+
+// A chunk of the gated layer's result, or of da and du: z and u hold the products
+// without their biases. da and du are rounded to the tensors' type, once, as gradients
+// that leave an operator are: their errors, independent, add half the result's own
+// rounding to the gradients' mean square (a factor of 1.41 in all). In two numbers each,
+// as gelu's dz above, they would cost twice the products and four times the bytes: 40000 x
+// 256 -> 2 x 512 bf16 moves 246 MB of da and du as it is.
+template <typename T, bool kGrad>
+__device__ __forceinline__ void finish_gated(const Product &a, int64_t row, int col, int left,
+                                             float (&z)[Piece<T>::kValues],
+                                             float (&u)[Piece<T>::kValues]) {
+  constexpr int kV = Piece<T>::kValues;
+  if (left <= 0) return;
+  if (a.bias != nullptr) {
+    float b[kV];
+    load_bias<T>(static_cast<const T *>(a.bias) + col, left, b);
+#pragma unroll
+    for (int i = 0; i < kV; ++i) z[i] += b[i];
+    load_bias<T>(static_cast<const T *>(a.bias) + a.n + col, left, b);
+#pragma unroll
+    for (int i = 0; i < kV; ++i) u[i] += b[i];
+  }
+  float slope[kV];
+#pragma unroll
+  for (int i = 0; i < kV; ++i) z[i] = gate_of(a.act, z[i], slope[i]);
+  if constexpr (!kGrad) {
+#pragma unroll
+    for (int i = 0; i < kV; ++i) z[i] *= u[i];
+    loose_store(static_cast<T *>(a.out) + row * a.n + col, pack<T>(z), left);
+  } else {
+    float g[kV];
+    unpack<T>(loose_load<T>(static_cast<const T *>(a.grad) + row * a.n + col, left), g);
+#pragma unroll
+    for (int i = 0; i < kV; ++i) {
+      slope[i] *= g[i] * u[i];
+      z[i] *= g[i];
+    }
+    T *to = static_cast<T *>(a.out) + row * a.ldz + col;
+    loose_store(to, pack<T>(slope), left);
+    loose_store(to + a.n, pack<T>(z), left);
+    if (left <= kV) {  // the row's last chunk: zeros up to whole chunks
+      for (int64_t i = 2 * static_cast<int64_t>(a.n) - col; i < a.ldz - col; ++i) {
+        to[i] = from_float<T>(0.0f);
+      }
+    }
+  }
+}
+
 // ------------------------------------------------------------- tile kernel ---
 
 // Three workgroups a CU where the registers allow it (168 of them): the loads and
@@ -407,12 +522,13 @@ __global__ __launch_bounds__(kThreads, (sizeof(T) == 4 && kTight) ? 3 : 2) void 
   constexpr int kStep = Piece<T>::kStep;
   constexpr bool kF32 = sizeof(T) == 4;
   constexpr bool kPAlong = kJob != Job::kWeight;
-  constexpr bool kQAlong = kJob == Job::kForward;
+  constexpr bool kQAlong = kJob == Job::kForward || gated(kJob);
   constexpr int WM = BM / 2, WN = BN / 2;  // a wavefront's quarter
+  constexpr int kColumns = gated(kJob) ? BN / 2 : BN;  // of the result
   constexpr int kI = WM / 32, kJ = WN / 32;
   // (the pair is this library's own tensor, its rows padded to whole chunks)
   using P = Loader<T, kPAlong, BM, kTight || kKind == Kind::kPair, kKind, false>;
-  using Q = Loader<T, kQAlong, BN, kTight, Kind::kPlain, kCodes>;
+  using Q = Loader<T, kQAlong, BN, kTight, gated(kJob) ? Kind::kGated : Kind::kPlain, kCodes>;
   constexpr int kStageLd = WN + 4;  // floats; the pad spreads rows over the banks
   constexpr int kTiles = P::kPlanes * P::kPlaneBytes + Q::kPlanes * Q::kPlaneBytes;
   constexpr int kTilesF32 = kF32 ? (BM + BN) * kRowBytes : 0;
@@ -427,7 +543,7 @@ __global__ __launch_bounds__(kThreads, (sizeof(T) == 4 && kTight) ? 3 : 2) void 
     split = tile / a.tiles;
     tile -= split * a.tiles;
   }
-  const int row0 = tile / a.tiles_n * BM, col0 = tile % a.tiles_n * BN;
+  const int row0 = tile / a.tiles_n * BM, col0 = tile % a.tiles_n * kColumns;
   const int k_begin = split * a.k_split;
   const int k_end = kJob == Job::kWeight && a.k - k_begin > a.k_split ? k_begin + a.k_split : a.k;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -593,10 +709,11 @@ __global__ __launch_bounds__(kThreads, (sizeof(T) == 4 && kTight) ? 3 : 2) void 
 
   // the tile, 32 rows of a wavefront at a time, through the wavefront's own LDS
   float *stage = reinterpret_cast<float *>(lds) + wave * 32 * kStageLd;
-  constexpr int kLanes = WN / kV;         // lanes per row
+  constexpr int kOut = gated(kJob) ? WN / 2 : WN;  // a wavefront's columns of the result
+  constexpr int kLanes = kOut / kV;       // lanes per row
   constexpr int kRows = kWave / kLanes;   // rows at a time
   const int chunk = lane % kLanes;
-  const int col = col0 + wc + chunk * kV, left = a.n - col;
+  const int col = col0 + (gated(kJob) ? wc / 2 : wc) + chunk * kV, left = a.n - col;
   float bias[kV] = {};
   if constexpr (kJob == Job::kForward) {
     if (a.bias != nullptr) load_bias<T>(static_cast<const T *>(a.bias) + col, left, bias);
@@ -628,7 +745,16 @@ __global__ __launch_bounds__(kThreads, (sizeof(T) == 4 && kTight) ? 3 : 2) void 
         for (int x = 0; x < 4; ++x) z[e + x] = v[x];
       }
       const int here = row < a.m ? left : 0;
-      if constexpr (kJob == Job::kForward) {
+      if constexpr (gated(kJob)) {
+        float u[kV];
+#pragma unroll
+        for (int e = 0; e < kV; e += 4) {
+          const f32x4 v = *reinterpret_cast<const f32x4 *>(src + kOut + e);
+#pragma unroll
+          for (int x = 0; x < 4; ++x) u[e + x] = v[x];
+        }
+        finish_gated<T, kJob == Job::kGatedGrad>(a, row, col, here, z, u);
+      } else if constexpr (kJob == Job::kForward) {
 #pragma unroll
         for (int e = 0; e < kV; ++e) z[e] += bias[e];
         finish_forward<T>(a, row, col, here, z);
@@ -654,8 +780,8 @@ __global__ __launch_bounds__(kThreads, (sizeof(T) == 4 && kTight) ? 3 : 2) void 
 
 // ------------------------------------------------------------ few results ---
 
-// kForward and kInput where the tiles would leave most CUs idle: a workgroup makes 32 x
-// 32 results and its kWaves wavefronts take turns at the steps of k, each with its own
+// kForward, kInput and the gated jobs where the tiles would leave most CUs idle: a workgroup
+// makes 32 x 32 results (gated: 32 x 16) and its kWaves wavefronts take turns at the steps of k, each with its own
 // tiles in LDS, so that none waits for another until the sums are joined, in wavefront
 // order. float32 is multiplied as it is: the time is that of the loads.
 template <typename T, Job kJob, int kWaves, bool kTight, Kind kKind>
@@ -663,16 +789,17 @@ __global__ __launch_bounds__(kWaves *kWave) void linear_few(const Product a) {
   constexpr int kV = Piece<T>::kValues;
   constexpr int kStep = Piece<T>::kStep;
   constexpr bool kF32 = sizeof(T) == 4;
-  constexpr bool kQAlong = kJob == Job::kForward;
+  constexpr bool kQAlong = kJob == Job::kForward || gated(kJob);
+  constexpr int kColumns = gated(kJob) ? 16 : 32;
   using P = Loader<T, true, 32, kTight || kKind == Kind::kPair, kKind, false, kWave>;
-  using Q = Loader<T, kQAlong, 32, kTight, Kind::kPlain, false, kWave>;
+  using Q = Loader<T, kQAlong, 32, kTight, gated(kJob) ? Kind::kGated : Kind::kPlain, false, kWave>;
   constexpr int kTile = 32 * kRowBytes;
   constexpr int kTiles = (P::kLoads + 1) * kTile;  // of a wavefront
   constexpr int kLd = 36;
   static_assert(32 * kLd * 4 <= kTiles, "a wavefront's sums exceed its tiles");
   __shared__ __attribute__((aligned(16))) char lds[kWaves * kTiles];
   const int tile = xcd_order(blockIdx.x, gridDim.x);
-  const int row0 = tile / a.tiles_n * 32, col0 = tile % a.tiles_n * 32;
+  const int row0 = tile / a.tiles_n * 32, col0 = tile % a.tiles_n * kColumns;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   char *const tile_p = lds + wave * kTiles, *const tile_q = tile_p + P::kLoads * kTile;
   P p;
@@ -734,7 +861,7 @@ __global__ __launch_bounds__(kWaves *kWave) void linear_few(const Product a) {
     *reinterpret_cast<f32x4 *>(sums + (lane & 31) * kLd + 8 * g + 4 * (lane >> 5)) = v;
   }
   __syncthreads();
-  constexpr int kLanes = 32 / kV;
+  constexpr int kLanes = kColumns / kV;
   // whole wavefronts take part (the mask's halves are exchanged between lanes)
   for (int i = threadIdx.x; i < 32 * kLanes; i += kWaves * kWave) {
     const int chunk = i % kLanes, r = i / kLanes;
@@ -748,7 +875,17 @@ __global__ __launch_bounds__(kWaves *kWave) void linear_few(const Product a) {
 #pragma unroll
       for (int e = 0; e < kV; ++e) z[e] += src[e];
     }
-    if constexpr (kJob == Job::kForward) {
+    if constexpr (gated(kJob)) {
+      float up[kV] = {};
+#pragma unroll
+      for (int u = 0; u < kWaves; ++u) {
+        const float *src =
+            reinterpret_cast<const float *>(lds + u * kTiles) + r * kLd + kColumns + chunk * kV;
+#pragma unroll
+        for (int e = 0; e < kV; ++e) up[e] += src[e];
+      }
+      finish_gated<T, kJob == Job::kGatedGrad>(a, row, col, left, z, up);
+    } else if constexpr (kJob == Job::kForward) {
       if (a.bias != nullptr) {
         float b[kV];
         load_bias<T>(static_cast<const T *>(a.bias) + col, a.n - col, b);
@@ -768,35 +905,39 @@ __global__ __launch_bounds__(kWaves *kWave) void linear_few(const Product a) {
 // flight on many CUs, not matrix cores that would multiply 32 rows. A wavefront takes
 // kCols rows of W whole, its lanes 16 bytes of each at a time, multiplies them with the
 // rows of x (in the caches after the first wavefront) on the vector unit and sums over its
-// lanes. A workgroup makes eight columns, a byte of the mask.
-template <typename T, int kRows, int kCols>
+// lanes. A workgroup makes eight columns, a byte of the mask. Gated: kCols rows of either
+// half of W.
+template <typename T, Job kJob, int kRows, int kCols>
 __global__ __launch_bounds__(8 / kCols *kWave) void linear_vector(const Product a) {
   constexpr int kV = Piece<T>::kValues;
   constexpr int kAhead = 4;  // of a lane's chunks, in flight together
   constexpr int kSpan = kWave * kV;
   constexpr int kLanes = 8 / kV;  // of a result row, at the end
-  static_assert(kRows * kLanes <= kWave && kRows * kCols <= kWave, "one wavefront ends it");
-  __shared__ __attribute__((aligned(16))) float lds[kRows * 8];
+  constexpr int kHalves = gated(kJob) ? 2 : 1;
+  constexpr int kW = kCols * kHalves;  // rows of W
+  static_assert(kRows * kLanes <= kWave && kRows * kW <= kWave, "one wavefront ends it");
+  __shared__ __attribute__((aligned(16))) float lds[kHalves][kRows * 8];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int first = blockIdx.x * 8, col0 = first + wave * kCols;
-  const T *w[kCols], *x[kRows];
+  const T *w[kW], *x[kRows];
 #pragma unroll
-  for (int c = 0; c < kCols; ++c) {
-    w[c] = static_cast<const T *>(a.q) + min(col0 + c, a.n - 1) * a.ldq;
+  for (int c = 0; c < kW; ++c) {
+    const int64_t row = min(col0 + c % kCols, a.n - 1) + (c < kCols ? 0 : a.n);
+    w[c] = static_cast<const T *>(a.q) + row * a.ldq;
   }
 #pragma unroll
   for (int m = 0; m < kRows; ++m) x[m] = static_cast<const T *>(a.p) + min(m, a.m - 1) * a.ldp;
   const int col = first + lane % kLanes * kV, row = lane / kLanes;
   float bias[kV] = {};
-  if (wave == 0 && a.bias != nullptr) {
+  if (!gated(kJob) && wave == 0 && a.bias != nullptr) {
     load_bias<T>(static_cast<const T *>(a.bias) + col, a.n - col, bias);
   }
-  float sum[kRows][kCols] = {};
+  float sum[kRows][kW] = {};
   // the products of one chunk each, but for the first `drop` values
-  auto add = [&](const u32x4(&wv)[kCols], const u32x4(&xv)[kRows], int drop) {
-    float f[kCols][kV];
+  auto add = [&](const u32x4(&wv)[kW], const u32x4(&xv)[kRows], int drop) {
+    float f[kW][kV];
 #pragma unroll
-    for (int c = 0; c < kCols; ++c) {
+    for (int c = 0; c < kW; ++c) {
       unpack<T>(wv[c], f[c]);
 #pragma unroll
       for (int e = 0; e < kV; ++e) f[c][e] = e < drop ? 0.0f : f[c][e];
@@ -808,7 +949,7 @@ __global__ __launch_bounds__(8 / kCols *kWave) void linear_vector(const Product 
 #pragma unroll
       for (int e = 0; e < kV; ++e) g[e] = e < drop ? 0.0f : g[e];
 #pragma unroll
-      for (int c = 0; c < kCols; ++c) {
+      for (int c = 0; c < kW; ++c) {
 #pragma unroll
         for (int e = 0; e < kV; ++e) sum[m][c] = fmaf(g[e], f[c][e], sum[m][c]);
       }
@@ -816,12 +957,12 @@ __global__ __launch_bounds__(8 / kCols *kWave) void linear_vector(const Product 
   };
   int k0 = lane * kV;
   for (; k0 - lane * kV + kAhead * kSpan <= a.k; k0 += kAhead * kSpan) {
-    u32x4 wv[kAhead][kCols], xv[kAhead][kRows];
+    u32x4 wv[kAhead][kW], xv[kAhead][kRows];
 #pragma unroll
     for (int i = 0; i < kAhead; ++i) {
       const int k = k0 + i * kSpan;
 #pragma unroll
-      for (int c = 0; c < kCols; ++c) wv[i][c] = reinterpret_cast<const Loose16 *>(w[c] + k)->v;
+      for (int c = 0; c < kW; ++c) wv[i][c] = reinterpret_cast<const Loose16 *>(w[c] + k)->v;
 #pragma unroll
       for (int m = 0; m < kRows; ++m) xv[i][m] = reinterpret_cast<const Loose16 *>(x[m] + k)->v;
     }
@@ -829,18 +970,18 @@ __global__ __launch_bounds__(8 / kCols *kWave) void linear_vector(const Product 
     for (int i = 0; i < kAhead; ++i) add(wv[i], xv[i], 0);
   }
   for (; k0 < a.k; k0 += kSpan) {
-    u32x4 wv[kCols], xv[kRows];
+    u32x4 wv[kW], xv[kRows];
     if (a.k >= kV) {
       // a chunk that passes the end: the rows' last 16 bytes, less what came before
       const int k = min(k0, a.k - kV);
 #pragma unroll
-      for (int c = 0; c < kCols; ++c) wv[c] = reinterpret_cast<const Loose16 *>(w[c] + k)->v;
+      for (int c = 0; c < kW; ++c) wv[c] = reinterpret_cast<const Loose16 *>(w[c] + k)->v;
 #pragma unroll
       for (int m = 0; m < kRows; ++m) xv[m] = reinterpret_cast<const Loose16 *>(x[m] + k)->v;
       add(wv, xv, k0 - k);
     } else {
 #pragma unroll
-      for (int c = 0; c < kCols; ++c) wv[c] = loose_load<T>(w[c], a.k);
+      for (int c = 0; c < kW; ++c) wv[c] = loose_load<T>(w[c], a.k);
 #pragma unroll
       for (int m = 0; m < kRows; ++m) xv[m] = loose_load<T>(x[m], a.k);
       add(wv, xv, 0);
@@ -850,21 +991,32 @@ __global__ __launch_bounds__(8 / kCols *kWave) void linear_vector(const Product 
 #pragma unroll
   for (int m = 0; m < kRows; ++m) {
 #pragma unroll
-    for (int c = 0; c < kCols; ++c) {
+    for (int c = 0; c < kW; ++c) {
       float v = sum[m][c];
       v = add_across<8>(add_across<4>(add_across<2>(add_across<1>(v))));
       v = add_across<32>(add_across<16>(v));
-      if (lane == m * kCols + c && col0 + c < a.n) mine = v;
+      if (lane == m * kW + c && col0 + c % kCols < a.n) mine = v;
     }
   }
-  if (lane < kRows * kCols) lds[lane / kCols * 8 + wave * kCols + lane % kCols] = mine;
+  if (lane < kRows * kW) {
+    lds[lane % kW / kCols][lane / kW * 8 + wave * kCols + lane % kCols] = mine;
+  }
   __syncthreads();
   if (wave != 0) return;
   float z[kV];
+  const int at = min(row, kRows - 1) * 8 + col - first;
 #pragma unroll
-  for (int e = 0; e < kV; ++e) z[e] = lds[min(row, kRows - 1) * 8 + col - first + e] + bias[e];
+  for (int e = 0; e < kV; ++e) z[e] = lds[0][at + e] + bias[e];
+  const int left = row < min(kRows, a.m) ? a.n - col : 0;
+  if constexpr (gated(kJob)) {
+    float u[kV];
+#pragma unroll
+    for (int e = 0; e < kV; ++e) u[e] = lds[kHalves - 1][at + e];
+    finish_gated<T, kJob == Job::kGatedGrad>(a, row, col, left, z, u);
+    return;
+  }
   // the whole wavefront: the mask's halves are exchanged between lanes
-  finish_forward<T>(a, row, col, row < min(kRows, a.m) ? a.n - col : 0, z);
+  finish_forward<T>(a, row, col, left, z);
 }
 
 // ----------------------------------------------------- gradient's last step ---

@@ -16,6 +16,7 @@ from .deformable_aggregation import (
     feature_maps_format,
 )
 from .dropout import dropout, dropout_pytorch
+from .gated_linear import gated_linear, gated_linear_pytorch
 from .layer_norm import layer_norm, layer_norm_pytorch
 from .linear import checkpoint_int8, checkpoint_restore, linear, linear_pytorch
 from .residual_norm import residual_norm, residual_norm_pytorch
@@ -31,6 +32,8 @@ __all__ = [
     "dropout_pytorch",
     "feature_maps_format",
     "explain_dispatch",
+    "gated_linear",
+    "gated_linear_pytorch",
     "layer_norm",
     "layer_norm_pytorch",
     "level_start_index_from_shapes",

@@ -22,7 +22,8 @@ MODULE_NAME = "muspace_layer_host"
 _BOUND = (
     "muspace_last_error", "linear_forward", "linear_checkpoint",
     "linear_backward_workspace_size_for", "linear_backward", "layer_norm_forward",
-    "layer_norm_backward_workspace_size", "layer_norm_backward", "dropout_forward",
+    "layer_norm_backward_workspace_size", "layer_norm_backward", "gated_linear_forward",
+    "gated_linear_backward_workspace_size", "gated_linear_backward", "dropout_forward",
     "residual_norm_forward", "residual_norm_backward_workspace_size", "residual_norm_backward",
 )
 

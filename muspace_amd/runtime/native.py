@@ -173,6 +173,17 @@ _EXPORTS: dict[str, tuple[Any, list[Any]]] = {
         [_c_ptr, _c_int, _c_ptr, _c_ptr, _c_int] + [_c_ptr] * 4
         + [_c_int64, _c_int64, _c_ptr, ctypes.c_size_t, _c_ptr],
     ),
+    "gated_linear_forward": (
+        _c_int, [_c_ptr, _c_int] + [_c_ptr] * 3 + [_c_int64] * 3 + [_c_int, _c_ptr]
+    ),
+    "gated_linear_backward_workspace_size": (
+        ctypes.c_size_t, [_c_int] + [_c_int64] * 3 + [_c_int] * 3
+    ),
+    "gated_linear_backward": (
+        _c_int,
+        [_c_ptr, _c_int] + [_c_ptr] * 6 + [_c_int64] * 3
+        + [_c_int, _c_ptr, ctypes.c_size_t, _c_ptr],
+    ),
     "dropout_forward": (
         _c_int,
         [_c_ptr, _c_int, _c_ptr, _c_ptr, _c_int64, ctypes.c_double, ctypes.c_uint64, _c_ptr,
