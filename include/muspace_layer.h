@@ -1,7 +1,7 @@
 /*
  * C-ABI of the dense operators around deformable attention in an encoder or
  * decoder layer: the linear layer with its epilogue and gradients, its 8-bit
- * input checkpoint, the gated layer, layer norm with its gradients, dropout, and the sum of a block
+ * input checkpoint, the gated layer, linear on 8-bit integers, layer norm with its gradients, dropout, and the sum of a block
  * with the residual stream and the norm after it. Part of `libmuspace_msda.so`,
  * MI355X (gfx950).
  *
@@ -110,6 +110,27 @@ MUSPACE_API int gated_linear_backward(const void *grad_output, int dtype, const 
                                       int64_t in_features, int64_t hidden_features,
                                       int activation, void *workspace, size_t workspace_bytes,
                                       void *stream);
+
+/* Rows in 8 bits: scales[r] = max(max |x[r]| / 127, 2^-126) in float32 (the quotient rounded
+ * once), codes[r][c] = x[r][c] / scales[r] rounded to the nearest integer, ties to even (of
+ * the float32 quotient), -127 to 127. A row with an infinity or NaN has scale NaN and codes 1.
+ * codes [rows, cols], scales [rows]; cols at most 2^20. */
+MUSPACE_API int quantize_int8(const void *x, int dtype, int8_t *codes, float *scales, int64_t rows,
+                              int64_t cols, void *stream);
+
+/* linear on 8-bit integers: x's rows are quantised as by quantize_int8, weight [out, in]
+ * are codes with a scale per row, weight_scales [out] float32:
+ *   z = sum of codes * scales[r] * weight_scales[o] + bias;  output = act(z) + residual
+ * with sums exact in int32 and the rest in float32, rounded once; activation 0 none,
+ * 1 relu, 2 gelu. in at most 2^17. The workspace (256-byte aligned) holds x's codes and
+ * scales. */
+MUSPACE_API size_t linear_int8_workspace_size(int dtype, int64_t rows, int64_t in_features,
+                                              int64_t out_features);
+MUSPACE_API int linear_int8_forward(const void *x, int dtype, const int8_t *weight,
+                                    const float *weight_scales, const void *bias,
+                                    const void *residual, void *output, int64_t rows,
+                                    int64_t in_features, int64_t out_features, int activation,
+                                    void *workspace, size_t workspace_bytes, void *stream);
 
 /* layer norm over the last dimension:
  *   c = x - mean(x);  s = 1 / sqrt(mean(c^2) + eps);  output = c s weight + bias

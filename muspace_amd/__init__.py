@@ -5,7 +5,8 @@ The exports mirror the MSDA part of the reference package
 dispatch explanation and the dispatch-report accessors. ``import muspace_amd
 as mu_space`` gives code written against the reference the same names. Next to
 them stand the dense operators of an attention layer (``linear``, its 8-bit
-checkpoints, ``gated_linear``, ``layer_norm``, ``dropout``, ``residual_norm``), which the reference leaves to torch.
+checkpoints, ``gated_linear``, ``linear_int8``, ``layer_norm``, ``dropout``,
+``residual_norm``), which the reference leaves to torch.
 """
 
 from .ops import (
@@ -16,11 +17,13 @@ from .ops import (
     gated_linear,
     layer_norm,
     linear,
+    linear_int8,
     multi_scale_deformable_attn,
     multi_scale_deformable_attn_pytorch,
     multi_scale_deformable_attn_pytorch_compat,
     multi_scale_deformable_attn_scatter_div,
     multi_scale_deformable_attn_softmax,
+    quantize_int8,
     residual_norm,
 )
 from .runtime.kernel_dispatch import (
@@ -47,10 +50,12 @@ __all__ = [
     "get_last_dispatch_report",
     "layer_norm",
     "linear",
+    "linear_int8",
     "multi_scale_deformable_attn",
     "multi_scale_deformable_attn_pytorch",
     "multi_scale_deformable_attn_pytorch_compat",
     "multi_scale_deformable_attn_scatter_div",
     "multi_scale_deformable_attn_softmax",
+    "quantize_int8",
     "residual_norm",
 ]

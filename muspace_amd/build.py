@@ -24,6 +24,7 @@ SOURCES = (
     PACKAGE_DIR / "csrc" / "linear_capi.hip",
     PACKAGE_DIR / "csrc" / "layer_norm_capi.hip",
     PACKAGE_DIR / "csrc" / "residual_norm_capi.hip",
+    PACKAGE_DIR / "csrc" / "int8_capi.hip",
 )
 DEPENDS = (
     PACKAGE_DIR / "csrc" / "capi_errors.hpp",
@@ -38,6 +39,7 @@ DEPENDS = (
     PACKAGE_DIR / "csrc" / "layer_norm_kernels.hpp",
     PACKAGE_DIR / "csrc" / "dropout_device.hpp",
     PACKAGE_DIR / "csrc" / "residual_norm_kernels.hpp",
+    PACKAGE_DIR / "csrc" / "int8_kernels.hpp",
     REPO_DIR / "include" / "muspace_msda.h",
     REPO_DIR / "include" / "muspace_dfa.h",
     REPO_DIR / "include" / "muspace_layer.h",

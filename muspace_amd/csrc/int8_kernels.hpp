@@ -1,0 +1,423 @@
+// The linear layer in 8-bit integers (include/muspace_layer.h):
+//
+//   s_r = max(max |x_r| / 127, 2^-126), q_rk = rint(x_rk / s_r)     rows of x, and of W before
+//   y = act(s_r t_o sum of q_rk w_ok + b_o) + residual              w codes, t scales of W
+//
+// Sums are exact, in int32 (in_features up to 2^17). The row's quotients are float32
+// divisions, so that codes are the same on any machine.
+//
+// int8_rows quantises; int8_product is linear_product (linear_kernels.hpp) with 128 codes a
+// step in the same 128 bytes: the same LDS layout serves, a lane's 16 bytes of a row are 16
+// codes, and v_mfma_i32_32x32x32_i8 takes 32 of k a time, at twice the 16-bit types' rate.
+// Rows of x's codes are padded with zeros to whole chunks, so what a weight's chunk holds
+// past the row's end (the next row's first codes) counts for nothing.
+#pragma once
+
+#include "linear_kernels.hpp"
+
+namespace dense {
+
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+typedef int i32x16 __attribute__((ext_vector_type(16)));
+
+constexpr int kCodeStep = kRowBytes;  // of k
+
+struct __attribute__((packed, aligned(1))) Bytes16 {
+  u32x4 v;
+};
+struct __attribute__((packed, aligned(1))) Bytes8 {
+  u32x2 v;
+};
+struct __attribute__((packed, aligned(1))) Bytes4 {
+  uint32_t v;
+};
+
+// ---------------------------------------------------------------- quantise ---
+
+constexpr int kQuantThreads = 512;
+
+struct Quantise {
+  const void *x;
+  int8_t *codes;
+  float *scales;
+  int64_t rows, ld;  // codes of a row in memory; zeros past cols
+  int cols;
+};
+
+// the largest magnitude of kLanes lanes (as bits), the same on all of them
+template <int kLanes>
+__device__ __forceinline__ uint32_t team_top(uint32_t v, uint32_t *lds) {
+  v = max(v, from_lane<1>(v));
+  v = max(v, from_lane<2>(v));
+  v = max(v, from_lane<4>(v));
+#pragma unroll
+  for (int d = 8; d < kWave && d < kLanes; d *= 2) {
+    v = max(v, static_cast<uint32_t>(__shfl_xor(static_cast<int>(v), d)));
+  }
+  if constexpr (kLanes > kWave) {
+    const int wave = threadIdx.x / kWave, first = threadIdx.x / kLanes * (kLanes / kWave);
+    __syncthreads();
+    if (threadIdx.x % kWave == 0) lds[wave] = v;
+    __syncthreads();
+    v = lds[first];
+#pragma unroll
+    for (int u = 1; u < kLanes / kWave; ++u) v = max(v, lds[first + u]);
+  }
+  return v;
+}
+
+// A row's scale from its largest magnitude; NaN for a row with an infinity or NaN.
+__device__ __forceinline__ float row_scale(uint32_t top) {
+  if (top >= 0x7f800000u) return __uint_as_float(0x7fc00000u);
+  return fmaxf(__uint_as_float(top) / 127.0f, 0x1p-126f);
+}
+
+// A piece's codes, four a word. (Codes of a row without a scale are 1: times NaN.)
+template <int kV>
+__device__ __forceinline__ void encode_row(const float (&v)[kV], float scale,
+                                           uint32_t (&w)[kV / 4]) {
+#pragma unroll
+  for (int i = 0; i < kV / 4; ++i) w[i] = 0;
+#pragma unroll
+  for (int e = 0; e < kV; ++e) {
+    const float q = scale == scale ? rintf(v[e] / scale) : 1.0f;
+    w[e / 4] |= (static_cast<uint32_t>(static_cast<int>(q)) & 0xffu) << (8 * (e & 3));
+  }
+}
+
+// `left` codes of a row in memory from `to` on
+template <int kV>
+__device__ __forceinline__ void store_codes(int8_t *to, const uint32_t (&w)[kV / 4], int64_t left) {
+  if (left >= kV) {
+    if constexpr (kV == 8) {
+      reinterpret_cast<Bytes8 *>(to)->v = u32x2{w[0], w[1]};
+    } else {
+      reinterpret_cast<Bytes4 *>(to)->v = w[0];
+    }
+    return;
+  }
+#pragma unroll
+  for (int e = 0; e < kV; ++e) {
+    if (e < left) to[e] = static_cast<int8_t>(w[e / 4] >> (8 * (e & 3)));
+  }
+}
+
+// Rows of up to kLanes pieces, a piece a lane; a wavefront holds several short rows.
+template <typename T, int kLanes>
+__global__ __launch_bounds__(kQuantThreads) void int8_rows(const Quantise a) {
+  constexpr int kV = Piece<T>::kValues;
+  constexpr int kGroups = kQuantThreads / kLanes;
+  __shared__ uint32_t lds[kQuantThreads / kWave];
+  const int lane = threadIdx.x % kLanes, col = lane * kV, left = a.cols - col;
+  for (int64_t base = static_cast<int64_t>(blockIdx.x) * kGroups; base < a.rows;
+       base += static_cast<int64_t>(gridDim.x) * kGroups) {
+    const int64_t row = base + threadIdx.x / kLanes;
+    const bool any = row < a.rows;
+    float v[kV];
+    unpack<T>(loose_load<T>(static_cast<const T *>(a.x) + row * a.cols + col, any ? left : 0), v);
+    uint32_t top = 0;
+#pragma unroll
+    for (int e = 0; e < kV; ++e) top = max(top, __float_as_uint(v[e]) & 0x7fffffffu);
+    const float scale = row_scale(team_top<kLanes>(top, lds));
+    if (!any) continue;
+    uint32_t w[kV / 4];
+    encode_row<kV>(v, scale, w);
+    store_codes<kV>(a.codes + row * a.ld + col, w, a.ld - col);
+    if (lane == 0) a.scales[row] = scale;
+  }
+}
+
+// Rows of any length: a workgroup a row, read twice, from the caches the second time.
+template <typename T>
+__global__ __launch_bounds__(kQuantThreads) void int8_rows_long(const Quantise a) {
+  constexpr int kV = Piece<T>::kValues;
+  __shared__ uint32_t lds[kQuantThreads / kWave];
+  for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+    const T *x = static_cast<const T *>(a.x) + row * a.cols;
+    uint32_t top = 0;
+    for (int col = threadIdx.x * kV; col < a.cols; col += kQuantThreads * kV) {
+      float v[kV];
+      unpack<T>(loose_load<T>(x + col, a.cols - col), v);
+#pragma unroll
+      for (int e = 0; e < kV; ++e) top = max(top, __float_as_uint(v[e]) & 0x7fffffffu);
+    }
+    const float scale = row_scale(team_top<kQuantThreads>(top, lds));
+    for (int64_t col = threadIdx.x * kV; col < a.ld; col += kQuantThreads * kV) {
+      float v[kV];
+      unpack<T>(loose_load<T>(x + col, static_cast<int>(a.cols - col)), v);
+      uint32_t w[kV / 4];
+      encode_row<kV>(v, scale, w);
+      store_codes<kV>(a.codes + row * a.ld + col, w, a.ld - col);
+    }
+    if (threadIdx.x == 0) a.scales[row] = scale;
+  }
+}
+
+// ----------------------------------------------------------------- product ---
+
+struct Codes {
+  const int8_t *x, *weight;             // x [m][ldx], weight [n][k]
+  const float *x_scales, *weight_scales;
+  int64_t ldx;
+  Product p;                            // m, n, k, tiles and the epilogue
+};
+
+// R rows by a step of codes, 16 bytes a chunk (see Loader). !kTight: rows of any length,
+// read at their own addresses; a chunk that would pass the end of the whole operand is
+// read as its last 16 bytes, moved to the front.
+template <int R, bool kTight, int kTeam = kThreads>
+struct CodeLoader {
+  static constexpr int kCount = R * 8 / kTeam;
+  static constexpr int kDown = kTeam / 8;
+  const int8_t *ptr;
+  int64_t ld, end;  // end: bytes of the operand
+  int row0, rows, r, c;
+  u32x4 v[kCount];
+
+  __device__ __forceinline__ void init(const int8_t *src, int64_t ld_, int row0_, int rows_) {
+    ptr = src;
+    ld = ld_;
+    row0 = row0_;
+    rows = rows_;
+    end = ld_ * rows_;
+    const int t = threadIdx.x % kTeam;
+    r = t >> 3;
+    c = t & 7;
+  }
+
+  __device__ __forceinline__ void fetch(int k0) {
+    if constexpr (kTight) {
+      Source s;
+      s.base = reinterpret_cast<const char *>(ptr + row0 * ld + k0);
+      const int64_t left = end - row0 * ld - k0;
+      s.bytes = left > 0x7fffffff ? 0x7fffffffu : static_cast<uint32_t>(left);
+      const bool inside = k0 + c * 16 < ld;
+#pragma unroll
+      for (int i = 0; i < kCount; ++i) {
+        const uint32_t off = static_cast<uint32_t>((r + kDown * i) * ld + c * 16);
+        v[i] = tight_load(s, inside ? off : kPast);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < kCount; ++i) {
+        const int64_t row = min(row0 + r + kDown * i, rows - 1);
+        const int64_t off = row * ld + k0 + c * 16;
+        if (end >= 16) {
+          const int64_t at = min(off, end - 16);
+          v[i] = reinterpret_cast<const Bytes16 *>(ptr + at)->v;
+          const int64_t skip = off - at;
+          if (skip > 0) v[i] = drop_front<int8_t>(v[i], skip > 16 ? 16 : static_cast<int>(skip));
+        } else {
+          u32x4 o = {0, 0, 0, 0};
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            if (off + e < end) {
+              o[e / 4] |= static_cast<uint32_t>(static_cast<uint8_t>(ptr[off + e])) << (8 * (e & 3));
+            }
+          }
+          v[i] = o;
+        }
+      }
+    }
+  }
+
+  __device__ __forceinline__ void put(char *tile) const {
+#pragma unroll
+    for (int i = 0; i < kCount; ++i) {
+      *reinterpret_cast<u32x4 *>(tile + along_offset<128>(r + kDown * i, c)) = v[i];
+    }
+  }
+};
+
+__device__ __forceinline__ i32x16 multiply_codes(const u32x4 &a, const u32x4 &b, i32x16 acc) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  return __builtin_amdgcn_mfma_i32_32x32x32_i8(__builtin_bit_cast(i32x4, a),
+                                               __builtin_bit_cast(i32x4, b), acc, 0, 0, 0);
+#else
+  return acc;
+#endif
+}
+
+// A chunk of the result from its integer sums. (A sum past 2^24 is rounded to float32,
+// relative 2^-24, as the two products with the scales are.)
+template <typename T>
+__device__ __forceinline__ void finish_codes(const Codes &a, int64_t row, int col, int left,
+                                             const int (&sum)[Piece<T>::kValues],
+                                             const float (&scale)[Piece<T>::kValues],
+                                             const float (&bias)[Piece<T>::kValues]) {
+  constexpr int kV = Piece<T>::kValues;
+  const float s = left > 0 ? a.x_scales[row] : 0.0f;
+  float z[kV];
+#pragma unroll
+  for (int e = 0; e < kV; ++e) z[e] = static_cast<float>(sum[e]) * s * scale[e] + bias[e];
+  finish_forward<T>(a.p, row, col, left, z);
+}
+
+// the weight's scales and the bias of a chunk of columns
+template <typename T>
+__device__ __forceinline__ void load_columns(const Codes &a, int col, int left,
+                                             float (&scale)[Piece<T>::kValues],
+                                             float (&bias)[Piece<T>::kValues]) {
+  constexpr int kV = Piece<T>::kValues;
+#pragma unroll
+  for (int e = 0; e < kV; e += 4) {
+    float f[4];
+    unpack<float>(loose_load<float>(a.weight_scales + col + e, left - e), f);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) scale[e + i] = f[i];
+  }
+#pragma unroll
+  for (int e = 0; e < kV; ++e) bias[e] = 0.0f;
+  if (a.p.bias != nullptr) load_bias<T>(static_cast<const T *>(a.p.bias) + col, left, bias);
+}
+
+template <typename T, int BM, int BN, bool kTight>
+__global__ __launch_bounds__(kThreads, 3) void int8_product(const Codes a) {
+  constexpr int kV = Piece<T>::kValues;
+  constexpr int WM = BM / 2, WN = BN / 2;  // a wavefront's quarter
+  constexpr int kI = WM / 32, kJ = WN / 32;
+  constexpr int kStageLd = WN + 4;  // ints; the pad spreads rows over the banks
+  constexpr int kStage = 4 * 32 * kStageLd * 4, kTiles = (BM + BN) * kRowBytes;
+  __shared__ __attribute__((aligned(16))) char lds[kStage > kTiles ? kStage : kTiles];
+  const int tile = xcd_order(blockIdx.x, gridDim.x);
+  const int row0 = tile / a.p.tiles_n * BM, col0 = tile % a.p.tiles_n * BN;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int wr = (wave >> 1) * WM, wc = (wave & 1) * WN;
+  CodeLoader<BM, true> p;
+  CodeLoader<BN, kTight> q;
+  p.init(a.x, a.ldx, row0, a.p.m);
+  q.init(a.weight, a.p.k, col0, a.p.n);
+  char *const tile_p = lds, *const tile_q = lds + BM * kRowBytes;
+  i32x16 acc[kI][kJ] = {};
+  if (a.p.k > 0) {
+    p.fetch(0);
+    q.fetch(0);
+  }
+  for (int k0 = 0; k0 < a.p.k; k0 += kCodeStep) {
+    p.put(tile_p);
+    q.put(tile_q);
+    __syncthreads();
+    if (k0 + kCodeStep < a.p.k) {
+      p.fetch(k0 + kCodeStep);
+      q.fetch(k0 + kCodeStep);
+    }
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {
+      u32x4 fp[kI], fq[kJ];
+#pragma unroll
+      for (int i = 0; i < kI; ++i) {
+        fp[i] = read_fragment<true, BM, 128>(tile_p, wr + 32 * i, s, lane);
+      }
+#pragma unroll
+      for (int j = 0; j < kJ; ++j) {
+        fq[j] = read_fragment<true, BN, 128>(tile_q, wc + 32 * j, s, lane);
+      }
+#pragma unroll
+      for (int i = 0; i < kI; ++i) {
+#pragma unroll
+        for (int j = 0; j < kJ; ++j) acc[i][j] = multiply_codes(fq[j], fp[i], acc[i][j]);
+      }
+    }
+    __syncthreads();
+  }
+  // the tile, 32 rows of a wavefront at a time, through the wavefront's own LDS
+  int *stage = reinterpret_cast<int *>(lds) + wave * 32 * kStageLd;
+  constexpr int kLanes = WN / kV, kRows = kWave / kLanes;
+  const int chunk = lane % kLanes;
+  const int col = col0 + wc + chunk * kV, left = a.p.n - col;
+  float scale[kV], bias[kV];
+  load_columns<T>(a, col, left, scale, bias);
+#pragma unroll
+  for (int i = 0; i < kI; ++i) {
+#pragma unroll
+    for (int j = 0; j < kJ; ++j) {
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        i32x4 v;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = acc[i][j][4 * g + e];
+        *reinterpret_cast<i32x4 *>(stage + (lane & 31) * kStageLd + 32 * j + 8 * g +
+                                   4 * (lane >> 5)) = v;
+      }
+    }
+    wave_lds_sync();
+#pragma unroll
+    for (int r0 = 0; r0 < 32; r0 += kRows) {
+      const int r = r0 + lane / kLanes;
+      const int64_t row = row0 + wr + 32 * i + r;
+      int sum[kV];
+#pragma unroll
+      for (int e = 0; e < kV; e += 4) {
+        const i32x4 v = *reinterpret_cast<const i32x4 *>(stage + r * kStageLd + chunk * kV + e);
+#pragma unroll
+        for (int x = 0; x < 4; ++x) sum[e + x] = v[x];
+      }
+      finish_codes<T>(a, row, col, row < a.p.m ? left : 0, sum, scale, bias);
+    }
+    wave_lds_sync();
+  }
+}
+
+// Where the tiles would leave most CUs idle (see linear_few): 32 x 32 results a workgroup,
+// whose wavefronts take turns at the steps of k.
+template <typename T, int kWaves, bool kTight>
+__global__ __launch_bounds__(kWaves *kWave) void int8_few(const Codes a) {
+  constexpr int kV = Piece<T>::kValues;
+  constexpr int kTile = 32 * kRowBytes;
+  constexpr int kLd = 36;
+  __shared__ __attribute__((aligned(16))) char lds[kWaves * 2 * kTile];
+  const int tile = xcd_order(blockIdx.x, gridDim.x);
+  const int row0 = tile / a.p.tiles_n * 32, col0 = tile % a.p.tiles_n * 32;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  char *const tile_p = lds + wave * 2 * kTile, *const tile_q = tile_p + kTile;
+  CodeLoader<32, true, kWave> p;
+  CodeLoader<32, kTight, kWave> q;
+  p.init(a.x, a.ldx, row0, a.p.m);
+  q.init(a.weight, a.p.k, col0, a.p.n);
+  i32x16 acc = {};
+  int k0 = wave * kCodeStep;
+  if (k0 < a.p.k) {
+    p.fetch(k0);
+    q.fetch(k0);
+  }
+  for (; k0 < a.p.k; k0 += kWaves * kCodeStep) {
+    p.put(tile_p);
+    q.put(tile_q);
+    wave_lds_sync();
+    if (k0 + kWaves * kCodeStep < a.p.k) {
+      p.fetch(k0 + kWaves * kCodeStep);
+      q.fetch(k0 + kWaves * kCodeStep);
+    }
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {
+      acc = multiply_codes(read_fragment<true, 32, 128>(tile_q, 0, s, lane),
+                           read_fragment<true, 32, 128>(tile_p, 0, s, lane), acc);
+    }
+    wave_lds_sync();
+  }
+  int *const sums = reinterpret_cast<int *>(tile_p);
+#pragma unroll
+  for (int g = 0; g < 4; ++g) {
+    const i32x4 v = {acc[4 * g], acc[4 * g + 1], acc[4 * g + 2], acc[4 * g + 3]};
+    *reinterpret_cast<i32x4 *>(sums + (lane & 31) * kLd + 8 * g + 4 * (lane >> 5)) = v;
+  }
+  __syncthreads();
+  constexpr int kLanes = 32 / kV;
+  for (int i = threadIdx.x; i < 32 * kLanes; i += kWaves * kWave) {
+    const int chunk = i % kLanes, r = i / kLanes;
+    const int col = col0 + chunk * kV;
+    const int64_t row = row0 + r;
+    int sum[kV] = {};
+#pragma unroll
+    for (int u = 0; u < kWaves; ++u) {
+      const int *src = reinterpret_cast<const int *>(lds + u * 2 * kTile) + r * kLd + chunk * kV;
+#pragma unroll
+      for (int e = 0; e < kV; ++e) sum[e] += src[e];
+    }
+    float scale[kV], bias[kV];
+    load_columns<T>(a, col, a.p.n - col, scale, bias);
+    finish_codes<T>(a, row, col, row < a.p.m ? a.p.n - col : 0, sum, scale, bias);
+  }
+}
+
+}  // namespace dense

@@ -43,6 +43,9 @@ void bind(const std::map<std::string, std::uintptr_t> &addresses) {
   bind_one(api.gated_forward, addresses, "gated_linear_forward");
   bind_one(api.gated_workspace, addresses, "gated_linear_backward_workspace_size");
   bind_one(api.gated_backward, addresses, "gated_linear_backward");
+  bind_one(api.quantize, addresses, "quantize_int8");
+  bind_one(api.int8_workspace, addresses, "linear_int8_workspace_size");
+  bind_one(api.int8_forward, addresses, "linear_int8_forward");
   bind_one(api.dropout_forward, addresses, "dropout_forward");
   bind_one(api.residual_forward, addresses, "residual_norm_forward");
   bind_one(api.residual_workspace, addresses, "residual_norm_backward_workspace_size");

@@ -39,6 +39,9 @@ struct Api {
   decltype(&::gated_linear_forward) gated_forward = nullptr;
   decltype(&::gated_linear_backward_workspace_size) gated_workspace = nullptr;
   decltype(&::gated_linear_backward) gated_backward = nullptr;
+  decltype(&::quantize_int8) quantize = nullptr;
+  decltype(&::linear_int8_workspace_size) int8_workspace = nullptr;
+  decltype(&::linear_int8_forward) int8_forward = nullptr;
   decltype(&::dropout_forward) dropout_forward = nullptr;
   decltype(&::residual_norm_forward) residual_forward = nullptr;
   decltype(&::residual_norm_backward_workspace_size) residual_workspace = nullptr;

@@ -1,5 +1,5 @@
 // Autograd nodes of a layer's blocks besides linear and layer norm: the gated layer,
-// dropout and the residual norm. The contract is that of layer_host.cpp.
+// dropout and the residual norm; and linear on 8-bit integers, which has no gradients. The contract is that of layer_host.cpp.
 #include <pybind11/stl.h>
 
 #include <cmath>
@@ -76,6 +76,64 @@ OptTensor gated_linear(const Tensor &input, const Tensor &weight, const OptTenso
     return GatedFunction::apply(x, w, opt(b), activation);
   }
   return gated_run(x, w, b, activation);
+}
+
+// ---------------------------------------------------------- 8-bit integers ---
+
+std::pair<Tensor, Tensor> quantize(const Tensor &input) {
+  refuse_tracing("quantize_int8");
+  const c10::DeviceGuard guard(input.device());
+  const Tensor x = dense(input);
+  std::pair<Tensor, Tensor> made{
+      at::empty(x.sizes(), x.options().dtype(at::kChar)),
+      at::empty(x.sizes().slice(0, x.dim() - 1), x.options().dtype(at::kFloat))};
+  check(api.quantize(x.data_ptr(), code_of(x.scalar_type(), "input"),
+                     static_cast<int8_t *>(made.first.data_ptr()),
+                     static_cast<float *>(made.second.data_ptr()), rows_of(x), x.size(-1),
+                     stream_of(x)),
+        "quantize_int8");
+  return made;
+}
+
+OptTensor linear_int8(const Tensor &input, const Tensor &weight, const Tensor &weight_scale,
+                      const OptTensor &bias, const OptTensor &residual, int64_t activation) {
+  const at::ScalarType type = input.scalar_type();
+  if (!supported(type) || input.dim() == 0 || weight.dim() != 2 ||
+      weight.size(1) != input.size(-1) || weight.scalar_type() != at::kChar ||
+      !row_of(weight_scale, weight.size(0), at::kFloat) || !row_of(bias, weight.size(0), type)) {
+    return OptTensor();
+  }
+  auto shape = input.sizes().vec();
+  shape.back() = weight.size(0);
+  if (residual.has_value() &&
+      (residual->scalar_type() != type || residual->sizes() != at::IntArrayRef(shape))) {
+    return OptTensor();
+  }
+  refuse_tracing("linear_int8");
+  const c10::DeviceGuard guard(input.device());
+  const Tensor x = dense(input);
+  const Tensor w = prepared(weight, x, "weight"), s = prepared(weight_scale, x, "weight_scale"),
+               b = prepared(bias, x, "bias"), r = prepared(residual, x, "residual");
+  refuse_tangents("linear_int8", {&x, &s, &b, &r});
+  if (at::GradMode::is_enabled()) {
+    for (const Tensor *t : {&x, &s, &b, &r}) {
+      if (wants_grad(*t)) {
+        throw std::runtime_error("linear_int8 has no gradients: call it under torch.no_grad() or "
+                                 "on tensors that require none");
+      }
+    }
+  }
+  Tensor output = at::empty(shape, x.options());
+  const int code = code_of(type, "input");
+  const int64_t rows = rows_of(x), cols = w.size(1), out = w.size(0);
+  const size_t bytes = api.int8_workspace(code, rows, cols, out);
+  const Tensor workspace = scratch(bytes, x);
+  check(api.int8_forward(x.data_ptr(), code, static_cast<const int8_t *>(w.data_ptr()),
+                         static_cast<const float *>(s.data_ptr()), pointer(b), pointer(r),
+                         output.data_ptr(), rows, cols, out, static_cast<int>(activation),
+                         pointer(workspace), bytes, stream_of(x)),
+        "linear_int8_forward");
+  return output;
 }
 
 // ----------------------------------------------------------------- dropout ---
@@ -341,6 +399,8 @@ namespace layer_host {
 void define_block(pybind11::module_ &m) {
   namespace py = pybind11;
   m.def("gated_linear", &gated_linear, py::call_guard<py::gil_scoped_release>());
+  m.def("quantize", &quantize, py::call_guard<py::gil_scoped_release>());
+  m.def("linear_int8", &linear_int8, py::call_guard<py::gil_scoped_release>());
   m.def("dropout", &dropout, py::call_guard<py::gil_scoped_release>());
   m.def("residual_norm", &residual_norm, py::call_guard<py::gil_scoped_release>());
 }

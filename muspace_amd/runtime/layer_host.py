@@ -23,7 +23,8 @@ _BOUND = (
     "muspace_last_error", "linear_forward", "linear_checkpoint",
     "linear_backward_workspace_size_for", "linear_backward", "layer_norm_forward",
     "layer_norm_backward_workspace_size", "layer_norm_backward", "gated_linear_forward",
-    "gated_linear_backward_workspace_size", "gated_linear_backward", "dropout_forward",
+    "gated_linear_backward_workspace_size", "gated_linear_backward", "quantize_int8",
+    "linear_int8_workspace_size", "linear_int8_forward", "dropout_forward",
     "residual_norm_forward", "residual_norm_backward_workspace_size", "residual_norm_backward",
 )
 

@@ -184,6 +184,13 @@ _EXPORTS: dict[str, tuple[Any, list[Any]]] = {
         [_c_ptr, _c_int] + [_c_ptr] * 6 + [_c_int64] * 3
         + [_c_int, _c_ptr, ctypes.c_size_t, _c_ptr],
     ),
+    "quantize_int8": (_c_int, [_c_ptr, _c_int, _c_ptr, _c_ptr, _c_int64, _c_int64, _c_ptr]),
+    "linear_int8_workspace_size": (ctypes.c_size_t, [_c_int] + [_c_int64] * 3),
+    "linear_int8_forward": (
+        _c_int,
+        [_c_ptr, _c_int] + [_c_ptr] * 5 + [_c_int64] * 3
+        + [_c_int, _c_ptr, ctypes.c_size_t, _c_ptr],
+    ),
     "dropout_forward": (
         _c_int,
         [_c_ptr, _c_int, _c_ptr, _c_ptr, _c_int64, ctypes.c_double, ctypes.c_uint64, _c_ptr,

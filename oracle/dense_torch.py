@@ -244,3 +244,39 @@ def gated_linear(x, weight, bias, activation, grad=None):
         results.append(value)
         bounds.append(err * (1 + u_step) + u_step * value.abs() + small)
     return results, bounds
+
+
+def quantize(x):
+    """(codes, scales) of the rows of x in 8 bits: the scale is a float32 number, the codes are
+    its float32 quotients' nearest integers. In float64, rounded to float32 where the definition
+    is (numbers of 24 bits divided in 53 and rounded to 24 are the correctly rounded quotient)."""
+    x = x.double()
+    top = x.abs().amax(-1, keepdim=True) if x.shape[-1] else x.new_zeros(x.shape[0], 1)
+    finite = x.isfinite().all(-1, keepdim=True)
+    scale = (top / 127.0).float().double().clamp_min(2.0**-126)
+    codes = torch.round((x / scale).float().double())
+    codes = torch.where(finite, codes, 1.0)
+    scale = torch.where(finite, scale, math.nan)
+    return codes.to(torch.int8), scale.squeeze(-1).float()
+
+
+def linear_int8(x, weight, weight_scale, bias, activation, residual):
+    """(y, bound): the sum of the codes' products is exact; it, its two products with the scales
+    and the sum with the bias round once each."""
+    dtype, u = x.dtype, half_step(x.dtype)
+    codes, scales = quantize(x)
+    z = (codes.double() @ weight.double().t()) * scales.double()[:, None] * weight_scale.double()
+    z_err = 2 * SUM_STEP * z.abs()
+    if bias is not None:
+        z = z + bias.double()
+        z_err = z_err + SUM_STEP * z.abs()
+    if activation == "relu":
+        y, y_err = z.clamp_min(0.0), z_err
+    elif activation == "gelu":
+        y, y_err = gelu(z), 1.13 * z_err + 8 * SUM_STEP * z.abs()
+    else:
+        y, y_err = z, z_err
+    if residual is not None:
+        y = y + residual.double()
+        y_err = y_err + SUM_STEP * y.abs()
+    return y, y_err * (1 + u) + u * y.abs() + tiny(dtype)
