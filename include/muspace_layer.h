@@ -167,12 +167,12 @@ MUSPACE_API int dropout_forward(const void *x, int dtype, const void *residual, 
 /* The sum of a block with the residual stream, and the norm after it:
  *   y = post_norm(block) (post_norm -1 none: the block; 0 layer, 1 rms)
  *   stream_values = residual_scale residual + gate dropout(y)
- *   output = norm(stream_values as stored)   (norm 0 layer, 1 rms)
+ *   output = norm(the same sum, before it is rounded)   (norm 0 layer, 1 rms)
  * block, residual, output, stream_values [rows, cols]; weight, bias, gate, post_weight,
  * post_bias [cols] of weight_dtype (dtype or float32), each may be NULL (ones; biases
  * zeros). The rms norm is x / sqrt(mean(x^2) + eps) weight + bias. dropout is that of
  * dropout_forward over the tensor's elements, p 0 for none. stream_values, statistics
- * and post_statistics ([rows, 2] float32, as layer norm's, for the backward) may be
+ * and post_statistics ([rows, 4] float32, 16-byte aligned, for the backward) may be
  * NULL. */
 MUSPACE_API int residual_norm_forward(const void *block, int dtype, const void *residual,
                                       const void *weight, const void *bias, const void *gate,
@@ -189,11 +189,13 @@ MUSPACE_API size_t residual_norm_backward_workspace_size(int dtype, int64_t rows
                                                          int sums);
 
 /* The gradients from those of output and stream_values (NULL: zeros). A NULL gradient
- * is not computed. block is read where there is a post norm or grad_gate is wanted, and
- * may be NULL otherwise; p, seed, device_seed's value and offset are the forward's. */
+ * is not computed. 16-bit types read block and residual (stream_values may be NULL);
+ * float32 reads stream_values, and block where there is a post norm or grad_gate is
+ * wanted (residual, and block otherwise, may be NULL). p, seed, device_seed's value and
+ * offset are the forward's. */
 MUSPACE_API int residual_norm_backward(
     const void *grad_output, const void *grad_stream, int dtype, const void *block,
-    const void *stream_values, const void *weight, const void *gate, const void *post_weight,
+    const void *residual, const void *stream_values, const void *weight, const void *gate, const void *post_weight,
     const void *post_bias, int weight_dtype, const float *statistics, const float *post_statistics,
     void *grad_block, void *grad_residual, void *grad_weight, void *grad_bias, void *grad_gate,
     void *grad_post_weight, void *grad_post_bias, int64_t rows, int64_t cols, int norm,

@@ -262,14 +262,16 @@ struct ResidualFunction : torch::autograd::Function<ResidualFunction> {
     const Vectors v{weight.value_or(Tensor()), bias.value_or(Tensor()), gate.value_or(Tensor()),
                     post_weight.value_or(Tensor()), post_bias.value_or(Tensor())};
     const auto stats = [&] {
-      return at::empty({rows_of(block), 2}, block.options().dtype(at::kFloat));
+      return at::empty({rows_of(block), 4}, block.options().dtype(at::kFloat));
     };
-    const NormKept kept{at::empty(block.sizes(), block.options()), stats(),
+    // what the backward reads (muspace_layer.h)
+    const bool sums = block.scalar_type() != at::kFloat;
+    const NormKept kept{sums && !want_stream ? Tensor() : at::empty(block.sizes(), block.options()), stats(),
                         n.post >= 0 ? stats() : Tensor()};
     Tensor output = residual_run(block, residual, v, n, drop, kept);
-    const bool block_kept = n.post >= 0 || wants_grad(v.gate);
-    ctx->save_for_backward({block_kept ? block : Tensor(), kept.stream, kept.stats, kept.post_stats,
-                            v.weight, v.gate, v.post_weight, v.post_bias, drop.device_seed});
+    const bool block_kept = sums || n.post >= 0 || wants_grad(v.gate);
+    ctx->save_for_backward({block_kept ? block : Tensor(), sums ? residual : kept.stream,
+                            kept.stats, kept.post_stats, v.weight, v.gate, v.post_weight, v.post_bias, drop.device_seed});
     drop.keep(ctx);
     ctx->saved_data["norm"] = n.norm;
     ctx->saved_data["post"] = n.post;
@@ -287,6 +289,7 @@ struct ResidualFunction : torch::autograd::Function<ResidualFunction> {
 
   static variable_list backward(AutogradContext *ctx, variable_list grads) {
     const variable_list saved = ctx->get_saved_variables();
+    // (the stream, or the residual that it is summed from)
     const Tensor &block = saved[0], &stream = saved[1], &stats = saved[2], &post_stats = saved[3];
     const auto type = static_cast<at::ScalarType>(ctx->saved_data["type"].toInt());
     const int64_t given = ctx->saved_data["given"].toInt();
@@ -318,8 +321,8 @@ struct ResidualFunction : torch::autograd::Function<ResidualFunction> {
       const size_t bytes = sums > 0 ? api.residual_workspace(code, rows, cols, sums) : 0;
       const Tensor workspace = scratch(bytes, stream);
       check(api.residual_backward(
-                pointer(g), pointer(gs), code, pointer(block), stream.data_ptr(), pointer(saved[4]),
-                pointer(saved[5]), pointer(saved[6]), pointer(saved[7]), code_of(type, "weight"),
+                pointer(g), pointer(gs), code, pointer(block), code != 0 ? stream.data_ptr() : nullptr,
+                code == 0 ? stream.data_ptr() : nullptr, pointer(saved[4]), pointer(saved[5]), pointer(saved[6]), pointer(saved[7]), code_of(type, "weight"),
                 static_cast<const float *>(stats.data_ptr()),
                 static_cast<const float *>(pointer(post_stats)), pointer(out[0]), pointer(out[1]),
                 pointer(out[2]), pointer(out[3]), pointer(out[4]), pointer(out[5]),

@@ -23,6 +23,7 @@ constexpr int64_t kMaxCols = 1 << 20;
 constexpr int64_t kMaxRows = INT_MAX - 256;
 
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+bool aligned16(const void *p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 
 template <typename F>
 void by_type(int dtype, F &&f) {
@@ -126,7 +127,7 @@ void launch_rows(const Residual &a, int blocks, bool block, hipStream_t st) {
   }
 }
 
-// `block`: forward: a post norm; backward: the block's output is read
+// `block`: forward: a post norm; backward: or the gate's gradient
 template <typename T, bool kBackward, int kLanes = 16>
 void launch(int lanes, const Residual &a, int blocks, bool block, hipStream_t st) {
   if (lanes != kLanes) {
@@ -184,6 +185,9 @@ int residual_norm_forward(const void *block, int dtype, const void *residual, co
   if (block == nullptr || residual == nullptr || output == nullptr) {
     return fail(MUSPACE_EINVAL, "%s: null tensor pointer", fn);
   }
+  if (!aligned16(statistics) || !aligned16(post_statistics)) {
+    return fail(MUSPACE_EINVAL, "%s: statistics must be 16-byte aligned", fn);
+  }
   Residual a = {};
   a.block = block;
   a.residual = residual;
@@ -229,8 +233,8 @@ size_t residual_norm_backward_workspace_size(int dtype, int64_t rows, int64_t co
 }
 
 int residual_norm_backward(const void *grad_output, const void *grad_stream, int dtype,
-                           const void *block, const void *stream_values, const void *weight,
-                           const void *gate, const void *post_weight, const void *post_bias,
+                           const void *block, const void *residual, const void *stream_values,
+                           const void *weight, const void *gate, const void *post_weight, const void *post_bias,
                            int weight_dtype, const float *statistics, const float *post_statistics,
                            void *grad_block, void *grad_residual, void *grad_weight,
                            void *grad_bias, void *grad_gate, void *grad_post_weight,
@@ -254,16 +258,18 @@ int residual_norm_backward(const void *grad_output, const void *grad_stream, int
   if (post_norm == dense::kNoNorm && (grad_post_weight != nullptr || grad_post_bias != nullptr)) {
     return fail(MUSPACE_EINVAL, "%s: gradients of a post norm without one", fn);
   }
-  // the block's output is read for the post norm and the gate's gradient
-  const bool reads_block = post_norm != dense::kNoNorm || grad_gate != nullptr;
+  // 16-bit types sum block and residual again; float32 reads the stream, and the block's
+  // output for the post norm and the gate's gradient
+  const bool of_block = post_norm != dense::kNoNorm || grad_gate != nullptr;
+  const bool reads_block = of_block || dtype != 0;
   if (rows > 0 &&
-      (stream_values == nullptr || statistics == nullptr || (reads_block && block == nullptr) ||
+      ((dtype == 0 ? stream_values : residual) == nullptr || statistics == nullptr ||
+       (reads_block && block == nullptr) ||
        (post_norm != dense::kNoNorm && post_statistics == nullptr))) {
     return fail(MUSPACE_EINVAL, "%s: null tensor pointer", fn);
   }
-  if (reinterpret_cast<uintptr_t>(statistics) % 8 != 0 ||
-      reinterpret_cast<uintptr_t>(post_statistics) % 8 != 0) {
-    return fail(MUSPACE_EINVAL, "%s: statistics must be 8-byte aligned", fn);
+  if (!aligned16(statistics) || !aligned16(post_statistics)) {
+    return fail(MUSPACE_EINVAL, "%s: statistics must be 16-byte aligned", fn);
   }
   const size_t need =
       a.sums > 0 ? residual_norm_backward_workspace_size(dtype, rows, cols, a.sums) : 0;
@@ -274,6 +280,7 @@ int residual_norm_backward(const void *grad_output, const void *grad_stream, int
   }
   const int lanes = plan_lanes(dtype, cols);
   a.block = reads_block ? block : nullptr;
+  a.residual = residual;
   a.stream_in = stream_values;
   a.grad_out = grad_output;
   a.grad_stream = grad_stream;
@@ -302,7 +309,7 @@ int residual_norm_backward(const void *grad_output, const void *grad_stream, int
     using T = decltype(t);
     if (rows > 0) {
       if (lanes != 0) {
-        launch<T, true>(lanes, a, blocks, reads_block, st);
+        launch<T, true>(lanes, a, blocks, of_block, st);
       } else {
         dense::residual_backward_long<T>
             <<<static_cast<int>(rows < 2048 ? rows : 2048), dense::kLongThreads, 0, st>>>(a);

@@ -15,11 +15,12 @@
 // whose statistics these are); the dropout's mask is computed in both directions
 // (dropout_device.hpp).
 //
-// `output` is the norm of the stream as it is stored, rounded to the tensors' type: the
-// backward keeps the stream alone and differentiates exactly what the forward
-// computed, and a stream read back gives the same norm. (With the norm of the unrounded
-// sum the backward would have to keep the block and the residual in its place, one
-// tensor more to keep and to read of five.)
+// `output` is the norm of the sum in float32, before it is rounded into the stream. In
+// 16-bit types the backward therefore sums the block and the residual again, rather than
+// read the stream: from the stored stream, h would carry its rounding, and the norm's
+// output and the weight's gradient would err by 1.3 to 1.66 times their own rounding. float32
+// reads the stream, which is the sum. Kept per norm and row: what is subtracted, in two
+// parts (Centre), and s.
 #pragma once
 
 #include "dropout_device.hpp"
@@ -33,10 +34,11 @@ constexpr int kSums = 5;  // dw, db, d gate, d post weight, d post bias
 
 struct Residual {
   const void *block, *residual, *weight, *bias, *gate, *post_weight, *post_bias;
-  const void *grad_out, *grad_stream, *stream_in;
+  const void *grad_out, *grad_stream;
+  const void *stream_in;           // float32's backward
   void *out, *stream;              // forward
   void *d_block, *d_residual;      // backward
-  float *stats, *post_stats;       // [rows][2] each, as layer norm's
+  float *stats, *post_stats;       // [rows][4] each: base, offset, s, 0
   float *partial;                  // [workgroups][sums][cols]
   float *row_sums;                 // rows of any length: [rows][4] for the column sums
   int slot[kSums];                 // a column sum's place in `partial` (-1: not wanted)
@@ -110,6 +112,15 @@ __device__ __forceinline__ float first_value(float v, float *lds) {
   }
 }
 
+__device__ __forceinline__ void keep_statistics(float *stats, int64_t row, const Centre &c, float s) {
+  reinterpret_cast<f32x4 *>(stats)[row] = f32x4{c.base, c.offset, s, 0.0f};
+}
+
+// x without its row's centre, times s; the forward's and the backward's
+__device__ __forceinline__ float unit_of(float x, const f32x4 &stats) {
+  return (x - stats[0] - stats[1]) * stats[2];
+}
+
 // Centre and factor of a row in registers. `v` keeps its values; `x0` is the first.
 template <int kLanes, bool kFull, int kV>
 __device__ __forceinline__ float row_statistics(const float (&v)[kV], int cols, int lane,
@@ -176,7 +187,7 @@ __global__ __launch_bounds__(kRowThreads) void residual_forward(const Residual a
       const float s = row_statistics<kLanes, kFull>(y, a.cols, lane, x0, a.post, inv, a.eps, lds,
                                                     centre);
       if (a.post_stats != nullptr && any && lane == 0) {
-        keep_centre(a.post_stats + 2 * row, x0, centre, s);
+        keep_statistics(a.post_stats, row, centre, s);
       }
 #pragma unroll
       for (int e = 0; e < kV; ++e) {
@@ -190,15 +201,13 @@ __global__ __launch_bounds__(kRowThreads) void residual_forward(const Residual a
     }
 #pragma unroll
     for (int e = 0; e < kV; ++e) v[e] = fmaf(a.scale, v[e], gate[e] * y[e]);
-    const u32x4 stored = pack<T>(v);
     if (a.stream != nullptr) {
-      loose_store(static_cast<T *>(a.stream) + row * a.cols + col, stored, any ? left : 0);
+      loose_store(static_cast<T *>(a.stream) + row * a.cols + col, pack<T>(v), any ? left : 0);
     }
-    unpack<T>(stored, v);
     const float x0 = first_value<kLanes>(v[0], lds);
     const float s = row_statistics<kLanes, kFull>(v, a.cols, lane, x0, a.norm, inv, a.eps, lds,
                                                   centre);
-    if (a.stats != nullptr && any && lane == 0) keep_centre(a.stats + 2 * row, x0, centre, s);
+    if (a.stats != nullptr && any && lane == 0) keep_statistics(a.stats, row, centre, s);
 #pragma unroll
     for (int e = 0; e < kV; ++e) {
       v[e] = (v[e] - centre.base - centre.offset) * s * w[e] + b[e];
@@ -207,17 +216,20 @@ __global__ __launch_bounds__(kRowThreads) void residual_forward(const Residual a
   }
 }
 
-// kBlock: the block's output is read again, for a post norm or the gate's gradient.
+// kBlock: for a post norm or the gate's gradient (float32 reads the block's output for
+// these alone).
 template <typename T, int kLanes, bool kFull, bool kBlock>
 __global__ __launch_bounds__(kRowThreads) void residual_backward(const Residual a) {
   constexpr int kGroups = kRowThreads / kLanes;  // rows at a time
   constexpr int kV = Piece<T>::kValues;
   constexpr int kCols = kLanes * kV;
   constexpr int kMine = kBlock ? kSums : 2;
+  constexpr bool kSum = sizeof(T) == 2;  // the stream is summed again
   using Pieces = RowPieces<T, kLanes, 1, kFull>;
   __shared__ float lds[kGroups > 1 ? kGroups * kCols : kTeamLds];
   const int lane = threadIdx.x % kLanes, group = threadIdx.x / kLanes;
-  const T *stream = static_cast<const T *>(a.stream_in), *block = static_cast<const T *>(a.block);
+  const T *stream = static_cast<const T *>(kSum ? a.residual : a.stream_in);
+  const T *block = static_cast<const T *>(a.block);
   const T *go = static_cast<const T *>(a.grad_out), *gs = static_cast<const T *>(a.grad_stream);
   const float inv = 1.0f / static_cast<float>(a.cols);
   const uint64_t seed = seed_of(a.drop);
@@ -233,37 +245,44 @@ __global__ __launch_bounds__(kRowThreads) void residual_backward(const Residual 
   const int64_t step = static_cast<int64_t>(gridDim.x) * kGroups;
   int64_t row = static_cast<int64_t>(blockIdx.x) * kGroups + group;
   Pieces n_stream, n_go = {}, n_gs = {}, n_block;
-  f32x2 n_stats = {0.0f, 0.0f}, n_post = {0.0f, 0.0f};
+  f32x4 n_stats, n_post = {0.0f, 0.0f, 1.0f, 0.0f};  // without a post norm: the block's output
   auto fetch = [&](int64_t r) {
     const int64_t at = min(r, a.rows - 1);
     n_stream.load(stream, r, a.rows, a.cols, lane);
     if (go != nullptr) n_go.load(go, r, a.rows, a.cols, lane);
     if (gs != nullptr) n_gs.load(gs, r, a.rows, a.cols, lane);
-    n_stats = reinterpret_cast<const f32x2 *>(a.stats)[at];
+    n_stats = reinterpret_cast<const f32x4 *>(a.stats)[at];
+    if constexpr (kBlock || kSum) n_block.load(block, r, a.rows, a.cols, lane);
     if constexpr (kBlock) {
-      n_block.load(block, r, a.rows, a.cols, lane);
-      if (a.post != kNoNorm) n_post = reinterpret_cast<const f32x2 *>(a.post_stats)[at];
+      if (a.post != kNoNorm) n_post = reinterpret_cast<const f32x4 *>(a.post_stats)[at];
     }
   };
   fetch(row);
   for (int64_t base = static_cast<int64_t>(blockIdx.x) * kGroups; base < a.rows;
        base += step, row += step) {
     const bool any = row < a.rows;
-    float h[kV], u[kV], ds[kV], y[kV];
+    const int64_t at = row * a.cols + col;
+    float h[kV], u[kV], ds[kV], unit[kV];
     n_stream.values(0, a.cols, lane, any, h);
     n_go.values(0, a.cols, lane, any && go != nullptr, u);
     n_gs.values(0, a.cols, lane, any && gs != nullptr, ds);
-    if constexpr (kBlock) n_block.values(0, a.cols, lane, any, y);
-    const f32x2 stats = n_stats, post = n_post;
+    if constexpr (kBlock || kSum) n_block.values(0, a.cols, lane, any, unit);
+    const f32x4 stats = n_stats, post = n_post;
     fetch(row + step);
-    const float x0 = first_value<kLanes>(h[0], lds);
-    const Centre centre = kept_centre(x0, stats[0], stats[1]);
-    const float s = fabsf(stats[1]);
+    // (no bits past the last row)
+    const uint32_t bits = !any ? 0u : a.drop.on ? kept_bits<kV>(a.drop, seed, at) : ~0u;
     float along[2] = {0.0f, 0.0f};
 #pragma unroll
     for (int e = 0; e < kV; ++e) {
-      // the operations of the forward, so that h is the forward's own
-      h[e] = inside<kFull>((h[e] - centre.base - centre.offset) * s, e, left);
+      if constexpr (kBlock) unit[e] = inside<kFull>(unit_of(unit[e], post), e, left);
+      if constexpr (kSum) {
+        // the operations of the forward
+        float y = unit[e];
+        if constexpr (kBlock) y = y * pw[e] + pb[e];
+        y = (bits >> e) & 1u ? y * a.drop.scale : 0.0f;
+        h[e] = fmaf(a.scale, h[e], gate[e] * y);
+      }
+      h[e] = inside<kFull>(unit_of(h[e], stats), e, left);
       sum[0][e] += u[e] * h[e];
       sum[1][e] += u[e];
       u[e] *= w[e];
@@ -276,22 +295,15 @@ __global__ __launch_bounds__(kRowThreads) void residual_backward(const Residual 
       team_sum<kLanes, 2>(along, lds);
       const float mu = a.norm == kLayerNorm ? along[0] * inv : 0.0f, mh = along[1] * inv;
 #pragma unroll
-      for (int e = 0; e < kV; ++e) ds[e] += s * (u[e] - mu - h[e] * mh);
+      for (int e = 0; e < kV; ++e) ds[e] += stats[2] * (u[e] - mu - h[e] * mh);
     }
-    float p0 = 0.0f;
-    if constexpr (kBlock) p0 = first_value<kLanes>(y[0], lds);
-    const Centre centre_p = kept_centre(p0, post[0], post[1]);
-    const float sp = fabsf(post[1]);
-    float across[2] = {0.0f, 0.0f};
-    const int64_t at = row * a.cols + col;
     if (a.d_residual != nullptr) {
       float r[kV];
 #pragma unroll
       for (int e = 0; e < kV; ++e) r[e] = a.scale * ds[e];
       loose_store(static_cast<T *>(a.d_residual) + at, pack<T>(r), any ? left : 0);
     }
-    // (no bits past the last row)
-    const uint32_t bits = !any ? 0u : a.drop.on ? kept_bits<kV>(a.drop, seed, at) : ~0u;
+    float across[2] = {0.0f, 0.0f};
 #pragma unroll
     for (int e = 0; e < kV; ++e) {
       const bool kept = (bits >> e) & 1u;
@@ -299,18 +311,13 @@ __global__ __launch_bounds__(kRowThreads) void residual_backward(const Residual 
       float dy = kept ? dt * gate[e] : 0.0f;
       if constexpr (kBlock) {
         dy = inside<kFull>(dy, e, left);
-        float unit = y[e];
-        if (a.post != kNoNorm) unit = (unit - centre_p.base - centre_p.offset) * sp;
-        unit = inside<kFull>(unit, e, left);
-        // with a post norm y is its result, otherwise the block's output
-        const float value = a.post != kNoNorm ? unit * pw[e] + pb[e] : unit;
-        sum[2][e] += kept && (kFull || e < left) ? dt * value : 0.0f;
-        sum[3][e] += dy * unit;
+        const float y = unit[e] * pw[e] + pb[e];
+        sum[2][e] += kept && (kFull || e < left) ? dt * y : 0.0f;
+        sum[3][e] += dy * unit[e];
         sum[4][e] += dy;
-        if (a.post != kNoNorm) dy *= pw[e];
+        dy *= pw[e];
         across[0] += dy;
-        across[1] += dy * unit;
-        y[e] = unit;
+        across[1] += dy * unit[e];
       }
       ds[e] = dy;
     }
@@ -320,7 +327,7 @@ __global__ __launch_bounds__(kRowThreads) void residual_backward(const Residual 
         team_sum<kLanes, 2>(across, lds);
         const float mv = a.post == kLayerNorm ? across[0] * inv : 0.0f, mh = across[1] * inv;
 #pragma unroll
-        for (int e = 0; e < kV; ++e) ds[e] = sp * (ds[e] - mv - y[e] * mh);
+        for (int e = 0; e < kV; ++e) ds[e] = post[2] * (ds[e] - mv - unit[e] * mh);
       }
     }
     loose_store(static_cast<T *>(a.d_block) + at, pack<T>(ds), any ? left : 0);
@@ -399,6 +406,92 @@ __device__ __forceinline__ float long_statistics(int cols, float x0, int norm, f
   return correct_centre(centre, sums, inv, eps);
 }
 
+// A row's pieces, forward and backward.
+template <typename T>
+struct LongRow {
+  static constexpr int kV = Piece<T>::kValues;
+  f32x4 stats, post;  // without a post norm: the block's output is its own unit row
+
+  // the post norm's unit row, and what the dropout is taken of
+  __device__ __forceinline__ void block(const Residual &a, int64_t row, int col, int left,
+                                        float (&unit)[kV], float (&y)[kV]) const {
+    unpack<T>(loose_load<T>(static_cast<const T *>(a.block) + row * a.cols + col,
+                            a.block != nullptr ? left : 0), unit);
+    float pw[kV], pb[kV];
+    load_vector<T>(a.post_weight, a.w32, col, left, pw, 1.0f);
+    load_vector<T>(a.post_bias, a.w32, col, left, pb, 0.0f);
+#pragma unroll
+    for (int e = 0; e < kV; ++e) {
+      unit[e] = e < left ? unit_of(unit[e], post) : 0.0f;
+      y[e] = unit[e] * pw[e] + pb[e];
+    }
+  }
+  // the stream, summed
+  __device__ __forceinline__ void stream(const Residual &a, uint64_t seed, int64_t row, int col,
+                                         int left, float (&v)[kV]) const {
+    const int64_t at = row * a.cols + col;
+    float unit[kV], y[kV], gate[kV];
+    block(a, row, col, left, unit, y);
+    unpack<T>(loose_load<T>(static_cast<const T *>(a.residual) + at, left), v);
+    load_vector<T>(a.gate, a.w32, col, left, gate, 1.0f);
+    const uint32_t bits = a.drop.on ? kept_bits<kV>(a.drop, seed, at) : ~0u;
+#pragma unroll
+    for (int e = 0; e < kV; ++e) {
+      y[e] = (bits >> e) & 1u ? y[e] * a.drop.scale : 0.0f;
+      v[e] = fmaf(a.scale, v[e], gate[e] * y[e]);
+    }
+  }
+  // backward: the statistics of a row
+  __device__ __forceinline__ void open(const Residual &a, int64_t row) {
+    stats = reinterpret_cast<const f32x4 *>(a.stats)[row];
+    post = f32x4{0.0f, 0.0f, 1.0f, 0.0f};
+    if (a.post != kNoNorm) post = reinterpret_cast<const f32x4 *>(a.post_stats)[row];
+  }
+  // h and g of the norm
+  __device__ __forceinline__ void unit(const Residual &a, uint64_t seed, int64_t row, int col,
+                                       int left, float (&h)[kV], float (&g)[kV]) const {
+    const int64_t at = row * a.cols + col;
+    if constexpr (sizeof(T) == 2) {
+      stream(a, seed, row, col, left, h);
+    } else {
+      unpack<T>(loose_load<T>(static_cast<const T *>(a.stream_in) + at, left), h);
+    }
+    unpack<T>(loose_load<T>(static_cast<const T *>(a.grad_out) + at, a.grad_out != nullptr ? left : 0),
+              g);
+#pragma unroll
+    for (int e = 0; e < kV; ++e) h[e] = e < left ? unit_of(h[e], stats) : 0.0f;
+  }
+  // the stream's gradient, given the means of u and u h
+  __device__ __forceinline__ void stream_grad(const Residual &a, int64_t row, int col, int left,
+                                              float mu, float mh, const float (&h)[kV],
+                                              const float (&g)[kV], float (&ds)[kV]) const {
+    const int64_t at = row * a.cols + col;
+    unpack<T>(loose_load<T>(static_cast<const T *>(a.grad_stream) + at,
+                            a.grad_stream != nullptr ? left : 0), ds);
+    if (a.grad_out == nullptr) return;
+    float w[kV];
+    load_vector<T>(a.weight, a.w32, col, left, w, 1.0f);
+#pragma unroll
+    for (int e = 0; e < kV; ++e) ds[e] += stats[2] * (g[e] * w[e] - mu - h[e] * mh);
+  }
+  // from ds: dy, the post norm's unit row (or the block's output) and the gate's term
+  __device__ __forceinline__ void block_grad(const Residual &a, uint64_t seed, int64_t row, int col,
+                                             int left, const float (&ds)[kV], float (&dy)[kV],
+                                             float (&unit)[kV], float (&gated)[kV]) const {
+    const uint32_t bits = a.drop.on ? kept_bits<kV>(a.drop, seed, row * a.cols + col) : ~0u;
+    float gate[kV], y[kV];
+    load_vector<T>(a.gate, a.w32, col, left, gate, 1.0f);
+    block(a, row, col, left, unit, y);
+#pragma unroll
+    for (int e = 0; e < kV; ++e) {
+      const bool kept = ((bits >> e) & 1u) && e < left;
+      const float dt = kept ? ds[e] * a.drop.scale : 0.0f;
+      dy[e] = kept ? dt * gate[e] : 0.0f;
+      gated[e] = kept ? dt * y[e] : 0.0f;
+    }
+  }
+};
+
 template <typename T>
 __global__ __launch_bounds__(kLongThreads) void residual_forward_long(const Residual a) {
   constexpr int kV = Piece<T>::kValues;
@@ -407,49 +500,25 @@ __global__ __launch_bounds__(kLongThreads) void residual_forward_long(const Resi
   const uint64_t seed = seed_of(a.drop);
   for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
     const T *block = static_cast<const T *>(a.block) + row * a.cols;
-    const T *residual = static_cast<const T *>(a.residual) + row * a.cols;
-    Centre centre_p = {0.0f, 0.0f};
-    float sp = 1.0f;
+    LongRow<T> r;
+    r.post = f32x4{0.0f, 0.0f, 1.0f, 0.0f};
+    Centre centre;
     if (a.post != kNoNorm) {
-      const float p0 = to_float(block[0]);
-      sp = long_statistics<T>(a.cols, p0, a.post, inv, a.eps, lds, centre_p,
-                              [&](int col, int left, float(&v)[kV]) {
-                                unpack<T>(loose_load<T>(block + col, left), v);
-                              });
+      const float s = long_statistics<T>(a.cols, to_float(block[0]), a.post, inv, a.eps, lds,
+                                         centre, [&](int col, int left, float(&v)[kV]) {
+                                           unpack<T>(loose_load<T>(block + col, left), v);
+                                         });
+      r.post = f32x4{centre.base, centre.offset, s, 0.0f};
       if (a.post_stats != nullptr && threadIdx.x == 0) {
-        keep_centre(a.post_stats + 2 * row, p0, centre_p, sp);
+        keep_statistics(a.post_stats, row, centre, s);
       }
     }
-    // the stream's piece as it is stored
-    auto stream = [&](int col, int left, float(&v)[kV]) {
-      float y[kV], gate[kV];
-      unpack<T>(loose_load<T>(block + col, left), y);
-      unpack<T>(loose_load<T>(residual + col, left), v);
-      load_vector<T>(a.gate, a.w32, col, left, gate, 1.0f);
-      if (a.post != kNoNorm) {
-        float pw[kV], pb[kV];
-        load_vector<T>(a.post_weight, a.w32, col, left, pw, 1.0f);
-        load_vector<T>(a.post_bias, a.w32, col, left, pb, 0.0f);
-#pragma unroll
-        for (int e = 0; e < kV; ++e) {
-          y[e] = (y[e] - centre_p.base - centre_p.offset) * sp * pw[e] + pb[e];
-        }
-      }
-      if (a.drop.on) {
-        const uint32_t bits = kept_bits<kV>(a.drop, seed, row * a.cols + col);
-#pragma unroll
-        for (int e = 0; e < kV; ++e) y[e] = (bits >> e) & 1u ? y[e] * a.drop.scale : 0.0f;
-      }
-#pragma unroll
-      for (int e = 0; e < kV; ++e) v[e] = fmaf(a.scale, v[e], gate[e] * y[e]);
-      unpack<T>(pack<T>(v), v);
-    };
+    auto stream = [&](int col, int left, float(&v)[kV]) { r.stream(a, seed, row, col, left, v); };
     float v0[kV] = {};
     if (threadIdx.x == 0) stream(0, a.cols, v0);
     const float x0 = first_value<kLongThreads>(v0[0], lds);
-    Centre centre;
     const float s = long_statistics<T>(a.cols, x0, a.norm, inv, a.eps, lds, centre, stream);
-    if (a.stats != nullptr && threadIdx.x == 0) keep_centre(a.stats + 2 * row, x0, centre, s);
+    if (a.stats != nullptr && threadIdx.x == 0) keep_statistics(a.stats, row, centre, s);
     over_row<T>(a.cols, [&](int col, int left) {
       float v[kV], w[kV], b[kV];
       stream(col, left, v);
@@ -467,81 +536,6 @@ __global__ __launch_bounds__(kLongThreads) void residual_forward_long(const Resi
   }
 }
 
-// A row's piece in the backward, given the means of u and u h.
-template <typename T>
-struct LongRow {
-  static constexpr int kV = Piece<T>::kValues;
-  Centre centre, centre_p;
-  float s, sp;
-
-  __device__ __forceinline__ void open(const Residual &a, int64_t row) {
-    const float k = a.stats[2 * row + 1];
-    s = fabsf(k);
-    centre = kept_centre(to_float(static_cast<const T *>(a.stream_in)[row * a.cols]),
-                         a.stats[2 * row], k);
-    centre_p = Centre{0.0f, 0.0f};
-    sp = 1.0f;
-    if (a.post != kNoNorm) {
-      const float kp = a.post_stats[2 * row + 1];
-      sp = fabsf(kp);
-      centre_p = kept_centre(to_float(static_cast<const T *>(a.block)[row * a.cols]),
-                             a.post_stats[2 * row], kp);
-    }
-  }
-  // h and g of the norm
-  __device__ __forceinline__ void unit(const Residual &a, int64_t row, int col, int left,
-                                       float (&h)[kV], float (&g)[kV]) const {
-    const int64_t at = row * a.cols + col;
-    unpack<T>(loose_load<T>(static_cast<const T *>(a.stream_in) + at, left), h);
-    unpack<T>(loose_load<T>(static_cast<const T *>(a.grad_out) + at, a.grad_out != nullptr ? left : 0),
-              g);
-#pragma unroll
-    for (int e = 0; e < kV; ++e) {
-      h[e] = e < left ? (h[e] - centre.base - centre.offset) * s : 0.0f;
-    }
-  }
-  // the stream's gradient
-  __device__ __forceinline__ void stream_grad(const Residual &a, int64_t row, int col, int left,
-                                              float mu, float mh, const float (&h)[kV],
-                                              const float (&g)[kV], float (&ds)[kV]) const {
-    const int64_t at = row * a.cols + col;
-    unpack<T>(loose_load<T>(static_cast<const T *>(a.grad_stream) + at,
-                            a.grad_stream != nullptr ? left : 0), ds);
-    if (a.grad_out == nullptr) return;
-    float w[kV];
-    load_vector<T>(a.weight, a.w32, col, left, w, 1.0f);
-#pragma unroll
-    for (int e = 0; e < kV; ++e) ds[e] += s * (g[e] * w[e] - mu - h[e] * mh);
-  }
-  // from ds: dy, the post norm's unit row (or the block's output) and what the gate
-  // multiplies
-  __device__ __forceinline__ void block_grad(const Residual &a, uint64_t seed, int64_t row, int col,
-                                             int left, const float (&ds)[kV], float (&dy)[kV],
-                                             float (&unit)[kV], float (&gated)[kV]) const {
-    const int64_t at = row * a.cols + col;
-    const uint32_t bits = a.drop.on ? kept_bits<kV>(a.drop, seed, at) : ~0u;
-    float gate[kV];
-    load_vector<T>(a.gate, a.w32, col, left, gate, 1.0f);
-    unpack<T>(loose_load<T>(static_cast<const T *>(a.block) + at, a.block != nullptr ? left : 0),
-              unit);
-    float pw[kV], pb[kV];
-    load_vector<T>(a.post_weight, a.w32, col, left, pw, 1.0f);
-    load_vector<T>(a.post_bias, a.w32, col, left, pb, 0.0f);
-#pragma unroll
-    for (int e = 0; e < kV; ++e) {
-      const bool kept = ((bits >> e) & 1u) && e < left;
-      const float dt = kept ? ds[e] * a.drop.scale : 0.0f;
-      dy[e] = kept ? dt * gate[e] : 0.0f;
-      float value = unit[e];
-      if (a.post != kNoNorm) {
-        unit[e] = e < left ? (unit[e] - centre_p.base - centre_p.offset) * sp : 0.0f;
-        value = unit[e] * pw[e] + pb[e];
-      }
-      gated[e] = kept ? dt * value : 0.0f;
-    }
-  }
-};
-
 template <typename T>
 __global__ __launch_bounds__(kLongThreads) void residual_backward_long(const Residual a) {
   constexpr int kV = Piece<T>::kValues;
@@ -555,7 +549,7 @@ __global__ __launch_bounds__(kLongThreads) void residual_backward_long(const Res
     if (a.grad_out != nullptr) {
       over_row<T>(a.cols, [&](int col, int left) {
         float h[kV], g[kV], w[kV];
-        r.unit(a, row, col, left, h, g);
+        r.unit(a, seed, row, col, left, h, g);
         load_vector<T>(a.weight, a.w32, col, left, w, 1.0f);
 #pragma unroll
         for (int e = 0; e < kV; ++e) {
@@ -573,7 +567,7 @@ __global__ __launch_bounds__(kLongThreads) void residual_backward_long(const Res
     }
     auto block_grad = [&](int col, int left, float(&ds)[kV], float(&dy)[kV], float(&unit)[kV]) {
       float h[kV], g[kV], gated[kV];
-      r.unit(a, row, col, left, h, g);
+      r.unit(a, seed, row, col, left, h, g);
       r.stream_grad(a, row, col, left, mean[0], mean[1], h, g, ds);
       r.block_grad(a, seed, row, col, left, ds, dy, unit, gated);
       if (a.post != kNoNorm) {
@@ -604,7 +598,7 @@ __global__ __launch_bounds__(kLongThreads) void residual_backward_long(const Res
       if (a.d_block != nullptr) {
         if (a.post != kNoNorm) {
 #pragma unroll
-          for (int e = 0; e < kV; ++e) dy[e] = r.sp * (dy[e] - mean_p[0] - unit[e] * mean_p[1]);
+          for (int e = 0; e < kV; ++e) dy[e] = r.post[2] * (dy[e] - mean_p[0] - unit[e] * mean_p[1]);
         }
         loose_store(static_cast<T *>(a.d_block) + at, pack<T>(dy), left);
       }
@@ -631,7 +625,7 @@ __global__ __launch_bounds__(kLongThreads) void residual_columns_long(const Resi
     LongRow<T> r;
     r.open(a, row);
     float h[kV], g[kV];
-    r.unit(a, row, col, left, h, g);
+    r.unit(a, seed, row, col, left, h, g);
 #pragma unroll
     for (int e = 0; e < kV; ++e) {
       sum[0][e] += g[e] * h[e];

@@ -9,9 +9,10 @@ Layers that norm after their blocks go on with ``normed``, layers that norm befo
 with both: ``normed`` into the next block, ``stream`` past it. A gate per channel and a
 norm on the block's own output are those of layers that norm on both sides or scale
 their branches. Every tensor is read and written once in either direction. ``normed``
-is the norm of the stream as it is stored, so the backward keeps that one tensor (and
-the block's output for a post norm or the gate's gradient); the dropout's mask is
-computed, not kept (see ``dropout``).
+is the norm of the sum before it is rounded into ``stream``: in 16-bit types the backward
+keeps the block's output and the residual and sums them again; in float32 it keeps the
+stream (and the block's output for a post norm or the gate's gradient). The dropout's
+mask is computed, not kept (see ``dropout``).
 
 No reference counterpart: the reference leaves these steps to torch.
 """
@@ -56,11 +57,6 @@ def residual_norm_pytorch(block, residual, weight=None, bias=None, *, norm="laye
     if gate is not None:
         y = gate.float() * y
     stream = residual_scale * residual.float() + y
-    if block.dtype != torch.float32:
-        # as it is stored, but still float32: both gradients of it are added before they
-        # are rounded (an infinity's difference from itself is no step)
-        step = (stream.to(block.dtype).float() - stream).detach()
-        stream = stream + torch.where(step.isnan(), 0.0, step)
     normed = _norm(stream, norm, weight, bias, eps).to(block.dtype)
     return (normed, stream.to(block.dtype)) if return_stream else normed
 

@@ -207,7 +207,7 @@ _EXPORTS: dict[str, tuple[Any, list[Any]]] = {
     ),
     "residual_norm_backward": (
         _c_int,
-        [_c_ptr, _c_ptr, _c_int] + [_c_ptr] * 6 + [_c_int] + [_c_ptr] * 9
+        [_c_ptr, _c_ptr, _c_int] + [_c_ptr] * 7 + [_c_int] + [_c_ptr] * 9
         + [_c_int64, _c_int64, _c_int, _c_int, ctypes.c_float, ctypes.c_double, ctypes.c_uint64,
            _c_ptr, ctypes.c_uint64, _c_ptr, ctypes.c_size_t, _c_ptr],
     ),

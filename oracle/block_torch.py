@@ -62,10 +62,11 @@ def dropout(x, keep, p, residual=None):
 class Unit:
     """A row's norm: its unit row h with its error, the factor s with its relative one."""
 
-    def __init__(self, x, kind, eps):
+    def __init__(self, x, kind, eps, x_err=0.0):
         cols = x.shape[-1]
         self.kind, self.depth = kind, 64 + cols // 256
         x = x.double()
+        x_err = x_err + torch.zeros_like(x)
         if kind == "layer":
             # the mean as an offset from a base, corrected by the mean of the differences
             # (see layer_norm in dense_torch)
@@ -73,9 +74,9 @@ class Unit:
             c = x - mean
             offset = torch.minimum(mean.abs(), (mean - x[:, :1]).abs())
             e = STEP * (2 * c.abs() + 2 * offset + self.depth * c.abs().mean(-1, keepdim=True))
-            e = e * (1 + 2.0**-10)
+            e = e * (1 + 2.0**-10) + x_err + x_err.mean(-1, keepdim=True)
         else:
-            c, e = x, torch.zeros_like(x)
+            c, e = x, x_err
         self.s = 1.0 / (c.square().mean(-1, keepdim=True) + eps).sqrt()
         self.s_rel = ((c.abs() * e + e * e).mean(-1, keepdim=True) * self.s * self.s
                       + (self.depth + 8) * STEP)
@@ -116,11 +117,9 @@ def column_sum(value, err, dtype):
 
 def residual_norm(block, residual, weight=None, bias=None, *, norm="layer", eps=1e-5,
                   post_norm=None, post_weight=None, post_bias=None, gate=None,
-                  residual_scale=1.0, p=0.0, keep=None, stream=None, grad=None,
-                  grad_stream=None):
+                  residual_scale=1.0, p=0.0, keep=None, grad=None, grad_stream=None):
     """{name: (value, bound)} of the outputs and, with a gradient of one of them, the
-    gradients of what is given. `keep`: the dropout's mask; `stream`: the stream as it was stored, of
-    which the norm is taken (by default the exact one, rounded)."""
+    gradients of what is given. `keep`: the dropout's mask."""
     dtype = block.dtype
     vectors = {"weight": weight, "bias": bias, "gate": gate, "post_weight": post_weight,
                "post_bias": post_bias}
@@ -142,9 +141,7 @@ def residual_norm(block, residual, weight=None, bias=None, *, norm="layer", eps=
     err = (gt.abs() * d_err + 2 * SUM_STEP * ((gt * d).abs() + total.abs()
                                               + (residual_scale * residual.double()).abs()))
     out = {"stream": rounded(total, err, dtype)}
-    if stream is None:
-        stream = total.to(dtype)
-    unit = Unit(stream, norm, eps)
+    unit = Unit(total, norm, eps, err)
     out["normed"] = rounded(*unit.scaled(w, b), dtype)
     if grad is None and grad_stream is None:
         return out

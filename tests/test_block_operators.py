@@ -112,8 +112,7 @@ def check_block(t, g, gs, p=0.0, seed=5, **kwargs):
     leaves = {k: v.detach().clone().requires_grad_() for k, v in t.items()}
     normed, stream = residual_norm(**leaves, dropout_p=p, seed=seed, offset=1, **kwargs)
     keep = block_torch.kept(0, t["block"].numel(), p, seed, 1).view(t["block"].shape)
-    want = block_torch.residual_norm(**t, p=p, keep=keep, stream=stream.detach(), grad=g,
-                                     grad_stream=gs, **kwargs)
+    want = block_torch.residual_norm(**t, p=p, keep=keep, grad=g, grad_stream=gs, **kwargs)
     outs = [o for o, d in ((normed, g), (stream, gs)) if d is not None]
     grads = torch.autograd.grad(outs, list(leaves.values()), [d for d in (g, gs) if d is not None],
                                 allow_unused=g is None)
@@ -338,6 +337,7 @@ def forward_args(**overrides):
         ({"block": None}, 1, "null tensor pointer"),
         ({"residual": None}, 1, "null tensor pointer"),
         ({"output": None}, 1, "null tensor pointer"),
+        ({"stats": FAR + 8}, 1, "16-byte aligned"),
     ],
 )
 def test_residual_norm_forward_abi_refuses(native_lib, overrides, code, message):
@@ -346,8 +346,8 @@ def test_residual_norm_forward_abi_refuses(native_lib, overrides, code, message)
 
 
 def backward_args(**overrides):
-    args = dict(grad=FAR, grad_stream=FAR, dtype=2, block=FAR, stream_values=FAR, weight=None,
-                gate=None, post_weight=None, post_bias=None, weight_dtype=0, stats=FAR,
+    args = dict(grad=FAR, grad_stream=FAR, dtype=2, block=FAR, residual=FAR, stream_values=FAR,
+                weight=None, gate=None, post_weight=None, post_bias=None, weight_dtype=0, stats=FAR,
                 post_stats=FAR, grad_block=FAR, grad_residual=FAR, grad_weight=FAR, grad_bias=None,
                 grad_gate=None, grad_post_weight=None, grad_post_bias=None, rows=4, cols=8, norm=0,
                 post_norm=-1, scale=1.0, p=0.0, seed=0, device_seed=None, offset=0, workspace=FAR,
@@ -363,10 +363,12 @@ def backward_args(**overrides):
         ({"cols": -1}, 1, "invalid dims"),
         ({"cols": 1 << 21}, 2, "32-bit"),
         ({"p": -0.5}, 1, "probability"),
-        ({"stream_values": None}, 1, "null tensor pointer"),
+        ({"residual": None}, 1, "null tensor pointer"),
+        ({"block": None}, 1, "null tensor pointer"),
+        ({"dtype": 0, "stream_values": None}, 1, "null tensor pointer"),
         ({"stats": None}, 1, "null tensor pointer"),
-        ({"stats": FAR + 4}, 1, "8-byte aligned"),
-        ({"grad_gate": FAR, "block": None}, 1, "null tensor pointer"),
+        ({"stats": FAR + 8}, 1, "16-byte aligned"),
+        ({"dtype": 0, "grad_gate": FAR, "block": None}, 1, "null tensor pointer"),
         ({"post_norm": 0, "post_stats": None}, 1, "null tensor pointer"),
         ({"grad_post_weight": FAR}, 1, "without one"),
         ({"workspace": None}, 1, "workspace"),
