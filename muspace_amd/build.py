@@ -40,6 +40,7 @@ DEPENDS = (
     PACKAGE_DIR / "csrc" / "dropout_device.hpp",
     PACKAGE_DIR / "csrc" / "residual_norm_kernels.hpp",
     PACKAGE_DIR / "csrc" / "int8_kernels.hpp",
+    PACKAGE_DIR / "csrc" / "wide_kernels.hpp",
     REPO_DIR / "include" / "muspace_msda.h",
     REPO_DIR / "include" / "muspace_dfa.h",
     REPO_DIR / "include" / "muspace_layer.h",

@@ -7,7 +7,7 @@
 
 #include "../../include/muspace_layer.h"
 #include "capi_errors.hpp"
-#include "int8_kernels.hpp"
+#include "wide_kernels.hpp"
 
 namespace {
 
@@ -89,6 +89,13 @@ void launch_product(Codes a, bool tight, hipStream_t st) {
 
 template <typename T>
 void run(Codes a, bool tight, hipStream_t st) {
+  if (tight && dense::wide_tiles(a.p.m, a.p.n, a.p.k)) {
+    a.p.tiles_n = static_cast<int>(ceil_div(a.p.n, dense::kWide));
+    a.p.tiles = static_cast<int>(ceil_div(a.p.m, dense::kWide)) * a.p.tiles_n;
+    dense::wide_product<int8_t, T, dense::Job::kForward>
+        <<<a.p.tiles, dense::kWideThreads, 0, st>>>(a);
+    return;
+  }
   const int64_t small = ceil_div(a.p.m, 64) * ceil_div(a.p.n, 64);
   if (small < 120) {
     constexpr int kWaves = 8;

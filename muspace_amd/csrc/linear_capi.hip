@@ -8,7 +8,7 @@
 
 #include "../../include/muspace_layer.h"
 #include "capi_errors.hpp"
-#include "linear_kernels.hpp"
+#include "wide_kernels.hpp"
 
 namespace {
 
@@ -298,6 +298,16 @@ template <Job kJob>
 void run_gated(int dtype, const Product &a, bool tight, hipStream_t st) {
   by_type(dtype, [&](auto t) {
     using T = decltype(t);
+    if constexpr (sizeof(T) == 2) {
+      if (tight && dense::wide_tiles(a.m, 2 * int64_t{a.n}, a.k)) {
+        dense::Codes c = {};
+        c.p = a;
+        c.p.tiles_n = static_cast<int>(ceil_div(a.n, dense::kWide / 2));
+        c.p.tiles = static_cast<int>(ceil_div(a.m, dense::kWide)) * c.p.tiles_n;
+        dense::wide_product<T, T, kJob><<<c.p.tiles, dense::kWideThreads, 0, st>>>(c);
+        return;
+      }
+    }
     if (few_rows<T>(a.m)) {
       run_vector<T, kJob>(a, st);
     } else {

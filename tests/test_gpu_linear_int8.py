@@ -73,7 +73,7 @@ SIZES = [
     (1, 1, 1), (1, 256, 256), (2, 8, 3), (3, 5, 7), (17, 33, 65), (31, 64, 32), (33, 129, 40),
     (130, 256, 520), (300, 96, 64), (257, 203, 131), (1000, 40, 24), (64, 2048, 100), (5, 5000, 17),
     (3, 131072, 5), (20011, 64, 32), (20000, 96, 160), (33001, 131, 77), (6000, 520, 1030),
-    (2049, 1024, 256), (513, 2048, 300),
+    (2049, 1024, 256), (513, 2048, 300), (4090, 1040, 3580), (16300, 1024, 900),
 ]
 
 
