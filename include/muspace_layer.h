@@ -122,8 +122,8 @@ MUSPACE_API int quantize_int8(const void *x, int dtype, int8_t *codes, float *sc
  * are codes with a scale per row, weight_scales [out] float32:
  *   z = sum of codes * scales[r] * weight_scales[o] + bias;  output = act(z) + residual
  * with sums exact in int32 and the rest in float32, rounded once; activation 0 none,
- * 1 relu, 2 gelu. in at most 2^17. The workspace (256-byte aligned) holds x's codes and
- * scales. */
+ * 1 relu, 2 gelu. in at most 2^17. The workspace (256-byte aligned; 0: none needed) holds
+ * x's codes and scales. */
 MUSPACE_API size_t linear_int8_workspace_size(int dtype, int64_t rows, int64_t in_features,
                                               int64_t out_features);
 MUSPACE_API int linear_int8_forward(const void *x, int dtype, const int8_t *weight,

@@ -87,25 +87,54 @@ void launch_product(Codes a, bool tight, hipStream_t st) {
   }
 }
 
+// So few results that workgroups of 32 x 32 are done sooner (see linear_capi's few_results).
+bool few_results(int64_t m, int64_t n) { return ceil_div(m, 64) * ceil_div(n, 64) < 120; }
+
+// Whether the product's own kernel quantises x: codes and scales are not written.
+bool few_rows(int64_t m, int64_t k) {
+  return m <= 4 && (m <= 2 ? m : 4) * padded(k) <= dense::kVectorCodes;
+}
+bool fused(int64_t m, int64_t n, int64_t k) {
+  return few_rows(m, k) || (few_results(m, n) && k <= dense::kFusedIn);
+}
+
+template <typename T, int kRows>
+void launch_vector(const Codes &a, hipStream_t st) {
+  dense::int8_vector<T, kRows><<<static_cast<int>(ceil_div(a.p.n, 16)), dense::kQuantThreads,
+                                 kRows * padded(a.p.k), st>>>(a);
+}
+
+template <typename T, bool kFused>
+void launch_few(Codes a, bool tight, hipStream_t st) {
+  constexpr int kWaves = 8;
+  a.p.tiles_n = static_cast<int>(ceil_div(a.p.n, 32));
+  a.p.tiles = static_cast<int>(ceil_div(a.p.m, 32)) * a.p.tiles_n;
+  if (tight) {
+    dense::int8_few<T, kWaves, true, kFused><<<a.p.tiles, kWaves * 64, 0, st>>>(a);
+  } else {
+    dense::int8_few<T, kWaves, false, kFused><<<a.p.tiles, kWaves * 64, 0, st>>>(a);
+  }
+}
+
 template <typename T>
 void run(Codes a, bool tight, hipStream_t st) {
-  if (tight && dense::wide_tiles(a.p.m, a.p.n, a.p.k)) {
+  if (few_rows(a.p.m, a.p.k)) {
+    if (a.p.m == 1) {
+      launch_vector<T, 1>(a, st);
+    } else if (a.p.m == 2) {
+      launch_vector<T, 2>(a, st);
+    } else {
+      launch_vector<T, 4>(a, st);
+    }
+  } else if (fused(a.p.m, a.p.n, a.p.k)) {
+    launch_few<T, true>(a, tight, st);
+  } else if (few_results(a.p.m, a.p.n)) {
+    launch_few<T, false>(a, tight, st);
+  } else if (tight && dense::wide_tiles(a.p.m, a.p.n, a.p.k)) {
     a.p.tiles_n = static_cast<int>(ceil_div(a.p.n, dense::kWide));
     a.p.tiles = static_cast<int>(ceil_div(a.p.m, dense::kWide)) * a.p.tiles_n;
     dense::wide_product<int8_t, T, dense::Job::kForward>
         <<<a.p.tiles, dense::kWideThreads, 0, st>>>(a);
-    return;
-  }
-  const int64_t small = ceil_div(a.p.m, 64) * ceil_div(a.p.n, 64);
-  if (small < 120) {
-    constexpr int kWaves = 8;
-    a.p.tiles_n = static_cast<int>(ceil_div(a.p.n, 32));
-    a.p.tiles = static_cast<int>(ceil_div(a.p.m, 32)) * a.p.tiles_n;
-    if (tight) {
-      dense::int8_few<T, kWaves, true><<<a.p.tiles, kWaves * 64, 0, st>>>(a);
-    } else {
-      dense::int8_few<T, kWaves, false><<<a.p.tiles, kWaves * 64, 0, st>>>(a);
-    }
   } else if (ceil_div(a.p.m, 128) * ceil_div(a.p.n, 128) * 2 >= 3 * kCus) {
     launch_product<T, 128>(a, tight, st);
   } else {
@@ -138,7 +167,7 @@ size_t linear_int8_workspace_size(int dtype, int64_t rows, int64_t in_features,
                                   int64_t out_features) {
   if (validate("linear_int8_workspace_size", dtype, rows, in_features, out_features) !=
           MUSPACE_OK ||
-      rows == 0 || out_features == 0) {
+      rows == 0 || out_features == 0 || fused(rows, out_features, in_features)) {
     return 0;
   }
   return pad256(static_cast<size_t>(rows) * padded(in_features)) +
@@ -162,23 +191,26 @@ int linear_int8_forward(const void *x, int dtype, const int8_t *weight, const fl
     return fail(MUSPACE_EINVAL, "%s: null tensor pointer", fn);
   }
   const size_t need = linear_int8_workspace_size(dtype, rows, in_features, out_features);
-  if (workspace == nullptr || workspace_bytes < need ||
-      reinterpret_cast<uintptr_t>(workspace) % 256 != 0) {
+  if (need > 0 && (workspace == nullptr || workspace_bytes < need ||
+                   reinterpret_cast<uintptr_t>(workspace) % 256 != 0)) {
     return fail(MUSPACE_EINVAL, "%s: needs a 256-byte aligned workspace of %zu bytes, got %zu", fn,
                 need, workspace == nullptr ? size_t{0} : workspace_bytes);
   }
   hipStream_t st = static_cast<hipStream_t>(stream);
   const int64_t ld = padded(in_features);
-  int8_t *codes = static_cast<int8_t *>(workspace);
-  float *scales = reinterpret_cast<float *>(static_cast<char *>(workspace) +
-                                            pad256(static_cast<size_t>(rows) * ld));
-  quantise(x, dtype, codes, scales, rows, in_features, ld, st);
   Codes a = {};
-  a.x = codes;
+  if (need > 0) {
+    int8_t *codes = static_cast<int8_t *>(workspace);
+    float *scales = reinterpret_cast<float *>(static_cast<char *>(workspace) +
+                                              pad256(static_cast<size_t>(rows) * ld));
+    quantise(x, dtype, codes, scales, rows, in_features, ld, st);
+    a.x = codes;
+    a.x_scales = scales;
+  }
   a.weight = weight;
-  a.x_scales = scales;
   a.weight_scales = weight_scales;
   a.ldx = ld;
+  a.p.p = x;
   a.p.m = static_cast<int>(rows);
   a.p.n = static_cast<int>(out_features);
   a.p.k = static_cast<int>(in_features);

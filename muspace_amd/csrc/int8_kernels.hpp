@@ -72,16 +72,31 @@ __device__ __forceinline__ float row_scale(uint32_t top) {
   return fmaxf(__uint_as_float(top) / 127.0f, 0x1p-126f);
 }
 
-// A piece's codes, four a word. (Codes of a row without a scale are 1: times NaN.)
+// A piece's codes, four a word. The quotient's nearest integer is that of the product with
+// the reciprocal, which errs by 3 * 2^-24 * 127 < 2^-15 at the most, but where that falls
+// as near as this to the middle of two: only then values are divided (a division takes ten
+// instructions, which was most of the kernel's time: 40000 x 256 bf16 10.9 us, now TODO).
+// Codes of a row without a scale are 1: times NaN.
 template <int kV>
-__device__ __forceinline__ void encode_row(const float (&v)[kV], float scale,
+__device__ __forceinline__ void encode_row(const float (&v)[kV], float scale, float inverse,
                                            uint32_t (&w)[kV / 4]) {
-#pragma unroll
-  for (int i = 0; i < kV / 4; ++i) w[i] = 0;
+  float q[kV], far = 0.0f;
 #pragma unroll
   for (int e = 0; e < kV; ++e) {
-    const float q = scale == scale ? rintf(v[e] / scale) : 1.0f;
-    w[e / 4] |= (static_cast<uint32_t>(static_cast<int>(q)) & 0xffu) << (8 * (e & 3));
+    const float product = v[e] * inverse;
+    q[e] = rintf(product);
+    far = fmaxf(far, fabsf(product - q[e]));
+  }
+  if (far > 0.5f - 0x1p-14f) {
+#pragma unroll
+    for (int e = 0; e < kV; ++e) q[e] = rintf(v[e] / scale);
+  }
+#pragma unroll
+  for (int i = 0; i < kV / 4; ++i) {
+    uint32_t c[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) c[e] = static_cast<uint32_t>(static_cast<int>(q[4 * i + e])) & 0xffu;
+    w[i] = scale == scale ? (c[0] | c[1] << 8) | (c[2] | c[3] << 8) << 16 : 0x01010101u;
   }
 }
 
@@ -121,7 +136,7 @@ __global__ __launch_bounds__(kQuantThreads) void int8_rows(const Quantise a) {
     const float scale = row_scale(team_top<kLanes>(top, lds));
     if (!any) continue;
     uint32_t w[kV / 4];
-    encode_row<kV>(v, scale, w);
+    encode_row<kV>(v, scale, 1.0f / scale, w);
     store_codes<kV>(a.codes + row * a.ld + col, w, a.ld - col);
     if (lane == 0) a.scales[row] = scale;
   }
@@ -146,7 +161,7 @@ __global__ __launch_bounds__(kQuantThreads) void int8_rows_long(const Quantise a
       float v[kV];
       unpack<T>(loose_load<T>(x + col, static_cast<int>(a.cols - col)), v);
       uint32_t w[kV / 4];
-      encode_row<kV>(v, scale, w);
+      encode_row<kV>(v, scale, 1.0f / scale, w);
       store_codes<kV>(a.codes + row * a.ld + col, w, a.ld - col);
     }
     if (threadIdx.x == 0) a.scales[row] = scale;
@@ -159,7 +174,7 @@ struct Codes {
   const int8_t *x, *weight;             // x [m][ldx], weight [n][k]
   const float *x_scales, *weight_scales;
   int64_t ldx;
-  Product p;                            // m, n, k, tiles and the epilogue
+  Product p;                            // m, n, k, tiles and the epilogue; p.p: x itself
 };
 
 // R rows by a step of codes, 16 bytes a chunk (see Loader). !kTight: rows of any length,
@@ -238,15 +253,14 @@ __device__ __forceinline__ i32x16 multiply_codes(const u32x4 &a, const u32x4 &b,
 #endif
 }
 
-// A chunk of the result from its integer sums. (A sum past 2^24 is rounded to float32,
+// A chunk of the result from its integer sums, of a row with scale `s`. (A sum past 2^24 is rounded to float32,
 // relative 2^-24, as the two products with the scales are.)
 template <typename T>
-__device__ __forceinline__ void finish_codes(const Codes &a, int64_t row, int col, int left,
+__device__ __forceinline__ void finish_codes(const Codes &a, float s, int64_t row, int col, int left,
                                              const int (&sum)[Piece<T>::kValues],
                                              const float (&scale)[Piece<T>::kValues],
                                              const float (&bias)[Piece<T>::kValues]) {
   constexpr int kV = Piece<T>::kValues;
-  const float s = left > 0 ? a.x_scales[row] : 0.0f;
   float z[kV];
 #pragma unroll
   for (int e = 0; e < kV; ++e) z[e] = static_cast<float>(sum[e]) * s * scale[e] + bias[e];
@@ -352,24 +366,37 @@ __global__ __launch_bounds__(kThreads, 3) void int8_product(const Codes a) {
 #pragma unroll
         for (int x = 0; x < 4; ++x) sum[e + x] = v[x];
       }
-      finish_codes<T>(a, row, col, row < a.p.m ? left : 0, sum, scale, bias);
+      finish_codes<T>(a, row < a.p.m && left > 0 ? a.x_scales[row] : 0.0f, row, col,
+                      row < a.p.m ? left : 0, sum, scale, bias);
     }
     wave_lds_sync();
   }
 }
 
 // Where the tiles would leave most CUs idle (see linear_few): 32 x 32 results a workgroup,
-// whose wavefronts take turns at the steps of k.
-template <typename T, int kWaves, bool kTight>
+// whose wavefronts take turns at the steps of k. kFused: the workgroup quantises its 32 rows
+// itself, into LDS, while the weight's first steps are on their way, in place of a launch
+// before (300 x 256 -> 256 float16: 3.1 + 4.0 us in two, TODO in one).
+constexpr int kFusedIn = 2048;  // of k at the most: 64 KB of codes
+
+template <typename T, int kWaves, bool kTight, bool kFused>
 __global__ __launch_bounds__(kWaves *kWave) void int8_few(const Codes a) {
   constexpr int kV = Piece<T>::kValues;
   constexpr int kTile = 32 * kRowBytes;
   constexpr int kLd = 36;
-  __shared__ __attribute__((aligned(16))) char lds[kWaves * 2 * kTile];
+  constexpr int kOwn = kFused ? kTile : 2 * kTile;  // of a wavefront
+  static_assert(32 * kLd * 4 <= 2 * kTile, "a wavefront's sums exceed its tiles");
+  // fused: 16 tiles of the rows' codes, then the wavefronts' tiles of the weight; the sums
+  // take the place of both
+  __shared__ __attribute__((aligned(16))) char
+      lds[kFused ? kFusedIn / kCodeStep * kTile + kWaves * kTile : kWaves * 2 * kTile];
+  __shared__ float row_scales[32];
   const int tile = xcd_order(blockIdx.x, gridDim.x);
   const int row0 = tile / a.p.tiles_n * 32, col0 = tile % a.p.tiles_n * 32;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  char *const tile_p = lds + wave * 2 * kTile, *const tile_q = tile_p + kTile;
+  char *const codes = lds;  // fused: of all steps
+  char *const tile_q =
+      kFused ? lds + kFusedIn / kCodeStep * kTile + wave * kOwn : lds + wave * kOwn + kTile;
   CodeLoader<32, true, kWave> p;
   CodeLoader<32, kTight, kWave> q;
   p.init(a.x, a.ldx, row0, a.p.m);
@@ -377,15 +404,48 @@ __global__ __launch_bounds__(kWaves *kWave) void int8_few(const Codes a) {
   i32x16 acc = {};
   int k0 = wave * kCodeStep;
   if (k0 < a.p.k) {
-    p.fetch(k0);
+    if constexpr (!kFused) p.fetch(k0);
     q.fetch(k0);
   }
+  if constexpr (kFused) {
+    // 16 threads a row: its largest magnitude, then its codes (read again, from the caches)
+    static_assert(kWaves * kWave == 32 * 16, "a row's threads are a row of lanes");
+    const int r = threadIdx.x / 16, t = threadIdx.x % 16;
+    const bool any = row0 + r < a.p.m;
+    const T *x = static_cast<const T *>(a.p.p) + static_cast<int64_t>(row0 + r) * a.p.k;
+    uint32_t top = 0;
+    for (int col = t * kV; col < a.p.k; col += 16 * kV) {
+      float v[kV];
+      unpack<T>(loose_load<T>(x + col, any ? a.p.k - col : 0), v);
+#pragma unroll
+      for (int e = 0; e < kV; ++e) top = max(top, __float_as_uint(v[e]) & 0x7fffffffu);
+    }
+    const float scale = row_scale(team_top<16>(top, nullptr)), inverse = 1.0f / scale;
+    if (t == 0) row_scales[r] = scale;
+    // zeros up to whole steps
+    const int steps_end = (a.p.k + kCodeStep - 1) / kCodeStep * kCodeStep;
+    for (int col = t * kV; col < steps_end; col += 16 * kV) {
+      float v[kV];
+      uint32_t w[kV / 4];
+      unpack<T>(loose_load<T>(x + col, any ? a.p.k - col : 0), v);
+      encode_row<kV>(v, scale, inverse, w);
+      char *to = codes + col / kCodeStep * kTile +
+                 along_offset<128>(r, col % kCodeStep / 16) + col % 16;
+      if constexpr (kV == 8) {
+        *reinterpret_cast<u32x2 *>(to) = u32x2{w[0], w[1]};
+      } else {
+        *reinterpret_cast<uint32_t *>(to) = w[0];
+      }
+    }
+    __syncthreads();
+  }
   for (; k0 < a.p.k; k0 += kWaves * kCodeStep) {
-    p.put(tile_p);
+    const char *const tile_p = kFused ? codes + k0 / kCodeStep * kTile : lds + wave * kOwn;
+    if constexpr (!kFused) p.put(lds + wave * kOwn);
     q.put(tile_q);
     wave_lds_sync();
     if (k0 + kWaves * kCodeStep < a.p.k) {
-      p.fetch(k0 + kWaves * kCodeStep);
+      if constexpr (!kFused) p.fetch(k0 + kWaves * kCodeStep);
       q.fetch(k0 + kWaves * kCodeStep);
     }
 #pragma unroll
@@ -395,7 +455,9 @@ __global__ __launch_bounds__(kWaves *kWave) void int8_few(const Codes a) {
     }
     wave_lds_sync();
   }
-  int *const sums = reinterpret_cast<int *>(tile_p);
+  if constexpr (kFused) __syncthreads();  // the codes are every wavefront's
+  constexpr int kSumBytes = 2 * kTile;
+  int *const sums = reinterpret_cast<int *>(lds + wave * kSumBytes);
 #pragma unroll
   for (int g = 0; g < 4; ++g) {
     const i32x4 v = {acc[4 * g], acc[4 * g + 1], acc[4 * g + 2], acc[4 * g + 3]};
@@ -407,17 +469,166 @@ __global__ __launch_bounds__(kWaves *kWave) void int8_few(const Codes a) {
     const int chunk = i % kLanes, r = i / kLanes;
     const int col = col0 + chunk * kV;
     const int64_t row = row0 + r;
+    const int left = row < a.p.m ? a.p.n - col : 0;
     int sum[kV] = {};
 #pragma unroll
     for (int u = 0; u < kWaves; ++u) {
-      const int *src = reinterpret_cast<const int *>(lds + u * 2 * kTile) + r * kLd + chunk * kV;
+      const int *src = reinterpret_cast<const int *>(lds + u * kSumBytes) + r * kLd + chunk * kV;
 #pragma unroll
       for (int e = 0; e < kV; ++e) sum[e] += src[e];
     }
     float scale[kV], bias[kV];
     load_columns<T>(a, col, a.p.n - col, scale, bias);
-    finish_codes<T>(a, row, col, row < a.p.m ? a.p.n - col : 0, sum, scale, bias);
+    finish_codes<T>(a, kFused ? row_scales[r] : left > 0 ? a.x_scales[row] : 0.0f, row, col, left, sum,
+                    scale, bias);
   }
+}
+
+// ------------------------------------------------------------ a row or a few ---
+
+// Lane l's sum over the wavefront's lanes (as add_across).
+__device__ __forceinline__ int sum_lanes(int v) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  v += __builtin_amdgcn_mov_dpp(v, 0xB1, 0xf, 0xf, true);
+  v += __builtin_amdgcn_mov_dpp(v, 0x4E, 0xf, 0xf, true);
+  v += __builtin_amdgcn_mov_dpp(v, 0x141, 0xf, 0xf, true);
+  v += __builtin_amdgcn_mov_dpp(v, 0x140, 0xf, 0xf, true);
+  u32x2 r = __builtin_bit_cast(u32x2, __builtin_amdgcn_permlane16_swap(v, v, false, false));
+  v = static_cast<int>(r[0] + r[1]);
+  r = __builtin_bit_cast(u32x2, __builtin_amdgcn_permlane32_swap(v, v, false, false));
+  v = static_cast<int>(r[0] + r[1]);
+#endif
+  return v;
+}
+
+__device__ __forceinline__ int dot_codes(const u32x4 &a, const u32x4 &b, int sum) {
+#if defined(__HIP_DEVICE_COMPILE__)
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    sum = __builtin_amdgcn_sdot4(static_cast<int>(a[i]), static_cast<int>(b[i]), sum, false);
+  }
+#endif
+  return sum;
+}
+
+// Up to kRows rows: reading the weight is all of it, as in linear_vector. A workgroup of
+// eight wavefronts makes 16 columns, two a wavefront; it quantises the rows itself while the
+// weight's first chunks are on their way.
+constexpr int kVectorCodes = 48 << 10;  // of the rows, in LDS, at the most
+
+template <typename T, int kRows>
+__global__ __launch_bounds__(kQuantThreads) void int8_vector(const Codes a) {
+  constexpr int kV = Piece<T>::kValues;
+  constexpr int kCols = 2, kAcross = 16;
+  constexpr int kAhead = 4;                // of a lane's chunks, in flight together
+  constexpr int kSpan = kWave * 16;        // of k, a chunk a lane
+  constexpr int kLanes = kAcross / kV;     // of a result row, at the end
+  static_assert(kRows * kLanes <= kWave, "one wavefront ends it");
+  extern __shared__ __attribute__((aligned(16))) char codes[];  // [kRows][pad16(k)]
+  __shared__ uint32_t tops[kQuantThreads / kWave];
+  __shared__ int sums[kRows][kAcross];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int first = blockIdx.x * kAcross, col0 = first + wave * kCols;
+  const int k = a.p.k, padded = (k + 15) & ~15;
+  const int8_t *w[kCols];
+#pragma unroll
+  for (int c = 0; c < kCols; ++c) {
+    w[c] = a.weight + static_cast<int64_t>(min(col0 + c, a.p.n - 1)) * k;
+  }
+  // the lane's chunk at `at`; one that passes the end as the row's last 16 bytes, moved
+  auto load = [&](int at, u32x4(&v)[kCols]) {
+    if (k >= 16) {
+      const int from = min(at, k - 16), skip = at - from;
+#pragma unroll
+      for (int c = 0; c < kCols; ++c) {
+        v[c] = reinterpret_cast<const Bytes16 *>(w[c] + from)->v;
+        if (skip > 0) v[c] = drop_front<int8_t>(v[c], min(skip, 16));
+      }
+    } else {
+#pragma unroll
+      for (int c = 0; c < kCols; ++c) {
+        v[c] = u32x4{0, 0, 0, 0};
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          if (at + e < k) {
+            v[c][e / 4] |= static_cast<uint32_t>(static_cast<uint8_t>(w[c][at + e])) << (8 * (e & 3));
+          }
+        }
+      }
+    }
+  };
+  u32x4 wv[kAhead][kCols];
+#pragma unroll
+  for (int i = 0; i < kAhead; ++i) {
+    if (i * kSpan < k) load(i * kSpan + lane * 16, wv[i]);
+  }
+  float scales[kRows];
+#pragma unroll
+  for (int m = 0; m < kRows; ++m) {
+    const T *x = static_cast<const T *>(a.p.p) + static_cast<int64_t>(min(m, a.p.m - 1)) * k;
+    uint32_t top = 0;
+    for (int col = threadIdx.x * kV; col < k; col += kQuantThreads * kV) {
+      float v[kV];
+      unpack<T>(loose_load<T>(x + col, k - col), v);
+#pragma unroll
+      for (int e = 0; e < kV; ++e) top = max(top, __float_as_uint(v[e]) & 0x7fffffffu);
+    }
+    const float scale = row_scale(team_top<kQuantThreads>(top, tops)), inverse = 1.0f / scale;
+    scales[m] = scale;
+    for (int col = threadIdx.x * kV; col < padded; col += kQuantThreads * kV) {
+      float v[kV];
+      uint32_t c[kV / 4];
+      unpack<T>(loose_load<T>(x + col, k - col), v);
+      encode_row<kV>(v, scale, inverse, c);
+      char *to = codes + m * padded + col;
+      if constexpr (kV == 8) {
+        *reinterpret_cast<u32x2 *>(to) = u32x2{c[0], c[1]};
+      } else {
+        *reinterpret_cast<uint32_t *>(to) = c[0];
+      }
+    }
+  }
+  __syncthreads();
+  int sum[kRows][kCols] = {};
+  for (int k0 = 0; k0 < k; k0 += kAhead * kSpan) {
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      const int at = k0 + i * kSpan + lane * 16;
+      if (at < k) {
+#pragma unroll
+        for (int m = 0; m < kRows; ++m) {
+          const u32x4 x = *reinterpret_cast<const u32x4 *>(codes + m * padded + at);
+#pragma unroll
+          for (int c = 0; c < kCols; ++c) sum[m][c] = dot_codes(wv[i][c], x, sum[m][c]);
+        }
+      }
+    }
+    if (k0 + kAhead * kSpan < k) {
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) load(k0 + (kAhead + i) * kSpan + lane * 16, wv[i]);
+    }
+  }
+#pragma unroll
+  for (int m = 0; m < kRows; ++m) {
+#pragma unroll
+    for (int c = 0; c < kCols; ++c) {
+      const int v = sum_lanes(sum[m][c]);
+      if (lane == 0) sums[m][wave * kCols + c] = v;
+    }
+  }
+  __syncthreads();
+  if (wave != 0) return;
+  const int row = lane / kLanes, chunk = lane % kLanes, col = first + chunk * kV;
+  const int left = row < min(kRows, a.p.m) ? a.p.n - col : 0;
+  int mine[kV];
+  float s = scales[0];
+#pragma unroll
+  for (int m = 1; m < kRows; ++m) s = row == m ? scales[m] : s;
+#pragma unroll
+  for (int e = 0; e < kV; ++e) mine[e] = sums[min(row, kRows - 1)][chunk * kV + e];
+  float scale[kV], bias[kV];
+  load_columns<T>(a, col, a.p.n - col, scale, bias);
+  finish_codes<T>(a, s, row, col, left, mine, scale, bias);
 }
 
 }  // namespace dense

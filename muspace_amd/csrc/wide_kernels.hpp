@@ -223,7 +223,7 @@ __global__ __launch_bounds__(kWideThreads, 2) void wide_product(const Codes a) {
         for (int x = 0; x < 4; ++x) z[e + x] = v[x];
       }
       if constexpr (kInt) {
-        finish_codes<Out>(a, row, col, here, z, scale, bias);
+        finish_codes<Out>(a, here > 0 ? a.x_scales[row] : 0.0f, row, col, here, z, scale, bias);
       } else {
         float u[kV];
 #pragma unroll

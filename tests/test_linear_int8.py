@@ -180,8 +180,8 @@ FAR = 1 << 12
     ],
 )
 def test_forward_abi_refuses(native_lib, overrides, code, message):
-    args = dict(x=FAR, dtype=0, weight=FAR, scales=FAR, bias=None, residual=None, output=FAR, rows=4,
-                inner=8, outer=8, activation=0, workspace=FAR, nbytes=1 << 20, stream=None)
+    args = dict(x=FAR, dtype=0, weight=FAR, scales=FAR, bias=None, residual=None, output=FAR,
+                rows=5, inner=2064, outer=8, activation=0, workspace=FAR, nbytes=1 << 20, stream=None)
     args.update(overrides)
     assert native_lib.raw("linear_int8_forward")(*args.values()) == code
     assert message in native_lib.last_error()
@@ -203,4 +203,7 @@ def test_abi_without_work_and_workspace(native_lib):
     size = native_lib.raw("linear_int8_workspace_size")
     assert size(7, 4, 8, 8) == size(0, 0, 8, 8) == 0
     # codes in rows of whole 16 bytes, then a scale a row
-    assert size(2, 100, 40, 8) == 4864 + 512
+    assert size(2, 100, 2050, 8) == 206592 + 512
+    # few rows and few results are quantised where they are multiplied
+    assert size(2, 4, 12288, 4096) == size(2, 1, 49152, 4096) == size(2, 300, 256, 256) == 0
+    assert size(2, 4, 12289, 4096) > 0 and size(2, 40000, 256, 512) > 0
