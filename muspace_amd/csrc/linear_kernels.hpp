@@ -995,10 +995,12 @@ __global__ __launch_bounds__(8 / kCols *kWave) void linear_vector(const Product 
     }
   };
   int k0 = lane * kV;
-  for (; k0 - lane * kV + kAhead * kSpan <= a.k; k0 += kAhead * kSpan) {
-    u32x4 wv[kAhead][kW], xv[kAhead][kRows];
+  // `kCount` whole spans
+  auto spans = [&](auto count) {
+    constexpr int kCount = decltype(count)::value;
+    u32x4 wv[kCount][kW], xv[kCount][kRows];
 #pragma unroll
-    for (int i = 0; i < kAhead; ++i) {
+    for (int i = 0; i < kCount; ++i) {
       const int k = k0 + i * kSpan;
 #pragma unroll
       for (int c = 0; c < kW; ++c) wv[i][c] = reinterpret_cast<const Loose16 *>(w[c] + k)->v;
@@ -1006,8 +1008,12 @@ __global__ __launch_bounds__(8 / kCols *kWave) void linear_vector(const Product 
       for (int m = 0; m < kRows; ++m) xv[i][m] = reinterpret_cast<const Loose16 *>(x[m] + k)->v;
     }
 #pragma unroll
-    for (int i = 0; i < kAhead; ++i) add(wv[i], xv[i], 0);
-  }
+    for (int i = 0; i < kCount; ++i) add(wv[i], xv[i], 0);
+    k0 += kCount * kSpan;
+  };
+  while (k0 - lane * kV + kAhead * kSpan <= a.k) spans(std::integral_constant<int, kAhead>{});
+  // (a row of two spans would take them one after the other: gated, 1024 -> 2 x 4096 bf16 TODO)
+  if (k0 - lane * kV + 2 * kSpan <= a.k) spans(std::integral_constant<int, 2>{});
   for (; k0 < a.k; k0 += kSpan) {
     u32x4 wv[kW], xv[kRows];
     if (a.k >= kV) {

@@ -71,11 +71,24 @@ __device__ __forceinline__ float inside(float v, int e, int left) {
 // 512 pieces. Short rows share a wavefront, long ones take several and join their sums
 // in LDS.
 constexpr int kRowThreads = 512;
-constexpr int kTeamLds = 2 * (kRowThreads / kWave);  // floats of team_sum
+constexpr int kTeamLds = 2 * (kRowThreads / kWave);  // floats of a Meeting's turn
+
+// Where wavefronts that share rows meet: two turns of LDS, taken one after the other, so
+// that a turn's readers are done when its next writers have passed the barrier between, and
+// one barrier a meeting is enough.
+struct Meeting {
+  float *lds;
+  int turn;
+
+  __device__ __forceinline__ float *next() {
+    turn ^= kTeamLds;
+    return lds + turn;
+  }
+};
 
 // kLanes lanes' sums, the same on all of them (every thread of the workgroup calls it)
 template <int kLanes, int N>
-__device__ __forceinline__ void team_sum(float (&v)[N], float *lds) {
+__device__ __forceinline__ void team_sum(float (&v)[N], Meeting &meet) {
 #pragma unroll
   for (int i = 0; i < N; ++i) {
     v[i] = add_across<8>(add_across<4>(add_across<2>(add_across<1>(v[i]))));
@@ -84,7 +97,7 @@ __device__ __forceinline__ void team_sum(float (&v)[N], float *lds) {
   }
   if constexpr (kLanes > kWave) {
     const int wave = threadIdx.x / kWave, first = threadIdx.x / kLanes * (kLanes / kWave);
-    __syncthreads();
+    float *lds = meet.next();
     if (threadIdx.x % kWave == 0) {
 #pragma unroll
       for (int i = 0; i < N; ++i) lds[wave * N + i] = v[i];
@@ -101,11 +114,11 @@ __device__ __forceinline__ void team_sum(float (&v)[N], float *lds) {
 
 // a row's first value, on all of its lanes
 template <int kLanes>
-__device__ __forceinline__ float first_value(float v, float *lds) {
+__device__ __forceinline__ float first_value(float v, Meeting &meet) {
   if constexpr (kLanes <= kWave) {
     return __shfl(v, 0, kLanes);
   } else {
-    __syncthreads();
+    float *lds = meet.next();
     if (threadIdx.x % kLanes == 0) lds[threadIdx.x / kLanes] = v;
     __syncthreads();
     return lds[threadIdx.x / kLanes];
@@ -121,19 +134,20 @@ __device__ __forceinline__ float unit_of(float x, const f32x4 &stats) {
   return (x - stats[0] - stats[1]) * stats[2];
 }
 
-// Centre and factor of a row in registers. `v` keeps its values; `x0` is the first.
+// Centre and factor of a row in registers. `v` keeps its values.
 template <int kLanes, bool kFull, int kV>
-__device__ __forceinline__ float row_statistics(const float (&v)[kV], int cols, int lane,
-                                                float x0, int norm, float inv, float eps,
-                                                float *lds, Centre &centre) {
+__device__ __forceinline__ float row_statistics(const float (&v)[kV], int cols, int lane, int norm,
+                                                float inv, float eps, Meeting &meet,
+                                                Centre &centre) {
   float sums[2] = {0.0f, 0.0f};
   centre = Centre{0.0f, 0.0f};
   if (norm == kLayerNorm) {
+    const float x0 = first_value<kLanes>(v[0], meet);
     float sum[1] = {0.0f};
     const int left = cols - lane * kV;
 #pragma unroll
     for (int e = 0; e < kV; ++e) sum[0] += inside<kFull>(v[e] - x0, e, left);
-    team_sum<kLanes, 1>(sum, lds);
+    team_sum<kLanes, 1>(sum, meet);
     centre = find_centre(x0, sum[0] * inv);
   }
   const int left = cols - lane * kV;
@@ -143,7 +157,7 @@ __device__ __forceinline__ float row_statistics(const float (&v)[kV], int cols, 
     sums[0] += c;
     sums[1] += c * c;
   }
-  team_sum<kLanes, 2>(sums, lds);
+  team_sum<kLanes, 2>(sums, meet);
   if (norm == kRmsNorm) return 1.0f / sqrtf(sums[1] * inv + eps);
   return correct_centre(centre, sums, inv, eps);
 }
@@ -153,7 +167,8 @@ __global__ __launch_bounds__(kRowThreads) void residual_forward(const Residual a
   constexpr int kGroups = kRowThreads / kLanes;  // rows at a time
   constexpr int kV = Piece<T>::kValues;
   using Pieces = RowPieces<T, kLanes, 1, kFull>;
-  __shared__ float lds[kTeamLds];
+  __shared__ float lds[2 * kTeamLds];
+  Meeting meet = {lds, 0};
   const int lane = threadIdx.x % kLanes;
   const T *block = static_cast<const T *>(a.block), *residual = static_cast<const T *>(a.residual);
   const float inv = 1.0f / static_cast<float>(a.cols);
@@ -183,9 +198,8 @@ __global__ __launch_bounds__(kRowThreads) void residual_forward(const Residual a
     next_r.load(residual, row + step, a.rows, a.cols, lane);
     Centre centre;
     if constexpr (kPost) {
-      const float x0 = first_value<kLanes>(y[0], lds);
-      const float s = row_statistics<kLanes, kFull>(y, a.cols, lane, x0, a.post, inv, a.eps, lds,
-                                                    centre);
+      const float s =
+          row_statistics<kLanes, kFull>(y, a.cols, lane, a.post, inv, a.eps, meet, centre);
       if (a.post_stats != nullptr && any && lane == 0) {
         keep_statistics(a.post_stats, row, centre, s);
       }
@@ -204,9 +218,7 @@ __global__ __launch_bounds__(kRowThreads) void residual_forward(const Residual a
     if (a.stream != nullptr) {
       loose_store(static_cast<T *>(a.stream) + row * a.cols + col, pack<T>(v), any ? left : 0);
     }
-    const float x0 = first_value<kLanes>(v[0], lds);
-    const float s = row_statistics<kLanes, kFull>(v, a.cols, lane, x0, a.norm, inv, a.eps, lds,
-                                                  centre);
+    const float s = row_statistics<kLanes, kFull>(v, a.cols, lane, a.norm, inv, a.eps, meet, centre);
     if (a.stats != nullptr && any && lane == 0) keep_statistics(a.stats, row, centre, s);
 #pragma unroll
     for (int e = 0; e < kV; ++e) {
@@ -226,7 +238,8 @@ __global__ __launch_bounds__(kRowThreads) void residual_backward(const Residual 
   constexpr int kMine = kBlock ? kSums : 2;
   constexpr bool kSum = sizeof(T) == 2;  // the stream is summed again
   using Pieces = RowPieces<T, kLanes, 1, kFull>;
-  __shared__ float lds[kGroups > 1 ? kGroups * kCols : kTeamLds];
+  __shared__ float lds[kGroups > 1 ? kGroups * kCols : 2 * kTeamLds];
+  Meeting meet = {lds, 0};
   const int lane = threadIdx.x % kLanes, group = threadIdx.x / kLanes;
   const T *stream = static_cast<const T *>(kSum ? a.residual : a.stream_in);
   const T *block = static_cast<const T *>(a.block);
@@ -292,7 +305,7 @@ __global__ __launch_bounds__(kRowThreads) void residual_backward(const Residual 
     // (without a gradient of the output both are zero, and rows that have no statistics
     // to speak of, of infinities, do not reach the stream's gradient)
     if (go != nullptr) {
-      team_sum<kLanes, 2>(along, lds);
+      team_sum<kLanes, 2>(along, meet);
       const float mu = a.norm == kLayerNorm ? along[0] * inv : 0.0f, mh = along[1] * inv;
 #pragma unroll
       for (int e = 0; e < kV; ++e) ds[e] += stats[2] * (u[e] - mu - h[e] * mh);
@@ -324,7 +337,7 @@ __global__ __launch_bounds__(kRowThreads) void residual_backward(const Residual 
     if (a.d_block == nullptr) continue;
     if constexpr (kBlock) {
       if (a.post != kNoNorm) {
-        team_sum<kLanes, 2>(across, lds);
+        team_sum<kLanes, 2>(across, meet);
         const float mv = a.post == kLayerNorm ? across[0] * inv : 0.0f, mh = across[1] * inv;
 #pragma unroll
         for (int e = 0; e < kV; ++e) ds[e] = post[2] * (ds[e] - mv - unit[e] * mh);
@@ -365,7 +378,6 @@ __global__ __launch_bounds__(kRowThreads) void residual_backward(const Residual 
 
 // A workgroup per row, its values computed from memory in every pass over it.
 constexpr int kLongThreads = 256;
-constexpr int kLongLds = 2 * (kLongThreads / kWave);  // floats of team_sum
 
 template <typename T, typename F>
 __device__ __forceinline__ void over_row(int cols, F &&f) {
@@ -376,7 +388,7 @@ __device__ __forceinline__ void over_row(int cols, F &&f) {
 // Centre and factor of a row whose pieces `values(col, left, v)` gives.
 template <typename T, typename F>
 __device__ __forceinline__ float long_statistics(int cols, float x0, int norm, float inv, float eps,
-                                                 float *lds, Centre &centre, F &&values) {
+                                                 Meeting &meet, Centre &centre, F &&values) {
   constexpr int kV = Piece<T>::kValues;
   float sums[2] = {0.0f, 0.0f};
   centre = Centre{0.0f, 0.0f};
@@ -388,7 +400,7 @@ __device__ __forceinline__ float long_statistics(int cols, float x0, int norm, f
 #pragma unroll
       for (int e = 0; e < kV; ++e) sum[0] += e < left ? v[e] - x0 : 0.0f;
     });
-    team_sum<kLongThreads, 1>(sum, lds);
+    team_sum<kLongThreads, 1>(sum, meet);
     centre = find_centre(x0, sum[0] * inv);
   }
   over_row<T>(cols, [&](int col, int left) {
@@ -401,7 +413,7 @@ __device__ __forceinline__ float long_statistics(int cols, float x0, int norm, f
       sums[1] += c * c;
     }
   });
-  team_sum<kLongThreads, 2>(sums, lds);
+  team_sum<kLongThreads, 2>(sums, meet);
   if (norm == kRmsNorm) return 1.0f / sqrtf(sums[1] * inv + eps);
   return correct_centre(centre, sums, inv, eps);
 }
@@ -495,7 +507,8 @@ struct LongRow {
 template <typename T>
 __global__ __launch_bounds__(kLongThreads) void residual_forward_long(const Residual a) {
   constexpr int kV = Piece<T>::kValues;
-  __shared__ float lds[kLongLds];
+  __shared__ float lds[2 * kTeamLds];
+  Meeting meet = {lds, 0};
   const float inv = 1.0f / static_cast<float>(a.cols);
   const uint64_t seed = seed_of(a.drop);
   for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
@@ -504,7 +517,7 @@ __global__ __launch_bounds__(kLongThreads) void residual_forward_long(const Resi
     r.post = f32x4{0.0f, 0.0f, 1.0f, 0.0f};
     Centre centre;
     if (a.post != kNoNorm) {
-      const float s = long_statistics<T>(a.cols, to_float(block[0]), a.post, inv, a.eps, lds,
+      const float s = long_statistics<T>(a.cols, to_float(block[0]), a.post, inv, a.eps, meet,
                                          centre, [&](int col, int left, float(&v)[kV]) {
                                            unpack<T>(loose_load<T>(block + col, left), v);
                                          });
@@ -516,8 +529,8 @@ __global__ __launch_bounds__(kLongThreads) void residual_forward_long(const Resi
     auto stream = [&](int col, int left, float(&v)[kV]) { r.stream(a, seed, row, col, left, v); };
     float v0[kV] = {};
     if (threadIdx.x == 0) stream(0, a.cols, v0);
-    const float x0 = first_value<kLongThreads>(v0[0], lds);
-    const float s = long_statistics<T>(a.cols, x0, a.norm, inv, a.eps, lds, centre, stream);
+    const float x0 = first_value<kLongThreads>(v0[0], meet);
+    const float s = long_statistics<T>(a.cols, x0, a.norm, inv, a.eps, meet, centre, stream);
     if (a.stats != nullptr && threadIdx.x == 0) keep_statistics(a.stats, row, centre, s);
     over_row<T>(a.cols, [&](int col, int left) {
       float v[kV], w[kV], b[kV];
@@ -539,7 +552,8 @@ __global__ __launch_bounds__(kLongThreads) void residual_forward_long(const Resi
 template <typename T>
 __global__ __launch_bounds__(kLongThreads) void residual_backward_long(const Residual a) {
   constexpr int kV = Piece<T>::kValues;
-  __shared__ float lds[kLongLds];
+  __shared__ float lds[2 * kTeamLds];
+  Meeting meet = {lds, 0};
   const float inv = 1.0f / static_cast<float>(a.cols);
   const uint64_t seed = seed_of(a.drop);
   for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
@@ -557,7 +571,7 @@ __global__ __launch_bounds__(kLongThreads) void residual_backward_long(const Res
           mean[1] += g[e] * w[e] * h[e];
         }
       });
-      team_sum<kLongThreads, 2>(mean, lds);
+      team_sum<kLongThreads, 2>(mean, meet);
       mean[0] = a.norm == kLayerNorm ? mean[0] * inv : 0.0f;
       mean[1] *= inv;
     }
@@ -587,7 +601,7 @@ __global__ __launch_bounds__(kLongThreads) void residual_backward_long(const Res
           mean_p[1] += dy[e] * unit[e];
         }
       });
-      team_sum<kLongThreads, 2>(mean_p, lds);
+      team_sum<kLongThreads, 2>(mean_p, meet);
       mean_p[0] = a.post == kLayerNorm ? mean_p[0] * inv : 0.0f;
       mean_p[1] *= inv;
     }

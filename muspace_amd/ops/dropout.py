@@ -26,6 +26,8 @@ _MASK32 = 0xFFFFFFFF
 def seed_arguments(seed, offset, p):
     """(seed tensor or None, seed, offset) as the host module takes them; a call without
     dropout needs no seed. ValueError or TypeError for others."""
+    if p == 0.0 and seed is None and offset == 0:  # a call without dropout
+        return None, 0, 0
     if not 0.0 <= p <= 1.0:
         raise ValueError(f"the dropout probability must be in [0, 1], got {p}")
     if not isinstance(offset, int) or not 0 <= offset < 1 << 64:
