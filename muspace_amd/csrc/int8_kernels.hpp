@@ -75,7 +75,7 @@ __device__ __forceinline__ float row_scale(uint32_t top) {
 // A piece's codes, four a word. The quotient's nearest integer is that of the product with
 // the reciprocal, which errs by 3 * 2^-24 * 127 < 2^-15 at the most, but where that falls
 // as near as this to the middle of two: only then values are divided (a division takes ten
-// instructions, which was most of the kernel's time: 40000 x 256 bf16 10.9 us, now TODO).
+// instructions: 40000 x 256 bf16 10.9 us with it, 10.3 without).
 // Codes of a row without a scale are 1: times NaN.
 template <int kV>
 __device__ __forceinline__ void encode_row(const float (&v)[kV], float scale, float inverse,
@@ -376,7 +376,7 @@ __global__ __launch_bounds__(kThreads, 3) void int8_product(const Codes a) {
 // Where the tiles would leave most CUs idle (see linear_few): 32 x 32 results a workgroup,
 // whose wavefronts take turns at the steps of k. kFused: the workgroup quantises its 32 rows
 // itself, into LDS, while the weight's first steps are on their way, in place of a launch
-// before (300 x 256 -> 256 float16: 3.1 + 4.0 us in two, TODO in one).
+// before (300 x 256 -> 256 float16: 3.1 + 4.0 us in two, 5.5 in one).
 constexpr int kFusedIn = 2048;  // of k at the most: 64 KB of codes
 
 template <typename T, int kWaves, bool kTight, bool kFused>

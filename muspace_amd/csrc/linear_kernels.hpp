@@ -1012,7 +1012,8 @@ __global__ __launch_bounds__(8 / kCols *kWave) void linear_vector(const Product 
     k0 += kCount * kSpan;
   };
   while (k0 - lane * kV + kAhead * kSpan <= a.k) spans(std::integral_constant<int, kAhead>{});
-  // (a row of two spans would take them one after the other: gated, 1024 -> 2 x 4096 bf16 TODO)
+  // (a row of two spans would take them one after the other: gated, 1024 -> 2 x 4096 bf16 6.2 us,
+  // so 5.9)
   if (k0 - lane * kV + 2 * kSpan <= a.k) spans(std::integral_constant<int, 2>{});
   for (; k0 < a.k; k0 += kSpan) {
     u32x4 wv[kW], xv[kRows];

@@ -88,21 +88,21 @@ int validate(const char *fn, int dtype, int weight_dtype, int64_t rows, int64_t 
 // Lanes that share a row, a 16-byte piece each: the least that hold it; 0: longer rows.
 int plan_lanes(int dtype, int64_t cols) {
   const int64_t n = ceil_div(cols, dtype == 0 ? 4 : 8);
-  for (int lanes = 16; lanes <= dense::kRowThreads; lanes *= 2) {
+  for (int lanes = 16; lanes <= dense::kMaxLanes; lanes *= 2) {
     if (n <= lanes) return lanes;
   }
   return 0;
 }
 
 int forward_blocks(int lanes, int64_t rows) {
-  const int64_t want = ceil_div(rows, lanes == 0 ? 1 : dense::kRowThreads / lanes);
-  return static_cast<int>(want < 2048 ? want : 2048);
+  const int64_t want = ceil_div(rows, lanes == 0 ? 1 : dense::row_threads(lanes) / lanes);
+  return static_cast<int>(want < 4096 ? want : 4096);
 }
 
 // Workgroups of the backward; each leaves a row of every column sum.
 int backward_blocks(int lanes, int64_t rows) {
   if (lanes == 0) return static_cast<int>(rows < 64 ? rows : 64);
-  const int64_t want = ceil_div(rows, dense::kRowThreads / lanes);
+  const int64_t want = ceil_div(rows, dense::row_threads(lanes) / lanes);
   return static_cast<int>(want < 512 ? want : 512);
 }
 
@@ -113,7 +113,7 @@ size_t row_bytes(int lanes, int64_t rows) {
 
 template <typename T, int kLanes, bool kFull, bool kBackward>
 void launch_rows(const Residual &a, int blocks, bool block, hipStream_t st) {
-  constexpr int kThreads = dense::kRowThreads;
+  constexpr int kThreads = dense::row_threads(kLanes);
   if constexpr (kBackward) {
     if (block) {
       dense::residual_backward<T, kLanes, kFull, true><<<blocks, kThreads, 0, st>>>(a);
@@ -131,7 +131,7 @@ void launch_rows(const Residual &a, int blocks, bool block, hipStream_t st) {
 template <typename T, bool kBackward, int kLanes = 16>
 void launch(int lanes, const Residual &a, int blocks, bool block, hipStream_t st) {
   if (lanes != kLanes) {
-    if constexpr (kLanes < dense::kRowThreads) {
+    if constexpr (kLanes < dense::kMaxLanes) {
       launch<T, kBackward, kLanes * 2>(lanes, a, blocks, block, st);
     }
   } else if (a.cols == kLanes * dense::Piece<T>::kValues) {

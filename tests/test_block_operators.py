@@ -387,5 +387,5 @@ def test_residual_norm_abi_without_work_is_a_no_op(native_lib):
     assert native_lib.raw("residual_norm_backward")(*backward_args(**none)) == 0
     size = native_lib.raw("residual_norm_backward_workspace_size")
     assert size(2, 100, 64, 0) == size(7, 100, 64, 2) == 0
-    # 8 pieces a row: 16 lanes, 32 rows a workgroup, 4 workgroups
-    assert size(2, 100, 64, 3) == 4 * 3 * 64 * 4
+    # 8 pieces a row: 16 lanes, 16 rows a workgroup, 7 workgroups
+    assert size(2, 100, 64, 3) == 7 * 3 * 64 * 4
