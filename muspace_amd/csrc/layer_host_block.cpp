@@ -346,8 +346,8 @@ bool residual_fits(const Tensor &block, const Tensor &residual,
                    const OptTensor &seed) {
   const at::ScalarType type = block.scalar_type();
   if (!supported(type) || block.dim() == 0 || residual.scalar_type() != type ||
-      residual.sizes() != block.sizes() || !(n.eps >= 0.0) || !std::isfinite(n.scale) ||
-      !drop_fits(p, seed)) {
+      residual.sizes() != block.sizes() || !(n.eps >= 0.0) ||
+      !std::isfinite(static_cast<float>(n.scale)) || !drop_fits(p, seed)) {
     return false;
   }
   OptTensor first;

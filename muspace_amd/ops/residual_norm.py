@@ -19,8 +19,6 @@ No reference counterpart: the reference leaves these steps to torch.
 
 from __future__ import annotations
 
-import math
-
 import torch
 import torch.nn.functional as F
 
@@ -77,8 +75,8 @@ def _validate(block, residual, vectors, norm, eps, post_norm, residual_scale, se
         raise ValueError(f"post_norm must be None, 'layer' or 'rms', got {post_norm!r}")
     if not eps >= 0.0:
         raise ValueError(f"eps must not be negative, got {eps}")
-    if not math.isfinite(residual_scale):
-        raise ValueError(f"residual_scale must be finite, got {residual_scale}")
+    if not abs(residual_scale) <= torch.finfo(torch.float32).max:
+        raise ValueError(f"residual_scale must be a finite float32 number, got {residual_scale}")
     validate_seed(seed, block)
     given = {name: tensor for name, tensor in vectors.items() if tensor is not None}
     for name, tensor in given.items():

@@ -231,6 +231,8 @@ def test_dropout_refuses(change, error, message):
         ({"eps": -1.0}, ValueError, "eps"),
         ({"eps": math.nan}, ValueError, "eps"),
         ({"residual_scale": math.inf}, ValueError, "residual_scale"),
+        ({"residual_scale": 1e300}, ValueError, "residual_scale"),
+        ({"residual_scale": math.nan}, ValueError, "residual_scale"),
         ({"dropout_p": 2.0}, ValueError, "probability"),
         ({"dropout_p": 0.1, "seed": None}, ValueError, "seed must be"),
         ({"seed": torch.zeros(1)}, TypeError, "seed tensor"),

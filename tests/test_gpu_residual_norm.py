@@ -189,6 +189,27 @@ def test_gradients_of_one_output(cols):
     assert torch.equal(got["block"], gs) and torch.equal(got["residual"], gs)
 
 
+def test_one_tensor_as_block_and_residual():
+    """Gradients of both add up, and gradients that are one result are not one tensor."""
+    t, g, gs = make(60, 256, torch.float32, names=("weight", "bias"))
+    for kwargs in ({}, {"dropout_p": 0.3, "seed": 2}, {"residual_scale": 0.5}):
+        a, b = (t["block"].clone().requires_grad_() for _ in range(2))
+        torch.autograd.backward(residual_norm(a, b, t["weight"], t["bias"], **kwargs), [g, gs])
+        x = t["block"].clone().requires_grad_()
+        torch.autograd.backward(residual_norm(x, x, t["weight"], t["bias"], **kwargs), [g, gs])
+        assert torch.equal(x.grad, a.grad + b.grad)
+        kept = b.grad.clone()
+        a.grad.zero_()
+        assert torch.equal(b.grad, kept)
+
+
+@pytest.mark.parametrize("scale", [1e300, -math.inf])
+def test_residual_scale_is_a_float32_number(scale):
+    t, _, _ = make(4, 8, torch.float32, names=())
+    with pytest.raises(ValueError, match="residual_scale must be a finite float32"):
+        residual_norm(**t, residual_scale=scale)
+
+
 def test_single_gradients_and_repeats():
     t, g, gs = make(9000, 200, torch.bfloat16)
 
