@@ -2,9 +2,10 @@
 
 Replaces the reference's ``mcc`` + TVM-FFI AOT build
 (/root/reference/native_build.py:27-65, sources listed in
-/root/reference/build_utils.py:12-30) with one ``hipcc`` invocation over the
-HIP sources in ``muspace_amd/csrc``. The library is built in-tree so that it
-travels with the source tree; ``python -m muspace_amd.build`` rebuilds it.
+/root/reference/build_utils.py:12-30) with one ``hipcc`` invocation for each of the
+HIP sources in ``muspace_amd/csrc``, side by side, and one that links them. The
+library is built in-tree so that it travels with the source tree; ``python -m
+muspace_amd.build`` rebuilds it.
 """
 
 from __future__ import annotations
@@ -14,6 +15,8 @@ import shutil
 import subprocess
 import sys
 import sysconfig
+import tempfile
+from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
 PACKAGE_DIR = Path(__file__).resolve().parent
@@ -87,8 +90,8 @@ def hipcc() -> str:
     raise FileNotFoundError("hipcc not found; ROCm is required to build libmuspace_msda.so")
 
 
-def build_command(output: Path, sources=SOURCES) -> list[str]:
-    return [hipcc(), *HIPCC_FLAGS, *(str(s) for s in sources), "-o", str(output)]
+def build_command(output: Path, sources=SOURCES, extra=()) -> list[str]:
+    return [hipcc(), *HIPCC_FLAGS, *extra, *(str(s) for s in sources), "-o", str(output)]
 
 
 def host_command(output: Path) -> list[str]:
@@ -128,12 +131,26 @@ def _compile(library: Path, command, verbose: bool) -> Path:
     return library
 
 
+def _compile_library(library: Path, sources, verbose: bool) -> Path:
+    """``library`` from objects of its ``sources``, which are compiled side by side."""
+    library.parent.mkdir(parents=True, exist_ok=True)
+    with tempfile.TemporaryDirectory(dir=library.parent, prefix="objects") as folder:
+        objects = [Path(folder) / f"{source.stem}.o" for source in sources]
+
+        def compile_one(source, target):
+            return _compile(target, lambda out: build_command(out, (source,), ("-c",)), verbose)
+
+        with ThreadPoolExecutor(max_workers=min(8, os.cpu_count() or 1)) as pool:
+            list(pool.map(compile_one, sources, objects))
+        return _compile(library, lambda out: build_command(out, objects), verbose)
+
+
 def build(verbose: bool = False) -> Path:
     """Compile the MSDA library, the probe library and the host module (always), each
     moved into place atomically; returns the MSDA library's path. The host module comes
     last: without a C++ compiler or torch's headers it is the only one that fails, and
     only the operators it holds are not there."""
-    _compile(LIBRARY, build_command, verbose)
+    _compile_library(LIBRARY, SOURCES, verbose)
     _compile(PROBE_LIBRARY, lambda out: build_command(out, PROBE_SOURCES), verbose)
     _compile(HOST_LIBRARY, host_command, verbose)
     return LIBRARY

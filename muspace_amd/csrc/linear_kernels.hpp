@@ -468,13 +468,7 @@ __device__ __forceinline__ float gate_of(int act, float z, float &slope) {
   return z;
 }
 
-// A chunk of the gated layer's result, or of da and du: z and u hold the products
-// without their biases. da and du are rounded to the tensors' type, once, as gradients
-// that leave an operator are: their errors, independent, add half the result's own
-// rounding to the gradients' mean square (a factor of 1.41 in all). In two numbers each,
-// as gelu's dz above, they would cost twice the products and four times the bytes: 40000 x
-// 256 -> 2 x 512 bf16 moves 246 MB of da and du as it is.
-// `bias` holds those of a chunk's z, then of its u; `grad` the chunk of g (kGrad).
+// The biases of a chunk's a, then of its u.
 template <typename T>
 __device__ __forceinline__ void load_biases(const Product &a, int col, int left,
                                             float (&bias)[2][Piece<T>::kValues]) {
@@ -493,6 +487,12 @@ __device__ __forceinline__ u32x4 load_grad(const Product &a, int64_t row, int co
   return loose_load<T>(static_cast<const T *>(a.grad) + row * a.n + col, left);
 }
 
+// A chunk of the gated layer's result, or of da and du: z and u hold the products
+// without their biases, `grad` the chunk of g (kGrad). da and du are rounded to the
+// tensors' type, once, as gradients that leave an operator are: their errors, independent,
+// are as large as the gradients' own rounding, 1.41 times it together. In two numbers each,
+// as gelu's dz below, they would cost twice the products and twice the bytes: 40000 x 256
+// -> 2 x 512 bf16 moves 246 MB of da and du as it is.
 template <typename T, bool kGrad>
 __device__ __forceinline__ void finish_gated(const Product &a, int64_t row, int col, int left,
                                              float (&z)[Piece<T>::kValues],
@@ -817,9 +817,9 @@ __global__ __launch_bounds__(kThreads, (sizeof(T) == 4 && kTight) ? 3 : 2) void 
 // ------------------------------------------------------------ few results ---
 
 // kForward, kInput and the gated jobs where the tiles would leave most CUs idle: a workgroup
-// makes 32 x 32 results (gated: 32 x 16) and its kWaves wavefronts take turns at the steps of k, each with its own
-// tiles in LDS, so that none waits for another until the sums are joined, in wavefront
-// order. float32 is multiplied as it is: the time is that of the loads.
+// makes 32 x 32 results (gated: 32 x 16) and its kWaves wavefronts take turns at the steps
+// of k, each with its own tiles in LDS, so that none waits for another until the sums are
+// joined, in wavefront order. float32 is multiplied as it is: the time is that of the loads.
 template <typename T, Job kJob, int kWaves, bool kTight, Kind kKind>
 __global__ __launch_bounds__(kWaves *kWave) void linear_few(const Product a) {
   constexpr int kV = Piece<T>::kValues;
