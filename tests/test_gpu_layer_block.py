@@ -151,14 +151,21 @@ def test_captured_steps_draw_new_masks():
     graph = torch.cuda.CUDAGraph()
     with torch.cuda.graph(graph):
         captured = step(seed)
+    # grad_value's sums at tile borders are added in no fixed order, so what is made of it alone is
+    # the same up to rounding: each run is within 2 * 40 * 2^-9 of float64 (test_layer_step), two
+    # runs within 4 * 40 * 2^-9 of each other
+    unordered = ("memory", "value.w", "value.b")
     seen = []
     for replay in range(1, 4):
         seed.add_(1)
         graph.replay()
         got = [t.clone() for t in captured]
         torch.cuda.synchronize()
-        for a, e in zip(got, step(SEED + replay)):
-            assert torch.equal(a, e)
+        for name, a, e in zip(("normed", "stream", *mine), got, step(SEED + replay)):
+            if name in unordered:
+                assert distance(a, e.cpu().double()) <= 4 * 40 * 2.0**-9, name
+            else:
+                assert torch.equal(a, e), name
         seen.append(got[0])
     assert not torch.equal(seen[0], seen[1]) and not torch.equal(seen[1], seen[2])
 
