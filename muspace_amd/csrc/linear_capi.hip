@@ -193,11 +193,10 @@ void launch_few(Product a, bool tight, hipStream_t st) {
 
 template <typename T, Job kJob, Kind kKind>
 void run_rows(const Product &a, bool tight, hipStream_t st) {
-  const int64_t columns = dense::gated(kJob) ? 2 * int64_t{a.n} : a.n;
-  if (few_results<T>(a.m, columns, a.k)) {
+  if (few_results<T>(a.m, a.n, a.k)) {
     launch_few<T, kJob, kKind>(a, tight, st);
   } else {
-    launch_product<T, kJob, kKind, false>(a, large_tiles(a.m, columns), tight, st);
+    launch_product<T, kJob, kKind, false>(a, large_tiles(a.m, a.n), tight, st);
   }
 }
 
@@ -294,12 +293,51 @@ void by_type(int dtype, F &&f) {
   }
 }
 
+// The gated layer's kernels: `columns` of the weight's rows, tight as for linear_product.
+enum class GatedKernel { kVector, kFew, kTiles64, kTiles128, kWide };
+
+template <typename T>
+GatedKernel gated_kernel(int64_t m, int64_t columns, int64_t k, bool tight) {
+  if (sizeof(T) == 2 && tight && dense::wide_tiles(m, columns, k)) return GatedKernel::kWide;
+  if (few_rows<T>(m)) return GatedKernel::kVector;
+  if (few_results<T>(m, columns, k)) return GatedKernel::kFew;
+  return large_tiles(m, columns) ? GatedKernel::kTiles128 : GatedKernel::kTiles64;
+}
+
+// Rows of sums that a kernel leaves: one a wavefront and part of the rows.
+template <typename T>
+int64_t gated_parts(GatedKernel kernel, int64_t m) {
+  switch (kernel) {
+    case GatedKernel::kVector:
+      return m;
+    case GatedKernel::kFew:
+      return ceil_div(m, 32) * (sizeof(T) == 4 ? 2 : 1);
+    case GatedKernel::kTiles64:
+      return ceil_div(m, 64) * 2;
+    case GatedKernel::kTiles128:
+      return ceil_div(m, 128) * 2;
+    default:
+      return ceil_div(m, dense::kWide) * 2;
+  }
+}
+
+// (without 256 x 256 tiles there are as many or more)
+size_t gated_sum_bytes(int dtype, int64_t rows, int64_t in, int64_t columns) {
+  int64_t parts = 0;
+  by_type(dtype, [&](auto t) {
+    using T = decltype(t);
+    parts = gated_parts<T>(gated_kernel<T>(rows, columns, in, false), rows);
+  });
+  return pad256(static_cast<size_t>(parts) * columns * 4);
+}
+
 template <Job kJob>
 void run_gated(int dtype, const Product &a, bool tight, hipStream_t st) {
   by_type(dtype, [&](auto t) {
     using T = decltype(t);
+    const GatedKernel kernel = gated_kernel<T>(a.m, 2 * int64_t{a.n}, a.k, tight);
     if constexpr (sizeof(T) == 2) {
-      if (tight && dense::wide_tiles(a.m, 2 * int64_t{a.n}, a.k)) {
+      if (kernel == GatedKernel::kWide) {
         dense::Codes c = {};
         c.p = a;
         c.p.tiles_n = static_cast<int>(ceil_div(a.n, dense::kWide / 2));
@@ -308,11 +346,25 @@ void run_gated(int dtype, const Product &a, bool tight, hipStream_t st) {
         return;
       }
     }
-    if (few_rows<T>(a.m)) {
+    if (kernel == GatedKernel::kVector) {
       run_vector<T, kJob>(a, st);
+    } else if (kernel == GatedKernel::kFew) {
+      launch_few<T, kJob, Kind::kPlain>(a, tight, st);
     } else {
-      run_rows<T, kJob, Kind::kPlain>(a, tight, st);
+      launch_product<T, kJob, Kind::kPlain, false>(a, kernel == GatedKernel::kTiles128, tight, st);
     }
+  });
+}
+
+// db from the rows of sums that run_gated<Job::kGatedGrad> left; zeros without rows.
+void run_gated_bias(int dtype, const Product &a, bool tight, void *db, hipStream_t st) {
+  by_type(dtype, [&](auto t) {
+    using T = decltype(t);
+    const int columns = 2 * a.n;
+    const int64_t parts =
+        a.m > 0 ? gated_parts<T>(gated_kernel<T>(a.m, columns, a.k, tight), a.m) : 0;
+    dense::gated_bias_sum<T><<<static_cast<int>(ceil_div(columns, 16)), dense::kThreads, 0, st>>>(
+        a.row_sums, static_cast<int>(parts), columns, static_cast<T *>(db));
   });
 }
 
@@ -334,6 +386,13 @@ Product gated_product(const void *x, const void *weight, const void *bias, int64
 
 bool gated_tight(int dtype, const void *x, const void *weight, int64_t in) {
   return in % chunk_values(dtype) == 0 && aligned16(x) && aligned16(weight);
+}
+
+size_t gated_bytes(int dtype, const Wanted &want, int64_t rows, int64_t in, int64_t out) {
+  Wanted products = want;
+  products.bias = false;
+  return dz_bytes(dtype, rows, out) + (want.bias ? gated_sum_bytes(dtype, rows, in, out) : 0) +
+         workspace_bytes_of(dtype, products, rows, in, out, dense::kNone);
 }
 
 // What the gradients' products read: dz [rows, ld] (and what rounding left of it), relu's
@@ -592,8 +651,7 @@ size_t gated_linear_backward_workspace_size(int dtype, int64_t rows, int64_t in_
   const Wanted want(want_input != 0, want_weight != 0, want_bias != 0, rows, in_features,
                     2 * hidden_features);
   if (!want.any()) return 0;
-  return dz_bytes(dtype, rows, 2 * hidden_features) +
-         workspace_bytes_of(dtype, want, rows, in_features, 2 * hidden_features, dense::kNone);
+  return gated_bytes(dtype, want, rows, in_features, 2 * hidden_features);
 }
 
 int gated_linear_backward(const void *grad_output, int dtype, const void *x, const void *weight,
@@ -624,12 +682,16 @@ int gated_linear_backward(const void *grad_output, int dtype, const void *x, con
   Product a = gated_product(x, weight, bias, rows, in_features, hidden_features, activation, ws);
   a.grad = grad_output;
   a.ldz = dz_chunks(dtype, out) * chunk_values(dtype);
-  if (summed) {
-    run_gated<Job::kGatedGrad>(dtype, a, gated_tight(dtype, x, weight, in_features), st);
-  }
+  const size_t sum_bytes = want.bias ? gated_sum_bytes(dtype, rows, in_features, out) : 0;
+  if (want.bias) a.row_sums = reinterpret_cast<float *>(ws + dz_bytes(dtype, rows, out));
+  const bool tight = gated_tight(dtype, x, weight, in_features);
+  if (summed) run_gated<Job::kGatedGrad>(dtype, a, tight, st);
   const Gradients g = {ws, nullptr, a.ldz, nullptr, x, nullptr, nullptr, weight, grad_input,
                        grad_weight, grad_bias, rows, in_features, out};
-  run_gradients(dtype, g, want, ws + dz_bytes(dtype, rows, out), st);
+  Wanted products = want;  // (db is of the sums above)
+  products.bias = false;
+  run_gradients(dtype, g, products, ws + dz_bytes(dtype, rows, out) + sum_bytes, st);
+  if (want.bias) run_gated_bias(dtype, a, tight, grad_bias, st);
   return check_launch(fn);
 }
 

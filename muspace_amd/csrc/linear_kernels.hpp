@@ -13,7 +13,9 @@
 //
 //   y  = act(a) u                    the same three kernels, Job::kGated
 //   da = g u act'(a), du = g act(a)  Job::kGatedGrad: a and u multiplied again
-//   dx = [da du] W, dW = [da du]^T x, db as above, from [da du] in memory
+//   dx = [da du] W, dW = [da du]^T x as above, from [da du] in memory
+//   db = sums of da and du           as they are made, a row of sums a wavefront, and
+//                                    gated_bias_sum
 //
 // A tile's rows of W are half Wg's and half Wu's, of the same results, 16 or 32 of each in
 // turn, so that a wavefront holds a and u of a result and neither is ever written.
@@ -64,9 +66,11 @@ struct Product {
   uint8_t *mask_out;     // kept sign bits (relu under training), as mask
   int act;
   uint8_t *codes, *code_scales;  // Kind::kKept: the checkpoint of x
-  // kGatedGrad: g [m, n]; out is [m, ldz], da, du and zeros up to whole chunks
+  // kGatedGrad: g [m, n]; out is [m, ldz], da, du and zeros up to whole chunks; sums of da
+  // and du over rows, before they are rounded, [parts of the rows][2 n] (0: none)
   const void *grad;
   int64_t ldz;
+  float *row_sums;
   // kWeight
   float *partial, *bias_partial;  // [splits][m][pad8(n)], [splits][m]
   void *bias_out;                 // splits == 1: db (0: none)
@@ -493,12 +497,15 @@ __device__ __forceinline__ u32x4 load_grad(const Product &a, int64_t row, int co
 // are as large as the gradients' own rounding, 1.41 times it together. In two numbers each,
 // as gelu's dz below, they would cost twice the products and twice the bytes: 40000 x 256
 // -> 2 x 512 bf16 moves 246 MB of da and du as it is.
+// `sums` gathers a lane's da and du as they are, for db: of few columns, sums of the rounded
+// ones erred by up to 1.6 times their own rounding, and these cost 5 of 155 us there.
 template <typename T, bool kGrad>
 __device__ __forceinline__ void finish_gated(const Product &a, int64_t row, int col, int left,
                                              float (&z)[Piece<T>::kValues],
                                              float (&u)[Piece<T>::kValues],
                                              const float (&bias)[2][Piece<T>::kValues],
-                                             const u32x4 &grad) {
+                                             const u32x4 &grad,
+                                             float (&sums)[2][Piece<T>::kValues]) {
   constexpr int kV = Piece<T>::kValues;
   if (left <= 0) return;
 #pragma unroll
@@ -520,6 +527,8 @@ __device__ __forceinline__ void finish_gated(const Product &a, int64_t row, int 
     for (int i = 0; i < kV; ++i) {
       slope[i] *= g[i] * u[i];
       z[i] *= g[i];
+      sums[0][i] += slope[i];
+      sums[1][i] += z[i];
     }
     T *to = static_cast<T *>(a.out) + row * a.ldz + col;
     loose_store(to, pack<T>(slope), left);
@@ -527,6 +536,37 @@ __device__ __forceinline__ void finish_gated(const Product &a, int64_t row, int 
     if (left <= kV) {  // the row's last chunk: zeros up to whole chunks
       for (int64_t i = 2 * static_cast<int64_t>(a.n) - col; i < a.ldz - col; ++i) {
         to[i] = from_float<T>(0.0f);
+      }
+    }
+  }
+}
+
+// The sums of a wavefront's rows: its lanes l, l + kLanes, l + 2 kLanes ... hold rows of the
+// same columns, and the first kLanes leave their sum as row `part` of row_sums.
+template <typename T, int kLanes>
+__device__ __forceinline__ void leave_sums(const Product &a, int part, int lane, int col, int left,
+                                           float (&sums)[2][Piece<T>::kValues]) {
+  constexpr int kV = Piece<T>::kValues;
+  if (a.row_sums == nullptr) return;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+#pragma unroll
+    for (int e = 0; e < kV; ++e) {
+      float v = sums[h][e];
+#if defined(__HIP_DEVICE_COMPILE__)
+      // rows of 16 lanes turned by 2, 4 and 8
+      if constexpr (kLanes <= 2) {
+        v += __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), 0x122, 0xf, 0xf, true));
+      }
+      if constexpr (kLanes <= 4) {
+        v += __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), 0x124, 0xf, 0xf, true));
+      }
+      v += __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), 0x128, 0xf, 0xf, true));
+#endif
+      static_assert(kLanes == 2 || kLanes == 4 || kLanes == 8, "a row's lanes");
+      v = add_across<32>(add_across<16>(v));
+      if (lane < kLanes && e < left) {
+        a.row_sums[(static_cast<int64_t>(part) * 2 + h) * a.n + col + e] = v;
       }
     }
   }
@@ -744,6 +784,7 @@ __global__ __launch_bounds__(kThreads, (sizeof(T) == 4 && kTight) ? 3 : 2) void 
   if constexpr (kJob == Job::kForward) {
     if (a.bias != nullptr) load_bias<T>(static_cast<const T *>(a.bias) + col, left, bias);
   }
+  float row_sums[2][kV] = {};
   if constexpr (gated(kJob)) load_biases<T>(a, col, left, biases);
 #pragma unroll
   for (int i = 0; i < kI; ++i) {
@@ -789,7 +830,7 @@ __global__ __launch_bounds__(kThreads, (sizeof(T) == 4 && kTight) ? 3 : 2) void 
           for (int x = 0; x < 4; ++x) u[e + x] = v[x];
         }
         finish_gated<T, kJob == Job::kGatedGrad>(a, row, col, here, z, u, biases,
-                                                 grads[r0 / kRows]);
+                                                 grads[r0 / kRows], row_sums);
       } else if constexpr (kJob == Job::kForward) {
 #pragma unroll
         for (int e = 0; e < kV; ++e) z[e] += bias[e];
@@ -811,6 +852,9 @@ __global__ __launch_bounds__(kThreads, (sizeof(T) == 4 && kTight) ? 3 : 2) void 
       }
     }
     wave_lds_sync();
+  }
+  if constexpr (kJob == Job::kGatedGrad) {
+    leave_sums<T, kLanes>(a, row0 / BM * 2 + (wave >> 1), lane, col, left, row_sums);
   }
 }
 
@@ -923,7 +967,13 @@ __global__ __launch_bounds__(kWaves *kWave) void linear_few(const Product a) {
       float biases[2][kV];
       load_biases<T>(a, col, left, biases);
       const u32x4 grad = kJob == Job::kGatedGrad ? load_grad<T>(a, row, col, left) : u32x4{};
-      finish_gated<T, kJob == Job::kGatedGrad>(a, row, col, left, z, up, biases, grad);
+      float row_sums[2][kV] = {};
+      finish_gated<T, kJob == Job::kGatedGrad>(a, row, col, left, z, up, biases, grad, row_sums);
+      if constexpr (kJob == Job::kGatedGrad) {
+        // (a wavefront's lanes are 16 rows of float32, or 32 of 16 bits)
+        constexpr int kParts = 32 * kLanes / kWave;
+        leave_sums<T, kLanes>(a, row0 / 32 * kParts + wave, lane, col, a.n - col, row_sums);
+      }
     } else if constexpr (kJob == Job::kForward) {
       if (a.bias != nullptr) {
         float b[kV];
@@ -1061,7 +1111,17 @@ __global__ __launch_bounds__(8 / kCols *kWave) void linear_vector(const Product 
     float biases[2][kV];
     load_biases<T>(a, col, left, biases);
     const u32x4 grad = kJob == Job::kGatedGrad ? load_grad<T>(a, row, col, left) : u32x4{};
-    finish_gated<T, kJob == Job::kGatedGrad>(a, row, col, left, z, u, biases, grad);
+    float row_sums[2][kV] = {};
+    finish_gated<T, kJob == Job::kGatedGrad>(a, row, col, left, z, u, biases, grad, row_sums);
+    if (kJob == Job::kGatedGrad && a.row_sums != nullptr && left > 0) {
+#pragma unroll
+      for (int e = 0; e < kV; ++e) {
+        if (e < left) {
+          a.row_sums[static_cast<int64_t>(row) * 2 * a.n + col + e] = row_sums[0][e];
+          a.row_sums[static_cast<int64_t>(row) * 2 * a.n + a.n + col + e] = row_sums[1][e];
+        }
+      }
+    }
     return;
   }
   // the whole wavefront: the mask's halves are exchanged between lanes
@@ -1122,6 +1182,36 @@ __global__ __launch_bounds__(kThreads) void linear_weight_sum(const float *parti
   } else if (bias) {
     db[i - count] = from_float<T>(s[0]);
   }
+}
+
+// db of the gated layer from its rows of sums, added in order: 16 columns by 16 runs of rows a
+// workgroup, runs joined in LDS.
+template <typename T>
+__global__ __launch_bounds__(kThreads) void gated_bias_sum(const float *rows, int parts, int columns,
+                                                           T *db) {
+  __shared__ float lds[16][17];
+  const int x = threadIdx.x & 15, y = threadIdx.x >> 4;
+  const int col = blockIdx.x * 16 + x;
+  float total = 0.0f;
+  if (col < columns) {
+    const float *src = rows + col;
+    int p = y;
+    for (; p + 7 * 16 < parts; p += 8 * 16) {
+      float v[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = src[static_cast<int64_t>(p + 16 * e) * columns];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) total += v[e];
+    }
+    for (; p < parts; p += 16) total += src[static_cast<int64_t>(p) * columns];
+  }
+  lds[y][x] = total;
+  __syncthreads();
+  if (y != 0 || col >= columns) return;
+  total = 0.0f;
+#pragma unroll
+  for (int e = 0; e < 16; ++e) total += lds[e][x];
+  db[col] = from_float<T>(total);
 }
 
 // ------------------------------------------------------------- elementwise ---

@@ -186,6 +186,7 @@ __global__ __launch_bounds__(kWideThreads, 2) void wide_product(const Codes a) {
   const int col = col0 + (gated(kJob) ? wc / 2 : wc) + chunk * kV, left = a.p.n - col;
   float scale[kV], bias[kV], biases[2][kV];
   if constexpr (kInt) load_columns<Out>(a, col, left, scale, bias);
+  float row_sums[2][kV] = {};
   if constexpr (gated(kJob)) load_biases<Out>(a.p, col, left, biases);
 #pragma unroll
   for (int i = 0; i < kI; ++i) {
@@ -233,10 +234,13 @@ __global__ __launch_bounds__(kWideThreads, 2) void wide_product(const Codes a) {
           for (int x = 0; x < 4; ++x) u[e + x] = v[x];
         }
         finish_gated<Out, kJob == Job::kGatedGrad>(a.p, row, col, here, z, u, biases,
-                                                   grads[r0 / kRows]);
+                                                   grads[r0 / kRows], row_sums);
       }
     }
     wave_lds_sync();
+  }
+  if constexpr (kJob == Job::kGatedGrad) {
+    leave_sums<Out, kLanes>(a.p, row0 / kWide * 2 + wave / 4, lane, col, left, row_sums);
   }
 }
 

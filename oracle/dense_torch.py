@@ -204,7 +204,7 @@ def gated_linear(x, weight, bias, activation, grad=None):
     in + 1 terms; the activations' derivatives are at most 1.13 and their second ones at
     most 0.8 (relu: a derivative may be either value where a lies within its error of zero);
     a value and a derivative take up to 16 float32 steps of their own. da and du are rounded
-    to the type once before they are multiplied."""
+    to the type once before they are multiplied, and not before they are summed."""
     dtype, u_step, small = x.dtype, half_step(x.dtype), tiny(x.dtype)
     x, w = x.double(), weight.double()
     rows, inner = x.shape
@@ -233,13 +233,14 @@ def gated_linear(x, weight, bias, activation, grad=None):
     du_err = g.abs() * h_err
     dz = torch.cat((da, du), -1)
     dz_err = torch.cat((da_err, du_err), -1) + 2 * SUM_STEP * dz.abs()
+    db, size = dz.sum(0), dz.abs() + dz_err
+    db_err = dz_err.sum(0) + (rows + 2) * SUM_STEP * size.sum(0)
     if dtype != torch.float32:
         dz_err = dz_err * (1 + u_step) + u_step * dz.abs() + small
     size = dz.abs() + dz_err
-    dx, dw, db = dz @ w, dz.t() @ x, dz.sum(0)
+    dx, dw = dz @ w, dz.t() @ x
     dx_err = dz_err @ w.abs() + (2 * hidden + 2) * SUM_STEP * (size @ w.abs())
     dw_err = dz_err.t() @ x.abs() + (rows + 2) * SUM_STEP * (size.t() @ x.abs())
-    db_err = dz_err.sum(0) + (rows + 2) * SUM_STEP * size.sum(0)
     for value, err in ((dx, dx_err), (dw, dw_err), (db, db_err)):
         results.append(value)
         bounds.append(err * (1 + u_step) + u_step * value.abs() + small)

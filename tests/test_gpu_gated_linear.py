@@ -159,8 +159,9 @@ def rms(a, e):
 
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_precision(dtype):
-    """Root mean squares. The output errs by its own rounding; the gradients by theirs and that
-    of da and du, two independent errors of one size: sqrt(2), 3% of room. float32: what
+    """Root mean squares. The output and the bias's gradient err by their own rounding; the
+    products by theirs and that of da and du, two independent errors of one size: sqrt(2), 3% of
+    room (384 sums scatter more: 4 deviations are 4 / sqrt(2 * 384), 14%). float32: what
     products of that many terms may lose, twice over for two in a row, and 8 steps of the
     activation."""
     x, w, b, g = make(8000, 256, 192, dtype, seed=5)
@@ -171,7 +172,7 @@ def test_precision(dtype):
         if dtype == torch.float32:
             limit = dense_torch.product_rms(256) + dense_torch.product_rms(8000) + 8 * 2.0**-24
         else:
-            limit = own * (1.03 * (math.sqrt(2) if i else 1.0))
+            limit = own * (1.03, 1.03 * math.sqrt(2), 1.03 * math.sqrt(2), 1.14)[i]
         assert rms(a, e) <= limit, (i, rms(a, e), own)
 
 
