@@ -130,7 +130,7 @@ void run(Codes a, bool tight, hipStream_t st) {
     launch_few<T, true>(a, tight, st);
   } else if (few_results(a.p.m, a.p.n)) {
     launch_few<T, false>(a, tight, st);
-  } else if (tight && dense::wide_tiles(a.p.m, a.p.n, a.p.k)) {
+  } else if (tight && dense::wide_tiles(a.p.m, a.p.n, a.p.k, 1)) {
     a.p.tiles_n = static_cast<int>(ceil_div(a.p.n, dense::kWide));
     a.p.tiles = static_cast<int>(ceil_div(a.p.m, dense::kWide)) * a.p.tiles_n;
     dense::wide_product<int8_t, T, dense::Job::kForward>

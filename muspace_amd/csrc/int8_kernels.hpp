@@ -95,7 +95,9 @@ __device__ __forceinline__ void encode_row(const float (&v)[kV], float scale, fl
   for (int i = 0; i < kV / 4; ++i) {
     uint32_t c[4];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) c[e] = static_cast<uint32_t>(static_cast<int>(q[4 * i + e])) & 0xffu;
+    for (int e = 0; e < 4; ++e) {
+      c[e] = static_cast<uint32_t>(static_cast<int>(q[4 * i + e])) & 0xffu;
+    }
     w[i] = scale == scale ? (c[0] | c[1] << 8) | (c[2] | c[3] << 8) << 16 : 0x01010101u;
   }
 }
@@ -253,11 +255,11 @@ __device__ __forceinline__ i32x16 multiply_codes(const u32x4 &a, const u32x4 &b,
 #endif
 }
 
-// A chunk of the result from its integer sums, of a row with scale `s`. (A sum past 2^24 is rounded to float32,
-// relative 2^-24, as the two products with the scales are.)
+// A chunk of the result from its integer sums, of a row with scale `s`. (A sum past 2^24 is
+// rounded to float32, relative 2^-24, as the two products with the scales are.)
 template <typename T>
-__device__ __forceinline__ void finish_codes(const Codes &a, float s, int64_t row, int col, int left,
-                                             const int (&sum)[Piece<T>::kValues],
+__device__ __forceinline__ void finish_codes(const Codes &a, float s, int64_t row, int col,
+                                             int left, const int (&sum)[Piece<T>::kValues],
                                              const float (&scale)[Piece<T>::kValues],
                                              const float (&bias)[Piece<T>::kValues]) {
   constexpr int kV = Piece<T>::kValues;
@@ -479,8 +481,8 @@ __global__ __launch_bounds__(kWaves *kWave) void int8_few(const Codes a) {
     }
     float scale[kV], bias[kV];
     load_columns<T>(a, col, a.p.n - col, scale, bias);
-    finish_codes<T>(a, kFused ? row_scales[r] : left > 0 ? a.x_scales[row] : 0.0f, row, col, left, sum,
-                    scale, bias);
+    finish_codes<T>(a, kFused ? row_scales[r] : left > 0 ? a.x_scales[row] : 0.0f, row, col, left,
+                    sum, scale, bias);
   }
 }
 

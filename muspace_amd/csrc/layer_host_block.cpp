@@ -1,5 +1,6 @@
 // Autograd nodes of a layer's blocks besides linear and layer norm: the gated layer,
-// dropout and the residual norm; and linear on 8-bit integers, which has no gradients. The contract is that of layer_host.cpp.
+// dropout and the residual norm; and linear on 8-bit integers, which has no gradients. The
+// contract is that of layer_host.cpp.
 #include <pybind11/stl.h>
 
 #include <cmath>
@@ -266,12 +267,14 @@ struct ResidualFunction : torch::autograd::Function<ResidualFunction> {
     };
     // what the backward reads (muspace_layer.h)
     const bool sums = block.scalar_type() != at::kFloat;
-    const NormKept kept{sums && !want_stream ? Tensor() : at::empty(block.sizes(), block.options()), stats(),
-                        n.post >= 0 ? stats() : Tensor()};
+    const NormKept kept{
+        sums && !want_stream ? Tensor() : at::empty(block.sizes(), block.options()), stats(),
+        n.post >= 0 ? stats() : Tensor()};
     Tensor output = residual_run(block, residual, v, n, drop, kept);
     const bool block_kept = sums || n.post >= 0 || wants_grad(v.gate);
     ctx->save_for_backward({block_kept ? block : Tensor(), sums ? residual : kept.stream,
-                            kept.stats, kept.post_stats, v.weight, v.gate, v.post_weight, v.post_bias, drop.device_seed});
+                            kept.stats, kept.post_stats, v.weight, v.gate, v.post_weight,
+                            v.post_bias, drop.device_seed});
     drop.keep(ctx);
     ctx->saved_data["norm"] = n.norm;
     ctx->saved_data["post"] = n.post;
@@ -321,8 +324,10 @@ struct ResidualFunction : torch::autograd::Function<ResidualFunction> {
       const size_t bytes = sums > 0 ? api.residual_workspace(code, rows, cols, sums) : 0;
       const Tensor workspace = scratch(bytes, stream);
       check(api.residual_backward(
-                pointer(g), pointer(gs), code, pointer(block), code != 0 ? stream.data_ptr() : nullptr,
-                code == 0 ? stream.data_ptr() : nullptr, pointer(saved[4]), pointer(saved[5]), pointer(saved[6]), pointer(saved[7]), code_of(type, "weight"),
+                pointer(g), pointer(gs), code, pointer(block),
+                code != 0 ? stream.data_ptr() : nullptr, code == 0 ? stream.data_ptr() : nullptr,
+                pointer(saved[4]), pointer(saved[5]), pointer(saved[6]), pointer(saved[7]),
+                code_of(type, "weight"),
                 static_cast<const float *>(stats.data_ptr()),
                 static_cast<const float *>(pointer(post_stats)), pointer(out[0]), pointer(out[1]),
                 pointer(out[2]), pointer(out[3]), pointer(out[4]), pointer(out[5]),

@@ -298,7 +298,9 @@ enum class GatedKernel { kVector, kFew, kTiles64, kTiles128, kWide };
 
 template <typename T>
 GatedKernel gated_kernel(int64_t m, int64_t columns, int64_t k, bool tight) {
-  if (sizeof(T) == 2 && tight && dense::wide_tiles(m, columns, k)) return GatedKernel::kWide;
+  if (sizeof(T) == 2 && tight && dense::wide_tiles(m, columns, k, sizeof(T))) {
+    return GatedKernel::kWide;
+  }
   if (few_rows<T>(m)) return GatedKernel::kVector;
   if (few_results<T>(m, columns, k)) return GatedKernel::kFew;
   return large_tiles(m, columns) ? GatedKernel::kTiles128 : GatedKernel::kTiles64;

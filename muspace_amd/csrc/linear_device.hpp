@@ -546,4 +546,29 @@ __device__ __forceinline__ void wave_lds_sync() {
   __builtin_amdgcn_wave_barrier();
 }
 
+// A column's sum over `parts` rows of `ld` floats, in order, by workgroups of 256 threads: 16
+// columns (threadIdx.x % 16) by 16 runs of rows, joined in LDS. The first 16 threads' results
+// are whole.
+__device__ __forceinline__ float add_rows(const float *src, int parts, int64_t ld) {
+  __shared__ float lds[16][17];
+  const int x = threadIdx.x & 15, y = threadIdx.x >> 4;
+  float total = 0.0f;
+  int p = y;
+  for (; p + 7 * 16 < parts; p += 8 * 16) {
+    float v[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = src[(p + 16 * e) * ld];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) total += v[e];
+  }
+  for (; p < parts; p += 16) total += src[p * ld];
+  lds[y][x] = total;
+  __syncthreads();
+  if (y != 0) return 0.0f;
+  total = 0.0f;
+#pragma unroll
+  for (int e = 0; e < 16; ++e) total += lds[e][x];
+  return total;
+}
+
 }  // namespace dense

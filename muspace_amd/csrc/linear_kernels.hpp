@@ -1184,34 +1184,14 @@ __global__ __launch_bounds__(kThreads) void linear_weight_sum(const float *parti
   }
 }
 
-// db of the gated layer from its rows of sums, added in order: 16 columns by 16 runs of rows a
-// workgroup, runs joined in LDS.
+// db of the gated layer from its rows of sums.
 template <typename T>
-__global__ __launch_bounds__(kThreads) void gated_bias_sum(const float *rows, int parts, int columns,
-                                                           T *db) {
-  __shared__ float lds[16][17];
-  const int x = threadIdx.x & 15, y = threadIdx.x >> 4;
-  const int col = blockIdx.x * 16 + x;
-  float total = 0.0f;
-  if (col < columns) {
-    const float *src = rows + col;
-    int p = y;
-    for (; p + 7 * 16 < parts; p += 8 * 16) {
-      float v[8];
-#pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = src[static_cast<int64_t>(p + 16 * e) * columns];
-#pragma unroll
-      for (int e = 0; e < 8; ++e) total += v[e];
-    }
-    for (; p < parts; p += 16) total += src[static_cast<int64_t>(p) * columns];
-  }
-  lds[y][x] = total;
-  __syncthreads();
-  if (y != 0 || col >= columns) return;
-  total = 0.0f;
-#pragma unroll
-  for (int e = 0; e < 16; ++e) total += lds[e][x];
-  db[col] = from_float<T>(total);
+__global__ __launch_bounds__(kThreads) void gated_bias_sum(const float *rows, int parts,
+                                                           int columns, T *db) {
+  static_assert(kThreads == 256, "add_rows");
+  const int col = blockIdx.x * 16 + (threadIdx.x & 15);
+  const float total = add_rows(rows + col, col < columns ? parts : 0, columns);
+  if (threadIdx.x < 16 && col < columns) db[col] = from_float<T>(total);
 }
 
 // ------------------------------------------------------------- elementwise ---

@@ -229,13 +229,14 @@ size_t residual_norm_backward_workspace_size(int dtype, int64_t rows, int64_t co
     return 0;
   }
   const int lanes = plan_lanes(dtype, cols);
-  return static_cast<size_t>(backward_blocks(lanes, rows)) * sums * cols * 4 + row_bytes(lanes, rows);
+  return static_cast<size_t>(backward_blocks(lanes, rows)) * sums * cols * 4 +
+         row_bytes(lanes, rows);
 }
 
 int residual_norm_backward(const void *grad_output, const void *grad_stream, int dtype,
                            const void *block, const void *residual, const void *stream_values,
-                           const void *weight, const void *gate, const void *post_weight, const void *post_bias,
-                           int weight_dtype, const float *statistics, const float *post_statistics,
+                           const void *weight, const void *gate, const void *post_weight,
+                           const void *post_bias, int weight_dtype, const float *statistics, const float *post_statistics,
                            void *grad_block, void *grad_residual, void *grad_weight,
                            void *grad_bias, void *grad_gate, void *grad_post_weight,
                            void *grad_post_bias, int64_t rows, int64_t cols, int norm,

@@ -40,7 +40,7 @@ struct Residual {
   void *d_block, *d_residual;      // backward
   float *stats, *post_stats;       // [rows][4] each: base, offset, s, 0
   float *partial;                  // [workgroups][sums][cols]
-  float *row_sums;                 // rows of any length: [rows][4] for the column sums
+  float *row_sums;                 // rows of any length: [rows][2], means of u and u h
   int slot[kSums];                 // a column sum's place in `partial` (-1: not wanted)
   int sums;                        // of them
   int64_t rows;
@@ -127,7 +127,8 @@ __device__ __forceinline__ float first_value(float v, Meeting &meet) {
   }
 }
 
-__device__ __forceinline__ void keep_statistics(float *stats, int64_t row, const Centre &c, float s) {
+__device__ __forceinline__ void keep_statistics(float *stats, int64_t row, const Centre &c,
+                                                float s) {
   reinterpret_cast<f32x4 *>(stats)[row] = f32x4{c.base, c.offset, s, 0.0f};
 }
 
@@ -220,7 +221,8 @@ __global__ __launch_bounds__(row_threads(kLanes)) void residual_forward(const Re
     if (a.stream != nullptr) {
       loose_store(static_cast<T *>(a.stream) + row * a.cols + col, pack<T>(v), any ? left : 0);
     }
-    const float s = row_statistics<kLanes, kFull>(v, a.cols, lane, a.norm, inv, a.eps, meet, centre);
+    const float s =
+        row_statistics<kLanes, kFull>(v, a.cols, lane, a.norm, inv, a.eps, meet, centre);
     if (a.stats != nullptr && any && lane == 0) keep_statistics(a.stats, row, centre, s);
 #pragma unroll
     for (int e = 0; e < kV; ++e) {
@@ -471,8 +473,8 @@ struct LongRow {
     } else {
       unpack<T>(loose_load<T>(static_cast<const T *>(a.stream_in) + at, left), h);
     }
-    unpack<T>(loose_load<T>(static_cast<const T *>(a.grad_out) + at, a.grad_out != nullptr ? left : 0),
-              g);
+    unpack<T>(loose_load<T>(static_cast<const T *>(a.grad_out) + at,
+                            a.grad_out != nullptr ? left : 0), g);
 #pragma unroll
     for (int e = 0; e < kV; ++e) h[e] = e < left ? unit_of(h[e], stats) : 0.0f;
   }
@@ -675,34 +677,14 @@ struct SumTargets {
   void *to[kSums];  // by place in `partial`
 };
 
-// The workgroups' rows of sums, added in order: 16 columns by 16 runs of rows a
-// workgroup, runs joined in LDS.
+// The workgroups' rows of sums, added in order.
 template <typename W>
 __global__ __launch_bounds__(256) void residual_sum_columns(const float *partial, int parts,
                                                             int cols, int sums, SumTargets out) {
-  __shared__ float lds[16][17];
-  const int x = threadIdx.x & 15, y = threadIdx.x >> 4;
   const int64_t ld = static_cast<int64_t>(sums) * cols;
-  const int64_t col = static_cast<int64_t>(blockIdx.x) * 16 + x;
-  float total = 0.0f;
-  if (col < ld) {
-    const float *src = partial + col;
-    int p = y;
-    for (; p + 7 * 16 < parts; p += 8 * 16) {
-      float v[8];
-#pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = src[(p + 16 * e) * ld];
-#pragma unroll
-      for (int e = 0; e < 8; ++e) total += v[e];
-    }
-    for (; p < parts; p += 16) total += src[p * ld];
-  }
-  lds[y][x] = total;
-  __syncthreads();
-  if (y != 0 || col >= ld) return;
-  total = 0.0f;
-#pragma unroll
-  for (int e = 0; e < 16; ++e) total += lds[e][x];
+  const int64_t col = static_cast<int64_t>(blockIdx.x) * 16 + (threadIdx.x & 15);
+  const float total = add_rows(partial + col, col < ld ? parts : 0, ld);
+  if (threadIdx.x >= 16 || col >= ld) return;
   const int k = static_cast<int>(col / cols);
   static_cast<W *>(out.to[k])[col - static_cast<int64_t>(k) * cols] = from_float<W>(total);
 }

@@ -10,8 +10,8 @@
 // moves chunks within their rows, is made by permuting which chunk of memory a lane
 // reads. Loads have no conditions: what lies beyond an operand, or k, reads as zeros.
 //
-// 16384 x 1024 -> 2 x 4096 bf16 274 us (0.99 PFLOP/s; in tiles of 128 331), of 2048 x 2048 -> 2 x 4096
-// 62 (87): a step takes 1.5 us, at 1.4 PFLOP/s, and the rest of a workgroup, 11 us, what
+// 16384 x 1024 -> 2 x 4096 bf16 274 us (0.99 PFLOP/s; in tiles of 128 331), 2048 x 2048 ->
+// 2 x 4096 62 (87): a step takes 1.5 us, at 1.4 PFLOP/s, and the rest of a workgroup, 11 us, what
 // ends its results above all, which nothing on the CU hides. Tiles of 256 x 128 at two
 // workgroups a CU hid it and read more of LDS and memory (290), as did 128 x 128 at four, loaded
 // like here (332).
@@ -95,7 +95,7 @@ __device__ __forceinline__ void wait_loads() {
 template <typename T, typename Out, Job kJob>
 __global__ __launch_bounds__(kWideThreads, 2) void wide_product(const Codes a) {
   constexpr bool kInt = std::is_same_v<T, int8_t>;
-  static_assert(kInt ? kJob == Job::kForward : gated(kJob), "the products with both operands along k");
+  static_assert(kInt ? kJob == Job::kForward : gated(kJob), "both operands lie along k");
   constexpr int kV = Piece<Out>::kValues;
   constexpr int kStep = kRowBytes / static_cast<int>(sizeof(T));
   constexpr int WM = 128, WN = 64, kI = WM / 32, kJ = WN / 32;  // a wavefront's part
@@ -244,16 +244,17 @@ __global__ __launch_bounds__(kWideThreads, 2) void wide_product(const Codes a) {
   }
 }
 
-// Whether m x n products of k values are made in these tiles: k long against the 11 us that
-// are not its, and the workgroups, one a CU, filling their rounds over the 256 CUs by 85%. In
-// tiles of 128 and in these, gated forward bf16: 8192 x 1024 -> 2 x 2048 (512 tiles) 83 and
-// 70 us, 12000 x 1024 -> 2 x 1536 (564) 88 and 95, 40000 x 256 -> 2 x 512 (628) 38 and 46,
-// 20000 x 512 -> 2 x 1024 (632) 54 and 60; integers: 16384 x 1024 -> 8192 (2048) 227 and 195,
-// 8192 x 1024 -> 4096 (512) 60 and 57, 12000 x 1024 -> 3072 (564) 65 and 76.
-inline bool wide_tiles(int64_t m, int64_t n, int64_t k) {
+// Whether m x n products of k values of `size` bytes are made in these tiles: k long against the
+// 11 us that are not its, and the workgroups, one a CU, filling their rounds over the 256 CUs by
+// 85%, or 70% of rows of 4096 bytes. In tiles of 128 and in these, gated forward bf16: 8192 x
+// 1024 -> 2 x 2048 (512 tiles, 100%) 83 and 70 us, 16384 x 1024 -> 2 x 1664 (832, 81%) 129 and
+// 130, 11000 x 1024 -> 2 x 1664 (559, 73%) 98 and 102, 11000 x 2048 -> 2 x 1664 194 and 172, 40000
+// x 256 -> 2 x 512 (628) 38 and 46, 20000 x 512 -> 2 x 1024 (632) 54 and 60; integers: 16384 x
+// 1024 -> 8192 (100%) 227 and 195, 16384 x 1024 -> 3328 (81%) 95 and 103, x 4096 325 and 291.
+inline bool wide_tiles(int64_t m, int64_t n, int64_t k, int size) {
   const int64_t tiles = ((m + kWide - 1) / kWide) * ((n + kWide - 1) / kWide);
   const int64_t rounds = (tiles + 255) / 256;
-  return k >= 1024 && tiles * 100 >= rounds * 256 * 85;
+  return k >= 1024 && tiles * 100 >= rounds * 256 * (k * size >= 4096 ? 70 : 85);
 }
 
 }  // namespace dense

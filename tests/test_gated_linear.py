@@ -171,7 +171,9 @@ def test_abi_without_work_and_workspace(native_lib):
     size = native_lib.raw("gated_linear_backward_workspace_size")
     assert size(9, 4, 8, 8, 1, 1, 1) == size(0, 4, 8, 8, 0, 0, 0) == 0
     # da and du in whole chunks, padded to 256 bytes; a short sum is not cut
-    assert size(0, 40, 8, 9, 1, 1, 1) == math.ceil(40 * 20 * 4 / 256) * 256
+    assert size(0, 40, 8, 9, 1, 1, 0) == math.ceil(40 * 20 * 4 / 256) * 256
+    # the bias's gradient: a row of sums per 16 rows, of two times 32
+    assert size(0, 40, 8, 9, 1, 1, 1) - size(0, 40, 8, 9, 1, 1, 0) == math.ceil(4 * 18 * 4 / 256) * 256
     assert size(2, 40, 8, 8, 1, 0, 0) == 40 * 16 * 2
     parts = native_lib.raw("linear_backward_workspace_size_for")
     assert (size(2, 40000, 256, 512, 1, 1, 0)

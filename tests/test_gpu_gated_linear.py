@@ -73,7 +73,8 @@ def test_small_sizes(size, dtype):
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("size", [(20011, 64, 32), (20000, 96, 80), (33001, 131, 77),
                                   (6000, 520, 515), (2049, 1024, 256), (513, 2048, 300),
-                                  (4090, 1032, 1790), (16300, 1024, 448)], ids=str)
+                                  (4090, 1032, 1790), (16300, 1024, 448), (11700, 2056, 500)],
+                         ids=str)
 def test_larger_sizes(size, dtype):
     check(*make(*size, dtype))
 
