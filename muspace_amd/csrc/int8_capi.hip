@@ -94,8 +94,16 @@ bool few_results(int64_t m, int64_t n) { return ceil_div(m, 64) * ceil_div(n, 64
 bool few_rows(int64_t m, int64_t k) {
   return m <= 4 && (m <= 2 ? m : 4) * padded(k) <= dense::kVectorCodes;
 }
+// Rows that workgroups quantise and multiply with all of the weight: many, so that one and a
+// half workgroups and more share a CU, and short ones; of a long weight 64 rows a time read too
+// much. In two kernels and in this one, us, bf16: 180000 x 256 -> 256 65.6 and 57.1, 40000 x 256
+// -> 512 32.2 and 29.7, 25000 x 256 -> 256 19.0 and 16.3, 100000 x 128 -> 128 25.4 and 22.7; 17000
+// x 256 -> 256 13.0 and 14.9, 33000 x 256 -> 1024 52 and 62.
+bool row_blocks(int64_t m, int64_t n, int64_t k) {
+  return k <= dense::kBlockIn && n <= 512 && ceil_div(m, dense::kBlockRows) * 2 >= 3 * kCus;
+}
 bool fused(int64_t m, int64_t n, int64_t k) {
-  return few_rows(m, k) || (few_results(m, n) && k <= dense::kFusedIn);
+  return few_rows(m, k) || (few_results(m, n) ? k <= dense::kFusedIn : row_blocks(m, n, k));
 }
 
 template <typename T, int kRows>
@@ -126,10 +134,19 @@ void run(Codes a, bool tight, hipStream_t st) {
     } else {
       launch_vector<T, 4>(a, st);
     }
-  } else if (fused(a.p.m, a.p.n, a.p.k)) {
-    launch_few<T, true>(a, tight, st);
   } else if (few_results(a.p.m, a.p.n)) {
-    launch_few<T, false>(a, tight, st);
+    if (a.p.k <= dense::kFusedIn) {
+      launch_few<T, true>(a, tight, st);
+    } else {
+      launch_few<T, false>(a, tight, st);
+    }
+  } else if (row_blocks(a.p.m, a.p.n, a.p.k)) {
+    const int blocks = static_cast<int>(ceil_div(a.p.m, dense::kBlockRows));
+    if (tight) {
+      dense::int8_row_block<T, true><<<blocks, dense::kThreads, 0, st>>>(a);
+    } else {
+      dense::int8_row_block<T, false><<<blocks, dense::kThreads, 0, st>>>(a);
+    }
   } else if (tight && dense::wide_tiles(a.p.m, a.p.n, a.p.k, 1)) {
     a.p.tiles_n = static_cast<int>(ceil_div(a.p.n, dense::kWide));
     a.p.tiles = static_cast<int>(ceil_div(a.p.m, dense::kWide)) * a.p.tiles_n;

@@ -6,9 +6,9 @@
 // Sums are exact, in int32 (in_features up to 2^17). The row's quotients are float32
 // divisions, so that codes are the same on any machine.
 //
-// int8_rows quantises; int8_product is linear_product (linear_kernels.hpp) with 128 codes a
-// step in the same 128 bytes: the same LDS layout serves, a lane's 16 bytes of a row are 16
-// codes, and v_mfma_i32_32x32x32_i8 takes 32 of k a time, at twice the 16-bit types' rate.
+// int8_rows quantises, or, of few rows or many short ones, the product's own kernel;
+// int8_product is linear_product (linear_kernels.hpp) with 128 codes a step in the same 128
+// bytes: the same LDS layout serves, a lane's 16 bytes of a row are 16 codes, and v_mfma_i32_32x32x32_i8 takes 32 of k a time, at twice the 16-bit types' rate.
 // Rows of x's codes are padded with zeros to whole chunks, so what a weight's chunk holds
 // past the row's end (the next row's first codes) counts for nothing.
 #pragma once
@@ -483,6 +483,132 @@ __global__ __launch_bounds__(kWaves *kWave) void int8_few(const Codes a) {
     load_columns<T>(a, col, a.p.n - col, scale, bias);
     finish_codes<T>(a, kFused ? row_scales[r] : left > 0 ? a.x_scales[row] : 0.0f, row, col, left,
                     sum, scale, bias);
+  }
+}
+
+// Many short rows: a workgroup quantises 64 rows into LDS, where their codes stay, and makes all
+// their results, 128 columns at a time, the weight's next step on its way over the ends of
+// results. x is read once, and nothing but results is written. 40000 x 256 -> 512 bf16 26.5 us,
+// 12 of them the bytes': a workgroup's steps wait for each other at barriers. With the weight's
+// fragments straight from the caches into registers none did, and it took 32.
+constexpr int kBlockRows = 64;
+constexpr int kBlockIn = 256;  // of k at the most: 16 KB of codes
+
+template <typename T, bool kTight>
+__global__ __launch_bounds__(kThreads, 3) void int8_row_block(const Codes a) {
+  constexpr int kV = Piece<T>::kValues;
+  constexpr int BN = 128, WN = BN / 2, kJ = WN / 32;  // a wavefront's part: 32 x 64
+  constexpr int kTile = kBlockRows * kRowBytes;
+  constexpr int kStageLd = WN + 4, kStage = 4 * 32 * kStageLd * 4;
+  static_assert(BN * kRowBytes <= kStage, "the weight's tile and the results take turns");
+  __shared__ __attribute__((aligned(16))) char codes[kBlockIn / kCodeStep * kTile], lds[kStage];
+  __shared__ float row_scales[kBlockRows];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int wr = (wave >> 1) * 32, wc = (wave & 1) * WN;
+  const int64_t row0 = static_cast<int64_t>(blockIdx.x) * kBlockRows;
+  CodeLoader<BN, kTight> q;
+  q.init(a.weight, a.p.k, 0, a.p.n);
+  if (a.p.k > 0) q.fetch(0);
+  {
+    // 16 threads a row, 16 rows at a time
+    constexpr int kTimes = kBlockRows / 16, kPieces = kBlockIn / (16 * kV);
+    const int r = threadIdx.x / 16, t = threadIdx.x % 16;
+    u32x4 piece[kTimes][kPieces];
+#pragma unroll
+    for (int u = 0; u < kTimes; ++u) {
+      const int64_t row = row0 + 16 * u + r;
+      const T *x = static_cast<const T *>(a.p.p) + row * a.p.k;
+#pragma unroll
+      for (int i = 0; i < kPieces; ++i) {
+        const int col = (t + 16 * i) * kV;
+        piece[u][i] = loose_load<T>(x + col, row < a.p.m ? a.p.k - col : 0);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < kTimes; ++u) {
+      uint32_t top = 0;
+#pragma unroll
+      for (int i = 0; i < kPieces; ++i) {
+        float v[kV];
+        unpack<T>(piece[u][i], v);
+#pragma unroll
+        for (int e = 0; e < kV; ++e) top = max(top, __float_as_uint(v[e]) & 0x7fffffffu);
+      }
+      const float scale = row_scale(team_top<16>(top, nullptr)), inverse = 1.0f / scale;
+      if (t == 0) row_scales[16 * u + r] = scale;
+#pragma unroll
+      for (int i = 0; i < kPieces; ++i) {
+        const int col = (t + 16 * i) * kV;
+        float v[kV];
+        uint32_t w[kV / 4];
+        unpack<T>(piece[u][i], v);
+        encode_row<kV>(v, scale, inverse, w);
+        char *to = codes + col / kCodeStep * kTile +
+                   along_offset<128>(16 * u + r, col % kCodeStep / 16) + col % 16;
+        if constexpr (kV == 8) {
+          *reinterpret_cast<u32x2 *>(to) = u32x2{w[0], w[1]};
+        } else {
+          *reinterpret_cast<uint32_t *>(to) = w[0];
+        }
+      }
+    }
+  }
+  __syncthreads();
+  int *stage = reinterpret_cast<int *>(lds) + wave * 32 * kStageLd;
+  constexpr int kLanes = WN / kV, kRows = kWave / kLanes;
+  const int chunk = lane % kLanes;
+  for (int col0 = 0; col0 < a.p.n; col0 += BN) {
+    i32x16 acc[kJ] = {};
+    for (int k0 = 0; k0 < a.p.k; k0 += kCodeStep) {
+      q.put(lds);
+      __syncthreads();
+      if (k0 + kCodeStep < a.p.k) {
+        q.fetch(k0 + kCodeStep);
+      } else if (col0 + BN < a.p.n) {
+        q.row0 = col0 + BN;
+        q.fetch(0);
+      }
+#pragma unroll
+      for (int s = 0; s < 4; ++s) {
+        const u32x4 fp =
+            read_fragment<true, kBlockRows, 128>(codes + k0 / kCodeStep * kTile, wr, s, lane);
+#pragma unroll
+        for (int j = 0; j < kJ; ++j) {
+          acc[j] = multiply_codes(read_fragment<true, BN, 128>(lds, wc + 32 * j, s, lane), fp,
+                                  acc[j]);
+        }
+      }
+      __syncthreads();
+    }
+    const int col = col0 + wc + chunk * kV, left = a.p.n - col;
+    float scale[kV], bias[kV];
+    load_columns<T>(a, col, left, scale, bias);
+#pragma unroll
+    for (int j = 0; j < kJ; ++j) {
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        i32x4 v;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = acc[j][4 * g + e];
+        *reinterpret_cast<i32x4 *>(stage + (lane & 31) * kStageLd + 32 * j + 8 * g +
+                                   4 * (lane >> 5)) = v;
+      }
+    }
+    wave_lds_sync();
+#pragma unroll
+    for (int r0 = 0; r0 < 32; r0 += kRows) {
+      const int r = r0 + lane / kLanes;
+      const int64_t row = row0 + wr + r;
+      int sum[kV];
+#pragma unroll
+      for (int e = 0; e < kV; e += 4) {
+        const i32x4 v = *reinterpret_cast<const i32x4 *>(stage + r * kStageLd + chunk * kV + e);
+#pragma unroll
+        for (int x = 0; x < 4; ++x) sum[e + x] = v[x];
+      }
+      finish_codes<T>(a, row_scales[wr + r], row, col, row < a.p.m ? left : 0, sum, scale, bias);
+    }
+    __syncthreads();
   }
 }
 

@@ -73,9 +73,9 @@ SIZES = [
     (1, 1, 1), (1, 256, 256), (2, 8, 3), (3, 5, 7), (17, 33, 65), (31, 64, 32), (33, 129, 40),
     (130, 256, 520), (300, 96, 64), (257, 203, 131), (1000, 40, 24), (64, 2048, 100), (5, 5000, 17),
     (3, 131072, 5), (4, 12288, 33), (3, 12300, 33), (2, 24570, 40), (1, 49150, 20),
-    (1, 4100, 500), (3, 2047, 19), (40, 2048, 70), (40, 2049, 70), (20011, 64, 32), (20000, 96, 160), (33001, 131, 77), (6000, 520, 1030),
-    (2049, 1024, 256), (513, 2048, 300), (4090, 1040, 3580), (16300, 1024, 900),
-    (11700, 4112, 1000),
+    (1, 4100, 500), (3, 2047, 19), (40, 2048, 70), (40, 2049, 70), (20011, 64, 32),
+    (20000, 96, 160), (33001, 131, 77), (6000, 520, 1030), (2049, 1024, 256), (513, 2048, 300), (4090, 1040, 3580), (16300, 1024, 900),
+    (11700, 4112, 1000), (24577, 256, 200), (24600, 64, 513), (30000, 240, 512), (25001, 3, 130),
 ]
 
 
@@ -102,7 +102,7 @@ def test_extreme_codes_and_sums():
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("rows", [3, 50, 9000])
+@pytest.mark.parametrize("rows", [3, 50, 9000, 25000])
 def test_infinity_and_nan_stay_in_their_rows(rows, dtype):
     x, w, s, b, r = make(rows, 200, 72, dtype)
     clean = linear_int8(x, w, s, b, residual=r)
@@ -186,7 +186,7 @@ def test_refused_on_the_device():
     assert not codes.requires_grad and not scales.requires_grad
 
 
-@pytest.mark.parametrize("rows", [1, 300, 9000])
+@pytest.mark.parametrize("rows", [1, 300, 9000, 25000])
 def test_streams_and_captured_calls(rows):
     """On another stream; captured, two graphs of it replayed in turn on new inputs with eager
     work in between (each has its own workspace)."""
