@@ -74,7 +74,8 @@ SIZES = [
     (130, 256, 520), (300, 96, 64), (257, 203, 131), (1000, 40, 24), (64, 2048, 100), (5, 5000, 17),
     (3, 131072, 5), (4, 12288, 33), (3, 12300, 33), (2, 24570, 40), (1, 49150, 20),
     (1, 4100, 500), (3, 2047, 19), (40, 2048, 70), (40, 2049, 70), (20011, 64, 32),
-    (20000, 96, 160), (33001, 131, 77), (6000, 520, 1030), (2049, 1024, 256), (513, 2048, 300), (4090, 1040, 3580), (16300, 1024, 900),
+    (20000, 96, 160), (33001, 131, 77), (6000, 520, 1030), (2049, 1024, 256), (513, 2048, 300),
+    (4090, 1040, 3580), (16300, 1024, 900),
     (11700, 4112, 1000), (24577, 256, 200), (24600, 64, 513), (30000, 240, 512), (25001, 3, 130),
 ]
 

@@ -206,4 +206,7 @@ def test_abi_without_work_and_workspace(native_lib):
     assert size(2, 100, 2050, 8) == 206592 + 512
     # few rows and few results are quantised where they are multiplied
     assert size(2, 4, 12288, 4096) == size(2, 1, 49152, 4096) == size(2, 300, 256, 256) == 0
-    assert size(2, 4, 12289, 4096) > 0 and size(2, 40000, 256, 512) > 0
+    assert size(2, 4, 12289, 4096) > 0 and size(2, 40000, 264, 512) > 0
+    # and many short rows
+    assert size(2, 40000, 256, 512) == 0 and size(2, 40000, 256, 513) > 0
+    assert size(2, 24512, 256, 512) > 0 and size(2, 24513, 256, 512) == 0
