@@ -100,6 +100,12 @@ MUSPACE_API size_t gated_linear_backward_workspace_size(int dtype, int64_t rows,
                                                         int64_t hidden_features, int want_input,
                                                         int want_weight, int want_bias);
 
+/* Rows of float32 sums of da and du, [2 hidden] each, that the backward leaves in its workspace
+ * for grad_bias (0 for invalid sizes): `aligned` is not 0 where x and weight start on 16-byte
+ * boundaries. The workspace's size covers either. */
+MUSPACE_API int64_t gated_linear_backward_sum_rows(int dtype, int64_t rows, int64_t in_features,
+                                                   int64_t hidden_features, int aligned);
+
 /* a and u are computed again; da = grad_output u act'(a) and du = grad_output act(a) are
  * rounded to the tensors' type (past its range: to infinities); grad_input = [da du]
  * weight, grad_weight = [da du]^T x, grad_bias their sums over the rows. A NULL gradient

@@ -56,7 +56,7 @@
 extern "C" {
 #endif
 
-#define MUSPACE_MSDA_ABI_VERSION 8
+#define MUSPACE_MSDA_ABI_VERSION 9
 
 /* the library is built with -fvisibility=hidden; only these symbols export */
 #if defined(__GNUC__)

@@ -2,6 +2,7 @@
 // Plans (tile sizes, parts of k) are functions of sizes, type and alignment only.
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <climits>
 #include <cstdint>
 #include <type_traits>
@@ -298,10 +299,10 @@ enum class GatedKernel { kVector, kFew, kTiles64, kTiles128, kWide };
 
 template <typename T>
 GatedKernel gated_kernel(int64_t m, int64_t columns, int64_t k, bool tight) {
+  if (few_rows<T>(m)) return GatedKernel::kVector;  // however wide the weight
   if (sizeof(T) == 2 && tight && dense::wide_tiles(m, columns, k, sizeof(T))) {
     return GatedKernel::kWide;
   }
-  if (few_rows<T>(m)) return GatedKernel::kVector;
   if (few_results<T>(m, columns, k)) return GatedKernel::kFew;
   return large_tiles(m, columns) ? GatedKernel::kTiles128 : GatedKernel::kTiles64;
 }
@@ -323,13 +324,20 @@ int64_t gated_parts(GatedKernel kernel, int64_t m) {
   }
 }
 
-// (without 256 x 256 tiles there are as many or more)
-size_t gated_sum_bytes(int dtype, int64_t rows, int64_t in, int64_t columns) {
+// Rows of sums that the kernel of these sizes leaves, tight operands or not.
+int64_t gated_sum_rows(int dtype, int64_t rows, int64_t in, int64_t columns, bool tight) {
   int64_t parts = 0;
   by_type(dtype, [&](auto t) {
     using T = decltype(t);
-    parts = gated_parts<T>(gated_kernel<T>(rows, columns, in, false), rows);
+    parts = gated_parts<T>(gated_kernel<T>(rows, columns, in, tight), rows);
   });
+  return parts;
+}
+
+// (the kernel goes by the operands' alignment too, which the workspace's size does not know)
+size_t gated_sum_bytes(int dtype, int64_t rows, int64_t in, int64_t columns) {
+  const int64_t parts = std::max(gated_sum_rows(dtype, rows, in, columns, true),
+                                 gated_sum_rows(dtype, rows, in, columns, false));
   return pad256(static_cast<size_t>(parts) * columns * 4);
 }
 
@@ -360,11 +368,10 @@ void run_gated(int dtype, const Product &a, bool tight, hipStream_t st) {
 
 // db from the rows of sums that run_gated<Job::kGatedGrad> left; zeros without rows.
 void run_gated_bias(int dtype, const Product &a, bool tight, void *db, hipStream_t st) {
+  const int columns = 2 * a.n;
+  const int64_t parts = a.m > 0 ? gated_sum_rows(dtype, a.m, a.k, columns, tight) : 0;
   by_type(dtype, [&](auto t) {
     using T = decltype(t);
-    const int columns = 2 * a.n;
-    const int64_t parts =
-        a.m > 0 ? gated_parts<T>(gated_kernel<T>(a.m, columns, a.k, tight), a.m) : 0;
     dense::gated_bias_sum<T><<<static_cast<int>(ceil_div(columns, 16)), dense::kThreads, 0, st>>>(
         a.row_sums, static_cast<int>(parts), columns, static_cast<T *>(db));
   });
@@ -656,6 +663,17 @@ size_t gated_linear_backward_workspace_size(int dtype, int64_t rows, int64_t in_
   return gated_bytes(dtype, want, rows, in_features, 2 * hidden_features);
 }
 
+int64_t gated_linear_backward_sum_rows(int dtype, int64_t rows, int64_t in_features,
+                                       int64_t hidden_features, int aligned) {
+  if (validate_gated("gated_linear_backward_sum_rows", dtype, rows, in_features, hidden_features,
+                     0) != MUSPACE_OK ||
+      rows == 0 || hidden_features == 0) {
+    return 0;
+  }
+  return gated_sum_rows(dtype, rows, in_features, 2 * hidden_features,
+                        aligned != 0 && in_features % chunk_values(dtype) == 0);
+}
+
 int gated_linear_backward(const void *grad_output, int dtype, const void *x, const void *weight,
                           const void *bias, void *grad_input, void *grad_weight, void *grad_bias,
                           int64_t rows, int64_t in_features, int64_t hidden_features,
@@ -685,8 +703,14 @@ int gated_linear_backward(const void *grad_output, int dtype, const void *x, con
   a.grad = grad_output;
   a.ldz = dz_chunks(dtype, out) * chunk_values(dtype);
   const size_t sum_bytes = want.bias ? gated_sum_bytes(dtype, rows, in_features, out) : 0;
-  if (want.bias) a.row_sums = reinterpret_cast<float *>(ws + dz_bytes(dtype, rows, out));
   const bool tight = gated_tight(dtype, x, weight, in_features);
+  if (want.bias) {
+    a.row_sums = reinterpret_cast<float *>(ws + dz_bytes(dtype, rows, out));
+    if (gated_sum_rows(dtype, rows, in_features, out, tight) * out * 4 >
+        static_cast<int64_t>(sum_bytes)) {
+      return fail(MUSPACE_EINVAL, "%s: the workspace's size is not this kernel's", fn);
+    }
+  }
   if (summed) run_gated<Job::kGatedGrad>(dtype, a, tight, st);
   const Gradients g = {ws, nullptr, a.ldz, nullptr, x, nullptr, nullptr, weight, grad_input,
                        grad_weight, grad_bias, rows, in_features, out};

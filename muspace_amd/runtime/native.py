@@ -28,7 +28,7 @@ from typing import Any, Callable
 import torch
 
 LIBRARY_RELPATH = "native/libmuspace_msda.so"
-ABI_VERSION = 8
+ABI_VERSION = 9
 
 DTYPE_F32, DTYPE_F16, DTYPE_BF16 = 0, 1, 2
 
@@ -179,6 +179,7 @@ _EXPORTS: dict[str, tuple[Any, list[Any]]] = {
     "gated_linear_backward_workspace_size": (
         ctypes.c_size_t, [_c_int] + [_c_int64] * 3 + [_c_int] * 3
     ),
+    "gated_linear_backward_sum_rows": (_c_int64, [_c_int] + [_c_int64] * 3 + [_c_int]),
     "gated_linear_backward": (
         _c_int,
         [_c_ptr, _c_int] + [_c_ptr] * 6 + [_c_int64] * 3

@@ -178,3 +178,35 @@ def test_abi_without_work_and_workspace(native_lib):
     parts = native_lib.raw("linear_backward_workspace_size_for")
     assert (size(2, 40000, 256, 512, 1, 1, 0)
             == 40000 * 1024 * 2 + parts(2, 40000, 256, 1024, 0, 1, 1, 0))
+
+
+def sums_and_room(native_lib, dtype, rows, inner, hidden):
+    """(rows of the bias's sums that the backward's kernel leaves, the most of either alignment;
+    those that its workspace holds)."""
+    size = native_lib.raw("gated_linear_backward_workspace_size")
+    left = native_lib.raw("gated_linear_backward_sum_rows")
+    room = size(dtype, rows, inner, hidden, 1, 1, 1) - size(dtype, rows, inner, hidden, 1, 1, 0)
+    return max(left(dtype, rows, inner, hidden, a) for a in (0, 1)), room / (2 * hidden * 4)
+
+
+@pytest.mark.parametrize("dtype", [0, 1, 2])
+@pytest.mark.parametrize("inner", [256, 1024, 2048, 8192])
+def test_the_workspace_holds_the_sums_of_the_kernel_taken(native_lib, inner, dtype):
+    """Of one row and of many, on both sides of the widths from which large tiles are taken."""
+    widths = [1, 24, 512, 4096, 11520, 16384, 22912, 22913, 22920, 23040, 27776, 27777, 28672, 32768,
+              40000, 65536]
+    for hidden in widths:
+        for rows in [*range(1, 301), 511, 513, 2048, 4095, 4096, 16384, 40000]:
+            left, room = sums_and_room(native_lib, dtype, rows, inner, hidden)
+            assert 0 < left <= room, (rows, inner, hidden, left, room)
+
+
+def test_sum_rows(native_lib):
+    left = native_lib.raw("gated_linear_backward_sum_rows")
+    assert left(3, 4, 8, 8, 1) == left(0, 0, 8, 8, 1) == left(0, 4, 8, 0, 1) == left(0, -1, 8, 8, 1) == 0
+    # a row of results is multiplied by itself, whatever the weight's width
+    for hidden in (64, 28672, 65536):
+        assert [left(2, rows, 8192, hidden, 1) for rows in (1, 2, 4)] == [1, 2, 4]
+    # two for each 32 rows of float32, for each 128 or 256 rows in tiles
+    assert left(0, 40, 8, 9, 1) == 4
+    assert left(2, 16384, 1024, 4096, 0) == 2 * left(2, 16384, 1024, 4096, 1) == 256

@@ -339,3 +339,30 @@ def test_streams_and_captured_steps(rows):
         torch.cuda.synchronize()
         for a, e in zip(got, run()):
             assert torch.equal(a, e)
+
+
+WIDE_ROWS = [(1, 1024, 28672), (1, 2048, 23040), (2, 1024, 27784), (4, 1024, 28672), (5, 1024, 28672)]
+
+
+@pytest.mark.parametrize("size", WIDE_ROWS, ids=str)
+def test_few_rows_of_a_wide_layer(size):
+    check(*make(*size, torch.bfloat16))
+
+
+@pytest.mark.parametrize("size", [*WIDE_ROWS, (1, 9, 7), (3, 64, 24), (33, 40, 17), (300, 256, 512),
+                                  (4096, 1024, 1792)], ids=str)
+def test_nothing_is_written_past_the_workspace(native_lib, size):
+    rows, inner, hidden = size
+    x, w, b, g = make(*size, torch.bfloat16)
+    need = native_lib.raw("gated_linear_backward_workspace_size")(2, rows, inner, hidden, 1, 1, 1)
+    # as much again behind it, or the sums of twice 256 rows, whichever is more
+    behind = max(need, 4 * 2 * hidden * 4)
+    space = torch.full((need + behind,), 0x5A, dtype=torch.uint8, device=DEV)
+    assert space.data_ptr() % 256 == 0
+    grads = [torch.empty_like(t) for t in (x, w, b)]
+    assert native_lib.raw("gated_linear_backward")(
+        g.data_ptr(), 2, x.data_ptr(), w.data_ptr(), b.data_ptr(), *(t.data_ptr() for t in grads),
+        rows, inner, hidden, 3, space.data_ptr(), need, torch.cuda.current_stream().cuda_stream) == 0
+    assert (space[need:] == 0x5A).all()
+    for got, want in zip(grads, step(x, w, b, g, "silu")[1:]):
+        assert torch.equal(got, want)
