@@ -246,15 +246,23 @@ __global__ __launch_bounds__(kWideThreads, 2) void wide_product(const Codes a) {
 
 // Whether m x n products of k values of `size` bytes are made in these tiles: k long against the
 // 11 us that are not its, and the workgroups, one a CU, filling their rounds over the 256 CUs by
-// 85%, or 70% of rows of 4096 bytes. In tiles of 128 and in these, gated forward bf16: 8192 x
+// 85%, or 70% of rows of 4096 bytes. us, in tiles of 128 and in these, gated forward bf16: 8192 x
 // 1024 -> 2 x 2048 (512 tiles, 100%) 83 and 70 us, 16384 x 1024 -> 2 x 1664 (832, 81%) 129 and
 // 130, 11000 x 1024 -> 2 x 1664 (559, 73%) 98 and 102, 11000 x 2048 -> 2 x 1664 194 and 172, 40000
 // x 256 -> 2 x 512 (628) 38 and 46, 20000 x 512 -> 2 x 1024 (632) 54 and 60; integers: 16384 x
 // 1024 -> 8192 (100%) 227 and 195, 16384 x 1024 -> 3328 (81%) 95 and 103, x 4096 325 and 291.
+// And where whole tiles are under a third more rows, and columns, than tiles of 128: 5 x 1024 -> 2 x
+// 28672 24 and 32, 128 rows 28 and 35, 160 rows 49 and 35, 288 rows 67 and 62, 288 x 2048 -> 2 x
+// 24576 103 and 111, 448 rows 122 and 113; 60000 x 1024 -> 2 x 64 23 and 32, 2 x 72 38 and 33, 2 x
+// 160 56 and 60; integers: 128 x 1024 -> 57344 22 and 28, 160 rows 35 and 29, 288 rows 48 and 49, 60000
+// x 1024 -> 128 57 and 64, 144 columns 65 and 65 (70 and 67 in another session), 320 76 and 85.
+inline int64_t whole(int64_t n, int tile) { return (n + tile - 1) / tile * tile; }
 inline bool wide_tiles(int64_t m, int64_t n, int64_t k, int size) {
-  const int64_t tiles = ((m + kWide - 1) / kWide) * ((n + kWide - 1) / kWide);
+  const int64_t tiles = whole(m, kWide) / kWide * (whole(n, kWide) / kWide);
   const int64_t rounds = (tiles + 255) / 256;
-  return k >= 1024 && tiles * 100 >= rounds * 256 * (k * size >= 4096 ? 70 : 85);
+  return k >= 1024 && whole(m, kWide) * 3 < whole(m, 128) * 4 &&
+         whole(n, kWide) * 3 < whole(n, 128) * 4 &&
+         tiles * 100 >= rounds * 256 * (k * size >= 4096 ? 70 : 85);
 }
 
 }  // namespace dense

@@ -210,3 +210,18 @@ def test_sum_rows(native_lib):
     # two for each 32 rows of float32, for each 128 or 256 rows in tiles
     assert left(0, 40, 8, 9, 1) == 4
     assert left(2, 16384, 1024, 4096, 0) == 2 * left(2, 16384, 1024, 4096, 1) == 256
+
+
+def test_large_tiles_are_not_half_empty(native_lib):
+    """Two rows of sums for 256 rows in large tiles, for 128 in others: large ones are taken where
+    they make less than a third more rows, and columns, than the others."""
+    left = native_lib.raw("gated_linear_backward_sum_rows")
+    rows = (5, 128, 129, 256, 257, 384, 385, 512)
+    assert [left(2, r, 2048, 28672, 0) for r in rows] == [2, 2, 4, 4, 6, 6, 8, 8]
+    assert [left(2, r, 2048, 28672, 1) for r in rows] == [2, 2, 2, 2, 6, 6, 4, 4]
+    wide, others = 2 * 235, 2 * 469  # of 60000 rows
+    for hidden, sums in ((64, others), (65, wide), (128, wide), (129, others), (192, others),
+                         (200, wide), (256, wide)):
+        assert left(2, 60000, 2048, hidden, 1) == sums, hidden
+    # float32 has none
+    assert left(0, 60000, 2048, 256, 1) == others

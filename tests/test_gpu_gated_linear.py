@@ -366,3 +366,9 @@ def test_nothing_is_written_past_the_workspace(native_lib, size):
     assert (space[need:] == 0x5A).all()
     for got, want in zip(grads, step(x, w, b, g, "silu")[1:]):
         assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("size", [(128, 1024, 28672), (130, 1024, 28672), (300, 1024, 28672), (60000, 1024, 64),
+                                  (60000, 1024, 68), (60000, 1024, 160)], ids=str)
+def test_borders_of_large_tiles(size):
+    check(*make(*size, torch.bfloat16))

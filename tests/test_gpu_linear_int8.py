@@ -214,3 +214,10 @@ def test_streams_and_captured_calls(rows):
         torch.cuda.synchronize()
         for _, source, out in graphs:
             assert torch.equal(out, linear_int8(source, w, s, b, residual=r))
+
+
+@pytest.mark.parametrize("size", [(5, 1024, 57344), (128, 1024, 57344), (130, 1024, 57344),
+                                  (60000, 1024, 128), (60000, 1024, 136), (60000, 1024, 320)], ids=str)
+def test_borders_of_large_tiles(size):
+    x, w, s, b, r = make(*size, torch.bfloat16)
+    check(x, w, s, b, r, "relu")
