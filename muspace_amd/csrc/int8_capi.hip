@@ -98,9 +98,12 @@ bool few_rows(int64_t m, int64_t k) {
 // half workgroups and more share a CU, and short ones; of a long weight 64 rows a time read too
 // much. In two kernels and in this one, us, bf16: 180000 x 256 -> 256 65.6 and 57.1, 40000 x 256
 // -> 512 32.2 and 29.7, 25000 x 256 -> 256 19.0 and 16.3, 100000 x 128 -> 128 25.4 and 22.7; 17000
-// x 256 -> 256 13.0 and 14.9, 33000 x 256 -> 1024 52 and 62.
+// x 256 -> 256 13.0 and 14.9, 33000 x 256 -> 1024 52 and 62. (A launch holds fewer than 2^32
+// threads; tiles are of twice as many rows.)
 bool row_blocks(int64_t m, int64_t n, int64_t k) {
-  return k <= dense::kBlockIn && n <= 512 && ceil_div(m, dense::kBlockRows) * 2 >= 3 * kCus;
+  const int64_t blocks = ceil_div(m, dense::kBlockRows);
+  return k <= dense::kBlockIn && n <= 512 && blocks * 2 >= 3 * kCus &&
+         blocks * dense::kThreads < int64_t{1} << 32;
 }
 bool fused(int64_t m, int64_t n, int64_t k) {
   return few_rows(m, k) || (few_results(m, n) ? k <= dense::kFusedIn : row_blocks(m, n, k));

@@ -221,3 +221,13 @@ def test_streams_and_captured_calls(rows):
 def test_borders_of_large_tiles(size):
     x, w, s, b, r = make(*size, torch.bfloat16)
     check(x, w, s, b, r, "relu")
+
+
+def test_more_rows_than_a_launch_of_row_blocks_holds():
+    rows = (1 << 30) + 777
+    x = torch.zeros((rows, 8), dtype=torch.bfloat16, device=DEV)
+    x[-500:] = torch.randn((500, 8), device=DEV).to(x.dtype)
+    w, s = quantize_int8(torch.randn((3, 8), device=DEV))
+    out = linear_int8(x, w, s)
+    assert_within(out[-500:], *dense_torch.linear_int8(x[-500:], w, s, None, None, None), "last rows")
+    assert not out[:-500].any()

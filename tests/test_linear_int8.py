@@ -210,3 +210,13 @@ def test_abi_without_work_and_workspace(native_lib):
     # and many short rows
     assert size(2, 40000, 256, 512) == 0 and size(2, 40000, 256, 513) > 0
     assert size(2, 24512, 256, 512) > 0 and size(2, 24513, 256, 512) == 0
+
+
+def test_no_launch_holds_too_many_threads(native_lib):
+    """2^32 threads are one too many: 2^24 workgroups of 256. Rows past 64 times that, less one
+    workgroup, are quantised into the workspace first, as longer rows are."""
+    size = native_lib.raw("linear_int8_workspace_size")
+    for rows in ((1 << 30) - 64, 1 << 20):
+        assert size(2, rows, 8, 16) == 0
+    for rows in ((1 << 30) - 63, 1 << 30, (1 << 30) + (1 << 20), (1 << 31) - 257):
+        assert size(2, rows, 8, 16) == 16 * rows + 4 * rows + -16 * rows % 256 + -4 * rows % 256
