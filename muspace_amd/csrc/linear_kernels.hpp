@@ -426,13 +426,14 @@ __device__ __forceinline__ void finish_forward(const Product &a, int64_t row, in
 }
 
 // The logistic function and one less it, from exp(-|z|), which has no overflow: both
-// keep their relative accuracy, 4e-7 (the exponent's product is carried to twice
-// float32's bits, rcp rounds to one step).
+// keep their relative accuracy, 6e-7 (the exponent's product is carried to twice
+// float32's bits, rcp rounds to one step), down to 2^-126, and steps of 2^-149 below, which
+// silu multiplies into normal numbers: exp2 has no such results, its square has.
 __device__ __forceinline__ float logistic(float z, float &other) {
   // (past 128 exp is zero; an infinity would be subtracted from itself, NaN stays)
   const float m = fabsf(z) > 128.0f ? -128.0f : -fabsf(z), p = m * 1.44269504f;
   const float rest = fmaf(m, 1.44269504f, -p) + m * 1.92596300e-8f;
-  const float power = __builtin_amdgcn_exp2f(p);
+  const float root = __builtin_amdgcn_exp2f(0.5f * p), power = root * root;
   const float e = fmaf(power * rest, 0.69314718f, power);
   const float large = __builtin_amdgcn_rcpf(1.0f + e), small = e * large;
   // (!(z < 0): NaN stays in both)
@@ -441,16 +442,23 @@ __device__ __forceinline__ float logistic(float z, float &other) {
 }
 
 // The gate's activation and its derivative; infinities have the limits' values. kShort:
-// for results of 16 bits, the logistic function in four instructions where the other takes
-// fifteen: the exponent's product is rounded once, relative 2^-24 |z|, and one less the
-// function is a difference, 2^-24 absolute (40000 x 256 -> 2 x 512 bf16 41 -> 38 us).
+// for results of 16 bits, the logistic function in seven instructions where the other takes
+// seventeen. The exponent's product is rounded once, which with log2(e)'s own rounding is relative
+// 2^-24 (1.3 |z| + 30) of either factor at the most, a hundredth of float16's own rounding.
+// Either is a product with the reciprocal r of 1 + exp(-z), and for silu of 2^-32 (1 + exp(-z)):
+// rcp has no results under 2^-126, but silu is a normal number down to z = -92. (40000 x 256 -> 2 x
+// 512 bf16 36.8 us; 36.6 with 1 - s for the other factor, which loses a saturated sigmoid's
+// derivative; 3 more with the float32 form.)
 template <bool kShort>
 __device__ __forceinline__ float gate_of(int act, float z, float &slope) {
   if (act == kSilu || act == kSigmoid) {
     float s, other;
     if constexpr (kShort) {
-      s = __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(z * -1.44269504f));
-      other = 1.0f - s;
+      const float shift = act == kSilu ? 32.0f : 0.0f, one = act == kSilu ? 0x1p-32f : 1.0f;
+      const float e = __builtin_amdgcn_exp2f(fmaf(z, -1.44269504f, -shift));
+      const float r = __builtin_amdgcn_rcpf(one + e);
+      s = one * r;
+      other = fminf(e, 0x1.fffffep127f) * r;  // (no infinity times zero)
     } else {
       s = logistic(z, other);
     }

@@ -372,3 +372,76 @@ def test_nothing_is_written_past_the_workspace(native_lib, size):
                                   (60000, 1024, 68), (60000, 1024, 160)], ids=str)
 def test_borders_of_large_tiles(size):
     check(*make(*size, torch.bfloat16))
+
+
+def gate_bounds(z, activation, dtype):
+    """(value, derivative, bounds of their errors before they are rounded) of a gate in a type.
+
+    16 bits: silu's and sigmoid's factors are off by a relative 2^-24 (1.3 |z| + 32), the
+    exponent's rounding and a few of operations; float32 and the other gates as in
+    test_the_whole_range_of_a_gate. The products keep silu to |z| steps of 2^-149; sigmoid and
+    its derivative may be zero where they are under 2^-126, and gelu's under 2^-119."""
+    value, slope = dense_torch.gate(z, activation)
+    near = dense_torch.SUM_STEP * (16 + (z.square() if activation == "gelu" else 0))
+    if dtype != torch.float32 and activation in ("silu", "sigmoid"):
+        near = 2.0**-24 * (1.3 * z.abs() + 40)
+    terms = slope.abs()
+    if activation == "gelu":
+        terms = (0.5 * torch.special.erfc(-z * math.sqrt(0.5))
+                 + z.abs() * torch.exp(-0.5 * z * z) / math.sqrt(2 * math.pi))
+    elif activation == "silu":
+        terms = torch.sigmoid(z) * (1 + z.abs() * torch.sigmoid(-z))
+    floor = {"silu": (z.abs() + 1) * 2.0**-149, "sigmoid": 2.0**-126, "gelu": 2.0**-119}.get(activation, 0)
+    # (2 near: the derivative has both factors, the sigmoid's their product)
+    return value, slope, near * value.abs() + floor, 2 * near * terms + floor
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("activation", GATES)
+def test_the_tails_of_a_gate_in_every_type(activation, dtype):
+    """As far as the type's numbers reach: a saturated sigmoid's derivative and silu's far left
+    keep their relative accuracy."""
+    a = torch.cat([torch.linspace(-130, 130, 4001, device=DEV), torch.linspace(-2, 2, 1001, device=DEV),
+                   torch.linspace(-95, -86, 181, device=DEV)]).to(dtype)
+    w = torch.tensor([[1.0], [0.0]], dtype=dtype, device=DEV)
+    b = torch.tensor([0.0, 1.0], dtype=dtype, device=DEV)
+    for x in (a[:, None], a[-4:, None], a[-40:, None]):  # in tiles, few rows, few results
+        xs = x.clone().requires_grad_()
+        out = gated_linear(xs, w, b, activation=activation)
+        dx, = torch.autograd.grad(out, [xs], torch.ones_like(out))
+        value, slope, value_err, slope_err = gate_bounds(x.double(), activation, dtype)
+        for got, e, err in ((out.detach(), value, value_err), (dx, slope, slope_err)):
+            # rounded once
+            u, small = dense_torch.half_step(dtype), dense_torch.tiny(dtype)
+            assert_within(got, e, err * (1 + u) + u * e.abs() + small, activation)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows", [2, 70, 5000])
+def test_limits_and_nan_in_every_type(rows, dtype):
+    """The limits of the gates and of their derivatives at infinities; NaN stays in its results."""
+    inf = math.inf
+    w = torch.ones((2, 1), dtype=dtype, device=DEV)
+    # the other half is a constant: its weight is zero, and no infinity meets it in the products
+    w[1] = 0.0
+    b = torch.tensor([inf, 1.0], dtype=dtype, device=DEV)
+    x = torch.zeros((rows, 1), dtype=dtype, device=DEV)
+    for activation, top, low, above, below in (
+            (None, inf, -inf, 1.0, 1.0), ("relu", inf, 0.0, 1.0, 0.0), ("gelu", inf, 0.0, 1.0, 0.0),
+            ("silu", inf, 0.0, 1.0, 0.0), ("sigmoid", 1.0, 0.0, 0.0, 0.0)):
+        for sign, value, slope in ((1.0, top, above), (-1.0, low, below)):
+            bias = (b * torch.tensor([sign, 1.0], dtype=dtype, device=DEV)).requires_grad_()
+            out = gated_linear(x, w, bias, activation=activation)
+            assert (out == value).all(), (activation, sign)
+            db, = torch.autograd.grad(out, [bias], torch.ones_like(out))
+            # (5000 rounds to the bfloat16 number 4992)
+            assert db[0] == torch.tensor(slope * rows).to(dtype), (activation, sign)
+        xs = x.clone()
+        xs[1] = math.nan
+        out = gated_linear(xs, w, activation=activation)
+        assert out[1].isnan() and not out[0].isnan()
+        # and in the gate's own derivative
+        xs.requires_grad_()
+        dx, = torch.autograd.grad(gated_linear(xs, w, activation=activation), [xs],
+                                  torch.ones((rows, 1), dtype=dtype, device=DEV))
+        assert dx[1].isnan() and not dx[0].isnan()
