@@ -36,7 +36,8 @@ def quantize_int8_pytorch(input: torch.Tensor) -> tuple[torch.Tensor, torch.Tens
     x = input.detach().float()
     top = x.abs().amax(-1) if x.shape[-1] else x.new_zeros(x.shape[:-1])
     finite = top.isfinite()
-    scales = torch.where(finite, (top / 127.0).clamp_min(2.0**-126), torch.nan)
+    # (by a tensor: on a GPU torch multiplies with a number's reciprocal, which rounds twice)
+    scales = torch.where(finite, (top / torch.full_like(top, 127.0)).clamp_min(2.0**-126), torch.nan)
     quotients = x / torch.where(finite, scales, 1.0).unsqueeze(-1)
     codes = torch.where(finite.unsqueeze(-1), torch.round(quotients), 1.0)
     return codes.to(torch.int8), scales

@@ -6,6 +6,7 @@ import pytest
 import torch
 
 from muspace_amd import get_last_dispatch_report, linear_int8, quantize_int8
+from muspace_amd.ops import quantize_int8_pytorch
 from oracle import dense_torch
 
 pytestmark = pytest.mark.gpu
@@ -231,3 +232,15 @@ def test_more_rows_than_a_launch_of_row_blocks_holds():
     out = linear_int8(x, w, s)
     assert_within(out[-500:], *dense_torch.linear_int8(x[-500:], w, s, None, None, None), "last rows")
     assert not out[:-500].any()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_the_pytorch_path_takes_the_same_codes(dtype):
+    """Scales are quotients by 127, which a product with its reciprocal would miss by a step."""
+    gen = torch.Generator(device=DEV).manual_seed(11)
+    x = torch.randn((20000, 96), generator=gen, device=DEV)
+    x = (x * torch.exp(torch.randn((20000, 1), generator=gen, device=DEV))).to(dtype)
+    codes, scales = quantize_int8(x)
+    for got, want in ((quantize_int8_pytorch(x), (codes, scales)),
+                      (dense_torch.quantize(x), (codes, scales))):
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
