@@ -98,12 +98,17 @@ bool few_rows(int64_t m, int64_t k) {
 // half workgroups and more share a CU, and short ones; of a long weight 64 rows a time read too
 // much. In two kernels and in this one, us, bf16: 180000 x 256 -> 256 65.6 and 57.1, 40000 x 256
 // -> 512 32.2 and 29.7, 25000 x 256 -> 256 19.0 and 16.3, 100000 x 128 -> 128 25.4 and 22.7; 17000
-// x 256 -> 256 13.0 and 14.9, 33000 x 256 -> 1024 52 and 62. (A launch holds fewer than 2^32
-// threads; tiles are of twice as many rows.)
+// x 256 -> 256 13.0 and 14.9, 33000 x 256 -> 1024 52 and 62; between, 40000 x 256 -> 640 33.4 and
+// 30.6, -> 768 34.5 and 33.6. With codes of 512 values in LDS, two workgroups a CU: 40000 x 320 ->
+// 512 35.9 and 40.9, x 512 39.1 and 47.7. Unaligned rows of the weight, which every workgroup reads
+// anew: 40000 x 100 -> 512 24.5 and 31.2, 180000 x 3 -> 256 44.5 and 57.3. Few products for a row:
+// 40000 x 32 -> 32 9.5 and 10.5, float32 9.0 and 10.7, x 64 -> 64 10.1 and 11.3; 40000 x 64 -> 256
+// float32 18.0 and 16.2, x 128 -> 64 13.4 and 11.7. (A launch holds fewer than 2^32 threads;
+// tiles are of twice as many rows.)
 bool row_blocks(int64_t m, int64_t n, int64_t k) {
   const int64_t blocks = ceil_div(m, dense::kBlockRows);
-  return k <= dense::kBlockIn && n <= 512 && blocks * 2 >= 3 * kCus &&
-         blocks * dense::kThreads < int64_t{1} << 32;
+  return k <= dense::kBlockIn && k % 16 == 0 && (k > 64 || n > 128) && n <= 512 &&
+         blocks * 2 >= 3 * kCus && blocks * dense::kThreads < int64_t{1} << 32;
 }
 bool fused(int64_t m, int64_t n, int64_t k) {
   return few_rows(m, k) || (few_results(m, n) ? k <= dense::kFusedIn : row_blocks(m, n, k));

@@ -244,3 +244,15 @@ def test_the_pytorch_path_takes_the_same_codes(dtype):
     for got, want in ((quantize_int8_pytorch(x), (codes, scales)),
                       (dense_torch.quantize(x), (codes, scales))):
         assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("size", [(24600, 80, 96), (24600, 64, 136), (24600, 64, 128), (25001, 100, 200),
+                                  (30007, 16, 512), (24577, 240, 40)], ids=str)
+def test_short_rows(size, dtype):
+    x, w, s, b, r = make(*size, dtype)
+    check(x, w, s, b, r, "relu")
+    # a weight that starts between 16-byte boundaries
+    buffer = torch.zeros(w.numel() + 16, dtype=torch.int8, device=DEV)
+    moved = buffer[3:3 + w.numel()].view(w.shape).copy_(w)
+    assert torch.equal(linear_int8(x, moved, s, b, residual=r), linear_int8(x, w, s, b, residual=r))

@@ -217,6 +217,15 @@ def test_no_launch_holds_too_many_threads(native_lib):
     workgroup, are quantised into the workspace first, as longer rows are."""
     size = native_lib.raw("linear_int8_workspace_size")
     for rows in ((1 << 30) - 64, 1 << 20):
-        assert size(2, rows, 8, 16) == 0
+        assert size(2, rows, 80, 16) == 0
     for rows in ((1 << 30) - 63, 1 << 30, (1 << 30) + (1 << 20), (1 << 31) - 257):
-        assert size(2, rows, 8, 16) == 16 * rows + 4 * rows + -16 * rows % 256 + -4 * rows % 256
+        assert size(2, rows, 80, 16) == 80 * rows + 4 * rows + -80 * rows % 256 + -4 * rows % 256
+
+
+def test_short_rows_that_two_kernels_do_sooner(native_lib):
+    """Unaligned rows of the weight, and few products for a row, take a workspace."""
+    size = native_lib.raw("linear_int8_workspace_size")
+    for dtype in (0, 1, 2):
+        assert size(dtype, 40000, 80, 128) == size(dtype, 40000, 64, 136) == size(dtype, 40000, 16, 512) == 0
+        for inner, outer in ((100, 512), (3, 256), (250, 256), (64, 128), (32, 32)):
+            assert size(dtype, 40000, inner, outer) > 0
