@@ -119,7 +119,10 @@ __device__ __forceinline__ void store_codes(int8_t *to, const uint32_t (&w)[kV /
   }
 }
 
-// Rows of up to kLanes pieces, a piece a lane; a wavefront holds several short rows.
+// Rows of up to kLanes pieces, a piece a lane; a wavefront holds several short rows. 40000 x 256
+// bf16 9.3 us of 6.0 for its bytes, 16384 x 2048 24.9 of 19.5: a row's loads, its largest value and
+// its codes follow one another, between barriers where a row takes several wavefronts, and no
+// next row is on its way (with one, 40000 x 256 took 10.9 for 10.2: more registers, fewer wavefronts).
 template <typename T, int kLanes>
 __global__ __launch_bounds__(kQuantThreads) void int8_rows(const Quantise a) {
   constexpr int kV = Piece<T>::kValues;
@@ -641,7 +644,8 @@ __device__ __forceinline__ int dot_codes(const u32x4 &a, const u32x4 &b, int sum
 
 // Up to kRows rows: reading the weight is all of it, as in linear_vector. A workgroup of
 // eight wavefronts makes 16 columns, two a wavefront; it quantises the rows itself while the
-// weight's first chunks are on their way.
+// weight's first chunks are on their way. bf16, one row: 4096 -> 16384 16.7 us (4.0 TB/s of the
+// weight), 4096 -> 4096 7.6, one round of loads and the call; four rows 28 and 12.
 constexpr int kVectorCodes = 48 << 10;  // of the rows, in LDS, at the most
 
 template <typename T, int kRows>

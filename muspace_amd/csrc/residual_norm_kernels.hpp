@@ -381,7 +381,13 @@ __global__ __launch_bounds__(row_threads(kLanes)) void residual_backward(const R
 
 // --------------------------------------------------- rows of any length ---
 
-// A workgroup per row, its values computed from memory in every pass over it.
+// A workgroup per row, its values computed from memory in every pass over it, the dropout's mask
+// among them: forward two passes (rms one) for the statistics and one that writes, as many as the
+// first again for a post norm; backward two, three with a post norm, and one for the columns' sums.
+// Layer norm, dropout, us of a forward and of a backward: 16384 x 4096 bf16, the longest rows in
+// registers, 108 and 171 (4.9 and 4.7 TB/s), 16384 x 5120 374 and 956, x 8192 508 and 1140; float32 x
+// 2048 100 and 138, x 5120 431 and 560, x 8192 679 and 786. The 16-bit backward is the slowest: it
+// sums block and residual again in each pass.
 constexpr int kLongThreads = 256;
 
 template <typename T, typename F>

@@ -6,9 +6,11 @@ product in one kernel.
 ``weight`` holds the gate's rows, then the others'. The products run on the matrix cores
 with float32 sums, a and u of a result in one wavefront's registers, and neither is
 written: the result is rounded once. The backward keeps the input alone and multiplies
-again for a and u, which costs a third of the products of a step and saves two tensors
-of the block's width, their writes and their reads; da and du are rounded to the
-tensors' type once, before they are multiplied with the weight and the input.
+again for a and u, a third of the products of a step more: that saves two tensors of the
+block's width in memory between the passes, and the rounding that 16 bits of them would
+give the gradients. It does not save time where rows are long: kept, they would be written and
+read sooner. da and du are rounded to the tensors' type once, before they are multiplied with the
+weight and the input.
 
 The second half of the block is ``linear``, with its residual. No reference counterpart:
 the reference leaves these products to torch.
